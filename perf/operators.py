@@ -232,7 +232,7 @@ def _attn_inputs(case, seed):
 
 def _attn_handles(case, st):
     ops, out = _ops(), torch.empty_like(st["q"])
-    plan = ops.PrefixPlan(case["rows"], case["heads"], case["kv_heads"], case["prefix"], "cuda")
+    plan = ops.PrefixPlan(case["rows"], case["heads"], case["kv_heads"], "cuda")
     ops.prefix_plan(st["slot"], st["group"], st["prefix"], plan)  # (once for all layers of a step)
     st["call"] = lambda: ops.paged_attention_shared(st["q"], st["k"], st["v"], st["table"], st["slot"], st["pos"], plan, case["heads"], out=out)
 
