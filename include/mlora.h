@@ -641,6 +641,49 @@ int mlora_delta_step(const void* d_x, int64_t ld, int32_t C, int32_t taps, int32
                      const int32_t* d_row_slot, const int32_t* d_row_pos, int32_t T, float* d_state, void* d_ring, void* d_out,
                      int32_t* d_status, int32_t f32, void* stream);
 
+/* ---- decode attention of a batch that shares prefixes -----------------------------------------------------------------
+ * Rows of a step whose sequences begin with the same pages (a system prompt, a document) read those pages once for all of them.
+ * A prefix has an id; d_prefix_id [n_slots] names the one a cache slot's sequence begins with (< 0: none), d_prefix_len [n_slots]
+ * its tokens: the first of them lie in the same pages for every slot with that id (any number; a page that only starts with shared
+ * tokens is each slot's own, with those tokens in it).
+ * mlora_prefix_plan: groups the rows of a step (d_row_slot [T]) by prefix, once for all layers.  Prefixes of fewer than 64 tokens
+ *   and groups of one row are left to the rows.  d_plan: mlora_prefix_plan_bytes(max_rows) bytes, 16-byte aligned; max_rows <= 1024.
+ * mlora_paged_attention_shared: out[t, h*D..] = softmax(scale q_t k^T) v over tokens 0..pos_t of the row's sequence (rows with
+ *   pos < 0: zeros), q as mlora_kv_append_rope leaves it (row stride ld) and the tokens' keys and values in the pages.  d_plan: of the
+ *   same rows, T, Hq and Hkv.  D 64 or 128, pages of 16 or 32, up to 42 query heads per key head.  Results do not depend on which
+ *   rows lie next to each other; the order of the sums depends on the groups.
+ *   d_work: mlora_paged_attention_shared_workspace bytes, zero-filled once before its first use (arrival counters, which reset
+ *   themselves, at a place that no call's sizes move); one buffer serves calls of any shape one after the other, calls that may run
+ *   at the same time need one each.  d_status as for mlora_prefill_attention. */
+size_t mlora_prefix_plan_bytes(int32_t max_rows);
+int mlora_prefix_plan(const int32_t* d_row_slot, int32_t T, const int32_t* d_prefix_id, const int32_t* d_prefix_len, int32_t n_slots,
+                      int32_t Hq, int32_t Hkv, int32_t* d_plan, int32_t max_rows, void* stream);
+size_t mlora_paged_attention_shared_workspace(int32_t T, int32_t Hq, int32_t Hkv, int32_t D);
+int mlora_paged_attention_shared(const void* d_q, int64_t ld, const void* d_k_pages, const void* d_v_pages, int32_t n_pages_total,
+                                 const int32_t* d_block_table, int32_t max_pages, const int32_t* d_row_slot,
+                                 const int32_t* d_row_pos, int32_t T, int32_t Hq, int32_t Hkv, int32_t D, int32_t page_size,
+                                 float scale, const int32_t* d_plan, int32_t plan_rows, void* d_out, int64_t ld_out, void* d_work,
+                                 size_t work_bytes, int32_t* d_status, void* stream);
+
+/* ---- the next tokens under rules ---------------------------------------------------------------------------------------
+ * tok[t] = first index of the row maximum of the logits d_logits [T, V] (fp32, row stride ld) after the rules of row t's request
+ * s = d_row_src[t] (NULL: s = t; outside 0..n-1, a row of padding: no rules), applied in this order, each step rounded to fp32:
+ *   v seen in the first d_prompt_len[s] tokens of d_prompt [n, ld_prompt] or the first d_answer_len[s] of d_answer [n, ld_answer]:
+ *       l = l > 0 ? l / repetition[s] : l * repetition[s]
+ *   c = how often the answer has v:  l = l - frequency[s] * c;  l = l - presence[s] where c > 0
+ *   l = l + bias of v in set b = d_bias_set[s] (outside 0..n_sets-1: none): entries d_bias_start[b] .. d_bias_start[b + 1] of
+ *       d_bias_token / d_bias_value [n_bias], ascending tokens (a token that is there twice gets the sum)
+ *   l = -inf where bit v % 32 of d_masks[d_mask_of[s] * ld_mask + v / 32] is 0 (mask_of outside 0..n_masks-1: everything is allowed)
+ * tok -1: no logit above -inf (a mask that allows nothing); NaN never wins, except that a mask turns it into -inf like any other.
+ * d_logits_out (optional, row stride ld_out, may be d_logits): the logits after the rules.  Every table may be NULL with its
+ * companions: no such rule. */
+int mlora_choose_tokens(const float* d_logits, int64_t ld, int32_t T, int32_t V, const int32_t* d_row_src, int32_t n,
+                        const float* d_repetition, const float* d_frequency, const float* d_presence, const int32_t* d_prompt,
+                        const int32_t* d_prompt_len, int64_t ld_prompt, const int32_t* d_answer, const int32_t* d_answer_len,
+                        int64_t ld_answer, const int32_t* d_bias_set, const int32_t* d_bias_start, const int32_t* d_bias_token,
+                        const float* d_bias_value, int32_t n_sets, int32_t n_bias, const int32_t* d_mask_of, const int32_t* d_masks,
+                        int32_t n_masks, int64_t ld_mask, float* d_logits_out, int64_t ld_out, int32_t* d_tok, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

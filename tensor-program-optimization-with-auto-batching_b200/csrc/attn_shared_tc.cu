@@ -1,0 +1,871 @@
+// Decode attention of a batch whose rows share long prefixes: the pages of a shared prefix are read once for all rows that have it
+// (the page-sharing counterpart of attention_with_fused_qkv, tvm/llama_auto_batcher/llama_for_causal_lm.py:55-64).
+//
+// softmax(q K^T) V over the keys of a row falls into ranges: with m, l and O the maximum, the sum of exp(s - m) and the sum of
+// exp(s - m) v of a range, two ranges make one with m = max(m1, m2), l = l1 e^(m1 - m) + l2 e^(m2 - m), O likewise.  So
+//
+//   prefix_plan_kernel     groups the rows of a step by the prefix their slot names (once a step, for all layers);
+//   prefix_attn_kernel     the prefix: up to 128 (row, query head) pairs that share a key head are the M rows of one tcgen05 tile, a CTA
+//                          takes a range of the prefix's keys and leaves m, l, O of its pairs in scratch;
+//   tail_attn_kernel       what follows the prefix, row by row, and the join of everything.
+//
+// The prefix has 2 D 2 bytes per key and key head against 4 D 128 flops of a full tile: bound by HBM up to some 128 pairs (rows x query
+// heads per key head), by the softmax beyond.  The tail is bound by HBM alone: its tiles have only the query heads of one key head, so
+// it uses mma.sync on 16 of them, with a ring of asynchronous copies in every warp.
+#include <math.h>
+
+#include <atomic>
+
+#include "common.cuh"
+#include "tc_ptx.cuh"
+
+namespace mlora {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kTile = 128;               // (row, query head) pairs of a tile = keys of a block
+constexpr int kSub = kTile * 64 * 2;     // one [128 x 64] bf16 sub-tile: 16 KB
+constexpr int kPxThreads = 160;          // warps 0..3: one thread per pair; warp 4: copies and MMA issue
+constexpr int kPlanMaxRows = 1024;
+constexpr int kPlanHeader = 8;           // int32: rows, tiles, items, parts
+constexpr int kTickets = 1024;           // arrival counters at the start of the scratch, whatever the call's sizes: zero between calls
+constexpr int kPlanMinRows = 2, kPlanMinKeys = 64;  // smaller groups and shorter prefixes are read row by row
+
+// A plan in int32: header, then two quads per tile (slot whose pages are read, keys, rows, first entry of `list` | first item, key ranges
+// per pair, first part, 0), then per row: `list` (rows by group), first key of the row's own part, its first part, its parts.
+struct PlanView {
+  int32_t *head, *tiles, *list, *first, *part, *n_part;
+};
+__host__ __device__ inline PlanView plan_view(int32_t* p, int max_rows) {
+  PlanView v;
+  v.head = p;
+  v.tiles = p + kPlanHeader;
+  v.list = v.tiles + 8 * (max_rows / kPlanMinRows + 1);
+  v.first = v.list + max_rows;
+  v.part = v.first + max_rows;
+  v.n_part = v.part + max_rows;
+  return v;
+}
+
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    n = 148;
+  }
+  return n;
+}
+
+// Rows of a tile; parts (a row's partial results over the key ranges of its prefix) that scratch has room for: an item is a tile's key
+// range and key head, there are at most `target` of them or one per tile and key head.
+int tile_rows(int rep) { return kTile / rep; }
+long long max_parts(int T, int rep, int Hkv, int target) {
+  const long long r = T < tile_rows(rep) ? T : tile_rows(rep), s = (target + Hkv - 1) / Hkv;
+  return r * s > T ? r * s : T;
+}
+
+__device__ __forceinline__ int block_sum_int(int v, int* sm /*[33]*/) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
+  __syncthreads();
+  int s = 0;
+  for (int w = 0; w < (int)(blockDim.x >> 5); ++w) s += sm[w];
+  return s;
+}
+
+// One CTA, a thread per row.  Rows of a group keep their order; groups are ordered by their first row.
+__global__ void __launch_bounds__(kPlanMaxRows) prefix_plan_kernel(const int32_t* __restrict__ row_slot, int T,
+                                                                   const int32_t* __restrict__ prefix_id, const int32_t* __restrict__ prefix_len,
+                                                                   int n_slots, int rt, int Hkv, int target, int cap_parts, int32_t* plan, int max_rows) {
+  __shared__ int s_id[kPlanMaxRows];     // prefix of the row, -1: none
+  __shared__ int s_lead[kPlanMaxRows];   // first row of its group, if the group is taken together
+  __shared__ int s_tile[kPlanMaxRows / kPlanMinRows + 1][4];  // blocks, rows, key ranges
+  __shared__ int s_red[33];
+  pdl_launch_dependents();
+  pdl_wait();
+  const PlanView v = plan_view(plan, max_rows);
+  const int t = threadIdx.x;
+  int id = -1, len = 0, slot = 0;
+  if (t < T) {
+    slot = row_slot[t];
+    if (slot >= 0 && slot < n_slots) id = prefix_id[slot], len = prefix_len[slot];
+  }
+  if (len < kPlanMinKeys) id = -1;
+  s_id[t] = id;
+  __syncthreads();
+  int rank = 0, count = 0, lead = t;
+  if (id >= 0)
+    for (int j = 0; j < T; ++j)
+      if (s_id[j] == id) {
+        if (j < lead) lead = j;
+        rank += j < t;
+        ++count;
+      }
+  const bool used = count >= kPlanMinRows;
+  s_lead[t] = used ? lead : -1;
+  __syncthreads();
+  const bool opens = used && rank % rt == 0;  // first row of a tile
+  const int n_tiles = block_sum_int(opens, s_red);
+  int place = 0, tile = 0;
+  if (used) {
+    for (int j = 0; j < T; ++j) place += s_lead[j] >= 0 && s_lead[j] < lead;
+  }
+  // tiles before this row's group: a group of n rows has ceil(n / rt); the group's first row knows n
+  __shared__ int s_group_tiles[kPlanMaxRows];
+  s_group_tiles[t] = used && rank == 0 ? (count + rt - 1) / rt : 0;
+  __syncthreads();
+  if (used) {
+    for (int j = 0; j < lead; ++j) tile += s_group_tiles[j];
+    tile += rank / rt;
+    place += rank;
+    v.list[place] = t;
+  }
+  int blocks = 0, rows = 0;
+  if (opens) {
+    rows = min(rt, count - rank);
+    blocks = (len + kTile - 1) / kTile;
+    s_tile[tile][0] = blocks;
+    s_tile[tile][1] = rows;
+  }
+  const int total = block_sum_int(blocks, s_red);
+  // keys per item, in blocks: as few as make no more than `target` items, which is what runs at once
+  int unit = max(1, (int)(((long long)total * Hkv + target - 1) / target));
+  for (;;) {
+    const int splits = opens ? (blocks + unit - 1) / unit : 0;
+    const int items = block_sum_int(splits, s_red) * Hkv, parts = block_sum_int(splits * rows, s_red);
+    const int longer = block_sum_int(opens && blocks > unit, s_red);
+    if (longer == 0 || (items <= target && parts <= cap_parts)) break;
+    unit += max(1, unit / 8);
+  }
+  const int splits = opens ? (blocks + unit - 1) / unit : 0;
+  if (opens) s_tile[tile][2] = splits;
+  __syncthreads();
+  int part_of_row = 0, n_part = 0;
+  if (used) {
+    int item = 0, part = 0;
+    for (int i = 0; i < tile; ++i) {
+      item += s_tile[i][2] * Hkv;
+      part += s_tile[i][1] * s_tile[i][2];
+    }
+    n_part = s_tile[tile][2];
+    part_of_row = part + (rank % rt) * n_part;
+    if (opens) {
+      reinterpret_cast<int4*>(v.tiles)[2 * tile] = make_int4(slot, len, rows, place);
+      reinterpret_cast<int4*>(v.tiles)[2 * tile + 1] = make_int4(item, splits, part, 0);
+    }
+  }
+  if (t < T) {
+    v.first[t] = used ? len : 0;
+    v.part[t] = part_of_row;
+    v.n_part[t] = n_part;
+  }
+  const int items = block_sum_int(splits, s_red) * Hkv, parts = block_sum_int(splits * rows, s_red);
+  if (t == 0) {
+    v.head[0] = T;
+    v.head[1] = n_tiles;
+    v.head[2] = items;
+    v.head[3] = parts;
+  }
+}
+
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+struct SharedArgs {
+  const bf16* q;
+  int64_t ld;
+  const bf16* k_pages;
+  const bf16* v_pages;
+  const int32_t* block_table;
+  int max_pages;
+  const int32_t* row_slot;
+  const int32_t* row_pos;
+  int T, Hq, Hkv, page_size;
+  int32_t* plan;
+  int plan_rows;
+  float* parts;     // [part][Hq][D + 2]: O, m, l of a row's key range (base-2 logarithms)
+  float* own;       // [T][Hq][n_splits][D + 2]
+  int32_t* tickets; // [T][Hkv][head tiles], zero between calls
+  int n_splits;
+  bf16* out;
+  int64_t ld_out;
+  float scale;      // of the scores, times log2(e)
+  int32_t* status;
+};
+
+// One item: a tile's pairs x a range of the prefix's blocks of 128 keys x one key head.  As in the prompt attention, S = Q K^T and
+// P V are tcgen05 products with S, P and O in TMEM, keys and values arrive page by page through the block table of the group's first
+// row, and one thread per pair runs the softmax against the exact running maximum.
+template <int ND, int PS>
+__global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid_constant__ CUtensorMap map_k,
+                                                                     const __grid_constant__ CUtensorMap map_v,
+                                                                     const __grid_constant__ CUtensorMap map_kr,
+                                                                     const __grid_constant__ CUtensorMap map_vr, SharedArgs a) {
+  constexpr int D = ND * 64, kPages = kTile / PS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sq = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* sk = sq + ND * kSub;
+  uint8_t* sv = sk + ND * kSub;
+  __shared__ uint64_t kbar, vbar;  // a block's keys / values have landed
+  __shared__ uint64_t sbar;        // S = Q K^T has retired, and every P V before it
+  __shared__ uint64_t pbar;        // the four softmax warps have written P, and taken the P V before into O
+  __shared__ uint64_t obar;        // P V has retired
+  __shared__ uint32_t tmem_slot;
+  __shared__ int s_abort, s_tile;
+
+  pdl_launch_dependents();  // (the tail's own keys do not depend on this kernel)
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const PlanView pv = plan_view(a.plan, a.plan_rows);
+  const int n_tiles = pv.head[1], item = blockIdx.x;
+  if (item >= pv.head[2]) return;  // (the whole CTA, before it has asked for anything)
+  for (int i = tid; i < n_tiles; i += kPxThreads) {
+    const int4 e = reinterpret_cast<const int4*>(pv.tiles)[2 * i + 1];
+    if (item >= e.x && item < e.x + e.y * a.Hkv) s_tile = i;
+  }
+  if (tid == 0) {
+    s_abort = 0;
+    mbar_init(&kbar, 1);
+    mbar_init(&vbar, 1);
+    mbar_init(&sbar, 1);
+    mbar_init(&pbar, 4);
+    mbar_init(&obar, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+    tma_prefetch_desc(&map_kr);
+    tma_prefetch_desc(&map_vr);
+  }
+  if (warp == 4) tmem_alloc(&tmem_slot, 256);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_slot, tmem_o = tmem_base + kTile;
+  const int4 t0 = reinterpret_cast<const int4*>(pv.tiles)[2 * s_tile], t1 = reinterpret_cast<const int4*>(pv.tiles)[2 * s_tile + 1];
+  const int rep = a.Hq / a.Hkv, kvh = (item - t1.x) / t1.y, split = (item - t1.x) % t1.y;
+  const int n_keys = min(t0.y, a.max_pages * PS);
+  const int blocks = (n_keys + kTile - 1) / kTile;
+  const int b0 = (int)((long long)blocks * split / t1.y), n_blocks = (int)((long long)blocks * (split + 1) / t1.y) - b0;
+  const int32_t* bt = a.block_table + (size_t)t0.x * a.max_pages;
+  const int n_pages = (n_keys + PS - 1) / PS;
+
+  // (the pairs' queries, as the tensor cores read them: rows of 128 bytes, 16-byte chunks XORed with the row)
+  int row = -1, head = 0;
+  if (tid < kTile) {
+    if (tid < t0.z * rep) {
+      row = pv.list[t0.w + tid / rep];
+      head = kvh * rep + tid % rep;
+    }
+    const uint4* src = reinterpret_cast<const uint4*>(a.q + (size_t)max(row, 0) * a.ld + (size_t)head * D);
+#pragma unroll
+    for (int c = 0; c < ND * 8; ++c)
+      *reinterpret_cast<uint4*>(sq + (c >> 3) * kSub + tid * 128 + (((c & 7) ^ (tid & 7)) << 4)) = row >= 0 ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  __syncthreads();
+
+  if (warp == 4) {
+    // ---- copies and MMAs: lane 0 waits and issues, one lane per page copies -----------------------------------------------
+    constexpr uint32_t idesc = make_idesc(kTile, kTile);
+    constexpr uint32_t idesc_pv = make_idesc(kTile, D) | (1u << 16);  // B operand MN-major
+    auto wait = [&](uint64_t* bar, uint32_t par) {
+      int w = 1;
+      if (lane == 0) w = mbar_wait(bar, par, &s_abort) ? 1 : 0;
+      w = __shfl_sync(0xffffffffu, w, 0);
+      if (!w) s_abort = 1;
+      return w != 0;
+    };
+    auto page_of = [&](int kb) {  // read one block ahead
+      const int pg = (b0 + kb) * kPages + lane;
+      return lane < kPages && kb < n_blocks && pg < n_pages ? bt[pg] : -1;
+    };
+    auto copy = [&](int kb, int page, uint8_t* dst, const CUtensorMap* map, const CUtensorMap* map_run, uint64_t* bar) {
+      const int valid = min(kPages, n_pages - (b0 + kb) * kPages);
+      const int first = __shfl_sync(0xffffffffu, page, 0);
+      if (valid == kPages && __all_sync(0xffffffffu, lane >= kPages || page == first + lane)) {
+        // pages that follow each other in the pool: one copy per 64 columns
+        if (lane == 0) {
+          mbar_expect_tx(bar, (uint32_t)(ND * kSub));
+          for (int j = 0; j < ND; ++j) tma_load_4d(dst + j * kSub, map_run, j * 64, 0, kvh, first, bar);
+        }
+        __syncwarp();
+        return;
+      }
+      if (lane == 0) mbar_expect_tx(bar, (uint32_t)(valid * ND * PS * 128));
+      __syncwarp();
+      if (lane < valid)
+        for (int j = 0; j < ND; ++j) tma_load_4d(dst + j * kSub + lane * (PS * 128), map, j * 64, 0, kvh, page, bar);
+      __syncwarp();
+    };
+    int page = page_of(0), page_next = page_of(1);
+    if (n_blocks > 0) {  // (a prefix longer than the block table is cut at its end)
+      copy(0, page, sk, &map_k, &map_kr, &kbar);
+      copy(0, page, sv, &map_v, &map_vr, &vbar);
+    }
+    for (int kb = 0; kb < n_blocks; ++kb) {
+      const uint32_t par = kb & 1;
+      if (!wait(&kbar, par)) break;
+      if (lane == 0) {
+        tc_fence_after();
+#pragma unroll
+        for (int j = 0; j < ND; ++j) {
+          const uint64_t adesc = make_smem_desc(smem_u32(sq + j * kSub));
+          const uint64_t bdesc = make_smem_desc(smem_u32(sk + j * kSub));
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma_bf16(tmem_base, adesc + 2 * k, bdesc + 2 * k, idesc, (j > 0 || k > 0) ? 1u : 0u);
+        }
+        umma_commit(&sbar);
+      }
+      if (kb > 0) {  // V's place is free once the P V before has retired
+        if (!wait(&obar, par ^ 1)) break;
+        copy(kb, page, sv, &map_v, &map_vr, &vbar);
+      }
+      if (kb + 1 < n_blocks) {
+        if (!wait(&sbar, par)) break;
+        page = page_next;
+        page_next = page_of(kb + 2);
+        copy(kb + 1, page, sk, &map_k, &map_kr, &kbar);
+      }
+      if (!wait(&vbar, par) || !wait(&pbar, par)) break;
+      if (lane == 0) {
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < kTile / 16; ++k)
+          umma_bf16_ta(tmem_o, tmem_base + k * 8, make_smem_desc_mn(smem_u32(sv + k * 2048), kSub, 1024), idesc_pv, k > 0 ? 1u : 0u);
+        umma_commit(&obar);
+      }
+      __syncwarp();
+    }
+    if (s_abort && lane == 0)  // copies may still be in flight: let them land before the shared memory goes to another CTA
+      for (int i = 0; i < 64; ++i) __nanosleep(1000);
+  } else {
+    // ---- softmax: one thread per pair; a warp without pairs only keeps step -------------------------------------------------
+    const bool busy = warp * 32 < t0.z * rep;
+    const int q_pos = row >= 0 ? a.row_pos[row] : -1;
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    float o[D];
+#pragma unroll
+    for (int i = 0; i < D; ++i) o[i] = 0.f;
+    float m_run = -INFINITY, l_run = 0.f;
+    bool ok = true;
+    for (int kb = 0; kb < n_blocks && ok; ++kb) {
+      const uint32_t par = kb & 1;
+      const int kstart = (b0 + kb) * kTile;
+      ok = __all_sync(0xffffffffu, mbar_wait(&sbar, par, &s_abort));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t s_addr = tmem_base + lanes;
+      const int hi = min(q_pos, n_keys - 1) - kstart;  // last key of the block that this pair sees
+      float corr = 0.f;
+      if (busy) {
+        const bool need_mask = __any_sync(0xffffffffu, hi < kTile - 1);
+        float buf[2][16];  // 16 scores at work, the next 16 on their way
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        auto maximum = [&](auto masked) {
+          tmem_ld16_issue(s_addr, buf[0]);
+#pragma unroll
+          for (int c = 0; c < kTile / 16; ++c) {
+            tmem_wait_ld16(buf[c & 1]);
+            if (c + 1 < kTile / 16) tmem_ld16_issue(s_addr + (c + 1) * 16, buf[(c + 1) & 1]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (!masked() || c * 16 + i <= hi) mx[i & 3] = fmaxf(mx[i & 3], buf[c & 1][i]);
+          }
+        };
+        if (need_mask)
+          maximum(std::true_type{});
+        else
+          maximum(std::false_type{});
+        const float m_new = fmaxf(m_run, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale);
+        corr = m_run == -INFINITY ? 0.f : fast_exp2(m_run - m_new);
+        const float neg_m = m_new == -INFINITY ? 0.f : -m_new;  // (-inf: nothing seen yet)
+        float sum = 0.f;
+        auto probabilities = [&](auto masked) {
+          tmem_ld16_issue(s_addr, buf[0]);
+#pragma unroll
+          for (int c = 0; c < kTile / 16; ++c) {
+            tmem_wait_ld16(buf[c & 1]);
+            if (c + 1 < kTile / 16) tmem_ld16_issue(s_addr + (c + 1) * 16, buf[(c + 1) & 1]);
+            uint32_t pk[8];
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              float p[2];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                p[e] = fast_exp2(fmaf(buf[c & 1][i + e], a.scale, neg_m));
+                if (masked() && c * 16 + i + e > hi) p[e] = 0.f;
+                sum += p[e];
+              }
+              const __nv_bfloat162 b = __floats2bfloat162_rn(p[0], p[1]);
+              pk[i / 2] = *reinterpret_cast<const uint32_t*>(&b);
+            }
+            tmem_st8_issue(s_addr + c * 8, pk);
+          }
+          tmem_wait_st();
+        };
+        if (need_mask)
+          probabilities(std::true_type{});
+        else
+          probabilities(std::false_type{});
+        l_run = fmaf(l_run, corr, sum);
+        m_run = m_new;
+      }
+      if (n_keys - kstart < kTile) {
+        // the prefix ends inside this block: values of keys that are not its own are zeroed (0 * NaN is not 0)
+        ok = __all_sync(0xffffffffu, mbar_wait(&vbar, par, &s_abort));
+        if (!ok) break;
+        if (tid >= n_keys - kstart) {
+#pragma unroll
+          for (int half = 0; half < ND; ++half)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) reinterpret_cast<uint4*>(sv + half * kSub + tid * 128)[c] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&pbar);
+      ok = __all_sync(0xffffffffu, mbar_wait(&obar, par, &s_abort));
+      if (!ok) break;
+      tc_fence_after();
+      if (busy) {
+        float buf[2][16];
+        tmem_ld16_issue(tmem_o + lanes, buf[0]);
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          tmem_wait_ld16(buf[c & 1]);
+          if (c + 1 < D / 16) tmem_ld16_issue(tmem_o + lanes + (c + 1) * 16, buf[(c + 1) & 1]);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[c * 16 + i] = fmaf(o[c * 16 + i], corr, buf[c & 1][i]);
+        }
+      }
+    }
+    if (!ok) s_abort = 1;
+    if (row >= 0) {
+      float* dst = a.parts + ((size_t)(pv.part[row] + split) * a.Hq + head) * (D + 4);
+#pragma unroll
+      for (int c = 0; c < D / 4; ++c) reinterpret_cast<float4*>(dst)[c] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+      *reinterpret_cast<float2*>(dst + D) = ok ? make_float2(m_run, l_run) : make_float2(-INFINITY, 0.f);
+    }
+    if (!ok && tid == 0 && a.status) atomicOr(a.status, 1);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4) tmem_dealloc(tmem_base, 256);
+}
+
+// ---- the tail -------------------------------------------------------------------------------------------------------------------
+constexpr int kTlWarps = 4, kTlThreads = kTlWarps * 32;
+constexpr int kTlKeys = 16;  // keys a warp works on at a time
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {  // the rest of the 16 becomes zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two probabilities as the sum of two pairs of bf16: the products with the values keep 16 bits of them.
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  const float2 f = __bfloat1622float2(h);
+  const __nv_bfloat162 r = __floats2bfloat162_rn(x - f.x, y - f.y);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// grid (Hkv x head tiles, T, key ranges): up to 16 query heads of a key head over the row's keys from `first` on (or a range of them).
+template <int D, int STAGES>
+__global__ void __launch_bounds__(kTlThreads) tail_attn_kernel(SharedArgs a) {
+  constexpr int kChunks = D / 8;                       // 16-byte pieces of a key
+  constexpr int kHalf = kTlKeys * D * 2;               // bytes of 16 keys
+  extern __shared__ __align__(128) uint8_t ring[];     // [warp][stage][K | V][16 keys][D]; then the warps' partial results
+  __shared__ float s_m[kTlWarps][16], s_l[kTlWarps][16];
+  __shared__ float s_w[64 + kTlWarps][16];             // factors of the ranges that are joined
+  __shared__ int s_last;
+
+  pdl_launch_dependents();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rep = a.Hq / a.Hkv, head_tiles = (rep + 15) / 16;
+  const int kvh = blockIdx.x / head_tiles, h0 = kvh * rep + (blockIdx.x % head_tiles) * 16, n_heads = min(16, kvh * rep + rep - h0);
+  const int t = blockIdx.y, split = blockIdx.z;
+  const PlanView pv = plan_view(a.plan, a.plan_rows);
+  const int slot = a.row_slot[t], pos = a.row_pos[t], first = pv.first[t], n_part = pv.n_part[t];
+  const int32_t* bt = a.block_table + (size_t)slot * a.max_pages;
+  const int PS = a.page_size;
+  const int n_tok = (int)min((long long)max(pos + 1, 0), (long long)a.max_pages * PS);
+  // units of 16 keys; a range has at least 8 units a warp, else fewer CTAs work on the row
+  const int u0 = min(first, n_tok) / kTlKeys, units = n_tok > first ? (n_tok + kTlKeys - 1) / kTlKeys - u0 : 0;
+  const int ranges = max(1, min(a.n_splits, units / (8 * kTlWarps)));
+  if (split >= ranges) return;
+  const int ub = u0 + (int)((long long)units * split / ranges), ue = u0 + (int)((long long)units * (split + 1) / ranges);
+
+  const uint32_t base = smem_u32(ring) + warp * STAGES * 2 * kHalf;
+  auto fetch = [&](int i) {  // unit ub + warp + 4 i -> stage i % STAGES
+    const int u = ub + warp + i * kTlWarps;
+    if (u < ue) {
+      const int key = u * kTlKeys, page = bt[key / PS];
+      const size_t at = (((size_t)page * a.Hkv + kvh) * PS + key % PS) * D;
+      const uint32_t dst = base + (i % STAGES) * 2 * kHalf;
+#pragma unroll
+      for (int c = 0; c < kTlKeys * kChunks / 32; ++c) {
+        const int p = c * 32 + lane, r = p / kChunks, ch = p % kChunks;
+        const int n = key + r >= first && key + r < n_tok ? 16 : 0;  // (what is not the row's own becomes zeros)
+        const uint32_t d = dst + r * (D * 2) + ((ch ^ (r & 7)) << 4);
+        cp_async16(d, a.k_pages + at + (size_t)r * D + ch * 8, n);
+        cp_async16(d + kHalf, a.v_pages + at + (size_t)r * D + ch * 8, n);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) fetch(i);
+
+  // queries as the A operand: rows = heads, a register pair of columns 16 s + 2 (lane % 4) and + 8
+  uint32_t qa[D / 16][4];
+  {
+    const int g = lane >> 2, c = (lane & 3) * 2;
+    const bf16* q0 = a.q + (size_t)t * a.ld + (size_t)(h0 + g) * D + c;
+    const bf16* q1 = q0 + 8 * D;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      qa[s][0] = g < n_heads ? *reinterpret_cast<const uint32_t*>(q0 + s * 16) : 0u;
+      qa[s][1] = g + 8 < n_heads ? *reinterpret_cast<const uint32_t*>(q1 + s * 16) : 0u;
+      qa[s][2] = g < n_heads ? *reinterpret_cast<const uint32_t*>(q0 + s * 16 + 8) : 0u;
+      qa[s][3] = g + 8 < n_heads ? *reinterpret_cast<const uint32_t*>(q1 + s * 16 + 8) : 0u;
+    }
+  }
+  float o[D / 8][4];
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  const int mr = lane & 7, mi = lane >> 3;  // row and matrix whose address this lane gives to ldmatrix
+
+  for (int i = 0; ub + warp + i * kTlWarps < ue; ++i) {
+    fetch(i + STAGES - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+    __syncwarp();
+    const int key = (ub + warp + i * kTlWarps) * kTlKeys;
+    const uint32_t sk = base + (i % STAGES) * 2 * kHalf, sv = sk + kHalf;
+    float s[2][4] = {};
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {  // matrices: keys 0-7 and 8-15, columns 16 k and + 8
+      uint32_t b[4];
+      const int r = (mi >> 1) * 8 + mr, ch = 2 * k + (mi & 1);
+      ldsm4(sk + r * (D * 2) + ((ch ^ mr) << 4), b);
+      mma16816(s[0], qa[k], b[0], b[1]);
+      mma16816(s[1], qa[k], b[2], b[3]);
+    }
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int kk = key + n * 8 + (lane & 3) * 2 + (e & 1);
+        s[n][e] = kk >= first && kk < n_tok ? s[n][e] * a.scale : -INFINITY;
+        mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
+      }
+    float corr[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+      const float mn = fmaxf(m[r], mx[r]);
+      corr[r] = m[r] == -INFINITY ? 0.f : fast_exp2(m[r] - mn);
+      l[r] *= corr[r];
+      m[r] = mn;
+    }
+    uint32_t ph[4], pl[4];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float x = s[n][2 * r] == -INFINITY ? 0.f : fast_exp2(s[n][2 * r] - m[r]);
+        const float y = s[n][2 * r + 1] == -INFINITY ? 0.f : fast_exp2(s[n][2 * r + 1] - m[r]);
+        l[r] += x + y;
+        split_pair(x, y, ph[n * 2 + r], pl[n * 2 + r]);
+      }
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {  // matrices: keys 0-7 and 8-15 of columns 16 c, then of 16 c + 8
+      uint32_t b[4];
+      const int r = (mi & 1) * 8 + mr, ch = 2 * c + (mi >> 1);
+      ldsm4t(sv + r * (D * 2) + ((ch ^ mr) << 4), b);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        float(&d)[4] = o[2 * c + n];
+        d[0] *= corr[0], d[1] *= corr[0], d[2] *= corr[1], d[3] *= corr[1];
+        mma16816(d, ph, b[2 * n], b[2 * n + 1]);
+        mma16816(d, pl, b[2 * n], b[2 * n + 1]);
+      }
+    }
+    __syncwarp();  // (the next copy overwrites what was read here)
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();  // every warp is done with the ring
+
+  // ---- the four warps' results, joined with what the prefix's key ranges left ---------------------------------------------------
+  float* acc = reinterpret_cast<float*>(ring);  // [warp][16][D]
+  {
+    const int g = lane >> 2, c = (lane & 3) * 2;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+      if ((lane & 3) == 0) s_m[warp][g + 8 * r] = m[r], s_l[warp][g + 8 * r] = l[r];
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+        *reinterpret_cast<float2*>(acc + ((size_t)warp * 16 + g + 8 * r) * D + n * 8 + c) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+    }
+  }
+  __syncthreads();
+  bool join = true;
+  int32_t* ticket = a.tickets + ((size_t)t * a.Hkv + kvh) * head_tiles + blockIdx.x % head_tiles;
+  if (ranges > 1) {  // this range's result into scratch; the last one of the row and key head joins them all
+    for (int i = tid; i < n_heads * (D / 4); i += kTlThreads) {
+      const int h = i / (D / 4), c = i % (D / 4);
+      float M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < kTlWarps; ++w) M = fmaxf(M, s_m[w][h]);
+      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kTlWarps; ++w) {
+        const float f = s_m[w][h] == -INFINITY ? 0.f : fast_exp2(s_m[w][h] - M);
+        const float4 x = reinterpret_cast<const float4*>(acc + ((size_t)w * 16 + h) * D)[c];
+        L = fmaf(s_l[w][h], f, L);
+        O.x = fmaf(x.x, f, O.x), O.y = fmaf(x.y, f, O.y), O.z = fmaf(x.z, f, O.z), O.w = fmaf(x.w, f, O.w);
+      }
+      float* dst = a.own + (((size_t)t * a.Hq + h0 + h) * a.n_splits + split) * (D + 4);
+      reinterpret_cast<float4*>(dst)[c] = O;
+      if (c == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(M, L);
+    }
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+      const int before = atomicAdd(ticket, 1);
+      s_last = before == ranges - 1;
+      if (s_last) *ticket = 0;
+    }
+    __syncthreads();
+    join = s_last;
+    __threadfence();
+  }
+  if (!join) return;
+  pdl_wait();  // the prefix's results (and, for whoever follows, that every kernel before this one is done)
+  const int n_own = ranges > 1 ? ranges : kTlWarps;
+  const auto own_ml = [&](int r, int h) {
+    if (ranges == 1) return make_float2(s_m[r][h], s_l[r][h]);
+    return __ldcg(reinterpret_cast<const float2*>(a.own + (((size_t)t * a.Hq + h0 + h) * a.n_splits + r) * (D + 4) + D));
+  };
+  const float* part0 = a.parts + ((size_t)pv.part[t] * a.Hq + h0) * (D + 4);
+  const size_t part_step = (size_t)a.Hq * (D + 4);
+  // factors exp2(m - M) / L of every range, 64 prefix ranges at a time in shared memory; the totals first
+  const int h = tid / (kTlThreads / 16), sub = tid % (kTlThreads / 16);  // 8 threads per head
+  float M = -INFINITY, L = 0.f;
+  if (h < n_heads) {
+    for (int r = sub; r < n_own + n_part; r += 8) {
+      const float2 ml = r < n_own ? own_ml(r, h) : __ldcg(reinterpret_cast<const float2*>(part0 + (size_t)(r - n_own) * part_step + (size_t)h * (D + 4) + D));
+      if (ml.x == -INFINITY) continue;
+      const float mn = fmaxf(M, ml.x);
+      L = L * fast_exp2(M - mn) + ml.y * fast_exp2(ml.x - mn);
+      M = mn;
+    }
+  }
+#pragma unroll
+  for (int x = 1; x < 8; x <<= 1) {
+    const float mo = __shfl_xor_sync(0xffffffffu, M, x), lo = __shfl_xor_sync(0xffffffffu, L, x), mn = fmaxf(M, mo);
+    if (mn != -INFINITY) L = (M == -INFINITY ? 0.f : L * fast_exp2(M - mn)) + (mo == -INFINITY ? 0.f : lo * fast_exp2(mo - mn));
+    M = mn;
+  }
+  const float inv = L > 0.f ? 1.f / L : 0.f;
+  // outputs: 4 columns of a head per thread, D / 4 threads a head
+  constexpr int kPer = kTlThreads / (D / 4);           // heads in work at once
+  constexpr int kSets = 16 / kPer;
+  float4 sum[kSets];
+#pragma unroll
+  for (int i = 0; i < kSets; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int c = tid % (D / 4), hs = tid / (D / 4);
+  for (int r0 = 0; r0 < n_own + n_part; r0 += 64) {
+    const int n = min(64, n_own + n_part - r0);
+    __syncthreads();
+    if (h < n_heads)
+      for (int r = sub; r < n; r += 8) {
+        const int x = r0 + r;
+        const float mx = x < n_own ? own_ml(x, h).x : __ldcg(part0 + (size_t)(x - n_own) * part_step + (size_t)h * (D + 4) + D);
+        s_w[r][h] = mx == -INFINITY ? 0.f : fast_exp2(mx - M) * inv;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSets; ++i) {
+      const int hh = i * kPer + hs;
+      if (hh >= n_heads) continue;
+#pragma unroll 4
+      for (int r = 0; r < n; ++r) {
+        const int x = r0 + r;
+        const float f = s_w[r][hh];
+        float4 v;
+        if (x >= n_own) v = __ldcg(reinterpret_cast<const float4*>(part0 + (size_t)(x - n_own) * part_step + (size_t)hh * (D + 4)) + c);
+        else if (ranges == 1) v = reinterpret_cast<const float4*>(acc + ((size_t)x * 16 + hh) * D)[c];
+        else v = __ldcg(reinterpret_cast<const float4*>(a.own + (((size_t)t * a.Hq + h0 + hh) * a.n_splits + x) * (D + 4)) + c);
+        sum[i].x = fmaf(v.x, f, sum[i].x), sum[i].y = fmaf(v.y, f, sum[i].y), sum[i].z = fmaf(v.z, f, sum[i].z), sum[i].w = fmaf(v.w, f, sum[i].w);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kSets; ++i) {
+    const int hh = i * kPer + hs;
+    if (hh >= n_heads) continue;
+    __nv_bfloat162 b[2] = {__floats2bfloat162_rn(sum[i].x, sum[i].y), __floats2bfloat162_rn(sum[i].z, sum[i].w)};
+    *reinterpret_cast<uint2*>(a.out + (size_t)t * a.ld_out + (size_t)(h0 + hh) * D + c * 4) = *reinterpret_cast<const uint2*>(b);
+  }
+}
+
+// Pages [n_pages][Hkv][PS][D], a box of `pages` pages of one head, 64 columns: rows of 128 bytes, swizzled.
+int page_map(CUtensorMap* m, const void* ptr, int n_pages, int Hkv, int PS, int D, int pages) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(MLORA_ECUDA, "paged_attention_shared: cuTensorMapEncodeTiled is not available from this driver");
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)PS, (cuuint64_t)Hkv, (cuuint64_t)n_pages};
+  cuuint64_t strides[3] = {(cuuint64_t)D * 2, (cuuint64_t)PS * D * 2, (cuuint64_t)Hkv * PS * D * 2};
+  cuuint32_t box[4] = {64, (cuuint32_t)PS, 1, (cuuint32_t)pages};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MLORA_ECUDA, "paged_attention_shared: cuTensorMapEncodeTiled failed with %d", (int)r);
+  return MLORA_OK;
+}
+
+template <typename K>
+int allow_smem(K kernel, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!((done.load(std::memory_order_acquire) >> (dev & 63)) & 1ull)) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return fail(MLORA_ECUDA, "paged_attention_shared: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    done.fetch_or(1ull << (dev & 63), std::memory_order_release);
+  }
+  return MLORA_OK;
+}
+
+constexpr int kTlStages = 3;
+
+template <int ND, int PS>
+int launch_shared(const SharedArgs& a, int n_pages_total, int max_items, cudaStream_t st) {
+  constexpr int D = ND * 64;
+  CUtensorMap mk, mv, mkr, mvr;
+  int rc = page_map(&mk, a.k_pages, n_pages_total, a.Hkv, PS, D, 1);
+  if (!rc) rc = page_map(&mv, a.v_pages, n_pages_total, a.Hkv, PS, D, 1);
+  if (!rc) rc = page_map(&mkr, a.k_pages, n_pages_total, a.Hkv, PS, D, kTile / PS);
+  if (!rc) rc = page_map(&mvr, a.v_pages, n_pages_total, a.Hkv, PS, D, kTile / PS);
+  if (rc) return rc;
+  constexpr int smem = 3 * ND * kSub + 1024, smem_tail = kTlWarps * kTlStages * 2 * kTlKeys * D * 2;
+  static_assert(smem_tail >= kTlWarps * 16 * D * 4, "the warps' results lie in the ring");
+  static std::atomic<unsigned long long> done{0}, done_tail{0};
+  rc = allow_smem(prefix_attn_kernel<ND, PS>, smem, done);
+  if (!rc) rc = allow_smem(tail_attn_kernel<D, kTlStages>, smem_tail, done_tail);
+  if (rc) return rc;
+  if (max_items > 0) {
+    prefix_attn_kernel<ND, PS><<<(unsigned)max_items, kPxThreads, smem, st>>>(mk, mv, mkr, mvr, a);
+    count_launch();
+    MLORA_CHECK_LAUNCH("prefix_attn_kernel");
+  }
+  const int head_tiles = (a.Hq / a.Hkv + 15) / 16;
+  const cudaError_t e = launch_pdl_if(max_items > 0 && pdl_enabled_tail(), tail_attn_kernel<D, kTlStages>, dim3((unsigned)(a.Hkv * head_tiles), (unsigned)a.T, (unsigned)a.n_splits),
+                                      dim3(kTlThreads), smem_tail, st, a);
+  if (e != cudaSuccess) return fail(MLORA_ECUDA, "tail_attn_kernel: %s", cudaGetErrorString(e));
+  count_launch();
+  MLORA_CHECK_LAUNCH("tail_attn_kernel");
+  return MLORA_OK;
+}
+
+// How a call's scratch is laid out: tickets | own parts | prefix parts, in floats.
+struct SharedSizes {
+  int target, max_items, n_splits;
+  long long tickets, own, parts, cap_parts;
+};
+SharedSizes sizes_of(int T, int Hq, int Hkv, int D) {
+  SharedSizes s;
+  const int rep = Hq / Hkv, ht = (rep + 15) / 16;
+  s.target = 2 * sm_count();
+  // tiles: a group has at least kPlanMinRows rows and a full tile has more, so there are at most T / kPlanMinRows
+  const int tiles = T / kPlanMinRows;
+  s.max_items = tiles == 0 ? 0 : (int)((long long)tiles * Hkv > s.target ? (long long)tiles * Hkv : s.target);
+  const long long ctas = (long long)T * Hkv * ht;
+  s.n_splits = ctas >= s.target || ctas > kTickets ? 1 : (int)((s.target + ctas - 1) / (ctas > 0 ? ctas : 1));
+  if (s.n_splits > 32) s.n_splits = 32;
+  s.tickets = kTickets;
+  s.own = s.n_splits > 1 ? (long long)T * Hq * s.n_splits * (D + 4) : 0;
+  s.cap_parts = max_parts(T, rep, Hkv, s.target);
+  s.parts = s.cap_parts * Hq * (D + 4);
+  return s;
+}
+
+bool shared_sizes_fit(int T, int Hq, int Hkv, int D) {
+  return T >= 0 && T <= kPlanMaxRows && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && kTile / (Hq / Hkv) > kPlanMinRows && Hq <= 1024 && (D == 64 || D == 128);
+}
+
+}  // namespace
+}  // namespace mlora
+
+using namespace mlora;
+
+extern "C" size_t mlora_prefix_plan_bytes(int32_t max_rows) {
+  return max_rows < 0 || max_rows > kPlanMaxRows ? 0 : 4u * (size_t)(kPlanHeader + 8 * (max_rows / kPlanMinRows + 1) + 4 * max_rows);
+}
+
+extern "C" int mlora_prefix_plan(const int32_t* d_row_slot, int32_t T, const int32_t* d_prefix_id, const int32_t* d_prefix_len, int32_t n_slots,
+                                 int32_t Hq, int32_t Hkv, int32_t* d_plan, int32_t max_rows, void* stream) {
+  MLORA_REQUIRE(shared_sizes_fit(T, Hq, Hkv, 64) && T <= max_rows && max_rows <= kPlanMaxRows && n_slots > 0,
+                "prefix_plan: bad sizes T=%d of %d, %d heads over %d key heads", T, max_rows, Hq, Hkv);
+  MLORA_REQUIRE(d_row_slot && d_prefix_id && d_prefix_len && d_plan && aligned16(d_plan), "prefix_plan: null pointer or unaligned plan");
+  if (T == 0) return MLORA_OK;
+  const int rep = Hq / Hkv, target = 2 * sm_count();
+  const int threads = (T + 31) / 32 * 32;
+  launch_pdl(prefix_plan_kernel, 1, threads, 0, (cudaStream_t)stream, d_row_slot, T, d_prefix_id, d_prefix_len, n_slots, tile_rows(rep), Hkv,
+             target, (int)max_parts(T, rep, Hkv, target), d_plan, max_rows);
+  count_launch();
+  MLORA_CHECK_LAUNCH("prefix_plan_kernel");
+  return MLORA_OK;
+}
+
+extern "C" size_t mlora_paged_attention_shared_workspace(int32_t T, int32_t Hq, int32_t Hkv, int32_t D) {
+  if (!shared_sizes_fit(T, Hq, Hkv, D)) return 0;
+  const SharedSizes s = sizes_of(T, Hq, Hkv, D);
+  return 4 * (size_t)(s.tickets + s.own + s.parts);
+}
+
+extern "C" int mlora_paged_attention_shared(const void* d_q, int64_t ld, const void* d_k_pages, const void* d_v_pages, int32_t n_pages_total,
+                                            const int32_t* d_block_table, int32_t max_pages, const int32_t* d_row_slot,
+                                            const int32_t* d_row_pos, int32_t T, int32_t Hq, int32_t Hkv, int32_t D, int32_t page_size,
+                                            float scale, const int32_t* d_plan, int32_t plan_rows, void* d_out, int64_t ld_out, void* d_work,
+                                            size_t work_bytes, int32_t* d_status, void* stream) {
+  MLORA_REQUIRE((D == 64 || D == 128) && (page_size == 16 || page_size == 32),
+                "paged_attention_shared: head_dim 64 or 128 and pages of 16 or 32 only (got %d, %d)", D, page_size);
+  MLORA_REQUIRE(shared_sizes_fit(T, Hq, Hkv, D) && T <= plan_rows && plan_rows <= kPlanMaxRows && n_pages_total > 0 && max_pages > 0 &&
+                    max_pages <= 2147483647 / page_size && scale > 0.f && ld >= (int64_t)Hq * D && ld_out >= (int64_t)Hq * D,
+                "paged_attention_shared: bad sizes T=%d Hq=%d Hkv=%d", T, Hq, Hkv);
+  MLORA_REQUIRE(d_q && d_k_pages && d_v_pages && d_block_table && d_row_slot && d_row_pos && d_plan && d_out, "paged_attention_shared: null pointer");
+  MLORA_REQUIRE(aligned16(d_q) && aligned16(d_k_pages) && aligned16(d_v_pages) && aligned16(d_out) && aligned16(d_plan) && aligned16(d_work) &&
+                    ld % 8 == 0 && ld_out % 8 == 0,
+                "paged_attention_shared: 16-byte alignment of tensors and row pitches");
+  if (T == 0) return MLORA_OK;
+  const SharedSizes s = sizes_of(T, Hq, Hkv, D);
+  if (!d_work || work_bytes < 4 * (size_t)(s.tickets + s.own + s.parts))
+    return fail(MLORA_ESIZE, "paged_attention_shared: scratch of %zu bytes needed, %zu given", 4 * (size_t)(s.tickets + s.own + s.parts), work_bytes);
+  float* w = (float*)d_work;
+  SharedArgs a{(const bf16*)d_q, ld, (const bf16*)d_k_pages, (const bf16*)d_v_pages, d_block_table, max_pages, d_row_slot, d_row_pos, T, Hq, Hkv,
+               page_size, const_cast<int32_t*>(d_plan), plan_rows, w + s.tickets + s.own, w + s.tickets, (int32_t*)w, s.n_splits, (bf16*)d_out, ld_out,
+               scale * kLog2e, d_status};
+  cudaStream_t st = (cudaStream_t)stream;
+  if (D == 64) return page_size == 16 ? launch_shared<1, 16>(a, n_pages_total, s.max_items, st) : launch_shared<1, 32>(a, n_pages_total, s.max_items, st);
+  return page_size == 16 ? launch_shared<2, 16>(a, n_pages_total, s.max_items, st) : launch_shared<2, 32>(a, n_pages_total, s.max_items, st);
+}

@@ -80,6 +80,7 @@ bool pdl_enabled_gemm();
 bool pdl_enabled_shrink();
 bool pdl_enabled_attn();
 bool pdl_enabled_norm();
+bool pdl_enabled_tail();
 
 // Programmatic dependent launch.  Every kernel of the decode step is launched with the
 // "programmatic stream serialization" attribute and begins with pdl_launch_dependents(), so the next

@@ -23,14 +23,15 @@ int fail(int code, const char* fmt, ...) {
 // Programmatic dependent launch policy.  Which kernels are launched programmatically dependent (may become
 // resident, and run whatever does not depend on earlier kernels, while the kernel before them still runs) is a
 // bit mask: bit 0 projection (its weight producer streams ahead), 1 LoRA shrink, 2 attention, 3 RMSNorm, 4 the
-// rest.  Measured on the benchmark's decode step (ms per step): none (0) 5.9, projection only (1) 4.98-5.60,
-// projection + RMSNorm (9) 5.00-5.53 -- the default --, + shrink (11) 5.01-5.57, + attention (13, 15, 31) 5.25-5.8
-// (its early-resident CTAs take registers and issue slots from the kernel before them).
-// The one documented switch: MLORA_PDL_MASK=<mask>.
+// rest, 5 the second launch of an operator that has two (it starts with what does not depend on the first).
+// Measured on the benchmark's decode step (ms per step), which has no kernel of bit 5: none (0) 5.9, projection
+// only (1) 4.98-5.60, projection + RMSNorm (9) 5.00-5.53 -- with bit 5 the default --, + shrink (11) 5.01-5.57,
+// + attention (13, 15, 31) 5.25-5.8 (its early-resident CTAs take registers and issue slots from the kernel
+// before them).  The one documented switch: MLORA_PDL_MASK=<mask>.
 static int pdl_mask() {
   static const int mask = [] {
     const char* e = getenv("MLORA_PDL_MASK");
-    return e ? atoi(e) : 9;
+    return e ? atoi(e) : 41;
   }();
   return mask;
 }
@@ -39,6 +40,7 @@ bool pdl_enabled_gemm() { return (pdl_mask() & 1) != 0; }
 bool pdl_enabled_shrink() { return (pdl_mask() & 2) != 0; }
 bool pdl_enabled_attn() { return (pdl_mask() & 4) != 0; }
 bool pdl_enabled_norm() { return (pdl_mask() & 8) != 0; }
+bool pdl_enabled_tail() { return (pdl_mask() & 32) != 0; }
 
 void count_launch(int n) { g_launches.fetch_add((uint64_t)n, std::memory_order_relaxed); }
 

@@ -864,3 +864,232 @@ def delta_step(x, r: DeltaRule, eps, row_slot, row_pos, state, ring, out, status
         eps, r.heads, r.kv_heads, r.dim, r.vdim, r.vdim_true, r.q_scale, _ptr(row_slot), _ptr(row_pos), x.shape[0], _ptr(state),
         _ptr(ring), _ptr(out), _ptr(status), int(x.dtype == torch.float32), _stream()), "mlora_delta_step")
     return out
+
+
+# ---------------------------------------------------------------- attention of a batch that shares prefixes
+def _one_device(*ts):
+    """Checks that the tensors lie on one CUDA device; None, or a context that makes it the current one."""
+    _need_cuda(*ts)
+    devs = {t.get_device() for t in ts if t is not None}
+    if len(devs) > 1:
+        raise ValueError("mlora: tensors of one call lie on one device")
+    dev = devs.pop()
+    return None if dev == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _int32_table(what, t, *shape):
+    """A contiguous int32 tensor of this shape (None: any size)."""
+    if t.dtype != torch.int32 or not t.is_contiguous() or t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+        raise ValueError(f"mlora: {what} must be contiguous int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+
+
+PREFIX_PLAN_MAX_ROWS = 1024
+
+
+class PrefixPlan:
+    """Which rows of a step share a prefix, for the attention of its layers (allocated once, filled by :func:`prefix_plan`)."""
+
+    def __init__(self, max_rows, Hq, Hkv, device):
+        if not 0 < max_rows <= PREFIX_PLAN_MAX_ROWS:
+            raise ValueError(f"mlora: a prefix plan holds 1 to {PREFIX_PLAN_MAX_ROWS} rows")
+        self.max_rows, self.Hq, self.Hkv, self.T = int(max_rows), int(Hq), int(Hkv), 0
+        self.table = torch.zeros(_lib.lib().mlora_prefix_plan_bytes(self.max_rows) // 4, dtype=torch.int32, device=device)
+
+
+def prefix_plan(row_slot, prefix_id, prefix_len, plan: PrefixPlan):
+    """Groups the rows by the prefix their slots begin with; see ``mlora_prefix_plan``."""
+    at = _one_device(row_slot, prefix_id, prefix_len, plan.table)
+    if at is not None:
+        with at:
+            return prefix_plan(row_slot, prefix_id, prefix_len, plan)
+    T, n = row_slot.numel(), prefix_id.numel()
+    _int32_table("row_slot", row_slot, T)
+    _int32_table("prefix_id", prefix_id, n)
+    _int32_table("prefix_len", prefix_len, n)
+    check(_lib.lib().mlora_prefix_plan(_ptr(row_slot), T, _ptr(prefix_id), _ptr(prefix_len), n, plan.Hq, plan.Hkv, _ptr(plan.table),
+                                       plan.max_rows, _stream()), "mlora_prefix_plan")
+    plan.T = T
+    return plan
+
+
+def paged_attention_shared_workspace(T, Hq, Hkv, D) -> int:
+    return int(_lib.lib().mlora_paged_attention_shared_workspace(T, Hq, Hkv, D))
+
+
+def paged_attention_shared(q, k_pages, v_pages, block_table, row_slot, row_pos, plan: PrefixPlan, Hq, out=None, work=None, status=None):
+    """One query row per (row, head) over the row's tokens 0..pos, prefixes of the plan read once; ``q`` [T, >= Hq D] as
+    :func:`kv_append_rope` leaves it.  ``work``: zero-initialised scratch of the caller (default: the per-stream fallback)."""
+    at = _one_device(q, k_pages, v_pages, block_table, row_slot, row_pos, plan.table, out, work, status)
+    if at is not None:
+        with at:
+            return paged_attention_shared(q, k_pages, v_pages, block_table, row_slot, row_pos, plan, Hq, out, work, status)
+    T, (n_pages, Hkv, ps, D) = q.shape[0], k_pages.shape
+    if out is None:
+        out = torch.empty(T, Hq * D, dtype=torch.bfloat16, device=q.device)
+    if (plan.T, plan.Hq, plan.Hkv) != (T, Hq, Hkv):
+        raise ValueError(f"mlora: the plan is for {plan.T} rows of {plan.Hq} heads over {plan.Hkv}, the call for {T} of {Hq} over {Hkv}")
+    if any(t.dtype != torch.bfloat16 for t in (q, k_pages, v_pages, out)) or v_pages.shape != k_pages.shape:
+        raise ValueError("mlora: shared attention takes bf16 queries, pages of one shape, and a bf16 result")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()) or q.stride(1) != 1 or out.stride(1) != 1 or q.shape[1] < Hq * D \
+            or tuple(out.shape) != (T, Hq * D):
+        raise ValueError("mlora: shared attention needs contiguous pages and rows of Hq * D columns")
+    _int32_table("block_table", block_table, None, None)
+    _int32_table("row_slot", row_slot, T)
+    _int32_table("row_pos", row_pos, T)
+    need = paged_attention_shared_workspace(T, Hq, Hkv, D)
+    if work is None:
+        work = workspace(need, q.device, "attn_shared")
+    check(_lib.lib().mlora_paged_attention_shared(
+        _ptr(q), q.stride(0), _ptr(k_pages), _ptr(v_pages), n_pages, _ptr(block_table), block_table.shape[1], _ptr(row_slot), _ptr(row_pos),
+        T, Hq, Hkv, D, ps, D ** -0.5, _ptr(plan.table), plan.max_rows, _ptr(out), out.stride(0), _ptr(work), work.numel(), _ptr(status),
+        _stream()), "mlora_paged_attention_shared")
+    return out
+
+
+# ---------------------------------------------------------------- the next tokens under rules
+@dataclass
+class LogitRules:
+    """Rules of ``n`` requests for :func:`choose_tokens`, on the device; what is None is no rule.
+
+    ``repetition`` (factor), ``frequency``, ``presence`` (fp32 [n]) look at the first ``prompt_len`` tokens of ``prompt`` and the first
+    ``answer_len`` of ``answer`` (int32 [n, any] and [n]).  ``bias_set`` (int32 [n], -1: none) names a set of biases: the entries
+    ``bias_start[set] .. bias_start[set + 1]`` of ``bias_token`` (ascending) and ``bias_value``.  ``mask_of`` (int32 [n], -1: all tokens)
+    names a row of ``masks`` (int32 [any, ceil(V / 32)]): bit v % 32 of word v / 32 allows token v.  :meth:`build` makes the
+    tables from Python values."""
+    repetition: torch.Tensor = None
+    frequency: torch.Tensor = None
+    presence: torch.Tensor = None
+    prompt: torch.Tensor = None
+    prompt_len: torch.Tensor = None
+    answer: torch.Tensor = None
+    answer_len: torch.Tensor = None
+    bias_set: torch.Tensor = None
+    bias_start: torch.Tensor = None
+    bias_token: torch.Tensor = None
+    bias_value: torch.Tensor = None
+    mask_of: torch.Tensor = None
+    masks: torch.Tensor = None
+
+    @classmethod
+    def build(cls, vocab, n, device, repetition=None, frequency=None, presence=None, prompts=None, biases=None, allowed=None):
+        """``repetition`` / ``frequency`` / ``presence``: a number, or one per request; ``prompts``: token lists; ``biases``: per request
+        None or {token: bias}; ``allowed``: per request None or the allowed tokens (a list, or a truth value per token).  Requests that
+        name the same object share a set."""
+        def per_request(v, name):
+            if v is None:
+                return None
+            v = torch.as_tensor(v, dtype=torch.float32)
+            if v.dim() and tuple(v.shape) != (n,):
+                raise ValueError(f"mlora: {name}: one number, or one per request")
+            return v.expand(n).contiguous().to(device)
+
+        def shared(values, name):  # (index of every request's set, the distinct sets)
+            if len(values) != n:
+                raise ValueError(f"mlora: {name}: one per request")
+            of, sets = {}, []
+            for v in values:
+                if v is not None and id(v) not in of:
+                    of[id(v)] = len(sets)
+                    sets.append(v)
+            return torch.tensor([-1 if v is None else of[id(v)] for v in values], dtype=torch.int32, device=device), sets
+
+        r = cls(*(per_request(v, name) for v, name in ((repetition, "repetition"), (frequency, "frequency"), (presence, "presence"))))
+        if prompts is not None:
+            if len(prompts) != n:
+                raise ValueError("mlora: prompts: one per request")
+            text = torch.zeros(n, max([len(p) for p in prompts] + [1]), dtype=torch.int32)
+            for i, p in enumerate(prompts):
+                text[i, :len(p)] = torch.as_tensor(list(p), dtype=torch.int32)
+            r.prompt, r.prompt_len = text.to(device), torch.tensor([len(p) for p in prompts], dtype=torch.int32, device=device)
+        if biases is not None:
+            r.bias_set, sets = shared(biases, "biases")
+            sets = [sorted((int(t), float(b)) for t, b in s.items()) for s in sets]
+            if any(not 0 <= t < vocab for s in sets for t, _ in s):
+                raise ValueError("mlora: biases name tokens of the vocabulary")
+            flat = [e for s in sets for e in s]
+            r.bias_start = torch.tensor(np.cumsum([0] + [len(s) for s in sets]), dtype=torch.int32, device=device)
+            r.bias_token = torch.tensor([t for t, _ in flat], dtype=torch.int32, device=device)
+            r.bias_value = torch.tensor([b for _, b in flat], dtype=torch.float32, device=device)
+        if allowed is not None:
+            r.mask_of, sets = shared(allowed, "allowed")
+            words = -(-vocab // 32)
+            bits = torch.zeros(len(sets), words * 32, dtype=torch.bool)
+            for i, s in enumerate(sets):
+                s = torch.as_tensor(s)
+                if s.dtype == torch.bool:
+                    if tuple(s.shape) != (vocab,):
+                        raise ValueError("mlora: allowed: a truth value per token of the vocabulary")
+                    bits[i, :vocab] = s
+                else:
+                    s = s.long()
+                    if s.numel() and not (0 <= int(s.min()) and int(s.max()) < vocab):
+                        raise ValueError("mlora: allowed names tokens of the vocabulary")
+                    bits[i, s] = True
+            v = (bits.view(len(sets), words, 32).long() << torch.arange(32)).sum(-1)
+            r.masks = torch.where(v >= 1 << 31, v - (1 << 32), v).int().to(device)
+        return r
+
+    @property
+    def n(self):
+        """Requests that have rules (0: none has any)."""
+        return next((t.shape[0] for t in (self.repetition, self.frequency, self.presence, self.bias_set, self.mask_of) if t is not None), 0)
+
+    def _check(self, V):
+        n = self.n
+        for name in ("repetition", "frequency", "presence"):
+            t = getattr(self, name)
+            if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (n,) or not t.is_contiguous()):
+                raise ValueError(f"mlora: {name} must be contiguous fp32 [{n}]")
+        for name in ("prompt", "answer"):
+            t, m = getattr(self, name), getattr(self, name + "_len")
+            if t is not None:
+                if m is None or t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != n or t.stride(1) != 1 or t.shape[1] == 0:
+                    raise ValueError(f"mlora: {name} must be int32 [{n}, any] with {name}_len")
+                _int32_table(name + "_len", m, n)
+        if self.bias_set is not None:
+            _int32_table("bias_set", self.bias_set, n)
+            if any(t is None for t in (self.bias_start, self.bias_token, self.bias_value)) or self.bias_value.dtype != torch.float32 \
+                    or not self.bias_value.is_contiguous() or self.bias_value.shape != self.bias_token.shape:
+                raise ValueError("mlora: bias sets are bias_start, bias_token and bias_value")
+            _int32_table("bias_start", self.bias_start, None)
+            _int32_table("bias_token", self.bias_token, None)
+        if self.mask_of is not None:
+            _int32_table("mask_of", self.mask_of, n)
+            if self.masks is None or self.masks.dim() != 2 or self.masks.shape[1] < -(-V // 32):
+                raise ValueError(f"mlora: masks must be int32 [any, {-(-V // 32)}]")
+            _int32_table("masks", self.masks, None, None)
+        return n
+
+
+def choose_tokens(logits, rules: LogitRules, row_src=None, out=None, logits_out=None):
+    """The greedy tokens of the logits under ``rules`` (-1: none is allowed); ``row_src`` int32 [T]: the request of every row (default:
+    its own number; outside the rules: none).  ``logits_out``: where the logits after the rules go (may be ``logits``)."""
+    r = rules
+    at = _one_device(logits, row_src, out, logits_out, *vars(r).values())
+    if at is not None:
+        with at:
+            return choose_tokens(logits, rules, row_src, out, logits_out)
+    T, V = logits.shape
+    n = r._check(V)
+    if out is None:
+        out = torch.empty(T, dtype=torch.int32, device=logits.device)
+    for t in (logits,) if logits_out is None else (logits, logits_out):
+        if t.dtype != torch.float32 or t.stride(1) != 1 or tuple(t.shape) != (T, V):
+            raise ValueError("mlora: choose_tokens takes fp32 logits [T, V]")
+    if row_src is not None:
+        _int32_table("row_src", row_src, T)
+    elif n and T > n:
+        raise ValueError(f"mlora: {T} rows, rules of {n} requests: row_src says which")
+    _int32_table("out", out, T)
+    sets = 0 if r.bias_set is None else r.bias_start.numel() - 1
+    masks = 0 if r.mask_of is None else r.masks.shape[0]
+    bias = r.bias_set is not None and sets > 0 and r.bias_token.numel() > 0
+    check(_lib.lib().mlora_choose_tokens(
+        _ptr(logits), logits.stride(0), T, V, _ptr(row_src), n, _ptr(r.repetition), _ptr(r.frequency), _ptr(r.presence),
+        _ptr(r.prompt), _ptr(r.prompt_len), r.prompt.stride(0) if r.prompt is not None else 0,
+        _ptr(r.answer), _ptr(r.answer_len), r.answer.stride(0) if r.answer is not None else 0,
+        _ptr(r.bias_set) if bias else None, _ptr(r.bias_start), _ptr(r.bias_token), _ptr(r.bias_value), sets,
+        r.bias_token.numel() if bias else 0, _ptr(r.mask_of) if masks else None, _ptr(r.masks), masks,
+        r.masks.stride(0) if masks else 0, _ptr(logits_out), logits_out.stride(0) if logits_out is not None else 0, _ptr(out), _stream()),
+        "mlora_choose_tokens")
+    return out
