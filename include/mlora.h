@@ -641,6 +641,30 @@ int mlora_delta_step(const void* d_x, int64_t ld, int32_t C, int32_t taps, int32
                      const int32_t* d_row_slot, const int32_t* d_row_pos, int32_t T, float* d_state, void* d_ring, void* d_out,
                      int32_t* d_status, int32_t f32, void* stream);
 
+/* ---- projections with 4-bit weights --------------------------------------------------------------------------------------
+ * W[o, k] = (q[o, k] - z[o, k / group]) * s[o, k / group], q and z in 0..15 (z = 8 where there are no zero points), s bf16, group 32,
+ * 64 or 128, in a multiple of it, any out.
+ * mlora_q4_quantize: q [out, in] (a byte each), s [out, in / group] and (d_zero not NULL) z of a bf16 matrix, every weight to its
+ *   nearest value: with zero points the 16 values span a group's range including 0, without them -7 .. 7 spans its largest magnitude.
+ * mlora_q4_pack: the layout that mlora_q4_linear reads (mlora_q4_bytes(out, in, group, d_zero != NULL) bytes, 16-byte aligned).
+ * mlora_q4_linear: mlora_linear with such weights: y = x W^T + scale[slot] * B_all[slot] u, MLORA_OUT_F32, MLORA_SILU_MUL (W's rows
+ *   interleaved as there), MLORA_ACT_*, MLORA_B_PACKED; MLORA_Q4_ZEROS says that the weights have zero points.  The other flags of
+ *   mlora_linear change nothing, but MLORA_B_SPLIT is refused.  The integers q - z are multiplied exactly, a group's sum and everything after it
+ *   are fp32; only the result is rounded.  Up to 16 rows need no scratch; more run on another kernel (other order of sums) and take
+ *   d_work of mlora_q4_linear_workspace bytes, zero-filled once before its first use; its status word and the caller's bytes are
+ *   those of mlora_linear's scratch (bit 1: a bounded wait expired, the output is undefined and the buffer must be zero-filled
+ *   again), and like that one it serves calls of any shape on one stream. */
+#define MLORA_Q4_ZEROS 4096
+size_t mlora_q4_bytes(int32_t out, int32_t in, int32_t group, int32_t zeros);
+int mlora_q4_quantize(const void* d_W, int32_t out, int32_t in, int32_t group, void* d_q, void* d_scale, void* d_zero, void* stream);
+int mlora_q4_pack(const void* d_q, const void* d_scale, const void* d_zero, int32_t out, int32_t in, int32_t group, void* d_Wq,
+                  void* stream);
+size_t mlora_q4_linear_workspace(int32_t T, int32_t in, int32_t out);
+int mlora_q4_linear(const void* d_x, int64_t ldx, const void* d_Wq, int32_t group, void* d_y, int64_t ldy, int32_t T, int32_t in,
+                    int32_t out, const float* d_u, const void* d_B_all, const float* d_scales, const int32_t* d_slots,
+                    int32_t n_adapters, int32_t r_max, int32_t n_mod, const int32_t* h_mod_offsets, int32_t flags, void* d_work,
+                    size_t work_bytes, void* stream);
+
 /* ---- decode attention of a batch that shares prefixes -----------------------------------------------------------------
  * Rows of a step whose sequences begin with the same pages (a system prompt, a document) read those pages once for all of them.
  * A prefix has an id; d_prefix_id [n_slots] names the one a cache slot's sequence begins with (< 0: none), d_prefix_len [n_slots]

@@ -1,0 +1,438 @@
+// Projections with 4-bit weights on the 5th-generation tensor cores, for more than 16 rows (see q4.cuh for the layout).
+//
+// Tiles of 128 outputs x BN rows of x.  Eight warps copy packed weights with rings of their own, turn them into bf16 integers q - z and
+// write them to TMEM (tcgen05.st.16x128b has the lanes where the packed order has them): weights go DRAM -> shared memory -> registers ->
+// TMEM and are never written to shared memory as bf16, whose 32 KB per 8 KB of weights would be more than its bandwidth.  The MMA takes
+// them from there as its A operand and the rows of x (TMA, 128-byte swizzle) as B.  A group's sums have an accumulator of their own, which
+// four warps scale in fp32 registers while the next one is filled: nothing but the output is rounded.
+//
+// Persistent, one CTA per SM; the units of 128 inputs of all tiles are dealt out in equal ranges.  A tile that several CTAs share is summed
+// by the last of them to arrive, in the order of the inputs, from the partial sums that each has left in scratch: no CTA waits for another.
+#include "q4.cuh"
+#include "tc_ptx.cuh"
+
+#include <atomic>
+
+namespace mlora {
+namespace {
+
+constexpr int kThreads = 512;            // warpgroups: 0 and 1 weights, 2 sums and outputs, 3 MMA issue and copies of x
+constexpr int kAbufs = 8, kXslots = 4;   // blocks of weights in TMEM, of x in shared memory
+constexpr int kWslots = 8;               // blocks in a weight warp's ring
+constexpr int kMaxCtas = 512;
+constexpr int kHeader = 256;             // bytes: status word, then the caller's
+constexpr int kWarpBlock = 1024 + 256;   // bytes of 32 outputs of a block, with their scales where there are zero points
+
+struct TcArgs {
+  Q4Args p;
+  int32_t* status;
+  int32_t* counters;  // [CTA that the tile begins in], zero between calls
+  float* parts;       // [CTA][2][BN][128]: sums of the tile it ends and of the tile it begins
+  int row_tiles, token_tiles, units;  // units of 128 inputs per tile
+};
+
+template <int N>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// 16 lanes x 32 columns from registers laid out as A operands of mma.m16n8k16
+__device__ __forceinline__ void tmem_st_16x128b_x8(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+               "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+
+// The blocks of 64 inputs of a CTA's range, one after the other.
+struct Cursor {
+  long long unit, end;
+  int tile, u, sub, units, n_kb;
+  __device__ Cursor(long long a, long long b, int units_, int n_kb_) : unit(a), end(b), sub(0), units(units_), n_kb(n_kb_) {
+    tile = (int)(a / units_);
+    u = (int)(a % units_);
+  }
+  __device__ bool valid() const { return unit < end; }
+  __device__ int kb() const { return 2 * u + sub; }
+  __device__ void next() {
+    if (sub == 0 && 2 * u + 1 < n_kb) {
+      sub = 1;
+      return;
+    }
+    sub = 0;
+    ++unit;
+    if (++u == units) u = 0, ++tile;
+  }
+};
+
+template <int BN, bool ZERO, int G>
+__global__ void __launch_bounds__(kThreads, 1) q4_tc_kernel(const __grid_constant__ CUtensorMap map_x, TcArgs t) {
+  constexpr int kDbufs = 2;
+  constexpr int kSums = G == 32 ? 2 : 1;                  // accumulators per block (G 128: one for two blocks)
+  constexpr int kEntry = ZERO ? 4 : 2;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sx = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* sw = sx + kXslots * BN * 128;                  // [weight warp][slot][kWarpBlock]
+  __shared__ uint64_t x_full[kXslots], x_empty[kXslots], a_full[kAbufs], a_empty[kAbufs], d_full[kDbufs], d_empty[kDbufs];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int s_abort, s_last;
+
+  pdl_launch_dependents();
+  const LinearArgs& a = t.p.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    s_abort = 0;
+    for (int i = 0; i < kXslots; ++i) mbar_init(&x_full[i], 1), mbar_init(&x_empty[i], 1);
+    for (int i = 0; i < kAbufs; ++i) mbar_init(&a_full[i], 4), mbar_init(&a_empty[i], 1);
+    for (int i = 0; i < kDbufs; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], 4);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    tma_prefetch_desc(&map_x);
+  }
+  if (warp == 12) tmem_alloc(&tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_a = tmem_slot + kDbufs * BN, tmem_d = tmem_slot;
+  const long long all = (long long)t.row_tiles * t.token_tiles * t.units;
+  const long long u_begin = all * blockIdx.x / gridDim.x, u_end = all * (blockIdx.x + 1) / gridDim.x;
+  const int n_kb = t.p.n_kb;
+  volatile int* abort = &s_abort;
+
+  if (warp < 8) {
+    // ---- weights -> TMEM: a warpgroup takes every other block, a warp its 32 outputs of it -------------------------------------
+    regs_down<96>();
+    const int wg = warp >> 2, quarter = warp & 3;
+    const uint8_t* weights = reinterpret_cast<const uint8_t*>(a.W) + quarter * 1024 + lane * 16;
+    const uint32_t ring = smem_u32(sw) + warp * kWslots * kWarpBlock;
+    const uint8_t* ring_p = sw + warp * kWslots * kWarpBlock;
+    Cursor ahead(u_begin, u_end, t.units, n_kb), now(u_begin, u_end, t.units, n_kb);
+    if (wg == 1) {
+      if (ahead.valid()) ahead.next();
+      if (now.valid()) now.next();
+    }
+    auto fetch = [&](int slot) {
+      if (ahead.valid()) {
+        const int row_tile = ahead.tile % t.row_tiles, kb = ahead.kb();
+        const uint8_t* src = weights + ((size_t)row_tile * n_kb + kb) * kQ4TileBytes;
+        const uint32_t dst = ring + slot * kWarpBlock;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + lane * 16), "l"(src) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 512 + lane * 16), "l"(src + 512) : "memory");
+        if (ZERO && lane < 8 * kSums) {
+          const int g = min(kSums == 2 ? 2 * kb + (lane >> 3) : kb * kQ4Block / G, t.p.n_groups - 1);
+          const uint8_t* e = t.p.table + (((size_t)row_tile * t.p.n_groups + g) * kQ4Tile + quarter * 32) * 4 + (lane & 7) * 16;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 1024 + lane * 16), "l"(e) : "memory");
+        }
+        ahead.next();
+        if (ahead.valid()) ahead.next();
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // (weights and scales are never written by an earlier kernel of a step: the copies need not wait for it)
+    for (int i = 0; i < kWslots - 1; ++i) fetch(i);
+    for (int i = 0; now.valid(); ++i) {
+      fetch((i + kWslots - 1) % kWslots);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kWslots - 1) : "memory");
+      __syncwarp();
+      const uint8_t* sp = ring_p + (i % kWslots) * kWarpBlock;
+      const int seq = 2 * i + wg, buf = seq % kAbufs;
+      if (!__all_sync(0xffffffffu, mbar_wait(&a_empty[buf], ((seq / kAbufs) & 1) ^ 1, abort))) {
+        s_abort = 1;
+        break;
+      }
+      tc_fence_after();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 w4 = *reinterpret_cast<const uint4*>(sp + h * 512 + lane * 16);
+        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+        uint32_t r[16];
+        uint32_t z0 = kQ4Middle, z1 = kQ4Middle;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (ZERO && (j == 0 || (kSums == 2 && j == 2))) {
+            const uint32_t* e = reinterpret_cast<const uint32_t*>(sp + 1024) + (kSums == 2 ? j / 2 : 0) * 32 + h * 16 + (lane >> 2);
+            const uint32_t e0 = e[0], e1 = e[8];
+            z0 = __byte_perm(e0, e0, 0x3232), z1 = __byte_perm(e1, e1, 0x3232);
+          }
+          uint32_t q[4];
+          q4_expand(w[j], z0, z1, q);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) r[4 * j + e] = q[e];
+        }
+        tmem_st_16x128b_x8(tmem_a + buf * 32 + ((uint32_t)(quarter * 32 + h * 16) << 16), r);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&a_full[buf]);
+      now.next();
+      if (now.valid()) now.next();
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+  } else if (warp < 12) {
+    // ---- sums and outputs: one thread per output ---------------------------------------------------------------------------------
+    regs_up<232>();
+    const int row = tid - 256;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    float acc[BN];
+#pragma unroll
+    for (int i = 0; i < BN; ++i) acc[i] = 0.f;
+    pdl_wait();  // (scratch and outputs belong to earlier kernels until here)
+    Cursor c(u_begin, u_end, t.units, n_kb);
+    int n = 0;  // accumulators taken
+    bool ok = true;
+    while (c.valid() && ok) {
+      const long long tile_begin = (long long)c.tile * t.units, seg_begin = c.unit;
+      const int tile = c.tile, row_tile = tile % t.row_tiles, token0 = tile / t.row_tiles * BN;
+      const uint8_t* table = t.p.table + ((size_t)row_tile * t.p.n_groups * kQ4Tile + row) * kEntry;
+      auto scale_of = [&](int g) {
+        const uint8_t* e = table + (size_t)min(g, t.p.n_groups - 1) * (kQ4Tile * kEntry);
+        return __uint_as_float((ZERO ? __ldg(reinterpret_cast<const uint32_t*>(e)) : (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(e))) << 16);
+      };
+      const long long seg_end = min(u_end, tile_begin + t.units);
+      const int g0 = (int)((seg_begin - tile_begin) * (128 / G)), g_end = min((int)((seg_end - tile_begin) * (128 / G)), G == 32 ? 2 * n_kb : (n_kb * kQ4Block + G - 1) / G);
+      float s_next = scale_of(g0);
+      for (int g = g0; g < g_end; ++g, ++n) {
+        const float s = s_next;
+        s_next = scale_of(g + 1);
+        const int d = n % kDbufs;
+        ok = __all_sync(0xffffffffu, mbar_wait(&d_full[d], (n / kDbufs) & 1, abort));
+        if (!ok) break;
+        tc_fence_after();
+        float v[2][16];
+        tmem_ld16_issue(tmem_d + d * BN + lanes, v[0]);
+#pragma unroll
+        for (int b = 0; b < BN / 16; ++b) {
+          tmem_wait_ld16(v[b & 1]);
+          if (b + 1 < BN / 16) tmem_ld16_issue(tmem_d + d * BN + lanes + (b + 1) * 16, v[(b + 1) & 1]);
+          if (b + 1 == BN / 16) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&d_empty[d]);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[b * 16 + i] = fmaf(s, v[b & 1][i], acc[b * 16 + i]);
+        }
+      }
+      ok = bar_all(1, ok);
+      if (!ok) break;
+      // the segment is done: output, or a share of a tile that others have a part of
+      const bool whole = seg_begin == tile_begin && seg_end == tile_begin + t.units;
+      bool write = true;
+      if (!whole) {
+        // first and last CTA of the tile: the ones whose ranges hold its first and last unit
+        auto cta_of = [&](long long unit) {
+          int k = (int)(unit * gridDim.x / all);
+          while (all * (k + 1) / gridDim.x <= unit) ++k;
+          while (all * k / gridDim.x > unit) --k;
+          return k;
+        };
+        const int c0 = cta_of(tile_begin), c1 = cta_of(tile_begin + t.units - 1);
+        float* mine = t.parts + ((size_t)blockIdx.x * 2 + (seg_begin == tile_begin ? 1 : 0)) * (BN * kQ4Tile) + row;
+#pragma unroll
+        for (int i = 0; i < BN; ++i) __stcg(mine + i * kQ4Tile, acc[i]);
+        __threadfence();
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (row == 0) {
+          const int before = atomicAdd(&t.counters[c0], 1);
+          s_last = before == c1 - c0;
+          if (before == c1 - c0) t.counters[c0] = 0;
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        write = s_last != 0;
+        if (write) {
+          __threadfence();
+          const float* from = t.parts + ((size_t)c0 * 2 + 1) * (BN * kQ4Tile) + row;
+#pragma unroll
+          for (int i = 0; i < BN; ++i) acc[i] = __ldcg(from + i * kQ4Tile);
+          for (int k = c0 + 1; k <= c1; ++k) {
+            from = t.parts + (size_t)k * 2 * (BN * kQ4Tile) + row;
+#pragma unroll
+            for (int i = 0; i < BN; ++i) acc[i] += __ldcg(from + i * kQ4Tile);
+          }
+        }
+      }
+      if (write) {
+        const int o = row_tile * kQ4Tile + row, n_tok = min(BN, a.T - token0);
+        if (a.u != nullptr && o < a.out) {
+          const float* u = a.u + (size_t)token0 * (a.r_max * a.n_mod) + module_of(a, o) * a.r_max;
+          for (int j = 0; j < a.r_max / 8; ++j) {
+            int have = -1, sw;
+            uint4 b = make_uint4(0u, 0u, 0u, 0u);
+            float alpha = 0.f;
+#pragma unroll
+            for (int i = 0; i < BN; ++i) {
+              const int s = i < n_tok ? a.slots[token0 + i] : -1;
+              if (s >= 0 && s < a.n_adapters) {
+                if (s != have) {
+                  b = ld_cached(q4_b_row(a, t.p.packed_b, s, o, j, sw));
+                  alpha = a.scales[s];
+                  have = s;
+                }
+                acc[i] = fmaf(alpha, dot8(b, u + (size_t)i * (a.r_max * a.n_mod) + 8 * j), acc[i]);
+              }
+            }
+          }
+        }
+        const int act = a.flags & (MLORA_ACT_RELU2 | MLORA_ACT_GELU);
+        if (a.flags & MLORA_SILU_MUL) {
+#pragma unroll
+          for (int i = 0; i < BN; ++i) {
+            const float up = __shfl_xor_sync(0xffffffffu, acc[i], 8);  // (8 gate outputs, then their 8 up outputs)
+            if (!(lane & 8) && o < a.out && i < n_tok) store_out(a, token0 + i, o / 16 * 8 + (o & 7), silu_mul(acc[i], up));
+          }
+        } else if (o < a.out) {
+#pragma unroll
+          for (int i = 0; i < BN; ++i)
+            if (i < n_tok) store_out(a, token0 + i, o, act_one(acc[i], act));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < BN; ++i) acc[i] = 0.f;
+      c = Cursor(seg_end, u_end, t.units, n_kb);
+    }
+    if (!ok) s_abort = 1;
+  } else {
+    regs_down<48>();
+    if (warp == 12) {
+      // ---- MMA issue -------------------------------------------------------------------------------------------------------------
+      constexpr uint32_t idesc = make_idesc(kQ4Tile, BN);
+      int seq = 0, n = 0;
+      bool ok = true;
+      for (Cursor c(u_begin, u_end, t.units, n_kb); c.valid() && ok; ++seq) {
+        const int buf = seq % kAbufs, slot = seq % kXslots, kb = c.kb();
+        const bool last_of_unit = c.sub == 1 || 2 * c.u + 1 >= n_kb;
+        int good = 1;
+        if (lane == 0) {
+          good = mbar_wait(&a_full[buf], (seq / kAbufs) & 1, abort) && mbar_wait(&x_full[slot], (seq / kXslots) & 1, abort);
+          tc_fence_after();
+          const uint64_t bdesc = make_smem_desc(smem_u32(sx + slot * BN * 128));
+#pragma unroll
+          for (int s = 0; s < kSums; ++s) {
+            const bool opens = G == 128 ? (kb & 1) == 0 : true, closes = G == 128 ? last_of_unit : true;
+            const int d = n % kDbufs;
+            if (good && opens) {
+              good = mbar_wait(&d_empty[d], ((n / kDbufs) & 1) ^ 1, abort);
+              tc_fence_after();
+            }
+            if (good) {
+              constexpr int steps = 4 / kSums;
+#pragma unroll
+              for (int k = 0; k < steps; ++k)
+                umma_bf16_ta(tmem_d + d * BN, tmem_a + buf * 32 + (s * steps + k) * 8, bdesc + 2 * (s * steps + k), idesc, (!opens || k > 0) ? 1u : 0u);
+              if (closes) {
+                umma_commit(&d_full[d]);
+                ++n;
+              }
+            }
+          }
+          if (good) {
+            umma_commit(&a_empty[buf]);
+            umma_commit(&x_empty[slot]);
+          }
+        }
+        good = __shfl_sync(0xffffffffu, good, 0);
+        if (!good) {
+          s_abort = 1;
+          ok = false;
+        }
+        c.next();
+      }
+    } else if (warp == 13) {
+      // ---- rows of x -------------------------------------------------------------------------------------------------------------
+      pdl_wait();
+      int seq = 0;
+      for (Cursor c(u_begin, u_end, t.units, n_kb); c.valid(); ++seq) {
+        const int slot = seq % kXslots;
+        int good = 1;
+        if (lane == 0) {
+          good = mbar_wait(&x_empty[slot], ((seq / kXslots) & 1) ^ 1, abort);
+          if (good) {
+            mbar_expect_tx(&x_full[slot], BN * 128);
+            tma_load_2d(sx + slot * BN * 128, &map_x, c.kb() * kQ4Block, c.tile / t.row_tiles * BN, &x_full[slot]);
+          }
+        }
+        good = __shfl_sync(0xffffffffu, good, 0);
+        if (!good) {
+          s_abort = 1;
+          break;
+        }
+        c.next();
+      }
+      if (*abort && lane == 0)  // copies may still be in flight: let them land before the shared memory goes to another CTA
+        for (int i = 0; i < 64; ++i) __nanosleep(1000);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && s_abort) atomicOr(t.status, 2);
+  if (warp == 12) tmem_dealloc(tmem_slot, 512);
+}
+
+int q4_ctas(long long units) {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    n = 148;
+  }
+  n = n < kMaxCtas ? n : kMaxCtas;
+  return (int)(units < n ? units : n);
+}
+int rows_per_tile(int T) { return T <= 32 ? 32 : T <= 64 ? 64 : 128; }
+
+template <int BN, bool ZERO, int G>
+int launch_tc_as(const TcArgs& t, int grid, cudaStream_t st) {
+  CUtensorMap mx;
+  const int rc = make_map(&mx, t.p.a.x, t.p.a.T, t.p.a.in, t.p.a.ldx, BN, kQ4Block);
+  if (rc) return rc;
+  constexpr int smem = 1024 + kXslots * BN * 128 + 8 * kWslots * kWarpBlock;
+  static std::atomic<unsigned long long> done{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!((done.load(std::memory_order_acquire) >> (dev & 63)) & 1ull)) {
+    const cudaError_t e = cudaFuncSetAttribute(q4_tc_kernel<BN, ZERO, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return fail(MLORA_ECUDA, "q4_linear: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    done.fetch_or(1ull << (dev & 63), std::memory_order_release);
+  }
+  const cudaError_t e = launch_pdl_if(pdl_enabled_gemm(), q4_tc_kernel<BN, ZERO, G>, dim3((unsigned)grid), dim3(kThreads), smem, st, mx, t);
+  if (e != cudaSuccess) return fail(MLORA_ECUDA, "q4_tc_kernel: %s", cudaGetErrorString(e));
+  count_launch();
+  MLORA_CHECK_LAUNCH("q4_tc_kernel");
+  return MLORA_OK;
+}
+template <int BN>
+int launch_tc_for(const TcArgs& t, int grid, cudaStream_t st) {
+  const bool zero = (t.p.a.flags & MLORA_Q4_ZEROS) != 0;
+  switch (t.p.group) {
+    case 32: return zero ? launch_tc_as<BN, true, 32>(t, grid, st) : launch_tc_as<BN, false, 32>(t, grid, st);
+    case 64: return zero ? launch_tc_as<BN, true, 64>(t, grid, st) : launch_tc_as<BN, false, 64>(t, grid, st);
+    default: return zero ? launch_tc_as<BN, true, 128>(t, grid, st) : launch_tc_as<BN, false, 128>(t, grid, st);
+  }
+}
+
+}  // namespace
+
+size_t q4_tc_workspace(int T, int in, int out) {
+  // (the largest tile and every CTA, whatever the sizes: one buffer serves them all)
+  (void)in, (void)out;
+  return kHeader + kMaxCtas * 4 + (size_t)q4_ctas(kMaxCtas) * 2 * rows_per_tile(T) * kQ4Tile * 4;
+}
+
+int launch_q4_tc(const Q4Args& p, void* work, size_t work_bytes, cudaStream_t st) {
+  const size_t need = q4_tc_workspace(p.a.T, p.a.in, p.a.out);
+  if (!work || work_bytes < need) return fail(MLORA_ESIZE, "q4_linear: scratch of %zu bytes needed, %zu given", need, work_bytes);
+  if (!aligned16(work)) return fail(MLORA_EINVAL, "q4_linear: the scratch must be 16-byte aligned");
+  TcArgs t{};
+  t.p = p;
+  t.status = (int32_t*)work;
+  t.counters = (int32_t*)((uint8_t*)work + kHeader);
+  t.parts = (float*)((uint8_t*)work + kHeader + kMaxCtas * 4);
+  const int bn = rows_per_tile(p.a.T);
+  t.row_tiles = (p.a.out + kQ4Tile - 1) / kQ4Tile;
+  t.token_tiles = (p.a.T + bn - 1) / bn;
+  t.units = (p.n_kb + 1) / 2;
+  if ((long long)t.row_tiles * t.token_tiles > 2147483647ll) return fail(MLORA_ESIZE, "q4_linear: too many tiles");
+  const int grid = q4_ctas((long long)t.row_tiles * t.token_tiles * t.units);
+  return bn == 32 ? launch_tc_for<32>(t, grid, st) : bn == 64 ? launch_tc_for<64>(t, grid, st) : launch_tc_for<128>(t, grid, st);
+}
+
+}  // namespace mlora

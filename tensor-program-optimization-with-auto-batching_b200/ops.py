@@ -17,6 +17,7 @@ from ._lib import check
 OUT_F32, SILU_MUL, FORCE_SIMT, W_PACKED, B_PACKED, SHARE_LORA_KERNEL, LORA_PER_ROW, B_SPLIT = 1, 2, 4, 8, 16, 32, 64, 128
 STABLE_SUMS = 1024
 ANY_SUMS = 2048
+Q4_ZEROS = 4096
 
 
 def _ptr(t):  # (plain numbers: the prototypes convert them)
@@ -213,13 +214,116 @@ class PackedWeight:
         return True
 
 
+class QuantWeight:
+    """W [out, in] in 4 bits, W[o, k] = (q[o, k] - zero[o, k / group]) scale[o, k / group] with q and zero in 0..15, in the layout of
+    ``mlora_q4_pack`` (see include/mlora.h).  ``group`` 32, 64 or 128 divides ``in``; ``zeros``: zero points per group, else 8 is the middle."""
+
+    def __init__(self, W, group=128, zeros=False):
+        """Quantises a bf16 matrix, every weight to its nearest value."""
+        _need_cuda(W)
+        if W.dtype != torch.bfloat16 or W.dim() != 2 or not W.is_contiguous():
+            raise ValueError("QuantWeight needs a contiguous bf16 matrix")
+        N, K = W.shape
+        if group not in (32, 64, 128) or K % group:
+            raise ValueError(f"QuantWeight: groups of 32, 64 or 128 that divide the {K} inputs, got {group}")
+        with torch.cuda.device(W.device):
+            q = torch.empty(N, K, dtype=torch.uint8, device=W.device)
+            s = torch.empty(N, K // group, dtype=torch.bfloat16, device=W.device)
+            z = torch.empty(N, K // group, dtype=torch.uint8, device=W.device) if zeros else None
+            check(_lib.lib().mlora_q4_quantize(_ptr(W), N, K, group, _ptr(q), _ptr(s), _ptr(z), _stream()), "mlora_q4_quantize")
+            self._pack(q, s, z, group)
+
+    @classmethod
+    def from_integers(cls, q, scale, zero=None, group=128):
+        """Weights that are quantised already: q [out, in] uint8, scale [out, in / group] bf16, zero likewise uint8 or None."""
+        _need_cuda(q, scale, zero)
+        if q.dtype != torch.uint8 or q.dim() != 2 or scale.dtype != torch.bfloat16 or (zero is not None and zero.dtype != torch.uint8):
+            raise ValueError("QuantWeight: q and zero are uint8, scale is bf16")
+        N, K = q.shape
+        if group not in (32, 64, 128) or K % group or any(t is not None and tuple(t.shape) != (N, K // group) for t in (scale, zero)):
+            raise ValueError(f"QuantWeight: groups of 32, 64 or 128 that divide the {K} inputs, a scale (and zero point) each, got {group}")
+        if any(t is not None and t.numel() and int(t.max()) > 15 for t in (q, zero)):
+            raise ValueError("QuantWeight: q and zero lie in 0..15")
+        W = cls.__new__(cls)
+        with torch.cuda.device(q.device):
+            W._pack(q.contiguous(), scale.contiguous(), None if zero is None else zero.contiguous(), group)
+        return W
+
+    def _pack(self, q, s, z, group):
+        self.shape, self.group, self.zeros, self.dtype = tuple(q.shape), int(group), z is not None, torch.bfloat16
+        n = _lib.lib().mlora_q4_bytes(*self.shape, group, int(self.zeros))
+        if not n:
+            raise ValueError(f"QuantWeight: no matrix of {self.shape}")
+        self.data = torch.empty(n, dtype=torch.uint8, device=q.device)
+        check(_lib.lib().mlora_q4_pack(_ptr(q), _ptr(s), _ptr(z), *self.shape, group, _ptr(self.data), _stream()), "mlora_q4_pack")
+
+    def data_ptr(self):
+        return self.data.data_ptr()
+
+    def get_device(self):
+        return self.data.get_device()
+
+    def numel(self):
+        return self.shape[0] * self.shape[1]
+
+    @property
+    def is_cuda(self):
+        return True
+
+
+def q4_linear_workspace(T, K, N) -> int:
+    return int(_lib.lib().mlora_q4_linear_workspace(T, K, N))
+
+
+def _linear_q4(x, W: QuantWeight, stack, slots, u, flags, out, work):
+    at = _one_device(x, W, slots, u, out, work)
+    if at is not None:
+        with at:
+            return _linear_q4(x, W, stack, slots, u, flags, out, work)
+    T, K = x.shape
+    N = W.shape[0]
+    cols = N // 2 if flags & SILU_MUL else N
+    dtype = torch.float32 if flags & OUT_F32 else torch.bfloat16
+    if x.dtype != torch.bfloat16 or K != W.shape[1] or x.stride(1) != 1:
+        raise ValueError(f"mlora.linear: bf16 rows of {W.shape[1]} columns, got {x.dtype} {list(x.shape)}")
+    if out is None:
+        out = torch.empty(T, cols, dtype=dtype, device=x.device)
+    elif out.dtype != dtype or tuple(out.shape) != (T, cols) or out.stride(1) != 1:
+        raise ValueError(f"mlora.linear: a result of {dtype} [{T}, {cols}], got {out.dtype} {list(out.shape)}")
+    mod = None
+    if stack is not None:
+        if slots is None:
+            raise ValueError("mlora.linear: adapters need the rows' slots")
+        _int32_table("slots", slots, T)
+        if u is None:
+            u = lora_shrink(x, stack, slots)
+        if u.dtype != torch.float32 or not u.is_contiguous() or u.numel() != T * stack.r_max * stack.n_mod:
+            raise ValueError("mlora.linear: u must be contiguous fp32 [T, n_mod * r_max]")
+        if stack.n_mod > 1 and not flags & SILU_MUL:
+            mod = (C.c_int32 * (stack.n_mod + 1))(*stack.mod_offsets)
+    flags = (flags & ~B_SPLIT) | (Q4_ZEROS if W.zeros else 0) | (B_PACKED if stack is not None and stack.b_packed else 0)
+    need = q4_linear_workspace(T, K, N)
+    if work is None and need:
+        work = workspace(need, x.device, "linear")
+    if work is not None and work.numel() < need:
+        raise ValueError(f"mlora.linear: scratch of {need} bytes needed, {work.numel()} given")
+    lora = stack is not None
+    check(_lib.lib().mlora_q4_linear(
+        _ptr(x), x.stride(0), _ptr(W), W.group, _ptr(out), out.stride(0), T, K, N, _ptr(u) if lora else None, _ptr(stack.B_all) if lora else None,
+        _ptr(stack.scales) if lora else None, _ptr(slots) if lora else None, stack.A_all.shape[0] if lora else 0, stack.r_max if lora else 0,
+        stack.n_mod if lora else 1, mod, flags, _ptr(work), work.numel() if work is not None else 0, _stream()), "mlora_q4_linear")
+    return out
+
+
 def linear(x, W, stack: LoraStack = None, slots=None, u=None, flags: int = 0, out=None, use_workspace=True,
            with_shrink=False, work=None):
     """y = x W^T (+ LoRA expand of ``u``) ; see ``mlora_linear`` in include/mlora.h.
-    ``W`` is a bf16 [out,in] tensor or a :class:`PackedWeight`.  ``with_shrink``: ``u`` is scratch and
+    ``W`` is a bf16 [out,in] tensor, a :class:`PackedWeight` or a :class:`QuantWeight` (``mlora_q4_linear``).  ``with_shrink``: ``u`` is scratch and
     the shrink is part of the call (``mlora_lora_linear``).  ``work``: the caller's own zero-initialised
     scratch buffer (default: the per-stream fallback buffer)."""
     _need_cuda(x, W)
+    if isinstance(W, QuantWeight):
+        return _linear_q4(x, W, stack, slots, None if with_shrink else u, flags, out, work)
     if x.dtype != torch.bfloat16 or W.dtype != torch.bfloat16:
         raise ValueError("mlora.linear needs bf16 x and W")
     if isinstance(W, PackedWeight):
