@@ -16,8 +16,9 @@
 namespace mlora {
 namespace {
 
-constexpr int kThreads = 512;            // warpgroups: 0 and 1 weights, 2 sums and outputs, 3 MMA issue and copies of x
-constexpr int kAbufs = 8, kXslots = 4;   // blocks of weights in TMEM, of x in shared memory
+// Warps 0..7: weights; then four or eight (tiles of 128 rows of x: half of the columns each) for sums and outputs, MMA issue, copies of x.
+constexpr int q4_threads(int bn) { return 32 * (8 + (bn == 128 ? 8 : 4) + 2); }
+constexpr int kBufs = 8;                 // blocks of weights in TMEM, and of x in shared memory
 constexpr int kWslots = 8;               // blocks in a weight warp's ring
 constexpr int kMaxCtas = 512;
 constexpr int kHeader = 256;             // bytes: status word, then the caller's
@@ -31,11 +32,21 @@ struct TcArgs {
   int row_tiles, token_tiles, units;  // units of 128 inputs per tile
 };
 
+// One verdict of the N threads that sum; see bar_all.
 template <int N>
-__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-
+__device__ __forceinline__ bool out_all(bool ok) {
+  uint32_t r;
+  __syncwarp();
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.aligned.pred q, 1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)ok), "n"(N)
+      : "memory");
+  return r != 0;
+}
 // 16 lanes x 32 columns from registers laid out as A operands of mma.m16n8k16
 __device__ __forceinline__ void tmem_st_16x128b_x8(uint32_t addr, const uint32_t (&r)[16]) {
   asm volatile("tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(r[0]),
@@ -66,14 +77,16 @@ struct Cursor {
 };
 
 template <int BN, bool ZERO, int G>
-__global__ void __launch_bounds__(kThreads, 1) q4_tc_kernel(const __grid_constant__ CUtensorMap map_x, TcArgs t) {
+__global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_constant__ CUtensorMap map_x, TcArgs t) {
   constexpr int kDbufs = 2;
+  constexpr int kOutWarps = BN == 128 ? 8 : 4, kMma = 8 + kOutWarps;  // first of the two warps behind them
+  constexpr int kCols = BN * 4 / kOutWarps;               // columns of a thread that sums
   constexpr int kSums = G == 32 ? 2 : 1;                  // accumulators per block (G 128: one for two blocks)
   constexpr int kEntry = ZERO ? 4 : 2;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sx = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint8_t* sw = sx + kXslots * BN * 128;                  // [weight warp][slot][kWarpBlock]
-  __shared__ uint64_t x_full[kXslots], x_empty[kXslots], a_full[kAbufs], a_empty[kAbufs], d_full[kDbufs], d_empty[kDbufs];
+  uint8_t* sw = sx + kBufs * BN * 128;                  // [weight warp][slot][kWarpBlock]
+  __shared__ uint64_t x_full[kBufs], a_full[kBufs], empty[kBufs], d_full[kDbufs], d_empty[kDbufs];
   __shared__ uint32_t tmem_slot;
   __shared__ int s_abort, s_last;
 
@@ -82,13 +95,12 @@ __global__ void __launch_bounds__(kThreads, 1) q4_tc_kernel(const __grid_constan
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     s_abort = 0;
-    for (int i = 0; i < kXslots; ++i) mbar_init(&x_full[i], 1), mbar_init(&x_empty[i], 1);
-    for (int i = 0; i < kAbufs; ++i) mbar_init(&a_full[i], 4), mbar_init(&a_empty[i], 1);
-    for (int i = 0; i < kDbufs; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], 4);
+    for (int i = 0; i < kBufs; ++i) mbar_init(&x_full[i], 1), mbar_init(&a_full[i], 4), mbar_init(&empty[i], 1);
+    for (int i = 0; i < kDbufs; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], kOutWarps);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     tma_prefetch_desc(&map_x);
   }
-  if (warp == 12) tmem_alloc(&tmem_slot, 512);
+  if (warp == kMma) tmem_alloc(&tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -100,7 +112,6 @@ __global__ void __launch_bounds__(kThreads, 1) q4_tc_kernel(const __grid_constan
 
   if (warp < 8) {
     // ---- weights -> TMEM: a warpgroup takes every other block, a warp its 32 outputs of it -------------------------------------
-    regs_down<96>();
     const int wg = warp >> 2, quarter = warp & 3;
     const uint8_t* weights = reinterpret_cast<const uint8_t*>(a.W) + quarter * 1024 + lane * 16;
     const uint32_t ring = smem_u32(sw) + warp * kWslots * kWarpBlock;
@@ -129,21 +140,27 @@ __global__ void __launch_bounds__(kThreads, 1) q4_tc_kernel(const __grid_constan
     };
     // (weights and scales are never written by an earlier kernel of a step: the copies need not wait for it)
     for (int i = 0; i < kWslots - 1; ++i) fetch(i);
+    int told = -1;  // block whose stores are on their way to TMEM: told to the MMA warp while the next one is being expanded
+    const auto tell = [&] {
+      if (told < 0) return;
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&a_full[told]);
+      __syncwarp();
+    };
     for (int i = 0; now.valid(); ++i) {
       fetch((i + kWslots - 1) % kWslots);
       asm volatile("cp.async.wait_group %0;" ::"n"(kWslots - 1) : "memory");
       __syncwarp();
       const uint8_t* sp = ring_p + (i % kWslots) * kWarpBlock;
-      const int seq = 2 * i + wg, buf = seq % kAbufs;
-      if (!__all_sync(0xffffffffu, mbar_wait(&a_empty[buf], ((seq / kAbufs) & 1) ^ 1, abort))) {
-        s_abort = 1;
-        break;
-      }
-      tc_fence_after();
+      const int seq = 2 * i + wg, buf = seq % kBufs;
+      uint4 w4[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) w4[h] = *reinterpret_cast<const uint4*>(sp + h * 512 + lane * 16);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint4 w4 = *reinterpret_cast<const uint4*>(sp + h * 512 + lane * 16);
-        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+        const uint32_t w[4] = {w4[h].x, w4[h].y, w4[h].z, w4[h].w};
         uint32_t r[16];
         uint32_t z0 = kQ4Middle, z1 = kQ4Middle;
 #pragma unroll
@@ -158,31 +175,38 @@ __global__ void __launch_bounds__(kThreads, 1) q4_tc_kernel(const __grid_constan
 #pragma unroll
           for (int e = 0; e < 4; ++e) r[4 * j + e] = q[e];
         }
+        if (h == 0) {
+          tell();
+          if (!__all_sync(0xffffffffu, mbar_wait(&empty[buf], ((seq / kBufs) & 1) ^ 1, abort))) {
+            s_abort = 1;
+            told = -1;
+            break;
+          }
+          tc_fence_after();
+          told = buf;
+        }
         tmem_st_16x128b_x8(tmem_a + buf * 32 + ((uint32_t)(quarter * 32 + h * 16) << 16), r);
       }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&a_full[buf]);
+      if (told < 0) break;
       now.next();
       if (now.valid()) now.next();
     }
+    tell();
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-  } else if (warp < 12) {
+  } else if (warp < kMma) {
     // ---- sums and outputs: one thread per output ---------------------------------------------------------------------------------
-    regs_up<232>();
-    const int row = tid - 256;
+    const int row = tid & 127, col0 = (warp - 8) / 4 * kCols;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    float acc[BN];
+    float acc[kCols];
 #pragma unroll
-    for (int i = 0; i < BN; ++i) acc[i] = 0.f;
+    for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
     pdl_wait();  // (scratch and outputs belong to earlier kernels until here)
     Cursor c(u_begin, u_end, t.units, n_kb);
     int n = 0;  // accumulators taken
     bool ok = true;
     while (c.valid() && ok) {
       const long long tile_begin = (long long)c.tile * t.units, seg_begin = c.unit;
-      const int tile = c.tile, row_tile = tile % t.row_tiles, token0 = tile / t.row_tiles * BN;
+      const int tile = c.tile, row_tile = tile % t.row_tiles, token0 = tile / t.row_tiles * BN + col0;
       const uint8_t* table = t.p.table + ((size_t)row_tile * t.p.n_groups * kQ4Tile + row) * kEntry;
       auto scale_of = [&](int g) {
         const uint8_t* e = table + (size_t)min(g, t.p.n_groups - 1) * (kQ4Tile * kEntry);
@@ -199,21 +223,24 @@ __global__ void __launch_bounds__(kThreads, 1) q4_tc_kernel(const __grid_constan
         if (!ok) break;
         tc_fence_after();
         float v[2][16];
-        tmem_ld16_issue(tmem_d + d * BN + lanes, v[0]);
+        const uint32_t from = tmem_d + d * BN + col0 + lanes;
+        tmem_ld16_issue(from, v[0]);
 #pragma unroll
-        for (int b = 0; b < BN / 16; ++b) {
+        for (int b = 0; b < kCols / 16; ++b) {
           tmem_wait_ld16(v[b & 1]);
-          if (b + 1 < BN / 16) tmem_ld16_issue(tmem_d + d * BN + lanes + (b + 1) * 16, v[(b + 1) & 1]);
-          if (b + 1 == BN / 16) {
+          if (b + 1 < kCols / 16) {
+            tmem_ld16_issue(from + (b + 1) * 16, v[(b + 1) & 1]);
+          } else {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&d_empty[d]);
+            __syncwarp();
           }
 #pragma unroll
           for (int i = 0; i < 16; ++i) acc[b * 16 + i] = fmaf(s, v[b & 1][i], acc[b * 16 + i]);
         }
       }
-      ok = bar_all(1, ok);
+      ok = out_all<32 * kOutWarps>(ok);
       if (!ok) break;
       // the segment is done: output, or a share of a tile that others have a part of
       const bool whole = seg_begin == tile_begin && seg_end == tile_begin + t.units;
@@ -227,32 +254,32 @@ __global__ void __launch_bounds__(kThreads, 1) q4_tc_kernel(const __grid_constan
           return k;
         };
         const int c0 = cta_of(tile_begin), c1 = cta_of(tile_begin + t.units - 1);
-        float* mine = t.parts + ((size_t)blockIdx.x * 2 + (seg_begin == tile_begin ? 1 : 0)) * (BN * kQ4Tile) + row;
+        float* mine = t.parts + ((size_t)blockIdx.x * 2 + (seg_begin == tile_begin ? 1 : 0)) * (BN * kQ4Tile) + col0 * kQ4Tile + row;
 #pragma unroll
-        for (int i = 0; i < BN; ++i) __stcg(mine + i * kQ4Tile, acc[i]);
+        for (int i = 0; i < kCols; ++i) __stcg(mine + i * kQ4Tile, acc[i]);
         __threadfence();
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        if (row == 0) {
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kOutWarps) : "memory");
+        if (tid == 256) {
           const int before = atomicAdd(&t.counters[c0], 1);
           s_last = before == c1 - c0;
           if (before == c1 - c0) t.counters[c0] = 0;
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kOutWarps) : "memory");
         write = s_last != 0;
         if (write) {
           __threadfence();
-          const float* from = t.parts + ((size_t)c0 * 2 + 1) * (BN * kQ4Tile) + row;
+          const float* from = t.parts + ((size_t)c0 * 2 + 1) * (BN * kQ4Tile) + col0 * kQ4Tile + row;
 #pragma unroll
-          for (int i = 0; i < BN; ++i) acc[i] = __ldcg(from + i * kQ4Tile);
+          for (int i = 0; i < kCols; ++i) acc[i] = __ldcg(from + i * kQ4Tile);
           for (int k = c0 + 1; k <= c1; ++k) {
-            from = t.parts + (size_t)k * 2 * (BN * kQ4Tile) + row;
+            from = t.parts + (size_t)k * 2 * (BN * kQ4Tile) + col0 * kQ4Tile + row;
 #pragma unroll
-            for (int i = 0; i < BN; ++i) acc[i] += __ldcg(from + i * kQ4Tile);
+            for (int i = 0; i < kCols; ++i) acc[i] += __ldcg(from + i * kQ4Tile);
           }
         }
       }
       if (write) {
-        const int o = row_tile * kQ4Tile + row, n_tok = min(BN, a.T - token0);
+        const int o = row_tile * kQ4Tile + row, n_tok = min(kCols, a.T - token0);
         if (a.u != nullptr && o < a.out) {
           const float* u = a.u + (size_t)token0 * (a.r_max * a.n_mod) + module_of(a, o) * a.r_max;
           for (int j = 0; j < a.r_max / 8; ++j) {
@@ -260,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, 1) q4_tc_kernel(const __grid_constan
             uint4 b = make_uint4(0u, 0u, 0u, 0u);
             float alpha = 0.f;
 #pragma unroll
-            for (int i = 0; i < BN; ++i) {
+            for (int i = 0; i < kCols; ++i) {
               const int s = i < n_tok ? a.slots[token0 + i] : -1;
               if (s >= 0 && s < a.n_adapters) {
                 if (s != have) {
@@ -276,76 +303,70 @@ __global__ void __launch_bounds__(kThreads, 1) q4_tc_kernel(const __grid_constan
         const int act = a.flags & (MLORA_ACT_RELU2 | MLORA_ACT_GELU);
         if (a.flags & MLORA_SILU_MUL) {
 #pragma unroll
-          for (int i = 0; i < BN; ++i) {
+          for (int i = 0; i < kCols; ++i) {
             const float up = __shfl_xor_sync(0xffffffffu, acc[i], 8);  // (8 gate outputs, then their 8 up outputs)
             if (!(lane & 8) && o < a.out && i < n_tok) store_out(a, token0 + i, o / 16 * 8 + (o & 7), silu_mul(acc[i], up));
           }
         } else if (o < a.out) {
 #pragma unroll
-          for (int i = 0; i < BN; ++i)
+          for (int i = 0; i < kCols; ++i)
             if (i < n_tok) store_out(a, token0 + i, o, act_one(acc[i], act));
         }
       }
 #pragma unroll
-      for (int i = 0; i < BN; ++i) acc[i] = 0.f;
+      for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
       c = Cursor(seg_end, u_end, t.units, n_kb);
     }
     if (!ok) s_abort = 1;
   } else {
-    regs_down<48>();
-    if (warp == 12) {
+    if (warp == kMma) {
       // ---- MMA issue -------------------------------------------------------------------------------------------------------------
       constexpr uint32_t idesc = make_idesc(kQ4Tile, BN);
-      int seq = 0, n = 0;
-      bool ok = true;
-      for (Cursor c(u_begin, u_end, t.units, n_kb); c.valid() && ok; ++seq) {
-        const int buf = seq % kAbufs, slot = seq % kXslots, kb = c.kb();
-        const bool last_of_unit = c.sub == 1 || 2 * c.u + 1 >= n_kb;
-        int good = 1;
-        if (lane == 0) {
-          good = mbar_wait(&a_full[buf], (seq / kAbufs) & 1, abort) && mbar_wait(&x_full[slot], (seq / kXslots) & 1, abort);
-          tc_fence_after();
-          const uint64_t bdesc = make_smem_desc(smem_u32(sx + slot * BN * 128));
+      constexpr int steps = 4 / kSums;
+      if (elect_one()) {  // (one thread: every instruction it spends per block bounds the rate)
+        const uint64_t b0 = make_smem_desc(smem_u32(sx));
+        const uint32_t a_full0 = smem_u32(a_full), x_full0 = smem_u32(x_full), empty0 = smem_u32(empty), d_full0 = smem_u32(d_full),
+                       d_empty0 = smem_u32(d_empty);
+        uint32_t buf = 0, par = 0, d = 0, d_par = 1;
+        bool ok = true, open = false;
+        for (Cursor c(u_begin, u_end, t.units, n_kb); c.valid(); c.next()) {
+          const bool closes = G != 128 || c.sub == 1 || 2 * c.u + 1 >= n_kb;
+          ok = mbar_wait_a(a_full0 + 8 * buf, par, abort) && mbar_wait_a(x_full0 + 8 * buf, par, abort);
+          if (!ok) break;
+          const uint64_t bdesc = b0 + (uint64_t)(buf * (BN * 128 >> 4));
+          const uint32_t a_tmem = tmem_a + buf * 32;
 #pragma unroll
           for (int s = 0; s < kSums; ++s) {
-            const bool opens = G == 128 ? (kb & 1) == 0 : true, closes = G == 128 ? last_of_unit : true;
-            const int d = n % kDbufs;
-            if (good && opens) {
-              good = mbar_wait(&d_empty[d], ((n / kDbufs) & 1) ^ 1, abort);
-              tc_fence_after();
+            if (!open) {
+              ok = mbar_wait_a(d_empty0 + 8 * d, d_par, abort);
+              if (!ok) break;
             }
-            if (good) {
-              constexpr int steps = 4 / kSums;
+            if (s == 0 || !open) tc_fence_after();
 #pragma unroll
-              for (int k = 0; k < steps; ++k)
-                umma_bf16_ta(tmem_d + d * BN, tmem_a + buf * 32 + (s * steps + k) * 8, bdesc + 2 * (s * steps + k), idesc, (!opens || k > 0) ? 1u : 0u);
-              if (closes) {
-                umma_commit(&d_full[d]);
-                ++n;
-              }
+            for (int k = 0; k < steps; ++k)
+              umma_bf16_ta(tmem_d + d * BN, a_tmem + (s * steps + k) * 8, bdesc + 2 * (s * steps + k), idesc, (open || k > 0) ? 1u : 0u);
+            open = !closes;
+            if (closes) {
+              umma_commit_a(d_full0 + 8 * d);
+              if (++d == kDbufs) d = 0, d_par ^= 1;
             }
           }
-          if (good) {
-            umma_commit(&a_empty[buf]);
-            umma_commit(&x_empty[slot]);
-          }
+          if (!ok) break;
+          umma_commit_a(empty0 + 8 * buf);
+          if (++buf == kBufs) buf = 0, par ^= 1;
         }
-        good = __shfl_sync(0xffffffffu, good, 0);
-        if (!good) {
-          s_abort = 1;
-          ok = false;
-        }
-        c.next();
+        if (!ok) s_abort = 1;
       }
-    } else if (warp == 13) {
+      __syncwarp();
+    } else {
       // ---- rows of x -------------------------------------------------------------------------------------------------------------
       pdl_wait();
       int seq = 0;
       for (Cursor c(u_begin, u_end, t.units, n_kb); c.valid(); ++seq) {
-        const int slot = seq % kXslots;
+        const int slot = seq % kBufs;
         int good = 1;
         if (lane == 0) {
-          good = mbar_wait(&x_empty[slot], ((seq / kXslots) & 1) ^ 1, abort);
+          good = mbar_wait(&empty[slot], ((seq / kBufs) & 1) ^ 1, abort);
           if (good) {
             mbar_expect_tx(&x_full[slot], BN * 128);
             tma_load_2d(sx + slot * BN * 128, &map_x, c.kb() * kQ4Block, c.tile / t.row_tiles * BN, &x_full[slot]);
@@ -358,6 +379,9 @@ __global__ void __launch_bounds__(kThreads, 1) q4_tc_kernel(const __grid_constan
         }
         c.next();
       }
+      // commits arrive at these barriers until the last block's: nobody leaves before
+      for (int k = max(seq - kBufs, 0); k < seq && !*abort; ++k)
+        if (!__all_sync(0xffffffffu, mbar_wait(&empty[k % kBufs], (k / kBufs) & 1, abort))) s_abort = 1;
       if (*abort && lane == 0)  // copies may still be in flight: let them land before the shared memory goes to another CTA
         for (int i = 0; i < 64; ++i) __nanosleep(1000);
     }
@@ -365,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) q4_tc_kernel(const __grid_constan
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && s_abort) atomicOr(t.status, 2);
-  if (warp == 12) tmem_dealloc(tmem_slot, 512);
+  if (warp == kMma) tmem_dealloc(tmem_slot, 512);
 }
 
 int q4_ctas(long long units) {
@@ -384,7 +408,7 @@ int launch_tc_as(const TcArgs& t, int grid, cudaStream_t st) {
   CUtensorMap mx;
   const int rc = make_map(&mx, t.p.a.x, t.p.a.T, t.p.a.in, t.p.a.ldx, BN, kQ4Block);
   if (rc) return rc;
-  constexpr int smem = 1024 + kXslots * BN * 128 + 8 * kWslots * kWarpBlock;
+  constexpr int smem = 1024 + kBufs * BN * 128 + 8 * kWslots * kWarpBlock;
   static std::atomic<unsigned long long> done{0};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -393,7 +417,7 @@ int launch_tc_as(const TcArgs& t, int grid, cudaStream_t st) {
     if (e != cudaSuccess) return fail(MLORA_ECUDA, "q4_linear: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     done.fetch_or(1ull << (dev & 63), std::memory_order_release);
   }
-  const cudaError_t e = launch_pdl_if(pdl_enabled_gemm(), q4_tc_kernel<BN, ZERO, G>, dim3((unsigned)grid), dim3(kThreads), smem, st, mx, t);
+  const cudaError_t e = launch_pdl_if(pdl_enabled_gemm(), q4_tc_kernel<BN, ZERO, G>, dim3((unsigned)grid), dim3(q4_threads(BN)), smem, st, mx, t);
   if (e != cudaSuccess) return fail(MLORA_ECUDA, "q4_tc_kernel: %s", cudaGetErrorString(e));
   count_launch();
   MLORA_CHECK_LAUNCH("q4_tc_kernel");
