@@ -1,13 +1,14 @@
 // Projections with 4-bit weights on the 5th-generation tensor cores, for more than 16 rows (see q4.cuh for the layout).
 //
-// Tiles of 128 outputs x BN rows of x.  Eight warps copy packed weights with rings of their own, turn them into bf16 integers q - z and
-// write them to TMEM (tcgen05.st.16x128b has the lanes where the packed order has them): weights go DRAM -> shared memory -> registers ->
-// TMEM and are never written to shared memory as bf16, whose 32 KB per 8 KB of weights would be more than its bandwidth.  The MMA takes
-// them from there as its A operand and the rows of x (TMA, 128-byte swizzle) as B.  A group's sums have an accumulator of their own, which
-// four warps scale in fp32 registers while the next one is filled: nothing but the output is rounded.
+// Tiles of 128 outputs x BN rows of x, in units of 128 inputs.  Eight warps take packed weights from rings of bulk copies, turn them into
+// bf16 integers q - z and write them to TMEM (tcgen05.st.16x128b has the lanes where the packed order has them): weights go DRAM -> shared
+// memory -> registers -> TMEM and are never written to shared memory as bf16, whose 32 KB per 8 KB of weights would be more than its
+// bandwidth.  The MMA takes them from there as its A operand -- 16 cycles per m128n32k16, against 40 from shared memory -- and the rows of
+// x (TMA, 128-byte swizzle) as B.  A group's sums have an accumulator of their own, which four or eight warps scale in fp32 registers
+// while the next ones are filled: nothing but the output is rounded.
 //
-// Persistent, one CTA per SM; the units of 128 inputs of all tiles are dealt out in equal ranges.  A tile that several CTAs share is summed
-// by the last of them to arrive, in the order of the inputs, from the partial sums that each has left in scratch: no CTA waits for another.
+// Persistent, one CTA per SM; the units of all tiles are dealt out in equal ranges.  A tile that several CTAs share is summed by the last
+// of them to arrive, in the order of the inputs, from the partial sums that each has left in scratch: no CTA waits for another.
 #include "q4.cuh"
 #include "tc_ptx.cuh"
 
@@ -18,11 +19,13 @@ namespace {
 
 // Warps 0..7: weights; then four or eight (tiles of 128 rows of x: half of the columns each) for sums and outputs, MMA issue, copies of x.
 constexpr int q4_threads(int bn) { return 32 * (8 + (bn == 128 ? 8 : 4) + 2); }
-constexpr int kBufs = 8;                 // blocks of weights in TMEM, and of x in shared memory
-constexpr int kWslots = 8;               // blocks in a weight warp's ring
+constexpr int kBufs = 4;                 // units of weights in TMEM, and of x in shared memory
+constexpr int kWslots = 4;               // packed units in a weight warpgroup's ring
+constexpr int kSlots = 8;                // units whose scales lie in shared memory
 constexpr int kMaxCtas = 512;
 constexpr int kHeader = 256;             // bytes: status word, then the caller's
-constexpr int kWarpBlock = 1024 + 256;   // bytes of 32 outputs of a block, with their scales where there are zero points
+constexpr int kScaleBytes = 4 * 512;     // scales of a unit's groups, at most
+constexpr int kSlotBytes = 2 * kQ4TileBytes + kScaleBytes;  // a unit, and its groups' scales where there are zero points
 
 struct TcArgs {
   Q4Args p;
@@ -55,38 +58,36 @@ __device__ __forceinline__ void tmem_st_16x128b_x8(uint32_t addr, const uint32_t
                : "memory");
 }
 
-// The blocks of 64 inputs of a CTA's range, one after the other.
+// The units of a CTA's range, one after the other.
 struct Cursor {
-  long long unit, end;
-  int tile, u, sub, units, n_kb;
-  __device__ Cursor(long long a, long long b, int units_, int n_kb_) : unit(a), end(b), sub(0), units(units_), n_kb(n_kb_) {
-    tile = (int)(a / units_);
-    u = (int)(a % units_);
+  int left, u, row_tile, token_tile, units, row_tiles;
+  __device__ Cursor(const TcArgs& t, long long a, long long b) : left((int)(b - a)), units(t.units), row_tiles(t.row_tiles) {
+    const int tile = (int)(a / t.units);
+    u = (int)(a % t.units);
+    row_tile = tile % t.row_tiles;
+    token_tile = tile / t.row_tiles;
   }
-  __device__ bool valid() const { return unit < end; }
-  __device__ int kb() const { return 2 * u + sub; }
   __device__ void next() {
-    if (sub == 0 && 2 * u + 1 < n_kb) {
-      sub = 1;
-      return;
-    }
-    sub = 0;
-    ++unit;
-    if (++u == units) u = 0, ++tile;
+    --left;
+    if (++u < units) return;
+    u = 0;
+    if (++row_tile == row_tiles) row_tile = 0, ++token_tile;
   }
 };
 
 template <int BN, bool ZERO, int G>
 __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_constant__ CUtensorMap map_x, TcArgs t) {
-  constexpr int kDbufs = 2;
+  constexpr int kDbufs = BN == 128 ? 2 : 4;
   constexpr int kOutWarps = BN == 128 ? 8 : 4, kMma = 8 + kOutWarps;  // first of the two warps behind them
   constexpr int kCols = BN * 4 / kOutWarps;               // columns of a thread that sums
-  constexpr int kSums = G == 32 ? 2 : 1;                  // accumulators per block (G 128: one for two blocks)
+  constexpr int kSums = 128 / G;                          // groups of a unit
   constexpr int kEntry = ZERO ? 4 : 2;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sx = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint8_t* sw = sx + kBufs * BN * 128;                  // [weight warp][slot][kWarpBlock]
-  __shared__ uint64_t x_full[kBufs], a_full[kBufs], empty[kBufs], d_full[kDbufs], d_empty[kDbufs];
+  uint8_t* sw = sx + kBufs * BN * 256;                    // [weight warpgroup][slot][kSlotBytes]
+  uint8_t* ss = sw + 2 * kWslots * kSlotBytes;            // [slot][kScaleBytes]
+  __shared__ uint64_t w_full[2 * kWslots], w_empty[2 * kWslots], x_full[kBufs], a_full[kBufs], empty[kBufs], d_full[kDbufs], d_empty[kDbufs],
+      s_full[kSlots], s_empty[kSlots];
   __shared__ uint32_t tmem_slot;
   __shared__ int s_abort, s_last;
 
@@ -95,7 +96,9 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     s_abort = 0;
+    for (int i = 0; i < 2 * kWslots; ++i) mbar_init(&w_full[i], 1), mbar_init(&w_empty[i], 4);
     for (int i = 0; i < kBufs; ++i) mbar_init(&x_full[i], 1), mbar_init(&a_full[i], 4), mbar_init(&empty[i], 1);
+    for (int i = 0; i < kSlots; ++i) mbar_init(&s_full[i], 1), mbar_init(&s_empty[i], kOutWarps);
     for (int i = 0; i < kDbufs; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], kOutWarps);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     tma_prefetch_desc(&map_x);
@@ -113,34 +116,31 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
   if (warp < 8) {
     // ---- weights -> TMEM: a warpgroup takes every other block, a warp its 32 outputs of it -------------------------------------
     const int wg = warp >> 2, quarter = warp & 3;
-    const uint8_t* weights = reinterpret_cast<const uint8_t*>(a.W) + quarter * 1024 + lane * 16;
-    const uint32_t ring = smem_u32(sw) + warp * kWslots * kWarpBlock;
-    const uint8_t* ring_p = sw + warp * kWslots * kWarpBlock;
-    Cursor ahead(u_begin, u_end, t.units, n_kb), now(u_begin, u_end, t.units, n_kb);
-    if (wg == 1) {
-      if (ahead.valid()) ahead.next();
-      if (now.valid()) now.next();
-    }
-    auto fetch = [&](int slot) {
-      if (ahead.valid()) {
-        const int row_tile = ahead.tile % t.row_tiles, kb = ahead.kb();
-        const uint8_t* src = weights + ((size_t)row_tile * n_kb + kb) * kQ4TileBytes;
-        const uint32_t dst = ring + slot * kWarpBlock;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + lane * 16), "l"(src) : "memory");
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 512 + lane * 16), "l"(src + 512) : "memory");
-        if (ZERO && lane < 8 * kSums) {
-          const int g = min(kSums == 2 ? 2 * kb + (lane >> 3) : kb * kQ4Block / G, t.p.n_groups - 1);
-          const uint8_t* e = t.p.table + (((size_t)row_tile * t.p.n_groups + g) * kQ4Tile + quarter * 32) * 4 + (lane & 7) * 16;
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 1024 + lane * 16), "l"(e) : "memory");
-        }
-        ahead.next();
-        if (ahead.valid()) ahead.next();
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
+    const uint8_t* weights = reinterpret_cast<const uint8_t*>(a.W);
+    uint8_t* ring = sw + wg * kWslots * kSlotBytes;
+    uint64_t *full = w_full + wg * kWslots, *freed = w_empty + wg * kWslots;
+    Cursor ahead(t, u_begin, u_end), now(t, u_begin, u_end);
+    if (wg == 1) ahead.next(), now.next();  // (a warpgroup takes every other unit)
+    // One thread copies for the warpgroup: a unit's 8 KB lie one after the other, and so do its groups' scales.
+    auto fetch = [&](int i) {
+      if (ahead.left <= 0) return true;
+      const int slot = i % kWslots;
+      if (!mbar_wait(&freed[slot], ((i / kWslots) & 1) ^ 1, abort)) return false;
+      const int blocks = min(2, n_kb - 2 * ahead.u), g = ahead.u * kSums, n_g = min(kSums, t.p.n_groups - g);
+      mbar_expect_tx(&full[slot], blocks * kQ4TileBytes + (ZERO ? n_g * 512 : 0));
+      bulk_load(ring + slot * kSlotBytes, weights + ((size_t)ahead.row_tile * n_kb + 2 * ahead.u) * kQ4TileBytes, blocks * kQ4TileBytes, &full[slot]);
+      if (ZERO)
+        bulk_load(ring + slot * kSlotBytes + 2 * kQ4TileBytes, t.p.table + ((size_t)ahead.row_tile * t.p.n_groups + g) * 512, n_g * 512, &full[slot]);
+      ahead.next();
+      ahead.next();
+      return true;
     };
+    const bool copies = quarter == 0 && lane == 0;
     // (weights and scales are never written by an earlier kernel of a step: the copies need not wait for it)
-    for (int i = 0; i < kWslots - 1; ++i) fetch(i);
-    int told = -1;  // block whose stores are on their way to TMEM: told to the MMA warp while the next one is being expanded
+    if (copies)
+      for (int i = 0; i < kWslots - 1; ++i) fetch(i);
+    __syncwarp();
+    int told = -1;  // unit whose stores are on their way to TMEM: told to the MMA warp while the next one is being expanded
     const auto tell = [&] {
       if (told < 0) return;
       tmem_wait_st();
@@ -149,26 +149,31 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
       if (lane == 0) mbar_arrive(&a_full[told]);
       __syncwarp();
     };
-    for (int i = 0; now.valid(); ++i) {
-      fetch((i + kWslots - 1) % kWslots);
-      asm volatile("cp.async.wait_group %0;" ::"n"(kWslots - 1) : "memory");
-      __syncwarp();
-      const uint8_t* sp = ring_p + (i % kWslots) * kWarpBlock;
+    for (int i = 0; now.left > 0; ++i, now.next(), now.next()) {
+      const int slot = i % kWslots;
+      bool good = true;
+      if (copies) good = fetch(i + kWslots - 1);
+      if (!__all_sync(0xffffffffu, good && mbar_wait(&full[slot], (i / kWslots) & 1, abort))) {
+        s_abort = 1;
+        told = -1;
+        break;
+      }
+      const uint8_t* sp = ring + slot * kSlotBytes + quarter * 1024 + lane * 16;
+      const uint32_t* zp = reinterpret_cast<const uint32_t*>(ring + slot * kSlotBytes + 2 * kQ4TileBytes) + quarter * 32 + (lane >> 2);
       const int seq = 2 * i + wg, buf = seq % kBufs;
-      uint4 w4[2];
+      uint4 w4[4];  // block, half of the warp's 32 outputs
 #pragma unroll
-      for (int h = 0; h < 2; ++h) w4[h] = *reinterpret_cast<const uint4*>(sp + h * 512 + lane * 16);
+      for (int h = 0; h < 4; ++h) w4[h] = *reinterpret_cast<const uint4*>(sp + (h >> 1) * kQ4TileBytes + (h & 1) * 512);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < 4; ++h) {
         const uint32_t w[4] = {w4[h].x, w4[h].y, w4[h].z, w4[h].w};
         uint32_t r[16];
         uint32_t z0 = kQ4Middle, z1 = kQ4Middle;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (ZERO && (j == 0 || (kSums == 2 && j == 2))) {
-            const uint32_t* e = reinterpret_cast<const uint32_t*>(sp + 1024) + (kSums == 2 ? j / 2 : 0) * 32 + h * 16 + (lane >> 2);
-            const uint32_t e0 = e[0], e1 = e[8];
-            z0 = __byte_perm(e0, e0, 0x3232), z1 = __byte_perm(e1, e1, 0x3232);
+          if (ZERO && (j == 0 || (G == 32 && j == 2))) {
+            const uint32_t* e = zp + (G == 32 ? (h >> 1) * 2 + j / 2 : G == 64 ? (h >> 1) : 0) * 128 + (h & 1) * 16;
+            z0 = __byte_perm(e[0], e[0], 0x3232), z1 = __byte_perm(e[8], e[8], 0x3232);
           }
           uint32_t q[4];
           q4_expand(w[j], z0, z1, q);
@@ -185,14 +190,18 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
           tc_fence_after();
           told = buf;
         }
-        tmem_st_16x128b_x8(tmem_a + buf * 32 + ((uint32_t)(quarter * 32 + h * 16) << 16), r);
+        if (h == 3) {  // (everything of the slot has been read)
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&freed[slot]);
+          __syncwarp();
+        }
+        tmem_st_16x128b_x8(tmem_a + buf * 64 + (h >> 1) * 32 + ((uint32_t)(quarter * 32 + (h & 1) * 16) << 16), r);
       }
       if (told < 0) break;
-      now.next();
-      if (now.valid()) now.next();
     }
     tell();
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (*abort && copies)  // copies may still be in flight: let them land before the shared memory goes to another CTA
+      for (int i = 0; i < 64; ++i) __nanosleep(1000);
   } else if (warp < kMma) {
     // ---- sums and outputs: one thread per output ---------------------------------------------------------------------------------
     const int row = tid & 127, col0 = (warp - 8) / 4 * kCols;
@@ -201,44 +210,45 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
 #pragma unroll
     for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
     pdl_wait();  // (scratch and outputs belong to earlier kernels until here)
-    Cursor c(u_begin, u_end, t.units, n_kb);
-    int n = 0;  // accumulators taken
+    Cursor c(t, u_begin, u_end);
+    long long unit = u_begin;
+    int n = 0, seq = 0;  // accumulators and units taken
     bool ok = true;
-    while (c.valid() && ok) {
-      const long long tile_begin = (long long)c.tile * t.units, seg_begin = c.unit;
-      const int tile = c.tile, row_tile = tile % t.row_tiles, token0 = tile / t.row_tiles * BN + col0;
-      const uint8_t* table = t.p.table + ((size_t)row_tile * t.p.n_groups * kQ4Tile + row) * kEntry;
-      auto scale_of = [&](int g) {
-        const uint8_t* e = table + (size_t)min(g, t.p.n_groups - 1) * (kQ4Tile * kEntry);
-        return __uint_as_float((ZERO ? __ldg(reinterpret_cast<const uint32_t*>(e)) : (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(e))) << 16);
-      };
-      const long long seg_end = min(u_end, tile_begin + t.units);
-      const int g0 = (int)((seg_begin - tile_begin) * (128 / G)), g_end = min((int)((seg_end - tile_begin) * (128 / G)), G == 32 ? 2 * n_kb : (n_kb * kQ4Block + G - 1) / G);
-      float s_next = scale_of(g0);
-      for (int g = g0; g < g_end; ++g, ++n) {
-        const float s = s_next;
-        s_next = scale_of(g + 1);
-        const int d = n % kDbufs;
-        ok = __all_sync(0xffffffffu, mbar_wait(&d_full[d], (n / kDbufs) & 1, abort));
-        if (!ok) break;
-        tc_fence_after();
-        float v[2][16];
-        const uint32_t from = tmem_d + d * BN + col0 + lanes;
-        tmem_ld16_issue(from, v[0]);
+    while (c.left > 0 && ok) {
+      const int u0 = c.u, row_tile = c.row_tile, token0 = c.token_tile * BN + col0, n_units = min(c.left, t.units - u0);
+      const long long seg_begin = unit, tile_begin = unit - u0, seg_end = unit + n_units;
+      for (int k = 0; k < n_units && ok; ++k, ++seq) {
+        const int slot = seq % kSlots, n_g = min(kSums, t.p.n_groups - (u0 + k) * kSums);
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[slot], (seq / kSlots) & 1, abort));
+        const uint8_t* scales = ss + slot * kScaleBytes + row * kEntry;
+#pragma unroll 1
+        for (int g = 0; g < n_g && ok; ++g, ++n) {
+          const float s = __uint_as_float((ZERO ? *reinterpret_cast<const uint32_t*>(scales + g * 512) : (uint32_t)*reinterpret_cast<const uint16_t*>(scales + g * 256)) << 16);
+          const int d = n % kDbufs;
+          ok = __all_sync(0xffffffffu, mbar_wait(&d_full[d], (n / kDbufs) & 1, abort));
+          if (!ok) break;
+          tc_fence_after();
+          float v[2][16];
+          const uint32_t from = tmem_d + d * BN + col0 + lanes;
+          tmem_ld16_issue(from, v[0]);
 #pragma unroll
-        for (int b = 0; b < kCols / 16; ++b) {
-          tmem_wait_ld16(v[b & 1]);
-          if (b + 1 < kCols / 16) {
-            tmem_ld16_issue(from + (b + 1) * 16, v[(b + 1) & 1]);
-          } else {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&d_empty[d]);
-            __syncwarp();
+          for (int b = 0; b < kCols / 16; ++b) {
+            tmem_wait_ld16(v[b & 1]);
+            if (b + 1 < kCols / 16) {
+              tmem_ld16_issue(from + (b + 1) * 16, v[(b + 1) & 1]);
+            } else {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&d_empty[d]);
+              __syncwarp();
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[b * 16 + i] = fmaf(s, v[b & 1][i], acc[b * 16 + i]);
           }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[b * 16 + i] = fmaf(s, v[b & 1][i], acc[b * 16 + i]);
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_empty[slot]);
+        __syncwarp();
       }
       ok = out_all<32 * kOutWarps>(ok);
       if (!ok) break;
@@ -315,40 +325,39 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
       }
 #pragma unroll
       for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
-      c = Cursor(seg_end, u_end, t.units, n_kb);
+      for (int k = 0; k < n_units; ++k) c.next();
+      unit = seg_end;
     }
     if (!ok) s_abort = 1;
   } else {
     if (warp == kMma) {
       // ---- MMA issue -------------------------------------------------------------------------------------------------------------
       constexpr uint32_t idesc = make_idesc(kQ4Tile, BN);
-      constexpr int steps = 4 / kSums;
-      if (elect_one()) {  // (one thread: every instruction it spends per block bounds the rate)
+      if (elect_one()) {  // (one thread: every instruction it spends per unit bounds the rate)
         const uint64_t b0 = make_smem_desc(smem_u32(sx));
         const uint32_t a_full0 = smem_u32(a_full), x_full0 = smem_u32(x_full), empty0 = smem_u32(empty), d_full0 = smem_u32(d_full),
                        d_empty0 = smem_u32(d_empty);
         uint32_t buf = 0, par = 0, d = 0, d_par = 1;
-        bool ok = true, open = false;
-        for (Cursor c(u_begin, u_end, t.units, n_kb); c.valid(); c.next()) {
-          const bool closes = G != 128 || c.sub == 1 || 2 * c.u + 1 >= n_kb;
+        bool ok = true;
+        for (Cursor c(t, u_begin, u_end); c.left > 0 && ok; c.next()) {
+          const int steps = min(8, (n_kb - 2 * c.u) * 4);  // of 16 inputs
           ok = mbar_wait_a(a_full0 + 8 * buf, par, abort) && mbar_wait_a(x_full0 + 8 * buf, par, abort);
           if (!ok) break;
-          const uint64_t bdesc = b0 + (uint64_t)(buf * (BN * 128 >> 4));
-          const uint32_t a_tmem = tmem_a + buf * 32;
+          const uint64_t bdesc = b0 + (uint64_t)(buf * (BN * 256 >> 4));
+          const uint32_t a_tmem = tmem_a + buf * 64;
 #pragma unroll
-          for (int s = 0; s < kSums; ++s) {
-            if (!open) {
-              ok = mbar_wait_a(d_empty0 + 8 * d, d_par, abort);
-              if (!ok) break;
-            }
-            if (s == 0 || !open) tc_fence_after();
-#pragma unroll
-            for (int k = 0; k < steps; ++k)
-              umma_bf16_ta(tmem_d + d * BN, a_tmem + (s * steps + k) * 8, bdesc + 2 * (s * steps + k), idesc, (open || k > 0) ? 1u : 0u);
-            open = !closes;
-            if (closes) {
-              umma_commit_a(d_full0 + 8 * d);
-              if (++d == kDbufs) d = 0, d_par ^= 1;
+          for (int k = 0; k < 8; ++k) {
+            if (k < steps && ok) {
+              const bool opens = k % (G / 16) == 0;
+              if (opens) {
+                ok = mbar_wait_a(d_empty0 + 8 * d, d_par, abort);
+                tc_fence_after();
+              }
+              if (ok) umma_bf16_ta(tmem_d + d * BN, a_tmem + k * 8, bdesc + 2 * (k & 3) + (k >> 2) * (BN * 128 >> 4), idesc, opens ? 0u : 1u);
+              if (ok && (k % (G / 16) == G / 16 - 1 || k + 1 == steps)) {
+                umma_commit_a(d_full0 + 8 * d);
+                if (++d == kDbufs) d = 0, d_par ^= 1;
+              }
             }
           }
           if (!ok) break;
@@ -359,17 +368,25 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
       }
       __syncwarp();
     } else {
-      // ---- rows of x -------------------------------------------------------------------------------------------------------------
+      // ---- rows of x, and the scales ------------------------------------------------------------------------------------------------
       pdl_wait();
       int seq = 0;
-      for (Cursor c(u_begin, u_end, t.units, n_kb); c.valid(); ++seq) {
-        const int slot = seq % kBufs;
+      for (Cursor c(t, u_begin, u_end); c.left > 0; c.next(), ++seq) {
+        const int slot = seq % kBufs, s_slot = seq % kSlots;
         int good = 1;
         if (lane == 0) {
           good = mbar_wait(&empty[slot], ((seq / kBufs) & 1) ^ 1, abort);
           if (good) {
-            mbar_expect_tx(&x_full[slot], BN * 128);
-            tma_load_2d(sx + slot * BN * 128, &map_x, c.kb() * kQ4Block, c.tile / t.row_tiles * BN, &x_full[slot]);
+            const int blocks = min(2, n_kb - 2 * c.u);
+            mbar_expect_tx(&x_full[slot], blocks * BN * 128);
+            for (int b = 0; b < blocks; ++b)
+              tma_load_2d(sx + (slot * 2 + b) * BN * 128, &map_x, (2 * c.u + b) * kQ4Block, c.token_tile * BN, &x_full[slot]);
+            good = mbar_wait(&s_empty[s_slot], ((seq / kSlots) & 1) ^ 1, abort);
+          }
+          if (good) {
+            const int g = c.u * kSums, bytes = min(kSums, t.p.n_groups - g) * kQ4Tile * kEntry;
+            mbar_expect_tx(&s_full[s_slot], bytes);
+            bulk_load(ss + s_slot * kScaleBytes, t.p.table + ((size_t)c.row_tile * t.p.n_groups + g) * kQ4Tile * kEntry, bytes, &s_full[s_slot]);
           }
         }
         good = __shfl_sync(0xffffffffu, good, 0);
@@ -377,7 +394,6 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
           s_abort = 1;
           break;
         }
-        c.next();
       }
       // commits arrive at these barriers until the last block's: nobody leaves before
       for (int k = max(seq - kBufs, 0); k < seq && !*abort; ++k)
@@ -408,7 +424,7 @@ int launch_tc_as(const TcArgs& t, int grid, cudaStream_t st) {
   CUtensorMap mx;
   const int rc = make_map(&mx, t.p.a.x, t.p.a.T, t.p.a.in, t.p.a.ldx, BN, kQ4Block);
   if (rc) return rc;
-  constexpr int smem = 1024 + kBufs * BN * 128 + 8 * kWslots * kWarpBlock;
+  constexpr int smem = 1024 + kBufs * BN * 256 + 2 * kWslots * kSlotBytes + kSlots * kScaleBytes;
   static std::atomic<unsigned long long> done{0};
   int dev = 0;
   cudaGetDevice(&dev);
