@@ -7,8 +7,10 @@
 // x (TMA, 128-byte swizzle) as B.  A group's sums have an accumulator of their own, which four or eight warps scale in fp32 registers
 // while the next ones are filled: nothing but the output is rounded.
 //
-// Persistent, one CTA per SM; the units of all tiles are dealt out in equal ranges.  A tile that several CTAs share is summed by the last
-// of them to arrive, in the order of the inputs, from the partial sums that each has left in scratch: no CTA waits for another.
+// Persistent, one CTA per SM; the units of all tiles are dealt out in equal ranges.  A tile that several CTAs share is finished by the one
+// that begins it: the others leave their sums in scratch -- the first thing each of them does -- and it adds them up in the order of the
+// inputs.  Adapters are expanded by a kernel of their own in front of this one, into fp32 scratch that is added to the sums: a thread here
+// has one output and many rows, whose adapters' rows it would have to wait for one after the other.
 #include "q4.cuh"
 #include "tc_ptx.cuh"
 
@@ -17,21 +19,26 @@
 namespace mlora {
 namespace {
 
-// Warps 0..7: weights; then four or eight (tiles of 128 rows of x: half of the columns each) for sums and outputs, MMA issue, copies of x.
-constexpr int q4_threads(int bn) { return 32 * (8 + (bn == 128 ? 8 : 4) + 2); }
 constexpr int kBufs = 4;                 // units of weights in TMEM, and of x in shared memory
-constexpr int kWslots = 4;               // packed units in a weight warpgroup's ring
-constexpr int kSlots = 8;                // units whose scales lie in shared memory
+constexpr int kSlots = 4;                // units whose scales lie in shared memory
 constexpr int kMaxCtas = 512;
 constexpr int kHeader = 256;             // bytes: status word, then the caller's
 constexpr int kScaleBytes = 4 * 512;     // scales of a unit's groups, at most
-constexpr int kSlotBytes = 2 * kQ4TileBytes + kScaleBytes;  // a unit, and its groups' scales where there are zero points
+constexpr int kSlice = 512;              // rows whose adapters' share lies in scratch at a time
+// Warps: weight warpgroups, then those that sum and write (32 columns of BN 32 and 64 each, 64 of 128), then MMA issue, copies of x,
+// copies of weights.
+constexpr int q4_weight_groups(int bn) { return bn == 32 ? 3 : 2; }
+constexpr int q4_out_warps(int bn) { return bn == 32 ? 4 : 8; }
+constexpr int q4_threads(int bn) { return 32 * (4 * q4_weight_groups(bn) + q4_out_warps(bn) + 3); }
+constexpr int q4_ring(int bn) { return bn == 128 ? 6 : 12; }  // packed units in shared memory
+constexpr int q4_slot_bytes(bool zero) { return 2 * kQ4TileBytes + (zero ? kScaleBytes : 0); }  // with zero points: and their groups' scales
 
 struct TcArgs {
   Q4Args p;
   int32_t* status;
-  int32_t* counters;  // [CTA that the tile begins in], zero between calls
-  float* parts;       // [CTA][2][BN][128]: sums of the tile it ends and of the tile it begins
+  int32_t* counters;  // [CTA that the tile begins in]: shares that have arrived, zero between calls
+  float* parts;       // [CTA][BN][128]: sums of a CTA's share of a tile that another CTA begins
+  const float* delta; // [rows][out]: the adapters' share, or NULL
   int row_tiles, token_tiles, units;  // units of 128 inputs per tile
 };
 
@@ -50,6 +57,13 @@ __device__ __forceinline__ bool out_all(bool ok) {
       : "memory");
   return r != 0;
 }
+template <int N>
+__device__ __forceinline__ void out_sync() {
+  __syncwarp();
+  asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory");
+}
+__device__ __noinline__ float act_apart(float v, int act) { return act_one(v, act); }  // (one copy of erf, not one per column)
+
 // 16 lanes x 32 columns from registers laid out as A operands of mma.m16n8k16
 __device__ __forceinline__ void tmem_st_16x128b_x8(uint32_t addr, const uint32_t (&r)[16]) {
   asm volatile("tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(r[0]),
@@ -78,28 +92,30 @@ struct Cursor {
 template <int BN, bool ZERO, int G>
 __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_constant__ CUtensorMap map_x, TcArgs t) {
   constexpr int kDbufs = BN == 128 ? 2 : 4;
-  constexpr int kOutWarps = BN == 128 ? 8 : 4, kMma = 8 + kOutWarps;  // first of the two warps behind them
-  constexpr int kCols = BN * 4 / kOutWarps;               // columns of a thread that sums
+  constexpr int kGroups = q4_weight_groups(BN), kWarpsOut = q4_out_warps(BN);
+  constexpr int kOut = 4 * kGroups, kMma = kOut + kWarpsOut;  // first warps of these roles
+  constexpr int kCols = BN * 4 / kWarpsOut;               // columns of a thread that sums
   constexpr int kSums = 128 / G;                          // groups of a unit
   constexpr int kEntry = ZERO ? 4 : 2;
+  constexpr int kWslots = q4_ring(BN), kSlotBytes = q4_slot_bytes(ZERO);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sx = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint8_t* sw = sx + kBufs * BN * 256;                    // [weight warpgroup][slot][kSlotBytes]
-  uint8_t* ss = sw + 2 * kWslots * kSlotBytes;            // [slot][kScaleBytes]
-  __shared__ uint64_t w_full[2 * kWslots], w_empty[2 * kWslots], x_full[kBufs], a_full[kBufs], empty[kBufs], d_full[kDbufs], d_empty[kDbufs],
+  uint8_t* sw = sx + kBufs * BN * 256;                    // [slot][kSlotBytes]
+  uint8_t* ss = sw + kWslots * kSlotBytes;                // [slot][kScaleBytes]
+  __shared__ uint64_t w_full[kWslots], w_empty[kWslots], x_full[kBufs], a_full[kBufs], empty[kBufs], d_full[kDbufs], d_empty[kDbufs],
       s_full[kSlots], s_empty[kSlots];
   __shared__ uint32_t tmem_slot;
-  __shared__ int s_abort, s_last;
+  __shared__ int s_abort;
 
   pdl_launch_dependents();
   const LinearArgs& a = t.p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     s_abort = 0;
-    for (int i = 0; i < 2 * kWslots; ++i) mbar_init(&w_full[i], 1), mbar_init(&w_empty[i], 4);
+    for (int i = 0; i < kWslots; ++i) mbar_init(&w_full[i], 1), mbar_init(&w_empty[i], 4);
     for (int i = 0; i < kBufs; ++i) mbar_init(&x_full[i], 1), mbar_init(&a_full[i], 4), mbar_init(&empty[i], 1);
-    for (int i = 0; i < kSlots; ++i) mbar_init(&s_full[i], 1), mbar_init(&s_empty[i], kOutWarps);
-    for (int i = 0; i < kDbufs; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], kOutWarps);
+    for (int i = 0; i < kSlots; ++i) mbar_init(&s_full[i], 1), mbar_init(&s_empty[i], kWarpsOut);
+    for (int i = 0; i < kDbufs; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], kWarpsOut);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     tma_prefetch_desc(&map_x);
   }
@@ -113,33 +129,9 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
   const int n_kb = t.p.n_kb;
   volatile int* abort = &s_abort;
 
-  if (warp < 8) {
-    // ---- weights -> TMEM: a warpgroup takes every other block, a warp its 32 outputs of it -------------------------------------
-    const int wg = warp >> 2, quarter = warp & 3;
-    const uint8_t* weights = reinterpret_cast<const uint8_t*>(a.W);
-    uint8_t* ring = sw + wg * kWslots * kSlotBytes;
-    uint64_t *full = w_full + wg * kWslots, *freed = w_empty + wg * kWslots;
-    Cursor ahead(t, u_begin, u_end), now(t, u_begin, u_end);
-    if (wg == 1) ahead.next(), now.next();  // (a warpgroup takes every other unit)
-    // One thread copies for the warpgroup: a unit's 8 KB lie one after the other, and so do its groups' scales.
-    auto fetch = [&](int i) {
-      if (ahead.left <= 0) return true;
-      const int slot = i % kWslots;
-      if (!mbar_wait(&freed[slot], ((i / kWslots) & 1) ^ 1, abort)) return false;
-      const int blocks = min(2, n_kb - 2 * ahead.u), g = ahead.u * kSums, n_g = min(kSums, t.p.n_groups - g);
-      mbar_expect_tx(&full[slot], blocks * kQ4TileBytes + (ZERO ? n_g * 512 : 0));
-      bulk_load(ring + slot * kSlotBytes, weights + ((size_t)ahead.row_tile * n_kb + 2 * ahead.u) * kQ4TileBytes, blocks * kQ4TileBytes, &full[slot]);
-      if (ZERO)
-        bulk_load(ring + slot * kSlotBytes + 2 * kQ4TileBytes, t.p.table + ((size_t)ahead.row_tile * t.p.n_groups + g) * 512, n_g * 512, &full[slot]);
-      ahead.next();
-      ahead.next();
-      return true;
-    };
-    const bool copies = quarter == 0 && lane == 0;
-    // (weights and scales are never written by an earlier kernel of a step: the copies need not wait for it)
-    if (copies)
-      for (int i = 0; i < kWslots - 1; ++i) fetch(i);
-    __syncwarp();
+  if (warp < kOut) {
+    // ---- weights -> TMEM: the warpgroups take the units in turn, a warp its 32 outputs -----------------------------------------
+    const int wg = warp >> 2, quarter = warp & 3, n_units = (int)(u_end - u_begin);
     int told = -1;  // unit whose stores are on their way to TMEM: told to the MMA warp while the next one is being expanded
     const auto tell = [&] {
       if (told < 0) return;
@@ -149,18 +141,15 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
       if (lane == 0) mbar_arrive(&a_full[told]);
       __syncwarp();
     };
-    for (int i = 0; now.left > 0; ++i, now.next(), now.next()) {
-      const int slot = i % kWslots;
-      bool good = true;
-      if (copies) good = fetch(i + kWslots - 1);
-      if (!__all_sync(0xffffffffu, good && mbar_wait(&full[slot], (i / kWslots) & 1, abort))) {
+    for (int seq = wg; seq < n_units; seq += kGroups) {
+      const int slot = seq % kWslots, buf = seq % kBufs;
+      if (!__all_sync(0xffffffffu, mbar_wait(&w_full[slot], (seq / kWslots) & 1, abort))) {
         s_abort = 1;
         told = -1;
         break;
       }
-      const uint8_t* sp = ring + slot * kSlotBytes + quarter * 1024 + lane * 16;
-      const uint32_t* zp = reinterpret_cast<const uint32_t*>(ring + slot * kSlotBytes + 2 * kQ4TileBytes) + quarter * 32 + (lane >> 2);
-      const int seq = 2 * i + wg, buf = seq % kBufs;
+      const uint8_t* sp = sw + slot * kSlotBytes + quarter * 1024 + lane * 16;
+      const uint32_t* zp = reinterpret_cast<const uint32_t*>(sw + slot * kSlotBytes + 2 * kQ4TileBytes) + quarter * 32 + (lane >> 2);
       uint4 w4[4];  // block, half of the warp's 32 outputs
 #pragma unroll
       for (int h = 0; h < 4; ++h) w4[h] = *reinterpret_cast<const uint4*>(sp + (h >> 1) * kQ4TileBytes + (h & 1) * 512);
@@ -192,7 +181,7 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
         }
         if (h == 3) {  // (everything of the slot has been read)
           __syncwarp();
-          if (lane == 0) mbar_arrive(&freed[slot]);
+          if (lane == 0) mbar_arrive(&w_empty[slot]);
           __syncwarp();
         }
         tmem_st_16x128b_x8(tmem_a + buf * 64 + (h >> 1) * 32 + ((uint32_t)(quarter * 32 + (h & 1) * 16) << 16), r);
@@ -200,11 +189,9 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
       if (told < 0) break;
     }
     tell();
-    if (*abort && copies)  // copies may still be in flight: let them land before the shared memory goes to another CTA
-      for (int i = 0; i < 64; ++i) __nanosleep(1000);
   } else if (warp < kMma) {
     // ---- sums and outputs: one thread per output ---------------------------------------------------------------------------------
-    const int row = tid & 127, col0 = (warp - 8) / 4 * kCols;
+    const int row = (warp - kOut) % 4 * 32 + lane, col0 = (warp - kOut) / 4 * kCols;  // (kOut is a multiple of 4: row / 32 = warp % 4)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     float acc[kCols];
 #pragma unroll
@@ -215,7 +202,7 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
     int n = 0, seq = 0;  // accumulators and units taken
     bool ok = true;
     while (c.left > 0 && ok) {
-      const int u0 = c.u, row_tile = c.row_tile, token0 = c.token_tile * BN + col0, n_units = min(c.left, t.units - u0);
+      const int u0 = c.u, token0 = c.token_tile * BN + col0, n_units = min(c.left, t.units - u0);
       const long long seg_begin = unit, tile_begin = unit - u0, seg_end = unit + n_units;
       for (int k = 0; k < n_units && ok; ++k, ++seq) {
         const int slot = seq % kSlots, n_g = min(kSums, t.p.n_groups - (u0 + k) * kSums);
@@ -250,77 +237,90 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
         if (lane == 0) mbar_arrive(&s_empty[slot]);
         __syncwarp();
       }
-      ok = out_all<32 * kOutWarps>(ok);
+      ok = out_all<32 * kWarpsOut>(ok);
       if (!ok) break;
-      // the segment is done: output, or a share of a tile that others have a part of
-      const bool whole = seg_begin == tile_begin && seg_end == tile_begin + t.units;
-      bool write = true;
+      const bool begins = seg_begin == tile_begin, whole = begins && seg_end == tile_begin + t.units;
+      int first = blockIdx.x, last = blockIdx.x;  // CTAs whose ranges hold the tile's first and last unit
       if (!whole) {
-        // first and last CTA of the tile: the ones whose ranges hold its first and last unit
-        auto cta_of = [&](long long unit) {
-          int k = (int)(unit * gridDim.x / all);
-          while (all * (k + 1) / gridDim.x <= unit) ++k;
-          while (all * k / gridDim.x > unit) --k;
+        const auto cta_of = [&](long long x) {
+          int k = (int)(x * gridDim.x / all);
+          while (all * (k + 1) / gridDim.x <= x) ++k;
+          while (all * k / gridDim.x > x) --k;
           return k;
         };
-        const int c0 = cta_of(tile_begin), c1 = cta_of(tile_begin + t.units - 1);
-        float* mine = t.parts + ((size_t)blockIdx.x * 2 + (seg_begin == tile_begin ? 1 : 0)) * (BN * kQ4Tile) + col0 * kQ4Tile + row;
+        first = cta_of(tile_begin), last = cta_of(tile_begin + t.units - 1);
+      }
+      if (!begins) {
+        float* mine = t.parts + (size_t)blockIdx.x * (BN * kQ4Tile) + col0 * kQ4Tile + row;
 #pragma unroll
         for (int i = 0; i < kCols; ++i) __stcg(mine + i * kQ4Tile, acc[i]);
-        __threadfence();
-        asm volatile("bar.sync 1, %0;" ::"n"(32 * kOutWarps) : "memory");
-        if (tid == 256) {
-          const int before = atomicAdd(&t.counters[c0], 1);
-          s_last = before == c1 - c0;
-          if (before == c1 - c0) t.counters[c0] = 0;
-        }
-        asm volatile("bar.sync 1, %0;" ::"n"(32 * kOutWarps) : "memory");
-        write = s_last != 0;
-        if (write) {
+        out_sync<32 * kWarpsOut>();
+        if (warp == kOut && lane == 0) {
           __threadfence();
-          const float* from = t.parts + ((size_t)c0 * 2 + 1) * (BN * kQ4Tile) + col0 * kQ4Tile + row;
-#pragma unroll
-          for (int i = 0; i < kCols; ++i) acc[i] = __ldcg(from + i * kQ4Tile);
-          for (int k = c0 + 1; k <= c1; ++k) {
-            from = t.parts + (size_t)k * 2 * (BN * kQ4Tile) + col0 * kQ4Tile + row;
-#pragma unroll
-            for (int i = 0; i < kCols; ++i) acc[i] += __ldcg(from + i * kQ4Tile);
-          }
+          atomicAdd(&t.counters[first], 1);
         }
-      }
-      if (write) {
-        const int o = row_tile * kQ4Tile + row, n_tok = min(kCols, a.T - token0);
-        if (a.u != nullptr && o < a.out) {
-          const float* u = a.u + (size_t)token0 * (a.r_max * a.n_mod) + module_of(a, o) * a.r_max;
-          for (int j = 0; j < a.r_max / 8; ++j) {
-            int have = -1, sw;
-            uint4 b = make_uint4(0u, 0u, 0u, 0u);
-            float alpha = 0.f;
-#pragma unroll
-            for (int i = 0; i < kCols; ++i) {
-              const int s = i < n_tok ? a.slots[token0 + i] : -1;
-              if (s >= 0 && s < a.n_adapters) {
-                if (s != have) {
-                  b = ld_cached(q4_b_row(a, t.p.packed_b, s, o, j, sw));
-                  alpha = a.scales[s];
-                  have = s;
-                }
-                acc[i] = fmaf(alpha, dot8(b, u + (size_t)i * (a.r_max * a.n_mod) + 8 * j), acc[i]);
-              }
+        __syncwarp();
+      } else {
+        if (!whole) {  // wait for the others' shares (each CTA writes its own before anything else)
+          if (lane == 0) {
+            ok = false;
+            for (uint32_t i = 0; i < kSpinLimit && !ok; ++i) {
+              int have;
+              asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(have) : "l"(&t.counters[first]) : "memory");
+              ok = have >= last - first;
+              if (!ok) __nanosleep(64);
+              if ((i & 255) == 255 && *abort) break;
             }
           }
+          ok = out_all<32 * kWarpsOut>(__shfl_sync(0xffffffffu, (int)ok, 0) != 0);
+          if (!ok) break;
+          if (warp == kOut && lane == 0) t.counters[first] = 0;  // (all of them have seen it)
         }
-        const int act = a.flags & (MLORA_ACT_RELU2 | MLORA_ACT_GELU);
-        if (a.flags & MLORA_SILU_MUL) {
+        const int o = c.row_tile * kQ4Tile + row, n_tok = min(kCols, a.T - token0), act = a.flags & (MLORA_ACT_RELU2 | MLORA_ACT_GELU);
+        const bool silu = (a.flags & MLORA_SILU_MUL) != 0, mine = o < a.out && (!silu || !(lane & 8));
+        const int col = silu ? o / 16 * 8 + (o & 7) : o;
+        // 16 columns at a time, with one copy of the code for them all: unrolled over the columns it would come from memory instruction
+        // by instruction, a tile at a time
+#pragma unroll 1
+        for (int c0 = 0; c0 < n_tok; c0 += 16) {
+          float v[16], add[16];
 #pragma unroll
-          for (int i = 0; i < kCols; ++i) {
-            const float up = __shfl_xor_sync(0xffffffffu, acc[i], 8);  // (8 gate outputs, then their 8 up outputs)
-            if (!(lane & 8) && o < a.out && i < n_tok) store_out(a, token0 + i, o / 16 * 8 + (o & 7), silu_mul(acc[i], up));
+          for (int i = 0; i < 16; ++i) v[i] = acc[i];
+#pragma unroll
+          for (int i = 0; i + 16 < kCols; ++i) acc[i] = acc[i + 16];
+          if (t.delta != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) add[i] = o < a.out && c0 + i < n_tok ? __ldcg(t.delta + (size_t)(token0 + c0 + i) * a.out + o) : 0.f;
           }
-        } else if (o < a.out) {
+#pragma unroll 1
+          for (int k = first + 1; k <= last; ++k) {
+            const float* from = t.parts + (size_t)k * (BN * kQ4Tile) + (col0 + c0) * kQ4Tile + row;
 #pragma unroll
-          for (int i = 0; i < kCols; ++i)
-            if (i < n_tok) store_out(a, token0 + i, o, act_one(acc[i], act));
+            for (int i = 0; i < 16; ++i) v[i] += __ldcg(from + i * kQ4Tile);
+          }
+          if (t.delta != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] += add[i];
+          }
+          if (silu) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = silu_mul(v[i], __shfl_xor_sync(0xffffffffu, v[i], 8));  // (8 gate outputs, then their 8 up outputs)
+          } else if (act) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = act_apart(v[i], act);
+          }
+          if (mine) {
+            const size_t at = (size_t)(token0 + c0) * a.ldy + col;
+            if (a.flags & MLORA_OUT_F32) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (c0 + i < n_tok) reinterpret_cast<float*>(a.y)[at + (size_t)i * a.ldy] = v[i];
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (c0 + i < n_tok) reinterpret_cast<bf16*>(a.y)[at + (size_t)i * a.ldy] = __float2bfloat16_rn(v[i]);
+            }
+          }
         }
       }
 #pragma unroll
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
         if (!ok) s_abort = 1;
       }
       __syncwarp();
-    } else {
+    } else if (warp == kMma + 1) {
       // ---- rows of x, and the scales ------------------------------------------------------------------------------------------------
       pdl_wait();
       int seq = 0;
@@ -400,12 +400,74 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
         if (!__all_sync(0xffffffffu, mbar_wait(&empty[k % kBufs], (k / kBufs) & 1, abort))) s_abort = 1;
       if (*abort && lane == 0)  // copies may still be in flight: let them land before the shared memory goes to another CTA
         for (int i = 0; i < 64; ++i) __nanosleep(1000);
+    } else if (lane == 0) {
+      // ---- packed weights: a unit's 8 KB lie one after the other, and so do its groups' scales (no earlier kernel of a step writes
+      // either, so the copies need not wait for it) --------------------------------------------------------------------------------
+      const uint8_t* weights = reinterpret_cast<const uint8_t*>(a.W);
+      int seq = 0;
+      for (Cursor c(t, u_begin, u_end); c.left > 0; c.next(), ++seq) {
+        const int slot = seq % kWslots;
+        if (!mbar_wait(&w_empty[slot], ((seq / kWslots) & 1) ^ 1, abort)) {
+          s_abort = 1;
+          break;
+        }
+        const int blocks = min(2, n_kb - 2 * c.u), g = c.u * kSums, n_g = min(kSums, t.p.n_groups - g);
+        mbar_expect_tx(&w_full[slot], blocks * kQ4TileBytes + (ZERO ? n_g * 512 : 0));
+        bulk_load(sw + slot * kSlotBytes, weights + ((size_t)c.row_tile * n_kb + 2 * c.u) * kQ4TileBytes, blocks * kQ4TileBytes, &w_full[slot]);
+        if (ZERO)
+          bulk_load(sw + slot * kSlotBytes + 2 * kQ4TileBytes, t.p.table + ((size_t)c.row_tile * t.p.n_groups + g) * 512, n_g * 512, &w_full[slot]);
+      }
+      if (*abort)
+        for (int i = 0; i < 64; ++i) __nanosleep(1000);
     }
   }
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && s_abort) atomicOr(t.status, 2);
   if (warp == kMma) tmem_dealloc(tmem_slot, 512);
+}
+
+// delta[t, o] = scale[slot] sum_j u[t, j] B[slot][o][j]: a thread per output, eight rows at a time; rows that follow each other with the
+// same adapter read its row once (up to 64 ranks wide).
+constexpr int kExThreads = 128, kExRows = 8, kExMaxU = 512;
+
+__global__ void __launch_bounds__(kExThreads) q4_expand_kernel(Q4Args p, float* __restrict__ delta) {
+  __shared__ __align__(16) float su[kExRows][kExMaxU];
+  __shared__ int s_slot[kExRows];
+  pdl_launch_dependents();
+  pdl_wait();
+  const LinearArgs& a = p.a;
+  const int o = blockIdx.x * kExThreads + threadIdx.x, t0 = blockIdx.y * kExRows, rows = min(kExRows, a.T - t0), width = a.r_max * a.n_mod;
+  if (threadIdx.x < kExRows) s_slot[threadIdx.x] = (int)threadIdx.x < rows ? a.slots[t0 + threadIdx.x] : -1;
+  const bool fits = width <= kExMaxU;
+  for (int i = threadIdx.x; fits && i < rows * width; i += kExThreads) su[i / width][i % width] = a.u[(size_t)t0 * width + i];
+  __syncthreads();
+  if (o >= a.out) return;
+  const int module = module_of(a, o) * a.r_max, n8 = a.r_max / 8;
+  uint4 b[8];
+  int have = -1, sw;
+  float alpha = 0.f;
+#pragma unroll 1
+  for (int r = 0; r < rows; ++r) {
+    const int s = s_slot[r];
+    float sum = 0.f;
+    if (s >= 0 && s < a.n_adapters) {
+      const float* u = fits ? &su[r][module] : a.u + (size_t)(t0 + r) * width + module;
+      if (s != have) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j < n8) b[j] = ld_cached(q4_b_row(a, p.packed_b, s, o, j, sw));
+        alpha = a.scales[s];
+        have = s;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < n8) sum += dot8(b[j], u + 8 * j);
+      for (int j = 8; j < n8; ++j) sum += dot8(ld_cached(q4_b_row(a, p.packed_b, s, o, j, sw)), u + 8 * j);
+      sum *= alpha;
+    }
+    delta[(size_t)(t0 + r) * a.out + o] = sum;
+  }
 }
 
 int q4_ctas(long long units) {
@@ -424,7 +486,7 @@ int launch_tc_as(const TcArgs& t, int grid, cudaStream_t st) {
   CUtensorMap mx;
   const int rc = make_map(&mx, t.p.a.x, t.p.a.T, t.p.a.in, t.p.a.ldx, BN, kQ4Block);
   if (rc) return rc;
-  constexpr int smem = 1024 + kBufs * BN * 256 + 2 * kWslots * kSlotBytes + kSlots * kScaleBytes;
+  constexpr int smem = 1024 + kBufs * BN * 256 + q4_ring(BN) * q4_slot_bytes(ZERO) + kSlots * kScaleBytes;
   static std::atomic<unsigned long long> done{0};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -451,10 +513,12 @@ int launch_tc_for(const TcArgs& t, int grid, cudaStream_t st) {
 
 }  // namespace
 
+size_t q4_base_bytes() { return kHeader + kMaxCtas * 4 + (size_t)q4_ctas(kMaxCtas) * 128 * kQ4Tile * 4; }
+
 size_t q4_tc_workspace(int T, int in, int out) {
-  // (the largest tile and every CTA, whatever the sizes: one buffer serves them all)
-  (void)in, (void)out;
-  return kHeader + kMaxCtas * 4 + (size_t)q4_ctas(kMaxCtas) * 2 * rows_per_tile(T) * kQ4Tile * 4;
+  // (counters and shares at places that no call's sizes move, then the adapters' share of a slice of rows)
+  (void)in;
+  return q4_base_bytes() + (size_t)(T < kSlice ? T : kSlice) * out * 4;
 }
 
 int launch_q4_tc(const Q4Args& p, void* work, size_t work_bytes, cudaStream_t st) {
@@ -462,17 +526,36 @@ int launch_q4_tc(const Q4Args& p, void* work, size_t work_bytes, cudaStream_t st
   if (!work || work_bytes < need) return fail(MLORA_ESIZE, "q4_linear: scratch of %zu bytes needed, %zu given", need, work_bytes);
   if (!aligned16(work)) return fail(MLORA_EINVAL, "q4_linear: the scratch must be 16-byte aligned");
   TcArgs t{};
-  t.p = p;
   t.status = (int32_t*)work;
   t.counters = (int32_t*)((uint8_t*)work + kHeader);
   t.parts = (float*)((uint8_t*)work + kHeader + kMaxCtas * 4);
-  const int bn = rows_per_tile(p.a.T);
-  t.row_tiles = (p.a.out + kQ4Tile - 1) / kQ4Tile;
-  t.token_tiles = (p.a.T + bn - 1) / bn;
-  t.units = (p.n_kb + 1) / 2;
-  if ((long long)t.row_tiles * t.token_tiles > 2147483647ll) return fail(MLORA_ESIZE, "q4_linear: too many tiles");
-  const int grid = q4_ctas((long long)t.row_tiles * t.token_tiles * t.units);
-  return bn == 32 ? launch_tc_for<32>(t, grid, st) : bn == 64 ? launch_tc_for<64>(t, grid, st) : launch_tc_for<128>(t, grid, st);
+  float* delta = p.a.u ? (float*)((uint8_t*)work + q4_base_bytes()) : nullptr;
+  const int slice = p.a.u ? kSlice : p.a.T;
+  for (int t0 = 0; t0 < p.a.T; t0 += slice) {
+    t.p = p;
+    LinearArgs& a = t.p.a;
+    a.T = p.a.T - t0 < slice ? p.a.T - t0 : slice;
+    a.x += (size_t)t0 * a.ldx;
+    a.y = (uint8_t*)a.y + (size_t)t0 * a.ldy * (a.flags & MLORA_OUT_F32 ? 4 : 2);
+    if (a.u) {
+      a.u += (size_t)t0 * a.r_max * a.n_mod;
+      a.slots += t0;
+      q4_expand_kernel<<<dim3((unsigned)((a.out + kExThreads - 1) / kExThreads), (unsigned)((a.T + kExRows - 1) / kExRows)), kExThreads, 0, st>>>(t.p, delta);
+      count_launch();
+      MLORA_CHECK_LAUNCH("q4_expand_kernel");
+      t.delta = delta;
+    }
+    const int bn = rows_per_tile(a.T);
+    t.row_tiles = (a.out + kQ4Tile - 1) / kQ4Tile;
+    t.token_tiles = (a.T + bn - 1) / bn;
+    t.units = (p.n_kb + 1) / 2;
+    const long long all = (long long)t.row_tiles * t.token_tiles * t.units;
+    if (all > 2147483647ll) return fail(MLORA_ESIZE, "q4_linear: too many tiles");
+    const int grid = q4_ctas(all);
+    const int rc = bn == 32 ? launch_tc_for<32>(t, grid, st) : bn == 64 ? launch_tc_for<64>(t, grid, st) : launch_tc_for<128>(t, grid, st);
+    if (rc) return rc;
+  }
+  return MLORA_OK;
 }
 
 }  // namespace mlora
