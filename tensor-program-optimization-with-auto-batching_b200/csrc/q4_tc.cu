@@ -19,19 +19,23 @@
 namespace mlora {
 namespace {
 
-constexpr int kBufs = 4;                 // units of weights in TMEM, and of x in shared memory
-constexpr int kSlots = 4;                // units whose scales lie in shared memory
+constexpr int kBufs = 4;                 // units of weights in TMEM
+constexpr int kSlots = 12;               // units whose scales lie in shared memory
 constexpr int kMaxCtas = 512;
 constexpr int kHeader = 256;             // bytes: status word, then the caller's
-constexpr int kScaleBytes = 4 * 512;     // scales of a unit's groups, at most
 constexpr int kSlice = 512;              // rows whose adapters' share lies in scratch at a time
 // Warps: weight warpgroups, then those that sum and write (32 columns of BN 32 and 64 each, 64 of 128), then MMA issue, copies of x,
 // copies of weights.
 constexpr int q4_weight_groups(int bn) { return bn == 32 ? 3 : 2; }
 constexpr int q4_out_warps(int bn) { return bn == 32 ? 4 : 8; }
 constexpr int q4_threads(int bn) { return 32 * (4 * q4_weight_groups(bn) + q4_out_warps(bn) + 3); }
-constexpr int q4_ring(int bn) { return bn == 128 ? 6 : 12; }  // packed units in shared memory
-constexpr int q4_slot_bytes(bool zero) { return 2 * kQ4TileBytes + (zero ? kScaleBytes : 0); }  // with zero points: and their groups' scales
+constexpr int q4_ring(int bn) { return bn == 32 ? 10 : bn == 64 ? 8 : 6; }  // packed units in shared memory
+constexpr int q4_x_ring(int bn) { return bn == 32 ? 8 : bn == 64 ? 6 : 4; }  // units of x (from L2, 1 us away)
+constexpr int q4_scale_bytes(bool zero, int g) { return 128 / g * kQ4Tile * (zero ? 4 : 2); }  // of a unit's groups
+constexpr int q4_slot_bytes(bool zero, int g) { return 2 * kQ4TileBytes + (zero ? q4_scale_bytes(zero, g) : 0); }
+constexpr int q4_smem(int bn, bool zero, int g) {
+  return 1024 + q4_x_ring(bn) * bn * 256 + q4_ring(bn) * q4_slot_bytes(zero, g) + kSlots * q4_scale_bytes(zero, g);
+}
 
 struct TcArgs {
   Q4Args p;
@@ -97,12 +101,12 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
   constexpr int kCols = BN * 4 / kWarpsOut;               // columns of a thread that sums
   constexpr int kSums = 128 / G;                          // groups of a unit
   constexpr int kEntry = ZERO ? 4 : 2;
-  constexpr int kWslots = q4_ring(BN), kSlotBytes = q4_slot_bytes(ZERO);
+  constexpr int kWslots = q4_ring(BN), kXslots = q4_x_ring(BN), kSlotBytes = q4_slot_bytes(ZERO, G), kScaleBytes = q4_scale_bytes(ZERO, G);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sx = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint8_t* sw = sx + kBufs * BN * 256;                    // [slot][kSlotBytes]
+  uint8_t* sw = sx + kXslots * BN * 256;                  // [slot][kSlotBytes]
   uint8_t* ss = sw + kWslots * kSlotBytes;                // [slot][kScaleBytes]
-  __shared__ uint64_t w_full[kWslots], w_empty[kWslots], x_full[kBufs], a_full[kBufs], empty[kBufs], d_full[kDbufs], d_empty[kDbufs],
+  __shared__ uint64_t w_full[kWslots], w_empty[kWslots], x_full[kXslots], x_empty[kXslots], a_full[kBufs], empty[kBufs], d_full[kDbufs], d_empty[kDbufs],
       s_full[kSlots], s_empty[kSlots];
   __shared__ uint32_t tmem_slot;
   __shared__ int s_abort;
@@ -113,7 +117,8 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
   if (tid == 0) {
     s_abort = 0;
     for (int i = 0; i < kWslots; ++i) mbar_init(&w_full[i], 1), mbar_init(&w_empty[i], 4);
-    for (int i = 0; i < kBufs; ++i) mbar_init(&x_full[i], 1), mbar_init(&a_full[i], 4), mbar_init(&empty[i], 1);
+    for (int i = 0; i < kXslots; ++i) mbar_init(&x_full[i], 1), mbar_init(&x_empty[i], 1);
+    for (int i = 0; i < kBufs; ++i) mbar_init(&a_full[i], 4), mbar_init(&empty[i], 1);
     for (int i = 0; i < kSlots; ++i) mbar_init(&s_full[i], 1), mbar_init(&s_empty[i], kWarpsOut);
     for (int i = 0; i < kDbufs; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], kWarpsOut);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -335,15 +340,15 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
       constexpr uint32_t idesc = make_idesc(kQ4Tile, BN);
       if (elect_one()) {  // (one thread: every instruction it spends per unit bounds the rate)
         const uint64_t b0 = make_smem_desc(smem_u32(sx));
-        const uint32_t a_full0 = smem_u32(a_full), x_full0 = smem_u32(x_full), empty0 = smem_u32(empty), d_full0 = smem_u32(d_full),
+        const uint32_t a_full0 = smem_u32(a_full), x_full0 = smem_u32(x_full), empty0 = smem_u32(empty), x_empty0 = smem_u32(x_empty), d_full0 = smem_u32(d_full),
                        d_empty0 = smem_u32(d_empty);
-        uint32_t buf = 0, par = 0, d = 0, d_par = 1;
+        uint32_t buf = 0, par = 0, x = 0, x_par = 0, d = 0, d_par = 1;
         bool ok = true;
         for (Cursor c(t, u_begin, u_end); c.left > 0 && ok; c.next()) {
           const int steps = min(8, (n_kb - 2 * c.u) * 4);  // of 16 inputs
-          ok = mbar_wait_a(a_full0 + 8 * buf, par, abort) && mbar_wait_a(x_full0 + 8 * buf, par, abort);
+          ok = mbar_wait_a(a_full0 + 8 * buf, par, abort) && mbar_wait_a(x_full0 + 8 * x, x_par, abort);
           if (!ok) break;
-          const uint64_t bdesc = b0 + (uint64_t)(buf * (BN * 256 >> 4));
+          const uint64_t bdesc = b0 + (uint64_t)(x * (BN * 256 >> 4));
           const uint32_t a_tmem = tmem_a + buf * 64;
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
@@ -362,60 +367,55 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
           }
           if (!ok) break;
           umma_commit_a(empty0 + 8 * buf);
+          umma_commit_a(x_empty0 + 8 * x);
           if (++buf == kBufs) buf = 0, par ^= 1;
+          if (++x == kXslots) x = 0, x_par ^= 1;
         }
         if (!ok) s_abort = 1;
       }
       __syncwarp();
     } else if (warp == kMma + 1) {
-      // ---- rows of x, and the scales ------------------------------------------------------------------------------------------------
-      pdl_wait();
-      int seq = 0;
-      for (Cursor c(t, u_begin, u_end); c.left > 0; c.next(), ++seq) {
-        const int slot = seq % kBufs, s_slot = seq % kSlots;
-        int good = 1;
-        if (lane == 0) {
-          good = mbar_wait(&empty[slot], ((seq / kBufs) & 1) ^ 1, abort);
-          if (good) {
-            const int blocks = min(2, n_kb - 2 * c.u);
-            mbar_expect_tx(&x_full[slot], blocks * BN * 128);
-            for (int b = 0; b < blocks; ++b)
-              tma_load_2d(sx + (slot * 2 + b) * BN * 128, &map_x, (2 * c.u + b) * kQ4Block, c.token_tile * BN, &x_full[slot]);
-            good = mbar_wait(&s_empty[s_slot], ((seq / kSlots) & 1) ^ 1, abort);
+      // ---- rows of x -----------------------------------------------------------------------------------------------------------------
+      if (lane == 0) {
+        pdl_wait();
+        int seq = 0;
+        for (Cursor c(t, u_begin, u_end); c.left > 0; c.next(), ++seq) {
+          const int slot = seq % kXslots, blocks = min(2, n_kb - 2 * c.u);
+          if (!mbar_wait(&x_empty[slot], ((seq / kXslots) & 1) ^ 1, abort)) {
+            s_abort = 1;
+            break;
           }
-          if (good) {
-            const int g = c.u * kSums, bytes = min(kSums, t.p.n_groups - g) * kQ4Tile * kEntry;
-            mbar_expect_tx(&s_full[s_slot], bytes);
-            bulk_load(ss + s_slot * kScaleBytes, t.p.table + ((size_t)c.row_tile * t.p.n_groups + g) * kQ4Tile * kEntry, bytes, &s_full[s_slot]);
-          }
+          mbar_expect_tx(&x_full[slot], blocks * BN * 128);
+          for (int b = 0; b < blocks; ++b)
+            tma_load_2d(sx + (slot * 2 + b) * BN * 128, &map_x, (2 * c.u + b) * kQ4Block, c.token_tile * BN, &x_full[slot]);
         }
-        good = __shfl_sync(0xffffffffu, good, 0);
-        if (!good) {
-          s_abort = 1;
-          break;
-        }
+        // commits arrive at these barriers until the last unit's: nobody leaves before
+        for (int k = max(seq - kXslots, 0); k < seq && !*abort; ++k)
+          if (!mbar_wait(&x_empty[k % kXslots], (k / kXslots) & 1, abort)) s_abort = 1;
+        for (int k = max(seq - kBufs, 0); k < seq && !*abort; ++k)
+          if (!mbar_wait(&empty[k % kBufs], (k / kBufs) & 1, abort)) s_abort = 1;
+        if (*abort)  // copies may still be in flight: let them land before the shared memory goes to another CTA
+          for (int i = 0; i < 64; ++i) __nanosleep(1000);
       }
-      // commits arrive at these barriers until the last block's: nobody leaves before
-      for (int k = max(seq - kBufs, 0); k < seq && !*abort; ++k)
-        if (!__all_sync(0xffffffffu, mbar_wait(&empty[k % kBufs], (k / kBufs) & 1, abort))) s_abort = 1;
-      if (*abort && lane == 0)  // copies may still be in flight: let them land before the shared memory goes to another CTA
-        for (int i = 0; i < 64; ++i) __nanosleep(1000);
     } else if (lane == 0) {
       // ---- packed weights: a unit's 8 KB lie one after the other, and so do its groups' scales (no earlier kernel of a step writes
       // either, so the copies need not wait for it) --------------------------------------------------------------------------------
       const uint8_t* weights = reinterpret_cast<const uint8_t*>(a.W);
       int seq = 0;
       for (Cursor c(t, u_begin, u_end); c.left > 0; c.next(), ++seq) {
-        const int slot = seq % kWslots;
-        if (!mbar_wait(&w_empty[slot], ((seq / kWslots) & 1) ^ 1, abort)) {
+        const int slot = seq % kWslots, s_slot = seq % kSlots;
+        if (!mbar_wait(&w_empty[slot], ((seq / kWslots) & 1) ^ 1, abort) || !mbar_wait(&s_empty[s_slot], ((seq / kSlots) & 1) ^ 1, abort)) {
           s_abort = 1;
           break;
         }
-        const int blocks = min(2, n_kb - 2 * c.u), g = c.u * kSums, n_g = min(kSums, t.p.n_groups - g);
-        mbar_expect_tx(&w_full[slot], blocks * kQ4TileBytes + (ZERO ? n_g * 512 : 0));
+        const int blocks = min(2, n_kb - 2 * c.u), g = c.u * kSums, n_g = min(kSums, t.p.n_groups - g), bytes = n_g * kQ4Tile * kEntry;
+        const uint8_t* table = t.p.table + ((size_t)c.row_tile * t.p.n_groups + g) * kQ4Tile * kEntry;
+        mbar_expect_tx(&w_full[slot], blocks * kQ4TileBytes + (ZERO ? bytes : 0));
         bulk_load(sw + slot * kSlotBytes, weights + ((size_t)c.row_tile * n_kb + 2 * c.u) * kQ4TileBytes, blocks * kQ4TileBytes, &w_full[slot]);
         if (ZERO)
-          bulk_load(sw + slot * kSlotBytes + 2 * kQ4TileBytes, t.p.table + ((size_t)c.row_tile * t.p.n_groups + g) * 512, n_g * 512, &w_full[slot]);
+          bulk_load(sw + slot * kSlotBytes + 2 * kQ4TileBytes, table, bytes, &w_full[slot]);
+        mbar_expect_tx(&s_full[s_slot], bytes);
+        bulk_load(ss + s_slot * kScaleBytes, table, bytes, &s_full[s_slot]);
       }
       if (*abort)
         for (int i = 0; i < 64; ++i) __nanosleep(1000);
@@ -486,7 +486,7 @@ int launch_tc_as(const TcArgs& t, int grid, cudaStream_t st) {
   CUtensorMap mx;
   const int rc = make_map(&mx, t.p.a.x, t.p.a.T, t.p.a.in, t.p.a.ldx, BN, kQ4Block);
   if (rc) return rc;
-  constexpr int smem = 1024 + kBufs * BN * 256 + q4_ring(BN) * q4_slot_bytes(ZERO) + kSlots * kScaleBytes;
+  constexpr int smem = q4_smem(BN, ZERO, G);
   static std::atomic<unsigned long long> done{0};
   int dev = 0;
   cudaGetDevice(&dev);
