@@ -1,13 +1,5 @@
-// 4-bit weights: quantising, packing, and the projection kernel of the smallest batches (see q4.cuh for the layout).
-//
-// Up to 16 rows: y = x W^T is bound by the weights' out in / 2 bytes.  A CTA owns 16 U outputs; its eight warps take the blocks of 64
-// inputs in turn, each with a ring of asynchronous copies of its own (weights, the rows of x, scales), multiply with mma.m16n8k16 --
-// weights as the 16-row operand, up to 8 or 16 rows of x as the 8-column one: at these sizes the legacy tensor path is a tenth busy, and
-// unlike a tcgen05 tile it needs neither 128 outputs per CTA nor a trip of the weights through TMEM -- and are added up at the end.
+// 4-bit weights: quantising, packing, and the entry point of their projections (see q4.cuh for the layout).
 #include "q4.cuh"
-#include "tc_ptx.cuh"
-
-#include <atomic>
 
 namespace mlora {
 namespace {
@@ -72,186 +64,72 @@ __global__ void q4_table_kernel(const bf16* __restrict__ scale, const uint8_t* _
   reinterpret_cast<__nv_bfloat162*>(table)[i] = __nv_bfloat162(s, z);
 }
 
-// ---- up to 16 rows ----------------------------------------------------------------------------------------------------------------
-constexpr int kQrWarps = 8, kQrThreads = kQrWarps * 32;
+// delta[t, o] = scale[slot] sum_j u[t, j] B[slot][o][j]: a thread per output, eight rows at a time; rows that follow each other with the
+// same adapter read its row once (up to 64 ranks wide).
+constexpr int kExThreads = 128, kExRows = 8, kExMaxU = 512;
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {  // the rest of the 16 becomes zeros
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// U: parts of 16 outputs of a CTA; N8: rows of x in eights; ZERO: zero points; SUB: groups of 32 (two in a block)
-template <int U, int N8, bool ZERO, bool SUB>
-struct Q4Ring {
-  static constexpr int kScaleBytes = ZERO ? 4 : 2, kSubs = SUB ? 2 : 1;
-  static constexpr int kX = U * 512, kS = kX + N8 * 1024, kStage = kS + kSubs * U * 16 * kScaleBytes;
-  static constexpr int kStages = U * N8 >= 4 ? 6 : 8;
-  static constexpr int kBytes = kQrWarps * kStages * kStage;
-  static_assert(kBytes >= kQrWarps * U * 16 * N8 * 8 * 4, "the warps' sums lie in the ring");
-};
-
-template <int U, int N8, bool ZERO, bool SUB>
-__global__ void __launch_bounds__(kQrThreads) q4_rows_kernel(Q4Args p) {
-  using R = Q4Ring<U, N8, ZERO, SUB>;
-  constexpr int kStages = R::kStages;
-  extern __shared__ __align__(128) uint8_t ring[];
+__global__ void __launch_bounds__(kExThreads) q4_expand_kernel(Q4Args p, float* __restrict__ delta) {
+  __shared__ __align__(16) float su[kExRows][kExMaxU];
+  __shared__ int s_slot[kExRows];
   pdl_launch_dependents();
+  pdl_wait();
   const LinearArgs& a = p.a;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int tile = blockIdx.x / (8 / U), part0 = blockIdx.x % (8 / U) * U;
-  const uint8_t* weights = reinterpret_cast<const uint8_t*>(a.W) + (size_t)tile * p.n_kb * kQ4TileBytes + part0 * 512 + lane * 16;
-  const uint8_t* scales = p.table + ((size_t)tile * p.n_groups * kQ4Tile + part0 * 16) * R::kScaleBytes;
-  const uint32_t base = smem_u32(ring) + warp * kStages * R::kStage;
-  pdl_wait();  // (before the first asynchronous copy of x)
-  auto fetch = [&](int i) {
-    const int kb = warp + i * kQrWarps;
-    if (kb < p.n_kb) {
-      const uint32_t st = base + (i % kStages) * R::kStage;
-#pragma unroll
-      for (int u = 0; u < U; ++u) cp16(st + u * 512 + lane * 16, weights + (size_t)kb * kQ4TileBytes + u * 512, 16);
-#pragma unroll
-      for (int c = 0; c < 2 * N8; ++c) {  // rows of 128 bytes, 16-byte pieces XORed with the row
-        const int t = c * 4 + (lane >> 3), ch = lane & 7, k = kb * kQ4Block + ch * 8;
-        const bool in_range = t < a.T && k < a.in;
-        cp16(st + R::kX + t * 128 + ((ch ^ (t & 7)) << 4), in_range ? a.x + (size_t)t * a.ldx + k : a.x, in_range ? 16 : 0);
-      }
-      constexpr int per = U * R::kScaleBytes;  // 16-byte pieces of a group's scales: U * 16 of them
-      if (lane < R::kSubs * per) {
-        const int g = min(SUB ? 2 * kb + lane / per : kb * kQ4Block / p.group, p.n_groups - 1);
-        cp16(st + R::kS + lane * 16, scales + (size_t)g * (kQ4Tile * R::kScaleBytes) + lane % per * 16, 16);
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) fetch(i);
-  float acc[U][N8][4];
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-#pragma unroll
-    for (int n = 0; n < N8; ++n) acc[u][n][0] = acc[u][n][1] = acc[u][n][2] = acc[u][n][3] = 0.f;
-  const int g = lane >> 2;
-  for (int i = 0; warp + i * kQrWarps < p.n_kb; ++i) {
-    fetch(i + kStages - 1);
-    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-    __syncwarp();
-    const uint32_t st = base + (i % kStages) * R::kStage;
-    const uint8_t* sp = ring + (st - smem_u32(ring));
-    uint32_t b[N8][2][4];  // rows 8 n .. of x: inputs 32 h .. 32 h + 31
-#pragma unroll
-    for (int n = 0; n < N8; ++n)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) ldmatrix4(st + R::kX + n * 1024 + (lane & 7) * 128 + (((h * 4 + (lane >> 3)) ^ (lane & 7)) << 4), b[n][h]);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint4 w4 = *reinterpret_cast<const uint4*>(sp + u * 512 + lane * 16);
-      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-      float sum[N8][4];
-      float s0 = 0.f, s1 = 0.f;
-      uint32_t z0 = kQ4Middle, z1 = kQ4Middle;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (j == 0 || (SUB && j == 2)) {  // a group begins
-          const uint8_t* e = sp + R::kS + ((SUB ? j / 2 : 0) * U * 16 + u * 16 + g) * R::kScaleBytes;
-          if constexpr (ZERO) {
-            const uint32_t e0 = *reinterpret_cast<const uint32_t*>(e), e1 = *reinterpret_cast<const uint32_t*>(e + 8 * 4);
-            s0 = __uint_as_float(e0 << 16), s1 = __uint_as_float(e1 << 16);
-            z0 = __byte_perm(e0, e0, 0x3232), z1 = __byte_perm(e1, e1, 0x3232);
-          } else {
-            s0 = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(e) << 16);
-            s1 = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(e + 8 * 2) << 16);
-          }
-#pragma unroll
-          for (int n = 0; n < N8; ++n) sum[n][0] = sum[n][1] = sum[n][2] = sum[n][3] = 0.f;
-        }
-        uint32_t r[4];
-        q4_expand(w[j], z0, z1, r);
-#pragma unroll
-        for (int n = 0; n < N8; ++n) mma_bf16(sum[n], r, b[n][j >> 1][(j & 1) * 2], b[n][j >> 1][(j & 1) * 2 + 1]);
-        if (j == 3 || (SUB && j == 1)) {
-#pragma unroll
-          for (int n = 0; n < N8; ++n) {
-            acc[u][n][0] = fmaf(s0, sum[n][0], acc[u][n][0]), acc[u][n][1] = fmaf(s0, sum[n][1], acc[u][n][1]);
-            acc[u][n][2] = fmaf(s1, sum[n][2], acc[u][n][2]), acc[u][n][3] = fmaf(s1, sum[n][3], acc[u][n][3]);
-          }
-        }
-      }
-    }
-    __syncwarp();  // (the next copy overwrites what was read here)
-  }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  const int o = blockIdx.x * kExThreads + threadIdx.x, t0 = blockIdx.y * kExRows, rows = min(kExRows, a.T - t0), width = a.r_max * a.n_mod;
+  if (threadIdx.x < kExRows) s_slot[threadIdx.x] = (int)threadIdx.x < rows ? a.slots[t0 + threadIdx.x] : -1;
+  const bool fits = width <= kExMaxU;
+  for (int i = threadIdx.x; fits && i < rows * width; i += kExThreads) su[i / width][i % width] = a.u[(size_t)t0 * width + i];
   __syncthreads();
-  // ---- the warps' sums: [warp][row of x][16 U outputs] -----------------------------------------------------------------------------
-  constexpr int kO = U * 16, kN = N8 * 8;
-  float* part = reinterpret_cast<float*>(ring);
+  if (o >= a.out) return;
+  const int module = module_of(a, o) * a.r_max, n8 = a.r_max / 8;
+  uint4 b[8];
+  int have = -1, sw;
+  float alpha = 0.f;
+#pragma unroll 1
+  for (int r = 0; r < rows; ++r) {
+    const int s = s_slot[r];
+    float sum = 0.f;
+    if (s >= 0 && s < a.n_adapters) {
+      const float* u = fits ? &su[r][module] : a.u + (size_t)(t0 + r) * width + module;
+      if (s != have) {
 #pragma unroll
-  for (int u = 0; u < U; ++u)
+        for (int j = 0; j < 8; ++j)
+          if (j < n8) b[j] = ld_cached(q4_b_row(a, p.packed_b, s, o, j, sw));
+        alpha = a.scales[s];
+        have = s;
+      }
 #pragma unroll
-    for (int n = 0; n < N8; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        part[(warp * kN + n * 8 + (lane & 3) * 2 + (e & 1)) * kO + u * 16 + g + (e >> 1) * 8] = acc[u][n][e];
-  __syncthreads();
-  const int o0 = tile * kQ4Tile + part0 * 16;
-  const auto total = [&](int t, int c) {
-    float s = 0.f;
-#pragma unroll
-    for (int w = 0; w < kQrWarps; ++w) s += part[(w * kN + t) * kO + c];
-    return o0 + c < a.out ? s + q4_adapter(a, p.packed_b, t, o0 + c) : 0.f;
-  };
-  if (a.flags & MLORA_SILU_MUL) {
-    for (int i = tid; i < a.T * (kO / 2); i += kQrThreads) {
-      const int t = i / (kO / 2), c = i % (kO / 2), at = (c >> 3) * 16 + (c & 7);  // (8 gate outputs, then their 8 up outputs)
-      if (o0 + at < a.out) store_out(a, t, o0 / 2 + c, silu_mul(total(t, at), total(t, at + 8)));
+      for (int j = 0; j < 8; ++j)
+        if (j < n8) sum += dot8(b[j], u + 8 * j);
+      for (int j = 8; j < n8; ++j) sum += dot8(ld_cached(q4_b_row(a, p.packed_b, s, o, j, sw)), u + 8 * j);
+      sum *= alpha;
     }
-  } else {
-    const int act = a.flags & (MLORA_ACT_RELU2 | MLORA_ACT_GELU);
-    for (int i = tid; i < a.T * kO; i += kQrThreads) {
-      const int t = i / kO, c = i % kO;
-      if (o0 + c < a.out) store_out(a, t, o0 + c, act_one(total(t, c), act));
-    }
+    delta[(size_t)(t0 + r) * a.out + o] = sum;
   }
-}
-
-template <int U, int N8, bool ZERO, bool SUB>
-int launch_rows_as(const Q4Args& p, cudaStream_t st) {
-  using R = Q4Ring<U, N8, ZERO, SUB>;
-  static std::atomic<unsigned long long> done{0};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (!((done.load(std::memory_order_acquire) >> (dev & 63)) & 1ull)) {
-    const cudaError_t e = cudaFuncSetAttribute(q4_rows_kernel<U, N8, ZERO, SUB>, cudaFuncAttributeMaxDynamicSharedMemorySize, R::kBytes);
-    if (e != cudaSuccess) return fail(MLORA_ECUDA, "q4_linear: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-    done.fetch_or(1ull << (dev & 63), std::memory_order_release);
-  }
-  const unsigned grid = (unsigned)((p.a.out + 16 * U - 1) / (16 * U));
-  const cudaError_t e = launch_pdl_if(pdl_enabled_gemm(), q4_rows_kernel<U, N8, ZERO, SUB>, dim3(grid), dim3(kQrThreads), R::kBytes, st, p);
-  if (e != cudaSuccess) return fail(MLORA_ECUDA, "q4_rows_kernel: %s", cudaGetErrorString(e));
-  count_launch();
-  MLORA_CHECK_LAUNCH("q4_rows_kernel");
-  return MLORA_OK;
-}
-template <int U, int N8>
-int launch_rows_for(const Q4Args& p, bool zero, cudaStream_t st) {
-  if (p.group == 32) return zero ? launch_rows_as<U, N8, true, true>(p, st) : launch_rows_as<U, N8, false, true>(p, st);
-  return zero ? launch_rows_as<U, N8, true, false>(p, st) : launch_rows_as<U, N8, false, false>(p, st);
 }
 
 }  // namespace
 
-int launch_q4_rows(const Q4Args& p, cudaStream_t st) {
-  const bool zero = (p.a.flags & MLORA_Q4_ZEROS) != 0;
-  // More outputs per CTA read the rows of x fewer times, as long as there are a few CTAs for every SM.
-  const int parts = (p.a.out + 15) / 16;
-  if (p.a.T <= 8) return parts >= 4 * 4 * 148 ? launch_rows_for<4, 1>(p, zero, st) : parts >= 2 * 4 * 148 ? launch_rows_for<2, 1>(p, zero, st) : launch_rows_for<1, 1>(p, zero, st);
-  return parts >= 4 * 2 * 148 ? launch_rows_for<4, 2>(p, zero, st) : parts >= 2 * 2 * 148 ? launch_rows_for<2, 2>(p, zero, st) : launch_rows_for<1, 2>(p, zero, st);
+int launch_q4_expand(const Q4Args& p, float* delta, cudaStream_t st) {
+  const dim3 grid((unsigned)((p.a.out + kExThreads - 1) / kExThreads), (unsigned)((p.a.T + kExRows - 1) / kExRows));
+  q4_expand_kernel<<<grid, kExThreads, 0, st>>>(p, delta);
+  count_launch();
+  MLORA_CHECK_LAUNCH("q4_expand_kernel");
+  return MLORA_OK;
+}
+
+int q4_ctas(long long units) {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    n = 148;
+  }
+  n = n < kQ4MaxCtas ? n : kQ4MaxCtas;
+  return (int)(units < n ? units : n);
+}
+
+// Counters and shares lie at places that no call's sizes move; behind them the adapters' share of a slice of rows.
+size_t q4_workspace(int T, int out) {
+  return kQ4Header + kQ4MaxCtas * 4 + (size_t)q4_ctas(kQ4MaxCtas) * 128 * kQ4Tile * 4 + (size_t)(T < kQ4Slice ? T : kQ4Slice) * out * 4;
 }
 
 }  // namespace mlora
@@ -297,7 +175,7 @@ extern "C" int mlora_q4_pack(const void* d_q, const void* d_scale, const void* d
 }
 
 extern "C" size_t mlora_q4_linear_workspace(int32_t T, int32_t in, int32_t out) {
-  return T <= 0 || in <= 0 || out <= 0 || T <= kQ4RowsMost ? 0 : q4_tc_workspace(T, in, out);
+  return T <= 0 || in <= 0 || out <= 0 ? 0 : q4_workspace(T, out);
 }
 
 extern "C" int mlora_q4_linear(const void* d_x, int64_t ldx, const void* d_Wq, int32_t group, void* d_y, int64_t ldy, int32_t T, int32_t in,
@@ -329,6 +207,27 @@ extern "C" int mlora_q4_linear(const void* d_x, int64_t ldx, const void* d_Wq, i
   }
   p.group = group, p.n_groups = in / group, p.n_kb = (in + kQ4Block - 1) / kQ4Block, p.packed_b = (flags & MLORA_B_PACKED) != 0;
   p.table = (const uint8_t*)d_Wq + q4_weight_bytes(out, in);
-  if (T <= kQ4RowsMost) return launch_q4_rows(p, (cudaStream_t)stream);
-  return launch_q4_tc(p, d_work, work_bytes, (cudaStream_t)stream);
+  const size_t need = q4_workspace(T, out);
+  if (!d_work || work_bytes < need) return fail(MLORA_ESIZE, "q4_linear: scratch of %zu bytes needed, %zu given", need, work_bytes);
+  MLORA_REQUIRE(aligned16(d_work), "q4_linear: the scratch must be 16-byte aligned");
+  Q4Work w{(int32_t*)d_work, (int32_t*)((uint8_t*)d_work + kQ4Header), (float*)((uint8_t*)d_work + kQ4Header + kQ4MaxCtas * 4), nullptr};
+  float* delta = (float*)((uint8_t*)d_work + q4_workspace(0, 0));
+  const cudaStream_t st = (cudaStream_t)stream;
+  const int slice = lora ? kQ4Slice : T;
+  for (int t0 = 0; t0 < T; t0 += slice) {
+    Q4Args s = p;
+    s.a.T = T - t0 < slice ? T - t0 : slice;
+    s.a.x += (size_t)t0 * ldx;
+    s.a.y = (uint8_t*)d_y + (size_t)t0 * ldy * (flags & MLORA_OUT_F32 ? 4 : 2);
+    if (lora) {
+      s.a.u += (size_t)t0 * a.r_max * a.n_mod;
+      s.a.slots += t0;
+      w.delta = delta;
+      const int rc = launch_q4_expand(s, delta, st);
+      if (rc) return rc;
+    }
+    const int rc = s.a.T <= kQ4SmallRows ? launch_q4_mm(s, w, st) : launch_q4_tc(s, w, st);
+    if (rc) return rc;
+  }
+  return MLORA_OK;
 }

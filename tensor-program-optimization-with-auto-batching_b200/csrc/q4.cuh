@@ -74,9 +74,28 @@ __device__ __forceinline__ float q4_adapter(const LinearArgs& a, int packed, int
   return a.scales[s] * sum;
 }
 
-int launch_q4_rows(const Q4Args& a, cudaStream_t st);
-size_t q4_tc_workspace(int T, int in, int out);
-int launch_q4_tc(const Q4Args& a, void* work, size_t work_bytes, cudaStream_t st);
-constexpr int kQ4RowsMost = 16;  // rows that launch_q4_rows takes
+// Scratch of a projection: the status word (and the caller's bytes), a counter and a share of 128 x 128 sums per CTA, and the adapters'
+// share of a slice of rows.
+constexpr int kQ4MaxCtas = 512, kQ4Header = 256, kQ4Slice = 512;
+struct Q4Work {
+  int32_t* status;
+  int32_t* counters;   // [CTA that a tile begins in]: shares of the tile that have arrived, zero between calls
+  float* parts;        // [CTA][128 x 128]: sums of a CTA's share of a tile that another CTA begins
+  const float* delta;  // [rows][out]: the adapters' share, or NULL
+};
+size_t q4_workspace(int T, int out);
+int q4_ctas(long long units);  // CTAs of a persistent launch over so many units: one per SM at most
+int launch_q4_expand(const Q4Args& p, float* delta, cudaStream_t st);
+int launch_q4_mm(const Q4Args& p, const Q4Work& w, cudaStream_t st);
+int launch_q4_tc(const Q4Args& p, const Q4Work& w, cudaStream_t st);
+constexpr int kQ4SmallRows = 64;  // rows that launch_q4_mm is for
+
+// Which CTAs of `ctas` share the units [begin, begin + n) of `all`, dealt out in equal ranges.
+__device__ __forceinline__ int q4_cta_of(long long unit, long long all, int ctas) {
+  int k = (int)(unit * ctas / all);
+  while (all * (k + 1) / ctas <= unit) ++k;
+  while (all * k / ctas > unit) --k;
+  return k;
+}
 
 }  // namespace mlora

@@ -1,0 +1,328 @@
+// Projections with 4-bit weights for up to 64 rows (see q4.cuh for the layout): y = x W^T is bound by the weights' out in / 2 bytes, and on
+// the way there by the integer pipe, which takes 14 cycles for the eight weights of a word -- 224 per 8 KB and SM sub-core, against the
+// 350 in which HBM delivers them.  So nothing else may cost much: weights go from bulk copies in shared memory to registers and from
+// there, as the A operand, straight into mma.m16n8k16, whose fragments the packed order has; the legacy tensor path is a third busy at 32
+// rows.  (A tcgen05 form of this kernel needs the weights in TMEM, four kinds of barriers per block and a trip of every group's sums
+// through registers: 567 instructions per sub-core and 8 KB, 30 us at 32 rows x 4096 x 22016 against XX here.)
+//
+// A CTA's tile is 128 outputs x 8, 16 or 32 rows; stages of 256 inputs -- 16 KB of weights, their scales, the rows of x -- arrive by bulk and
+// TMA copies.  Sixteen warps: four ranges of 32 outputs x four blocks of 64 inputs.  Persistent, one CTA per SM, the stages of all tiles
+// dealt out in equal ranges; a tile that several CTAs share is finished by the one that begins it, from the sums that the others have
+// left in scratch -- the first thing each of them does.
+#include "q4.cuh"
+#include "tc_ptx.cuh"
+
+#include <atomic>
+
+namespace mlora {
+namespace {
+
+constexpr int kMmWarps = 16, kMmThreads = 32 * (kMmWarps + 1);  // and one warp for the copies
+constexpr int kMmBlocks = 4;                                    // of 64 inputs per stage
+constexpr int kMmPitch = 132;                                   // floats between rows of x in the sums
+
+struct MmArgs {
+  Q4Args p;
+  Q4Work w;
+  int row_tiles, token_tiles, units;  // stages per tile
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_more(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// One verdict of the 512 threads that multiply; see bar_all.
+__device__ __forceinline__ bool mm_all(bool ok) {
+  uint32_t r;
+  __syncwarp();
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.aligned.pred q, 1, 512, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)ok)
+      : "memory");
+  return r != 0;
+}
+
+// N8: rows of x in eights; ZERO: zero points; G: inputs per group
+template <int N8, bool ZERO, int G>
+struct MmStage {
+  static constexpr int kEntry = ZERO ? 4 : 2, kGroups = 256 / G;
+  static constexpr int kW = kMmBlocks * kQ4TileBytes, kX = kMmBlocks * N8 * 1024, kS = kGroups * kQ4Tile * kEntry;
+  static constexpr int kBytes = (kW + kX + kS + 1023) / 1024 * 1024;  // (x is swizzled: 1024-byte places)
+  static constexpr int kSums = 4 * N8 * 8 * kMmPitch * 4;  // of the four blocks' warps
+  static constexpr int kStages = (227 * 1024 - 1024 - 512 - kSums) / kBytes < 8 ? (227 * 1024 - 1024 - 512 - kSums) / kBytes : 8;
+  static constexpr int kSmem = 1024 + kStages * kBytes + kSums;
+};
+
+template <int N8, bool ZERO, int G>
+__global__ void __launch_bounds__(kMmThreads, 1) q4_mm_kernel(const __grid_constant__ CUtensorMap map_x, MmArgs t) {
+  using S = MmStage<N8, ZERO, G>;
+  constexpr int kStages = S::kStages, kEntry = S::kEntry;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);  // [stage][x | W | scales]
+  float* sums = reinterpret_cast<float*>(ring + kStages * S::kBytes);                                            // [block][row of x][kMmPitch]
+  __shared__ uint64_t full[kStages], empty[kStages];
+  __shared__ int s_abort;
+
+  pdl_launch_dependents();
+  const LinearArgs& a = t.p.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    s_abort = 0;
+    for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], kMmWarps);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    tma_prefetch_desc(&map_x);
+  }
+  __syncthreads();
+  const long long all = (long long)t.row_tiles * t.token_tiles * t.units;
+  const long long u_begin = all * blockIdx.x / gridDim.x, u_end = all * (blockIdx.x + 1) / gridDim.x;
+  const int n_kb = t.p.n_kb, left = (int)(u_end - u_begin);
+  volatile int* abort = &s_abort;
+  int tile = (int)(u_begin / t.units), u = (int)(u_begin % t.units);  // of the unit at work
+
+  if (warp == kMmWarps) {
+    // ---- copies --------------------------------------------------------------------------------------------------------------------
+    if (lane == 0) {
+      const uint8_t* weights = reinterpret_cast<const uint8_t*>(a.W);
+      int row_tile = tile % t.row_tiles, token = tile / t.row_tiles * (N8 * 8);
+      const auto copy_x = [&](int slot, int at, int at_token) {
+        const int blocks = min(kMmBlocks, n_kb - at * kMmBlocks);
+        for (int b = 0; b < blocks; ++b)
+          tma_load_2d(ring + slot * S::kBytes + b * N8 * 1024, &map_x, (at * kMmBlocks + b) * kQ4Block, at_token, &full[slot]);
+      };
+      const auto copy_w = [&](int slot) {
+        const int blocks = min(kMmBlocks, n_kb - u * kMmBlocks), g = u * S::kGroups, bytes = min(S::kGroups, t.p.n_groups - g) * kQ4Tile * kEntry;
+        uint8_t* dst = ring + slot * S::kBytes + S::kX;
+        mbar_expect_tx(&full[slot], blocks * (kQ4TileBytes + N8 * 1024) + bytes);
+        bulk_load(dst, weights + ((size_t)row_tile * n_kb + u * kMmBlocks) * kQ4TileBytes, blocks * kQ4TileBytes, &full[slot]);
+        bulk_load(dst + S::kW, t.p.table + ((size_t)row_tile * t.p.n_groups + g) * kQ4Tile * kEntry, bytes, &full[slot]);
+      };
+      const auto next = [&] {
+        if (++u < t.units) return;
+        u = 0;
+        if (++row_tile == t.row_tiles) row_tile = 0, token += N8 * 8;
+      };
+      // the first stages' weights and scales, which no earlier kernel of a step writes; then, behind that kernel, their rows of x
+      const int u0 = u, row0 = row_tile, token0 = token, ahead = min(left, kStages);
+      for (int i = 0; i < ahead; ++i, next()) copy_w(i);
+      const int u1 = u, row1 = row_tile, token1 = token;
+      pdl_wait();
+      u = u0, row_tile = row0, token = token0;
+      for (int i = 0; i < ahead; ++i, next()) copy_x(i, u, token);
+      u = u1, row_tile = row1, token = token1;
+      for (int i = ahead; i < left; ++i, next()) {
+        const int slot = i % kStages;
+        if (!mbar_wait(&empty[slot], ((i / kStages) & 1) ^ 1, abort)) {
+          s_abort = 1;
+          break;
+        }
+        copy_w(slot);
+        copy_x(slot, u, token);
+      }
+      if (*abort)  // copies may still be in flight: let them land before the shared memory goes to another CTA
+        for (int i = 0; i < 64; ++i) __nanosleep(1000);
+    }
+  } else {
+    // ---- products --------------------------------------------------------------------------------------------------------------------
+    const int quarter = warp >> 2, block = warp & 3, g = lane >> 2;
+    float acc[2][N8][4];
+    const auto clear = [&] {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int n = 0; n < N8; ++n) acc[h][n][0] = acc[h][n][1] = acc[h][n][2] = acc[h][n][3] = 0.f;
+    };
+    clear();
+    bool ok = true, waited = false;
+    for (int i = 0; i < left;) {
+      const int seg = min(left - i, t.units - u);  // stages of this tile
+      const int u_first = u;
+      for (int e = i + seg; i < e; ++i, ++u) {
+        const int slot = i % kStages;
+        ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], (i / kStages) & 1, abort));
+        if (!ok) break;
+        if (u * kMmBlocks + block < n_kb) {
+          const uint8_t* st = ring + slot * S::kBytes;
+          const uint32_t sx = smem_u32(st) + block * N8 * 1024 + (lane & 7) * 128;
+          const uint8_t* sw = st + S::kX + block * kQ4TileBytes + quarter * 1024 + lane * 16;
+          const uint8_t* ss = st + S::kX + S::kW + (quarter * 32 + g) * kEntry;
+          uint4 w4[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) w4[h] = *reinterpret_cast<const uint4*>(sw + h * 512);
+          uint32_t b[N8][2][4];  // rows 8 n .. of x: inputs 32 h .. 32 h + 31 of the block
+#pragma unroll
+          for (int n = 0; n < N8; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) ldmatrix4(sx + n * 1024 + (((h * 4 + (lane >> 3)) ^ (lane & 7)) << 4), b[n][h]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t w[4] = {w4[h].x, w4[h].y, w4[h].z, w4[h].w};
+            float sum[N8][4], s0 = 0.f, s1 = 0.f;
+            uint32_t z0 = kQ4Middle, z1 = kQ4Middle;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              constexpr int kWords = G == 32 ? 2 : 4;  // of a group in this block
+              if (j % kWords == 0) {
+                // (inputs that end inside a block: its second group is not there, and x is 0)
+                const int group = G == 32 ? min(block * 2 + j / 2, t.p.n_groups - u * S::kGroups - 1) : G == 64 ? block : block / 2;
+                const uint8_t* e = ss + (group * kQ4Tile + h * 16) * kEntry;
+                if constexpr (ZERO) {
+                  const uint32_t e0 = *reinterpret_cast<const uint32_t*>(e), e1 = *reinterpret_cast<const uint32_t*>(e + 8 * 4);
+                  s0 = __uint_as_float(e0 << 16), s1 = __uint_as_float(e1 << 16);
+                  z0 = __byte_perm(e0, e0, 0x3232), z1 = __byte_perm(e1, e1, 0x3232);
+                } else {
+                  s0 = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(e) << 16);
+                  s1 = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(e + 8 * 2) << 16);
+                }
+              }
+              uint32_t r[4];
+              q4_expand(w[j], z0, z1, r);
+#pragma unroll
+              for (int n = 0; n < N8; ++n) {
+                if (j % kWords == 0)
+                  mma_first(sum[n], r, b[n][j >> 1][(j & 1) * 2], b[n][j >> 1][(j & 1) * 2 + 1]);
+                else
+                  mma_more(sum[n], r, b[n][j >> 1][(j & 1) * 2], b[n][j >> 1][(j & 1) * 2 + 1]);
+              }
+              if (j % kWords == kWords - 1) {
+#pragma unroll
+                for (int n = 0; n < N8; ++n) {
+                  acc[h][n][0] = fmaf(s0, sum[n][0], acc[h][n][0]), acc[h][n][1] = fmaf(s0, sum[n][1], acc[h][n][1]);
+                  acc[h][n][2] = fmaf(s1, sum[n][2], acc[h][n][2]), acc[h][n][3] = fmaf(s1, sum[n][3], acc[h][n][3]);
+                }
+              }
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[slot]);
+      }
+      ok = mm_all(ok);  // (also: the sums before have been read)
+      if (!ok) break;
+      // ---- the segment is done: the four blocks' sums, then output, or a share of a tile that another CTA finishes -----------------
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int n = 0; n < N8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            sums[(block * N8 * 8 + n * 8 + (lane & 3) * 2 + (e & 1)) * kMmPitch + quarter * 32 + h * 16 + (e >> 1) * 8 + g] = acc[h][n][e];
+      clear();
+      if (!waited) {
+        pdl_wait();  // (scratch and outputs belong to earlier kernels until here)
+        waited = true;
+      }
+      mm_all(true);
+      const long long tile_begin = (long long)tile * t.units;
+      const int row0 = tile % t.row_tiles * kQ4Tile, token0 = tile / t.row_tiles * (N8 * 8), n_tok = min(N8 * 8, a.T - token0);
+      const auto total = [&](int tok, int c) {
+        const float* s = sums + tok * kMmPitch + c;
+        return (s[0] + s[N8 * 8 * kMmPitch]) + (s[2 * N8 * 8 * kMmPitch] + s[3 * N8 * 8 * kMmPitch]);
+      };
+      if (u_first != 0) {
+        float* mine = t.w.parts + (size_t)blockIdx.x * (kQ4Tile * kQ4Tile);
+        const int first = q4_cta_of(tile_begin, all, gridDim.x);
+        for (int k = tid; k < n_tok * kQ4Tile; k += 512) __stcg(mine + k, total(k >> 7, k & 127));
+        mm_all(true);
+        if (tid == 0) {
+          __threadfence();
+          atomicAdd(&t.w.counters[first], 1);
+        }
+      } else {
+        int last = blockIdx.x;
+        if (u != t.units) {  // others have a part: each of them writes it before anything else
+          last = q4_cta_of(tile_begin + t.units - 1, all, gridDim.x);
+          if (tid == 0) {
+            ok = false;
+            for (uint32_t k = 0; k < kSpinLimit && !ok; ++k) {
+              int have;
+              asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(have) : "l"(&t.w.counters[blockIdx.x]) : "memory");
+              ok = have >= last - (int)blockIdx.x;
+              if (!ok) __nanosleep(64);
+              if ((k & 255) == 255 && *abort) break;
+            }
+            t.w.counters[blockIdx.x] = 0;
+          }
+          ok = mm_all(ok);
+          if (!ok) break;
+        }
+        const auto value = [&](int tok, int c) {
+          float v = total(tok, c);
+          for (int k = blockIdx.x + 1; k <= last; ++k) v += __ldcg(t.w.parts + (size_t)k * (kQ4Tile * kQ4Tile) + tok * kQ4Tile + c);
+          return t.w.delta != nullptr && row0 + c < a.out ? v + __ldcg(t.w.delta + (size_t)(token0 + tok) * a.out + row0 + c) : v;
+        };
+        if (a.flags & MLORA_SILU_MUL) {
+          for (int k = tid; k < n_tok * (kQ4Tile / 2); k += 512) {
+            const int tok = k >> 6, c = k & 63, at = (c >> 3) * 16 + (c & 7);  // (8 gate outputs, then their 8 up outputs)
+            if (row0 + at < a.out) store_out(a, token0 + tok, row0 / 2 + c, silu_mul(value(tok, at), value(tok, at + 8)));
+          }
+        } else {
+          const int act = a.flags & (MLORA_ACT_RELU2 | MLORA_ACT_GELU);
+          for (int k = tid; k < n_tok * kQ4Tile; k += 512) {
+            const int tok = k >> 7, c = k & 127;
+            if (row0 + c < a.out) store_out(a, token0 + tok, row0 + c, act_one(value(tok, c), act));
+          }
+        }
+      }
+      if (u == t.units) u = 0, ++tile;
+    }
+    if (!ok) s_abort = 1;
+  }
+  __syncthreads();
+  if (tid == 0 && s_abort) atomicOr(t.w.status, 2);
+}
+
+template <int N8, bool ZERO, int G>
+int launch_mm_as(const MmArgs& t, int grid, cudaStream_t st) {
+  CUtensorMap mx;
+  const int rc = make_map(&mx, t.p.a.x, t.p.a.T, t.p.a.in, t.p.a.ldx, N8 * 8, kQ4Block);
+  if (rc) return rc;
+  constexpr int smem = MmStage<N8, ZERO, G>::kSmem;
+  static std::atomic<unsigned long long> done{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!((done.load(std::memory_order_acquire) >> (dev & 63)) & 1ull)) {
+    const cudaError_t e = cudaFuncSetAttribute(q4_mm_kernel<N8, ZERO, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return fail(MLORA_ECUDA, "q4_linear: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    done.fetch_or(1ull << (dev & 63), std::memory_order_release);
+  }
+  const cudaError_t e = launch_pdl_if(pdl_enabled_gemm(), q4_mm_kernel<N8, ZERO, G>, dim3((unsigned)grid), dim3(kMmThreads), smem, st, mx, t);
+  if (e != cudaSuccess) return fail(MLORA_ECUDA, "q4_mm_kernel: %s", cudaGetErrorString(e));
+  count_launch();
+  MLORA_CHECK_LAUNCH("q4_mm_kernel");
+  return MLORA_OK;
+}
+template <int N8>
+int launch_mm_for(const MmArgs& t, int grid, cudaStream_t st) {
+  const bool zero = (t.p.a.flags & MLORA_Q4_ZEROS) != 0;
+  switch (t.p.group) {
+    case 32: return zero ? launch_mm_as<N8, true, 32>(t, grid, st) : launch_mm_as<N8, false, 32>(t, grid, st);
+    case 64: return zero ? launch_mm_as<N8, true, 64>(t, grid, st) : launch_mm_as<N8, false, 64>(t, grid, st);
+    default: return zero ? launch_mm_as<N8, true, 128>(t, grid, st) : launch_mm_as<N8, false, 128>(t, grid, st);
+  }
+}
+
+}  // namespace
+
+int launch_q4_mm(const Q4Args& p, const Q4Work& w, cudaStream_t st) {
+  const int n8 = p.a.T <= 8 ? 1 : p.a.T <= 16 ? 2 : 4;
+  MmArgs t{p, w, (p.a.out + kQ4Tile - 1) / kQ4Tile, (p.a.T + n8 * 8 - 1) / (n8 * 8), (p.n_kb + kMmBlocks - 1) / kMmBlocks};
+  const long long all = (long long)t.row_tiles * t.token_tiles * t.units;
+  if (all > 2147483647ll) return fail(MLORA_ESIZE, "q4_linear: too many tiles");
+  const int grid = q4_ctas(all);
+  return n8 == 1 ? launch_mm_for<1>(t, grid, st) : n8 == 2 ? launch_mm_for<2>(t, grid, st) : launch_mm_for<4>(t, grid, st);
+}
+
+}  // namespace mlora

@@ -21,9 +21,6 @@ namespace {
 
 constexpr int kBufs = 4;                 // units of weights in TMEM
 constexpr int kSlots = 12;               // units whose scales lie in shared memory
-constexpr int kMaxCtas = 512;
-constexpr int kHeader = 256;             // bytes: status word, then the caller's
-constexpr int kSlice = 512;              // rows whose adapters' share lies in scratch at a time
 // Warps: weight warpgroups, then those that sum and write (32 columns of BN 32 and 64 each, 64 of 128), then MMA issue, copies of x,
 // copies of weights.
 constexpr int q4_weight_groups(int bn) { return bn == 32 ? 3 : 2; }
@@ -247,13 +244,7 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
       const bool begins = seg_begin == tile_begin, whole = begins && seg_end == tile_begin + t.units;
       int first = blockIdx.x, last = blockIdx.x;  // CTAs whose ranges hold the tile's first and last unit
       if (!whole) {
-        const auto cta_of = [&](long long x) {
-          int k = (int)(x * gridDim.x / all);
-          while (all * (k + 1) / gridDim.x <= x) ++k;
-          while (all * k / gridDim.x > x) --k;
-          return k;
-        };
-        first = cta_of(tile_begin), last = cta_of(tile_begin + t.units - 1);
+        first = q4_cta_of(tile_begin, all, gridDim.x), last = q4_cta_of(tile_begin + t.units - 1, all, gridDim.x);
       }
       if (!begins) {
         float* mine = t.parts + (size_t)blockIdx.x * (BN * kQ4Tile) + col0 * kQ4Tile + row;
@@ -345,7 +336,7 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
         uint32_t buf = 0, par = 0, x = 0, x_par = 0, d = 0, d_par = 1;
         bool ok = true;
         for (Cursor c(t, u_begin, u_end); c.left > 0 && ok; c.next()) {
-          const int steps = min(8, (n_kb - 2 * c.u) * 4);  // of 16 inputs
+          const int steps = min(8, (a.in - c.u * 128) / 16);  // of 16 inputs (a group that is not there has no accumulator)
           ok = mbar_wait_a(a_full0 + 8 * buf, par, abort) && mbar_wait_a(x_full0 + 8 * x, x_par, abort);
           if (!ok) break;
           const uint64_t bdesc = b0 + (uint64_t)(x * (BN * 256 >> 4));
@@ -427,59 +418,7 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
   if (warp == kMma) tmem_dealloc(tmem_slot, 512);
 }
 
-// delta[t, o] = scale[slot] sum_j u[t, j] B[slot][o][j]: a thread per output, eight rows at a time; rows that follow each other with the
-// same adapter read its row once (up to 64 ranks wide).
-constexpr int kExThreads = 128, kExRows = 8, kExMaxU = 512;
-
-__global__ void __launch_bounds__(kExThreads) q4_expand_kernel(Q4Args p, float* __restrict__ delta) {
-  __shared__ __align__(16) float su[kExRows][kExMaxU];
-  __shared__ int s_slot[kExRows];
-  pdl_launch_dependents();
-  pdl_wait();
-  const LinearArgs& a = p.a;
-  const int o = blockIdx.x * kExThreads + threadIdx.x, t0 = blockIdx.y * kExRows, rows = min(kExRows, a.T - t0), width = a.r_max * a.n_mod;
-  if (threadIdx.x < kExRows) s_slot[threadIdx.x] = (int)threadIdx.x < rows ? a.slots[t0 + threadIdx.x] : -1;
-  const bool fits = width <= kExMaxU;
-  for (int i = threadIdx.x; fits && i < rows * width; i += kExThreads) su[i / width][i % width] = a.u[(size_t)t0 * width + i];
-  __syncthreads();
-  if (o >= a.out) return;
-  const int module = module_of(a, o) * a.r_max, n8 = a.r_max / 8;
-  uint4 b[8];
-  int have = -1, sw;
-  float alpha = 0.f;
-#pragma unroll 1
-  for (int r = 0; r < rows; ++r) {
-    const int s = s_slot[r];
-    float sum = 0.f;
-    if (s >= 0 && s < a.n_adapters) {
-      const float* u = fits ? &su[r][module] : a.u + (size_t)(t0 + r) * width + module;
-      if (s != have) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (j < n8) b[j] = ld_cached(q4_b_row(a, p.packed_b, s, o, j, sw));
-        alpha = a.scales[s];
-        have = s;
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < n8) sum += dot8(b[j], u + 8 * j);
-      for (int j = 8; j < n8; ++j) sum += dot8(ld_cached(q4_b_row(a, p.packed_b, s, o, j, sw)), u + 8 * j);
-      sum *= alpha;
-    }
-    delta[(size_t)(t0 + r) * a.out + o] = sum;
-  }
-}
-
-int q4_ctas(long long units) {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
-    cudaGetLastError();
-    n = 148;
-  }
-  n = n < kMaxCtas ? n : kMaxCtas;
-  return (int)(units < n ? units : n);
-}
-int rows_per_tile(int T) { return T <= 32 ? 32 : T <= 64 ? 64 : 128; }
+int rows_per_tile(int T) { return T <= 64 ? 64 : 128; }
 
 template <int BN, bool ZERO, int G>
 int launch_tc_as(const TcArgs& t, int grid, cudaStream_t st) {
@@ -513,49 +452,17 @@ int launch_tc_for(const TcArgs& t, int grid, cudaStream_t st) {
 
 }  // namespace
 
-size_t q4_base_bytes() { return kHeader + kMaxCtas * 4 + (size_t)q4_ctas(kMaxCtas) * 128 * kQ4Tile * 4; }
-
-size_t q4_tc_workspace(int T, int in, int out) {
-  // (counters and shares at places that no call's sizes move, then the adapters' share of a slice of rows)
-  (void)in;
-  return q4_base_bytes() + (size_t)(T < kSlice ? T : kSlice) * out * 4;
-}
-
-int launch_q4_tc(const Q4Args& p, void* work, size_t work_bytes, cudaStream_t st) {
-  const size_t need = q4_tc_workspace(p.a.T, p.a.in, p.a.out);
-  if (!work || work_bytes < need) return fail(MLORA_ESIZE, "q4_linear: scratch of %zu bytes needed, %zu given", need, work_bytes);
-  if (!aligned16(work)) return fail(MLORA_EINVAL, "q4_linear: the scratch must be 16-byte aligned");
+int launch_q4_tc(const Q4Args& p, const Q4Work& w, cudaStream_t st) {
   TcArgs t{};
-  t.status = (int32_t*)work;
-  t.counters = (int32_t*)((uint8_t*)work + kHeader);
-  t.parts = (float*)((uint8_t*)work + kHeader + kMaxCtas * 4);
-  float* delta = p.a.u ? (float*)((uint8_t*)work + q4_base_bytes()) : nullptr;
-  const int slice = p.a.u ? kSlice : p.a.T;
-  for (int t0 = 0; t0 < p.a.T; t0 += slice) {
-    t.p = p;
-    LinearArgs& a = t.p.a;
-    a.T = p.a.T - t0 < slice ? p.a.T - t0 : slice;
-    a.x += (size_t)t0 * a.ldx;
-    a.y = (uint8_t*)a.y + (size_t)t0 * a.ldy * (a.flags & MLORA_OUT_F32 ? 4 : 2);
-    if (a.u) {
-      a.u += (size_t)t0 * a.r_max * a.n_mod;
-      a.slots += t0;
-      q4_expand_kernel<<<dim3((unsigned)((a.out + kExThreads - 1) / kExThreads), (unsigned)((a.T + kExRows - 1) / kExRows)), kExThreads, 0, st>>>(t.p, delta);
-      count_launch();
-      MLORA_CHECK_LAUNCH("q4_expand_kernel");
-      t.delta = delta;
-    }
-    const int bn = rows_per_tile(a.T);
-    t.row_tiles = (a.out + kQ4Tile - 1) / kQ4Tile;
-    t.token_tiles = (a.T + bn - 1) / bn;
-    t.units = (p.n_kb + 1) / 2;
-    const long long all = (long long)t.row_tiles * t.token_tiles * t.units;
-    if (all > 2147483647ll) return fail(MLORA_ESIZE, "q4_linear: too many tiles");
-    const int grid = q4_ctas(all);
-    const int rc = bn == 32 ? launch_tc_for<32>(t, grid, st) : bn == 64 ? launch_tc_for<64>(t, grid, st) : launch_tc_for<128>(t, grid, st);
-    if (rc) return rc;
-  }
-  return MLORA_OK;
+  t.p = p, t.status = w.status, t.counters = w.counters, t.parts = w.parts, t.delta = w.delta;
+  const int bn = rows_per_tile(p.a.T);
+  t.row_tiles = (p.a.out + kQ4Tile - 1) / kQ4Tile;
+  t.token_tiles = (p.a.T + bn - 1) / bn;
+  t.units = (p.n_kb + 1) / 2;
+  const long long all = (long long)t.row_tiles * t.token_tiles * t.units;
+  if (all > 2147483647ll) return fail(MLORA_ESIZE, "q4_linear: too many tiles");
+  const int grid = q4_ctas(all);
+  return bn == 64 ? launch_tc_for<64>(t, grid, st) : launch_tc_for<128>(t, grid, st);
 }
 
 }  // namespace mlora

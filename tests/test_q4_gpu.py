@@ -39,7 +39,8 @@ def _packed(ops, q, s, z, group, cuda):
 CASES = [  # rows, in, out
     (1, 32, 1), (1, 4096, 4096), (2, 96, 500), (3, 160, 130), (5, 11008, 257), (8, 512, 16), (9, 544, 48), (16, 4096, 2100), (13, 352, 9500),
     (17, 32, 1), (17, 4096, 128), (31, 96, 300), (33, 2080, 1000), (64, 512, 4096), (65, 160, 130), (101, 5120, 1100), (128, 96, 129), (129, 544, 260),
-    (300, 1024, 513), (40, 11008, 130)]
+    (300, 1024, 513), (40, 11008, 130),
+    (5, 96, 60000), (33, 160, 40000), (70, 96, 60000), (130, 160, 20001)]  # (inputs that end inside a block, many tiles per CTA)
 
 
 @pytest.mark.parametrize("T,K,N", CASES)
