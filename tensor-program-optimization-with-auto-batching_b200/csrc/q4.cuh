@@ -90,6 +90,8 @@ int launch_q4_mm(const Q4Args& p, const Q4Work& w, cudaStream_t st);
 int launch_q4_tc(const Q4Args& p, const Q4Work& w, cudaStream_t st);
 constexpr int kQ4SmallRows = 64;  // rows that launch_q4_mm is for
 
+__device__ __noinline__ static float q4_act(float v, int act) { return act_one(v, act); }  // (one copy of erf, not one per value)
+
 // Which CTAs of `ctas` share the units [begin, begin + n) of `all`, dealt out in equal ranges.
 __device__ __forceinline__ int q4_cta_of(long long unit, long long all, int ctas) {
   int k = (int)(unit * ctas / all);

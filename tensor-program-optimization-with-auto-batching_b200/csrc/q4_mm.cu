@@ -31,12 +31,12 @@ __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void mma_more(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -226,24 +226,37 @@ __global__ void __launch_bounds__(kMmThreads, 1) q4_mm_kernel(const __grid_const
       }
       mm_all(true);
       const long long tile_begin = (long long)tile * t.units;
-      const int row0 = tile % t.row_tiles * kQ4Tile, token0 = tile / t.row_tiles * (N8 * 8), n_tok = min(N8 * 8, a.T - token0);
-      const auto total = [&](int tok, int c) {
-        const float* s = sums + tok * kMmPitch + c;
-        return (s[0] + s[N8 * 8 * kMmPitch]) + (s[2 * N8 * 8 * kMmPitch] + s[3 * N8 * 8 * kMmPitch]);
-      };
+      const int row0 = tile % t.row_tiles * kQ4Tile, token0 = tile / t.row_tiles * (N8 * 8), n_tok = a.T - token0;
+      // a thread: one output of every fourth row of x
+      constexpr int kMine = N8 * 2;
+      const int c = tid & 127, tok0 = tid >> 7;
+      float v[kMine];
+#pragma unroll
+      for (int k = 0; k < kMine; ++k) {
+        const float* s = sums + (tok0 + 4 * k) * kMmPitch + c;
+        v[k] = (s[0] + s[N8 * 8 * kMmPitch]) + (s[2 * N8 * 8 * kMmPitch] + s[3 * N8 * 8 * kMmPitch]);
+      }
       if (u_first != 0) {
-        float* mine = t.w.parts + (size_t)blockIdx.x * (kQ4Tile * kQ4Tile);
-        const int first = q4_cta_of(tile_begin, all, gridDim.x);
-        for (int k = tid; k < n_tok * kQ4Tile; k += 512) __stcg(mine + k, total(k >> 7, k & 127));
+        float* mine = t.w.parts + (size_t)blockIdx.x * (kQ4Tile * kQ4Tile) + tok0 * kQ4Tile + c;
+#pragma unroll
+        for (int k = 0; k < kMine; ++k) __stcg(mine + 4 * k * kQ4Tile, v[k]);
         mm_all(true);
         if (tid == 0) {
           __threadfence();
-          atomicAdd(&t.w.counters[first], 1);
+          atomicAdd(&t.w.counters[q4_cta_of(tile_begin, all, gridDim.x)], 1);
         }
       } else {
-        int last = blockIdx.x;
+        const int o = row0 + c;
+        const bool there = o < a.out;
+        if (t.w.delta != nullptr) {
+          float add[kMine];
+#pragma unroll
+          for (int k = 0; k < kMine; ++k) add[k] = there && tok0 + 4 * k < n_tok ? __ldcg(t.w.delta + (size_t)(token0 + tok0 + 4 * k) * a.out + o) : 0.f;
+#pragma unroll
+          for (int k = 0; k < kMine; ++k) v[k] += add[k];
+        }
         if (u != t.units) {  // others have a part: each of them writes it before anything else
-          last = q4_cta_of(tile_begin + t.units - 1, all, gridDim.x);
+          const int last = q4_cta_of(tile_begin + t.units - 1, all, gridDim.x);
           if (tid == 0) {
             ok = false;
             for (uint32_t k = 0; k < kSpinLimit && !ok; ++k) {
@@ -257,23 +270,26 @@ __global__ void __launch_bounds__(kMmThreads, 1) q4_mm_kernel(const __grid_const
           }
           ok = mm_all(ok);
           if (!ok) break;
+#pragma unroll 1
+          for (int part = blockIdx.x + 1; part <= last; ++part) {
+            const float* from = t.w.parts + (size_t)part * (kQ4Tile * kQ4Tile) + tok0 * kQ4Tile + c;
+#pragma unroll
+            for (int k = 0; k < kMine; ++k) v[k] += __ldcg(from + 4 * k * kQ4Tile);
+          }
         }
-        const auto value = [&](int tok, int c) {
-          float v = total(tok, c);
-          for (int k = blockIdx.x + 1; k <= last; ++k) v += __ldcg(t.w.parts + (size_t)k * (kQ4Tile * kQ4Tile) + tok * kQ4Tile + c);
-          return t.w.delta != nullptr && row0 + c < a.out ? v + __ldcg(t.w.delta + (size_t)(token0 + tok) * a.out + row0 + c) : v;
-        };
-        if (a.flags & MLORA_SILU_MUL) {
-          for (int k = tid; k < n_tok * (kQ4Tile / 2); k += 512) {
-            const int tok = k >> 6, c = k & 63, at = (c >> 3) * 16 + (c & 7);  // (8 gate outputs, then their 8 up outputs)
-            if (row0 + at < a.out) store_out(a, token0 + tok, row0 / 2 + c, silu_mul(value(tok, at), value(tok, at + 8)));
-          }
-        } else {
-          const int act = a.flags & (MLORA_ACT_RELU2 | MLORA_ACT_GELU);
-          for (int k = tid; k < n_tok * kQ4Tile; k += 512) {
-            const int tok = k >> 7, c = k & 127;
-            if (row0 + c < a.out) store_out(a, token0 + tok, row0 + c, act_one(value(tok, c), act));
-          }
+        const bool silu = (a.flags & MLORA_SILU_MUL) != 0;
+        const int act = a.flags & (MLORA_ACT_RELU2 | MLORA_ACT_GELU), col = silu ? o / 16 * 8 + (o & 7) : o;
+        if (silu) {
+#pragma unroll
+          for (int k = 0; k < kMine; ++k) v[k] = silu_mul(v[k], __shfl_xor_sync(0xffffffffu, v[k], 8));  // (8 gate outputs, then their 8 up outputs)
+        } else if (act) {
+#pragma unroll
+          for (int k = 0; k < kMine; ++k) v[k] = q4_act(v[k], act);
+        }
+        if (there && (!silu || !(c & 8))) {
+#pragma unroll
+          for (int k = 0; k < kMine; ++k)
+            if (tok0 + 4 * k < n_tok) store_out(a, token0 + tok0 + 4 * k, col, v[k]);
         }
       }
       if (u == t.units) u = 0, ++tile;

@@ -63,7 +63,6 @@ __device__ __forceinline__ void out_sync() {
   __syncwarp();
   asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory");
 }
-__device__ __noinline__ float act_apart(float v, int act) { return act_one(v, act); }  // (one copy of erf, not one per column)
 
 // 16 lanes x 32 columns from registers laid out as A operands of mma.m16n8k16
 __device__ __forceinline__ void tmem_st_16x128b_x8(uint32_t addr, const uint32_t (&r)[16]) {
@@ -303,7 +302,7 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
             for (int i = 0; i < 16; ++i) v[i] = silu_mul(v[i], __shfl_xor_sync(0xffffffffu, v[i], 8));  // (8 gate outputs, then their 8 up outputs)
           } else if (act) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = act_apart(v[i], act);
+            for (int i = 0; i < 16; ++i) v[i] = q4_act(v[i], act);
           }
           if (mine) {
             const size_t at = (size_t)(token0 + c0) * a.ldy + col;
