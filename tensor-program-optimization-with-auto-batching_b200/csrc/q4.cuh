@@ -84,11 +84,11 @@ struct Q4Work {
   const float* delta;  // [rows][out]: the adapters' share, or NULL
 };
 size_t q4_workspace(int T, int out);
-int q4_ctas(long long units);  // CTAs of a persistent launch over so many units: one per SM at most
+int q4_ctas(long long tiles, int units);  // CTAs of a persistent launch over tiles of so many units
 int launch_q4_expand(const Q4Args& p, float* delta, cudaStream_t st);
 int launch_q4_mm(const Q4Args& p, const Q4Work& w, cudaStream_t st);
 int launch_q4_tc(const Q4Args& p, const Q4Work& w, cudaStream_t st);
-constexpr int kQ4SmallRows = 64;  // rows that launch_q4_mm is for
+constexpr int kQ4SmallRows = 16;  // rows that launch_q4_mm is for
 
 __device__ __noinline__ static float q4_act(float v, int act) { return act_one(v, act); }  // (one copy of erf, not one per value)
 

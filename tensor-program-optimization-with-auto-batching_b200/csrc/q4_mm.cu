@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) q4_mm_kernel(const __grid_const
           }
           ok = mm_all(ok);
           if (!ok) break;
-#pragma unroll 1
+#pragma unroll 4
           for (int part = blockIdx.x + 1; part <= last; ++part) {
             const float* from = t.w.parts + (size_t)part * (kQ4Tile * kQ4Tile) + tok0 * kQ4Tile + c;
 #pragma unroll
@@ -337,7 +337,7 @@ int launch_q4_mm(const Q4Args& p, const Q4Work& w, cudaStream_t st) {
   MmArgs t{p, w, (p.a.out + kQ4Tile - 1) / kQ4Tile, (p.a.T + n8 * 8 - 1) / (n8 * 8), (p.n_kb + kMmBlocks - 1) / kMmBlocks};
   const long long all = (long long)t.row_tiles * t.token_tiles * t.units;
   if (all > 2147483647ll) return fail(MLORA_ESIZE, "q4_linear: too many tiles");
-  const int grid = q4_ctas(all);
+  const int grid = q4_ctas(t.row_tiles * (long long)t.token_tiles, t.units);
   return n8 == 1 ? launch_mm_for<1>(t, grid, st) : n8 == 2 ? launch_mm_for<2>(t, grid, st) : launch_mm_for<4>(t, grid, st);
 }
 

@@ -19,19 +19,21 @@
 namespace mlora {
 namespace {
 
-constexpr int kBufs = 4;                 // units of weights in TMEM
-constexpr int kSlots = 12;               // units whose scales lie in shared memory
 // Warps: weight warpgroups, then those that sum and write (32 columns of BN 32 and 64 each, 64 of 128), then MMA issue, copies of x,
 // copies of weights.
 constexpr int q4_weight_groups(int bn) { return bn == 32 ? 3 : 2; }
 constexpr int q4_out_warps(int bn) { return bn == 32 ? 4 : 8; }
 constexpr int q4_threads(int bn) { return 32 * (4 * q4_weight_groups(bn) + q4_out_warps(bn) + 3); }
 constexpr int q4_ring(int bn) { return bn == 32 ? 10 : bn == 64 ? 8 : 6; }  // packed units in shared memory
-constexpr int q4_x_ring(int bn) { return bn == 32 ? 8 : bn == 64 ? 6 : 4; }  // units of x (from L2, 1 us away)
+constexpr int q4_bufs(int bn) { return bn == 128 ? 4 : 6; }  // units of weights in TMEM, and of x in shared memory (from L2, 1 us away)
+// Units whose scales lie in shared memory.  A slot is filled again without asking: copies are at most q4_bufs units ahead of the MMAs,
+// which are at most as many accumulators (q4_sums, one or more a unit) ahead of the warps that read scales.
+constexpr int q4_sums(int bn) { return bn == 32 ? 4 : 2; }
+constexpr int q4_scale_slots(int bn) { return q4_bufs(bn) + q4_sums(bn) + 1; }
 constexpr int q4_scale_bytes(bool zero, int g) { return 128 / g * kQ4Tile * (zero ? 4 : 2); }  // of a unit's groups
 constexpr int q4_slot_bytes(bool zero, int g) { return 2 * kQ4TileBytes + (zero ? q4_scale_bytes(zero, g) : 0); }
 constexpr int q4_smem(int bn, bool zero, int g) {
-  return 1024 + q4_x_ring(bn) * bn * 256 + q4_ring(bn) * q4_slot_bytes(zero, g) + kSlots * q4_scale_bytes(zero, g);
+  return 1024 + q4_bufs(bn) * bn * 256 + q4_ring(bn) * q4_slot_bytes(zero, g) + q4_scale_slots(bn) * q4_scale_bytes(zero, g);
 }
 
 struct TcArgs {
@@ -57,6 +59,25 @@ __device__ __forceinline__ bool out_all(bool ok) {
       : "r"((uint32_t)ok), "n"(N)
       : "memory");
   return r != 0;
+}
+__device__ __forceinline__ void tmem_ld32_issue(uint32_t taddr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,"
+      "%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+// (the registers go through the wait, so that nothing that reads them is scheduled before it)
+template <int N>
+__device__ __forceinline__ void tmem_wait_ld_all(float* v) {
+#pragma unroll
+  for (int i = 0; i < N; i += 16) tmem_wait_ld16(v + i);
 }
 template <int N>
 __device__ __forceinline__ void out_sync() {
@@ -91,19 +112,18 @@ struct Cursor {
 
 template <int BN, bool ZERO, int G>
 __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_constant__ CUtensorMap map_x, TcArgs t) {
-  constexpr int kDbufs = BN == 128 ? 2 : 4;
+  constexpr int kDbufs = q4_sums(BN), kSlots = q4_scale_slots(BN);
   constexpr int kGroups = q4_weight_groups(BN), kWarpsOut = q4_out_warps(BN);
   constexpr int kOut = 4 * kGroups, kMma = kOut + kWarpsOut;  // first warps of these roles
   constexpr int kCols = BN * 4 / kWarpsOut;               // columns of a thread that sums
   constexpr int kSums = 128 / G;                          // groups of a unit
   constexpr int kEntry = ZERO ? 4 : 2;
-  constexpr int kWslots = q4_ring(BN), kXslots = q4_x_ring(BN), kSlotBytes = q4_slot_bytes(ZERO, G), kScaleBytes = q4_scale_bytes(ZERO, G);
+  constexpr int kWslots = q4_ring(BN), kBufs = q4_bufs(BN), kSlotBytes = q4_slot_bytes(ZERO, G), kScaleBytes = q4_scale_bytes(ZERO, G);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sx = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint8_t* sw = sx + kXslots * BN * 256;                  // [slot][kSlotBytes]
+  uint8_t* sw = sx + kBufs * BN * 256;                  // [slot][kSlotBytes]
   uint8_t* ss = sw + kWslots * kSlotBytes;                // [slot][kScaleBytes]
-  __shared__ uint64_t w_full[kWslots], w_empty[kWslots], x_full[kXslots], x_empty[kXslots], a_full[kBufs], empty[kBufs], d_full[kDbufs], d_empty[kDbufs],
-      s_full[kSlots], s_empty[kSlots];
+  __shared__ uint64_t w_full[kWslots], w_empty[kWslots], full[kBufs], empty[kBufs], d_full[kDbufs], d_empty[kDbufs];
   __shared__ uint32_t tmem_slot;
   __shared__ int s_abort;
 
@@ -113,9 +133,7 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
   if (tid == 0) {
     s_abort = 0;
     for (int i = 0; i < kWslots; ++i) mbar_init(&w_full[i], 1), mbar_init(&w_empty[i], 4);
-    for (int i = 0; i < kXslots; ++i) mbar_init(&x_full[i], 1), mbar_init(&x_empty[i], 1);
-    for (int i = 0; i < kBufs; ++i) mbar_init(&a_full[i], 4), mbar_init(&empty[i], 1);
-    for (int i = 0; i < kSlots; ++i) mbar_init(&s_full[i], 1), mbar_init(&s_empty[i], kWarpsOut);
+    for (int i = 0; i < kBufs; ++i) mbar_init(&full[i], 4 + 1), mbar_init(&empty[i], 1);  // (four weight warps, and the copies of x)
     for (int i = 0; i < kDbufs; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], kWarpsOut);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     tma_prefetch_desc(&map_x);
@@ -139,7 +157,7 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&a_full[told]);
+      if (lane == 0) mbar_arrive(&full[told]);
       __syncwarp();
     };
     for (int seq = wg; seq < n_units; seq += kGroups) {
@@ -200,43 +218,40 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
     pdl_wait();  // (scratch and outputs belong to earlier kernels until here)
     Cursor c(t, u_begin, u_end);
     long long unit = u_begin;
-    int n = 0, seq = 0;  // accumulators and units taken
+    int seq = 0;  // units taken
+    uint32_t d = 0, d_par = 0;
+    const uint32_t d_full0 = smem_u32(d_full);
     bool ok = true;
     while (c.left > 0 && ok) {
       const int u0 = c.u, token0 = c.token_tile * BN + col0, n_units = min(c.left, t.units - u0);
       const long long seg_begin = unit, tile_begin = unit - u0, seg_end = unit + n_units;
       for (int k = 0; k < n_units && ok; ++k, ++seq) {
-        const int slot = seq % kSlots, n_g = min(kSums, t.p.n_groups - (u0 + k) * kSums);
-        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[slot], (seq / kSlots) & 1, abort));
-        const uint8_t* scales = ss + slot * kScaleBytes + row * kEntry;
+        const int n_g = min(kSums, t.p.n_groups - (u0 + k) * kSums);
+        const uint8_t* scales = ss + seq % kSlots * kScaleBytes + row * kEntry;
 #pragma unroll 1
-        for (int g = 0; g < n_g && ok; ++g, ++n) {
-          const float s = __uint_as_float((ZERO ? *reinterpret_cast<const uint32_t*>(scales + g * 512) : (uint32_t)*reinterpret_cast<const uint16_t*>(scales + g * 256)) << 16);
-          const int d = n % kDbufs;
-          ok = __all_sync(0xffffffffu, mbar_wait(&d_full[d], (n / kDbufs) & 1, abort));
+        for (int g = 0; g < n_g; ++g, scales += kQ4Tile * kEntry) {
+          // (a unit's scales arrive at the barrier of its rows of x, which the MMAs have waited for)
+          ok = __all_sync(0xffffffffu, mbar_wait_a(d_full0 + 8 * d, d_par, abort));
           if (!ok) break;
           tc_fence_after();
-          float v[2][16];
           const uint32_t from = tmem_d + d * BN + col0 + lanes;
-          tmem_ld16_issue(from, v[0]);
+          const float s = __uint_as_float((ZERO ? *reinterpret_cast<const uint32_t*>(scales) : (uint32_t)*reinterpret_cast<const uint16_t*>(scales)) << 16);
+          constexpr int kStep = kCols == 32 ? 32 : 16;  // (64 sums leave registers for 16 columns on their way)
 #pragma unroll
-          for (int b = 0; b < kCols / 16; ++b) {
-            tmem_wait_ld16(v[b & 1]);
-            if (b + 1 < kCols / 16) {
-              tmem_ld16_issue(from + (b + 1) * 16, v[(b + 1) & 1]);
-            } else {
+          for (int c0 = 0; c0 < kCols; c0 += kStep) {
+            float v[kStep];
+            if constexpr (kStep == 32) tmem_ld32_issue(from + c0, v); else tmem_ld16_issue(from + c0, v);
+            tmem_wait_ld_all<kStep>(v);
+            if (c0 + kStep == kCols) {
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive(&d_empty[d]);
-              __syncwarp();
+              if (++d == kDbufs) d = 0, d_par ^= 1;
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[b * 16 + i] = fmaf(s, v[b & 1][i], acc[b * 16 + i]);
+            for (int i = 0; i < kStep; ++i) acc[c0 + i] = fmaf(s, v[i], acc[c0 + i]);
           }
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_empty[slot]);
-        __syncwarp();
       }
       ok = out_all<32 * kWarpsOut>(ok);
       if (!ok) break;
@@ -274,6 +289,18 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
         const int o = c.row_tile * kQ4Tile + row, n_tok = min(kCols, a.T - token0), act = a.flags & (MLORA_ACT_RELU2 | MLORA_ACT_GELU);
         const bool silu = (a.flags & MLORA_SILU_MUL) != 0, mine = o < a.out && (!silu || !(lane & 8));
         const int col = silu ? o / 16 * 8 + (o & 7) : o;
+#pragma unroll 1
+        for (int k = first + 1; k <= last; ++k) {
+          const float* from = t.parts + (size_t)k * (BN * kQ4Tile) + col0 * kQ4Tile + row;
+#pragma unroll
+          for (int c0 = 0; c0 < kCols; c0 += 16) {
+            float v[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = __ldcg(from + (c0 + i) * kQ4Tile);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[c0 + i] += v[i];
+          }
+        }
         // 16 columns at a time, with one copy of the code for them all: unrolled over the columns it would come from memory instruction
         // by instruction, a tile at a time
 #pragma unroll 1
@@ -286,12 +313,6 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
           if (t.delta != nullptr) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) add[i] = o < a.out && c0 + i < n_tok ? __ldcg(t.delta + (size_t)(token0 + c0 + i) * a.out + o) : 0.f;
-          }
-#pragma unroll 1
-          for (int k = first + 1; k <= last; ++k) {
-            const float* from = t.parts + (size_t)k * (BN * kQ4Tile) + (col0 + c0) * kQ4Tile + row;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] += __ldcg(from + i * kQ4Tile);
           }
           if (t.delta != nullptr) {
 #pragma unroll
@@ -328,60 +349,60 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
     if (warp == kMma) {
       // ---- MMA issue -------------------------------------------------------------------------------------------------------------
       constexpr uint32_t idesc = make_idesc(kQ4Tile, BN);
-      if (elect_one()) {  // (one thread: every instruction it spends per unit bounds the rate)
-        const uint64_t b0 = make_smem_desc(smem_u32(sx));
-        const uint32_t a_full0 = smem_u32(a_full), x_full0 = smem_u32(x_full), empty0 = smem_u32(empty), x_empty0 = smem_u32(x_empty), d_full0 = smem_u32(d_full),
-                       d_empty0 = smem_u32(d_empty);
-        uint32_t buf = 0, par = 0, x = 0, x_par = 0, d = 0, d_par = 1;
+      if (elect_one()) {  // (one thread: its instructions come one after the other, and all of them bound the rate)
+        const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty), d_full0 = smem_u32(d_full), d_empty0 = smem_u32(d_empty);
+        const uint64_t desc = make_smem_desc(smem_u32(sx));
+        const uint32_t desc_hi = (uint32_t)(desc >> 32), desc_lo = (uint32_t)desc;
+        const int n_units = (int)(u_end - u_begin), last_steps = (a.in - (t.units - 1) * 128) / 16;  // (a group that is not there has no accumulator)
+        int u = (int)(u_begin % t.units);
+        uint32_t buf = 0, par = 0, d = 0, d_par = 1;
         bool ok = true;
-        for (Cursor c(t, u_begin, u_end); c.left > 0 && ok; c.next()) {
-          const int steps = min(8, (a.in - c.u * 128) / 16);  // of 16 inputs (a group that is not there has no accumulator)
-          ok = mbar_wait_a(a_full0 + 8 * buf, par, abort) && mbar_wait_a(x_full0 + 8 * x, x_par, abort);
+        for (int i = 0; i < n_units; ++i) {
+          ok = mbar_wait_a(full0 + 8 * buf, par, abort);
           if (!ok) break;
-          const uint64_t bdesc = b0 + (uint64_t)(x * (BN * 256 >> 4));
-          const uint32_t a_tmem = tmem_a + buf * 64;
+          const uint32_t b_lo = desc_lo + buf * (BN * 256 >> 4), a_tmem = tmem_a + buf * 64;
+          const bool last = u == t.units - 1;
+          u = last ? 0 : u + 1;
+          const int groups = last ? (last_steps + G / 16 - 1) / (G / 16) : kSums;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            if (k < steps && ok) {
-              const bool opens = k % (G / 16) == 0;
-              if (opens) {
-                ok = mbar_wait_a(d_empty0 + 8 * d, d_par, abort);
-                tc_fence_after();
-              }
-              if (ok) umma_bf16_ta(tmem_d + d * BN, a_tmem + k * 8, bdesc + 2 * (k & 3) + (k >> 2) * (BN * 128 >> 4), idesc, opens ? 0u : 1u);
-              if (ok && (k % (G / 16) == G / 16 - 1 || k + 1 == steps)) {
-                umma_commit_a(d_full0 + 8 * d);
-                if (++d == kDbufs) d = 0, d_par ^= 1;
-              }
+          for (int s = 0; s < kSums; ++s) {
+            if (s < groups && ok) {
+              ok = mbar_wait_a(d_empty0 + 8 * d, d_par, abort);
+              tc_fence_after();
+              const uint32_t d_tmem = tmem_d + d * BN;
+#pragma unroll
+              for (int k = s * (G / 16); k < (s + 1) * (G / 16); ++k)
+                if (G != 128 || !last || k < last_steps)
+                  umma_bf16_ta(d_tmem, a_tmem + k * 8, (uint64_t)desc_hi << 32 | (b_lo + 2 * (k & 3) + (k >> 2) * (BN * 128 >> 4)), idesc, k % (G / 16) != 0);
+              umma_commit_a(d_full0 + 8 * d);
+              if (++d == kDbufs) d = 0, d_par ^= 1;
             }
           }
           if (!ok) break;
           umma_commit_a(empty0 + 8 * buf);
-          umma_commit_a(x_empty0 + 8 * x);
           if (++buf == kBufs) buf = 0, par ^= 1;
-          if (++x == kXslots) x = 0, x_par ^= 1;
         }
         if (!ok) s_abort = 1;
       }
       __syncwarp();
     } else if (warp == kMma + 1) {
-      // ---- rows of x -----------------------------------------------------------------------------------------------------------------
+      // ---- rows of x and scales -----------------------------------------------------------------------------------------------------------------
       if (lane == 0) {
         pdl_wait();
         int seq = 0;
         for (Cursor c(t, u_begin, u_end); c.left > 0; c.next(), ++seq) {
-          const int slot = seq % kXslots, blocks = min(2, n_kb - 2 * c.u);
-          if (!mbar_wait(&x_empty[slot], ((seq / kXslots) & 1) ^ 1, abort)) {
+          const int slot = seq % kBufs, blocks = min(2, n_kb - 2 * c.u);
+          if (!mbar_wait(&empty[slot], ((seq / kBufs) & 1) ^ 1, abort)) {
             s_abort = 1;
             break;
           }
-          mbar_expect_tx(&x_full[slot], blocks * BN * 128);
+          const int g = c.u * kSums, bytes = min(kSums, t.p.n_groups - g) * kQ4Tile * kEntry;
+          mbar_expect_tx(&full[slot], blocks * BN * 128 + bytes);
+          bulk_load(ss + seq % kSlots * kScaleBytes, t.p.table + ((size_t)c.row_tile * t.p.n_groups + g) * kQ4Tile * kEntry, bytes, &full[slot]);
           for (int b = 0; b < blocks; ++b)
-            tma_load_2d(sx + (slot * 2 + b) * BN * 128, &map_x, (2 * c.u + b) * kQ4Block, c.token_tile * BN, &x_full[slot]);
+            tma_load_2d(sx + (slot * 2 + b) * BN * 128, &map_x, (2 * c.u + b) * kQ4Block, c.token_tile * BN, &full[slot]);
         }
         // commits arrive at these barriers until the last unit's: nobody leaves before
-        for (int k = max(seq - kXslots, 0); k < seq && !*abort; ++k)
-          if (!mbar_wait(&x_empty[k % kXslots], (k / kXslots) & 1, abort)) s_abort = 1;
         for (int k = max(seq - kBufs, 0); k < seq && !*abort; ++k)
           if (!mbar_wait(&empty[k % kBufs], (k / kBufs) & 1, abort)) s_abort = 1;
         if (*abort)  // copies may still be in flight: let them land before the shared memory goes to another CTA
@@ -393,8 +414,8 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
       const uint8_t* weights = reinterpret_cast<const uint8_t*>(a.W);
       int seq = 0;
       for (Cursor c(t, u_begin, u_end); c.left > 0; c.next(), ++seq) {
-        const int slot = seq % kWslots, s_slot = seq % kSlots;
-        if (!mbar_wait(&w_empty[slot], ((seq / kWslots) & 1) ^ 1, abort) || !mbar_wait(&s_empty[s_slot], ((seq / kSlots) & 1) ^ 1, abort)) {
+        const int slot = seq % kWslots;
+        if (!mbar_wait(&w_empty[slot], ((seq / kWslots) & 1) ^ 1, abort)) {
           s_abort = 1;
           break;
         }
@@ -404,8 +425,6 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
         bulk_load(sw + slot * kSlotBytes, weights + ((size_t)c.row_tile * n_kb + 2 * c.u) * kQ4TileBytes, blocks * kQ4TileBytes, &w_full[slot]);
         if (ZERO)
           bulk_load(sw + slot * kSlotBytes + 2 * kQ4TileBytes, table, bytes, &w_full[slot]);
-        mbar_expect_tx(&s_full[s_slot], bytes);
-        bulk_load(ss + s_slot * kScaleBytes, table, bytes, &s_full[s_slot]);
       }
       if (*abort)
         for (int i = 0; i < 64; ++i) __nanosleep(1000);
@@ -417,7 +436,7 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
   if (warp == kMma) tmem_dealloc(tmem_slot, 512);
 }
 
-int rows_per_tile(int T) { return T <= 64 ? 64 : 128; }
+int rows_per_tile(int T) { return T <= 32 ? 32 : T <= 64 ? 64 : 128; }
 
 template <int BN, bool ZERO, int G>
 int launch_tc_as(const TcArgs& t, int grid, cudaStream_t st) {
@@ -460,8 +479,8 @@ int launch_q4_tc(const Q4Args& p, const Q4Work& w, cudaStream_t st) {
   t.units = (p.n_kb + 1) / 2;
   const long long all = (long long)t.row_tiles * t.token_tiles * t.units;
   if (all > 2147483647ll) return fail(MLORA_ESIZE, "q4_linear: too many tiles");
-  const int grid = q4_ctas(all);
-  return bn == 64 ? launch_tc_for<64>(t, grid, st) : launch_tc_for<128>(t, grid, st);
+  const int grid = q4_ctas(t.row_tiles * (long long)t.token_tiles, t.units);
+  return bn == 32 ? launch_tc_for<32>(t, grid, st) : bn == 64 ? launch_tc_for<64>(t, grid, st) : launch_tc_for<128>(t, grid, st);
 }
 
 }  // namespace mlora
