@@ -95,41 +95,58 @@ __global__ void __launch_bounds__(kMmThreads, 1) q4_mm_kernel(const __grid_const
   if (warp == kMmWarps) {
     // ---- copies --------------------------------------------------------------------------------------------------------------------
     if (lane == 0) {
-      const uint8_t* weights = reinterpret_cast<const uint8_t*>(a.W);
-      int row_tile = tile % t.row_tiles, token = tile / t.row_tiles * (N8 * 8);
-      const auto copy_x = [&](int slot, int at, int at_token) {
-        const int blocks = min(kMmBlocks, n_kb - at * kMmBlocks);
-        for (int b = 0; b < blocks; ++b)
-          tma_load_2d(ring + slot * S::kBytes + b * N8 * 1024, &map_x, (at * kMmBlocks + b) * kQ4Block, at_token, &full[slot]);
+      // (one thread's instructions come one after the other: counters and running pointers instead of remainders and products; weights
+      // and scales lie one stage after the other, whole tiles and all)
+      struct Place {
+        int u, row_tile, token;
+        const uint8_t *weights, *table;
       };
-      const auto copy_w = [&](int slot) {
-        const int blocks = min(kMmBlocks, n_kb - u * kMmBlocks), g = u * S::kGroups, bytes = min(S::kGroups, t.p.n_groups - g) * kQ4Tile * kEntry;
-        uint8_t* dst = ring + slot * S::kBytes + S::kX;
+      const uint8_t* weights0 = reinterpret_cast<const uint8_t*>(a.W);
+      const int row_tile = tile % t.row_tiles, last_blocks = n_kb - (t.units - 1) * kMmBlocks;
+      const int last_scales = (t.p.n_groups - (t.units - 1) * S::kGroups) * kQ4Tile * kEntry;
+      Place at{u, row_tile, tile / t.row_tiles * (N8 * 8), weights0 + ((size_t)row_tile * n_kb + u * kMmBlocks) * kQ4TileBytes,
+               t.p.table + ((size_t)row_tile * t.p.n_groups + u * S::kGroups) * kQ4Tile * kEntry};
+      const auto copy_x = [&](int slot, uint8_t* dst) {
+        const int blocks = at.u == t.units - 1 ? last_blocks : kMmBlocks;
+#pragma unroll
+        for (int b = 0; b < kMmBlocks; ++b)
+          if (b < blocks) tma_load_2d(dst + b * N8 * 1024, &map_x, at.u * (kMmBlocks * kQ4Block) + b * kQ4Block, at.token, &full[slot]);
+      };
+      const auto copy_w = [&](int slot, uint8_t* dst) {
+        const bool last = at.u == t.units - 1;
+        const int blocks = last ? last_blocks : kMmBlocks, bytes = last ? last_scales : S::kS;
         mbar_expect_tx(&full[slot], blocks * (kQ4TileBytes + N8 * 1024) + bytes);
-        bulk_load(dst, weights + ((size_t)row_tile * n_kb + u * kMmBlocks) * kQ4TileBytes, blocks * kQ4TileBytes, &full[slot]);
-        bulk_load(dst + S::kW, t.p.table + ((size_t)row_tile * t.p.n_groups + g) * kQ4Tile * kEntry, bytes, &full[slot]);
+        bulk_load(dst + S::kX, at.weights, blocks * kQ4TileBytes, &full[slot]);
+        bulk_load(dst + S::kX + S::kW, at.table, bytes, &full[slot]);
+        at.weights += blocks * kQ4TileBytes;
+        at.table += bytes;
       };
       const auto next = [&] {
-        if (++u < t.units) return;
-        u = 0;
-        if (++row_tile == t.row_tiles) row_tile = 0, token += N8 * 8;
+        if (++at.u < t.units) return;
+        at.u = 0;
+        if (++at.row_tile == t.row_tiles) at.row_tile = 0, at.token += N8 * 8, at.weights = weights0, at.table = t.p.table;
       };
       // the first stages' weights and scales, which no earlier kernel of a step writes; then, behind that kernel, their rows of x
-      const int u0 = u, row0 = row_tile, token0 = token, ahead = min(left, kStages);
-      for (int i = 0; i < ahead; ++i, next()) copy_w(i);
-      const int u1 = u, row1 = row_tile, token1 = token;
+      const int ahead = min(left, kStages);
+      const Place begin = at;
+      for (int i = 0; i < ahead; ++i, next()) copy_w(i, ring + i * S::kBytes);
+      const Place then = at;
       pdl_wait();
-      u = u0, row_tile = row0, token = token0;
-      for (int i = 0; i < ahead; ++i, next()) copy_x(i, u, token);
-      u = u1, row_tile = row1, token = token1;
+      at = begin;
+      for (int i = 0; i < ahead; ++i, next()) copy_x(i, ring + i * S::kBytes);
+      at = then;
+      uint32_t par = 0;
+      int slot = 0;
+      uint8_t* dst = ring;
       for (int i = ahead; i < left; ++i, next()) {
-        const int slot = i % kStages;
-        if (!mbar_wait(&empty[slot], ((i / kStages) & 1) ^ 1, abort)) {
+        if (!mbar_wait(&empty[slot], par, abort)) {
           s_abort = 1;
           break;
         }
-        copy_w(slot);
-        copy_x(slot, u, token);
+        copy_w(slot, dst);
+        copy_x(slot, dst);
+        dst += S::kBytes;
+        if (++slot == kStages) slot = 0, par ^= 1, dst = ring;
       }
       if (*abort)  // copies may still be in flight: let them land before the shared memory goes to another CTA
         for (int i = 0; i < 64; ++i) __nanosleep(1000);

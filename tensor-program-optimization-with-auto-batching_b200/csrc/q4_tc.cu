@@ -389,19 +389,38 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
       // ---- rows of x and scales -----------------------------------------------------------------------------------------------------------------
       if (lane == 0) {
         pdl_wait();
-        int seq = 0;
-        for (Cursor c(t, u_begin, u_end); c.left > 0; c.next(), ++seq) {
-          const int slot = seq % kBufs, blocks = min(2, n_kb - 2 * c.u);
-          if (!mbar_wait(&empty[slot], ((seq / kBufs) & 1) ^ 1, abort)) {
+        // (as in the MMA warp one thread's instructions bound the rate: counters instead of remainders, and scales lie one unit after the
+        // other, whole tiles and all)
+        const int n_units = (int)(u_end - u_begin);
+        int u = (int)(u_begin % t.units), row_tile = (int)(u_begin / t.units) % t.row_tiles, token = (int)(u_begin / t.units / t.row_tiles) * BN;
+        const int last_blocks = n_kb - 2 * (t.units - 1), last_bytes = (t.p.n_groups - (t.units - 1) * kSums) * kQ4Tile * kEntry;
+        const uint8_t* table = t.p.table + ((size_t)row_tile * t.p.n_groups + u * kSums) * kQ4Tile * kEntry;
+        int slot = 0, s_slot = 0;
+        uint32_t par = 1;
+        uint8_t *dst = sx, *s_dst = ss;
+        for (int i = 0; i < n_units; ++i) {
+          if (!mbar_wait(&empty[slot], par, abort)) {
             s_abort = 1;
             break;
           }
-          const int g = c.u * kSums, bytes = min(kSums, t.p.n_groups - g) * kQ4Tile * kEntry;
-          mbar_expect_tx(&full[slot], blocks * BN * 128 + bytes);
-          bulk_load(ss + seq % kSlots * kScaleBytes, t.p.table + ((size_t)c.row_tile * t.p.n_groups + g) * kQ4Tile * kEntry, bytes, &full[slot]);
-          for (int b = 0; b < blocks; ++b)
-            tma_load_2d(sx + (slot * 2 + b) * BN * 128, &map_x, (2 * c.u + b) * kQ4Block, c.token_tile * BN, &full[slot]);
+          const bool last = u == t.units - 1;
+          const int bytes = last ? last_bytes : kScaleBytes;
+          mbar_expect_tx(&full[slot], (last && last_blocks == 1 ? BN * 128 : BN * 256) + bytes);
+          tma_load_2d(dst, &map_x, u * 128, token, &full[slot]);
+          if (!last || last_blocks == 2) tma_load_2d(dst + BN * 128, &map_x, u * 128 + 64, token, &full[slot]);
+          bulk_load(s_dst, table, bytes, &full[slot]);
+          table += bytes;
+          ++u;
+          if (last) {
+            u = 0;
+            if (++row_tile == t.row_tiles) row_tile = 0, token += BN, table = t.p.table;
+          }
+          dst += BN * 256;
+          if (++slot == kBufs) slot = 0, par ^= 1, dst = sx;
+          s_dst += kScaleBytes;
+          if (++s_slot == kSlots) s_slot = 0, s_dst = ss;
         }
+        const int seq = n_units;
         // commits arrive at these barriers until the last unit's: nobody leaves before
         for (int k = max(seq - kBufs, 0); k < seq && !*abort; ++k)
           if (!mbar_wait(&empty[k % kBufs], (k / kBufs) & 1, abort)) s_abort = 1;
@@ -411,20 +430,32 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
     } else if (lane == 0) {
       // ---- packed weights: a unit's 8 KB lie one after the other, and so do its groups' scales (no earlier kernel of a step writes
       // either, so the copies need not wait for it) --------------------------------------------------------------------------------
-      const uint8_t* weights = reinterpret_cast<const uint8_t*>(a.W);
-      int seq = 0;
-      for (Cursor c(t, u_begin, u_end); c.left > 0; c.next(), ++seq) {
-        const int slot = seq % kWslots;
-        if (!mbar_wait(&w_empty[slot], ((seq / kWslots) & 1) ^ 1, abort)) {
+      const int n_units = (int)(u_end - u_begin);
+      int u = (int)(u_begin % t.units), row_tile = (int)(u_begin / t.units) % t.row_tiles, slot = 0;
+      const int last_bytes = (n_kb - 2 * (t.units - 1)) * kQ4TileBytes, last_scales = (t.p.n_groups - (t.units - 1) * kSums) * kQ4Tile * kEntry;
+      const uint8_t* weights = reinterpret_cast<const uint8_t*>(a.W) + ((size_t)row_tile * n_kb + 2 * u) * kQ4TileBytes;
+      const uint8_t* table = t.p.table + ((size_t)row_tile * t.p.n_groups + u * kSums) * kQ4Tile * kEntry;
+      uint32_t par = 1;
+      uint8_t* dst = sw;
+      for (int i = 0; i < n_units; ++i) {
+        if (!mbar_wait(&w_empty[slot], par, abort)) {
           s_abort = 1;
           break;
         }
-        const int blocks = min(2, n_kb - 2 * c.u), g = c.u * kSums, n_g = min(kSums, t.p.n_groups - g), bytes = n_g * kQ4Tile * kEntry;
-        const uint8_t* table = t.p.table + ((size_t)c.row_tile * t.p.n_groups + g) * kQ4Tile * kEntry;
-        mbar_expect_tx(&w_full[slot], blocks * kQ4TileBytes + (ZERO ? bytes : 0));
-        bulk_load(sw + slot * kSlotBytes, weights + ((size_t)c.row_tile * n_kb + 2 * c.u) * kQ4TileBytes, blocks * kQ4TileBytes, &w_full[slot]);
-        if (ZERO)
-          bulk_load(sw + slot * kSlotBytes + 2 * kQ4TileBytes, table, bytes, &w_full[slot]);
+        const bool last = u == t.units - 1;
+        const int bytes = last ? last_bytes : 2 * kQ4TileBytes, scales = !ZERO ? 0 : last ? last_scales : kScaleBytes;
+        mbar_expect_tx(&w_full[slot], bytes + scales);
+        bulk_load(dst, weights, bytes, &w_full[slot]);
+        if (ZERO) bulk_load(dst + 2 * kQ4TileBytes, table, scales, &w_full[slot]);
+        weights += bytes;
+        table += scales;
+        ++u;
+        if (last) {
+          u = 0;
+          if (++row_tile == t.row_tiles) row_tile = 0, weights = reinterpret_cast<const uint8_t*>(a.W), table = t.p.table;
+        }
+        dst += kSlotBytes;
+        if (++slot == kWslots) slot = 0, par ^= 1, dst = sw;
       }
       if (*abort)
         for (int i = 0; i < 64; ++i) __nanosleep(1000);
