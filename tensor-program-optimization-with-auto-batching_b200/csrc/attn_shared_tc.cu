@@ -31,19 +31,21 @@ constexpr int kPlanHeader = 8;           // int32: rows, tiles, items, parts
 constexpr int kTickets = 1024;           // arrival counters at the start of the scratch, whatever the call's sizes: zero between calls
 constexpr int kPlanMinRows = 2, kPlanMinKeys = 64;  // smaller groups and shorter prefixes are read row by row
 
-// A plan in int32: header, then two quads per tile (slot whose pages are read, keys, rows, first entry of `list` | first item, key ranges
-// per pair, first part, 0), then per row: `list` (rows by group), first key of the row's own part, its first part, its parts.
+// A plan in int32: header; per row a quad (first key of its own part, its first part, its parts, 0) and its entry of `list` (rows by group);
+// then two quads per item, all that a CTA needs to begin: (slot whose pages are read, first block, blocks, keys of the prefix | first entry
+// of `list`, rows, key head, key range).
 struct PlanView {
-  int32_t *head, *tiles, *list, *first, *part, *n_part;
+  int32_t* head;
+  int4* row;
+  int32_t* list;
+  int4* item;
 };
 __host__ __device__ inline PlanView plan_view(int32_t* p, int max_rows) {
   PlanView v;
   v.head = p;
-  v.tiles = p + kPlanHeader;
-  v.list = v.tiles + 8 * (max_rows / kPlanMinRows + 1);
-  v.first = v.list + max_rows;
-  v.part = v.first + max_rows;
-  v.n_part = v.part + max_rows;
+  v.row = reinterpret_cast<int4*>(p + kPlanHeader);
+  v.list = p + kPlanHeader + 4 * max_rows;
+  v.item = reinterpret_cast<int4*>(v.list + (max_rows + 3) / 4 * 4);
   return v;
 }
 
@@ -54,6 +56,12 @@ int sm_count() {
     n = 148;
   }
   return n;
+}
+
+// Items of a call: a tile has at least kPlanMinRows rows, and more where it is full, so there are at most T / kPlanMinRows tiles.
+int max_items_of(int T, int Hkv, int target) {
+  const long long tiles = T / kPlanMinRows;
+  return tiles == 0 ? 0 : (int)(tiles * Hkv > target ? tiles * Hkv : target);
 }
 
 // Rows of a tile; parts (a row's partial results over the key ranges of its prefix) that scratch has room for: an item is a tile's key
@@ -81,7 +89,7 @@ __global__ void __launch_bounds__(kPlanMaxRows) prefix_plan_kernel(const int32_t
                                                                    int n_slots, int rt, int Hkv, int target, int cap_parts, int32_t* plan, int max_rows) {
   __shared__ int s_id[kPlanMaxRows];     // prefix of the row, -1: none
   __shared__ int s_lead[kPlanMaxRows];   // first row of its group, if the group is taken together
-  __shared__ int s_tile[kPlanMaxRows / kPlanMinRows + 1][4];  // blocks, rows, key ranges
+  __shared__ int s_tile[kPlanMaxRows / kPlanMinRows + 1][8];  // blocks, rows, key ranges, first item, slot, keys, first entry of the list
   __shared__ int s_red[33];
   pdl_launch_dependents();
   pdl_wait();
@@ -151,22 +159,26 @@ __global__ void __launch_bounds__(kPlanMaxRows) prefix_plan_kernel(const int32_t
     }
     n_part = s_tile[tile][2];
     part_of_row = part + (rank % rt) * n_part;
-    if (opens) {
-      reinterpret_cast<int4*>(v.tiles)[2 * tile] = make_int4(slot, len, rows, place);
-      reinterpret_cast<int4*>(v.tiles)[2 * tile + 1] = make_int4(item, splits, part, 0);
-    }
+    if (opens) s_tile[tile][3] = item, s_tile[tile][4] = slot, s_tile[tile][5] = len, s_tile[tile][6] = place;
   }
-  if (t < T) {
-    v.first[t] = used ? len : 0;
-    v.part[t] = part_of_row;
-    v.n_part[t] = n_part;
-  }
+  if (t < T) v.row[t] = make_int4(used ? len : 0, part_of_row, n_part, 0);
   const int items = block_sum_int(splits, s_red) * Hkv, parts = block_sum_int(splits * rows, s_red);
   if (t == 0) {
     v.head[0] = T;
     v.head[1] = n_tiles;
     v.head[2] = items;
     v.head[3] = parts;
+  }
+  for (int i = t; i < items; i += blockDim.x) {
+    int lo = 0, hi = n_tiles - 1;  // the last tile whose first item is not behind this one
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (s_tile[mid][3] <= i) lo = mid; else hi = mid - 1;
+    }
+    const int* e = s_tile[lo];
+    const int r = i - e[3], split = r % e[2], b0 = (int)((long long)e[0] * split / e[2]), b1 = (int)((long long)e[0] * (split + 1) / e[2]);
+    v.item[2 * i] = make_int4(e[4], b0, b1 - b0, e[5]);
+    v.item[2 * i + 1] = make_int4(e[6], e[1], r / e[2], split);
   }
 }
 
@@ -216,17 +228,19 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
   __shared__ uint64_t pbar;        // the four softmax warps have written P, and taken the P V before into O
   __shared__ uint64_t obar;        // P V has retired
   __shared__ uint32_t tmem_slot;
-  __shared__ int s_abort, s_tile;
+  __shared__ int s_abort;
 
-  pdl_launch_dependents();  // (the tail's own keys do not depend on this kernel)
+  pdl_wait();
+  pdl_launch_dependents();  // (behind the wait: the tail may begin when everything before this kernel is done; its own keys do not depend on it)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const PlanView pv = plan_view(a.plan, a.plan_rows);
-  const int n_tiles = pv.head[1], item = blockIdx.x;
-  if (item >= pv.head[2]) return;  // (the whole CTA, before it has asked for anything)
-  for (int i = tid; i < n_tiles; i += kPxThreads) {
-    const int4 e = reinterpret_cast<const int4*>(pv.tiles)[2 * i + 1];
-    if (item >= e.x && item < e.x + e.y * a.Hkv) s_tile = i;
-  }
+  const int n_items = pv.head[2];
+  const int4 i0 = pv.item[2 * blockIdx.x], i1 = pv.item[2 * blockIdx.x + 1];  // (there is room for as many as there are CTAs)
+  if ((int)blockIdx.x >= n_items) return;  // (the whole CTA, before it has asked for anything)
+  const int rep = a.Hq / a.Hkv, kvh = i1.z, split = i1.w;
+  const int n_keys = min(i0.w, a.max_pages * PS), n_pages = (n_keys + PS - 1) / PS;
+  const int b0 = i0.y, n_blocks = max(0, min(i0.y + i0.z, (n_keys + kTile - 1) / kTile) - i0.y);  // (a prefix longer than the block table is cut)
+  const int32_t* bt = a.block_table + (size_t)i0.x * a.max_pages;
   if (tid == 0) {
     s_abort = 0;
     mbar_init(&kbar, 1);
@@ -235,29 +249,23 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
     mbar_init(&pbar, 4);
     mbar_init(&obar, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    tma_prefetch_desc(&map_k);
-    tma_prefetch_desc(&map_v);
-    tma_prefetch_desc(&map_kr);
-    tma_prefetch_desc(&map_vr);
   }
-  if (warp == 4) tmem_alloc(&tmem_slot, 256);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem_base = tmem_slot, tmem_o = tmem_base + kTile;
-  const int4 t0 = reinterpret_cast<const int4*>(pv.tiles)[2 * s_tile], t1 = reinterpret_cast<const int4*>(pv.tiles)[2 * s_tile + 1];
-  const int rep = a.Hq / a.Hkv, kvh = (item - t1.x) / t1.y, split = (item - t1.x) % t1.y;
-  const int n_keys = min(t0.y, a.max_pages * PS);
-  const int blocks = (n_keys + kTile - 1) / kTile;
-  const int b0 = (int)((long long)blocks * split / t1.y), n_blocks = (int)((long long)blocks * (split + 1) / t1.y) - b0;
-  const int32_t* bt = a.block_table + (size_t)t0.x * a.max_pages;
-  const int n_pages = (n_keys + PS - 1) / PS;
+  if (warp == 4) {
+    if (lane == 0) {
+      tma_prefetch_desc(&map_k);
+      tma_prefetch_desc(&map_v);
+      tma_prefetch_desc(&map_kr);
+      tma_prefetch_desc(&map_vr);
+    }
+    __syncwarp();
+    tmem_alloc(&tmem_slot, 256);
+  }
 
   // (the pairs' queries, as the tensor cores read them: rows of 128 bytes, 16-byte chunks XORed with the row)
   int row = -1, head = 0;
   if (tid < kTile) {
-    if (tid < t0.z * rep) {
-      row = pv.list[t0.w + tid / rep];
+    if (tid < i1.y * rep) {
+      row = pv.list[i1.x + tid / rep];
       head = kvh * rep + tid % rep;
     }
     const uint4* src = reinterpret_cast<const uint4*>(a.q + (size_t)max(row, 0) * a.ld + (size_t)head * D);
@@ -266,7 +274,10 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
       *reinterpret_cast<uint4*>(sq + (c >> 3) * kSub + tid * 128 + (((c & 7) ^ (tid & 7)) << 4)) = row >= 0 ? src[c] : make_uint4(0u, 0u, 0u, 0u);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
+  tc_fence_before();
   __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_slot, tmem_o = tmem_base + kTile;
 
   if (warp == 4) {
     // ---- copies and MMAs: lane 0 waits and issues, one lane per page copies -----------------------------------------------
@@ -344,7 +355,7 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
       for (int i = 0; i < 64; ++i) __nanosleep(1000);
   } else {
     // ---- softmax: one thread per pair; a warp without pairs only keeps step -------------------------------------------------
-    const bool busy = warp * 32 < t0.z * rep;
+    const bool busy = warp * 32 < i1.y * rep;
     const int q_pos = row >= 0 ? a.row_pos[row] : -1;
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     float o[D];
@@ -446,7 +457,7 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
     }
     if (!ok) s_abort = 1;
     if (row >= 0) {
-      float* dst = a.parts + ((size_t)(pv.part[row] + split) * a.Hq + head) * (D + 4);
+      float* dst = a.parts + ((size_t)(pv.row[row].y + split) * a.Hq + head) * (D + 4);
 #pragma unroll
       for (int c = 0; c < D / 4; ++c) reinterpret_cast<float4*>(dst)[c] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
       *reinterpret_cast<float2*>(dst + D) = ok ? make_float2(m_run, l_run) : make_float2(-INFINITY, 0.f);
@@ -462,9 +473,6 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
 constexpr int kTlWarps = 4, kTlThreads = kTlWarps * 32;
 constexpr int kTlKeys = 16;  // keys a warp works on at a time
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {  // the rest of the 16 becomes zeros
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
@@ -487,21 +495,24 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint3
 
 // grid (Hkv x head tiles, T, key ranges): up to 16 query heads of a key head over the row's keys from `first` on (or a range of them).
 template <int D, int STAGES>
-__global__ void __launch_bounds__(kTlThreads) tail_attn_kernel(SharedArgs a) {
-  constexpr int kChunks = D / 8;                       // 16-byte pieces of a key
-  constexpr int kHalf = kTlKeys * D * 2;               // bytes of 16 keys
-  extern __shared__ __align__(128) uint8_t ring[];     // [warp][stage][K | V][16 keys][D]; then the warps' partial results
+__global__ void __launch_bounds__(kTlThreads) tail_attn_kernel(const __grid_constant__ CUtensorMap map_k,
+                                                               const __grid_constant__ CUtensorMap map_v, SharedArgs a) {
+  constexpr int kHalf = kTlKeys * D * 2;               // bytes of 16 keys: D / 64 sub-tiles [16][64], 128-byte swizzle
+  extern __shared__ uint8_t smem_raw[];                // [warp][stage][K | V]; then the warps' partial results
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ uint64_t full[kTlWarps][STAGES];
   __shared__ float s_m[kTlWarps][16], s_l[kTlWarps][16];
   __shared__ float s_w[64 + kTlWarps][16];             // factors of the ranges that are joined
-  __shared__ int s_last;
+  __shared__ int s_last, s_abort;
 
   pdl_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rep = a.Hq / a.Hkv, head_tiles = (rep + 15) / 16;
   const int kvh = blockIdx.x / head_tiles, h0 = kvh * rep + (blockIdx.x % head_tiles) * 16, n_heads = min(16, kvh * rep + rep - h0);
   const int t = blockIdx.y, split = blockIdx.z;
-  const PlanView pv = plan_view(a.plan, a.plan_rows);
-  const int slot = a.row_slot[t], pos = a.row_pos[t], first = pv.first[t], n_part = pv.n_part[t];
+  const int slot = a.row_slot[t], pos = a.row_pos[t];
+  const int4 plan = plan_view(a.plan, a.plan_rows).row[t];
+  const int first = plan.x, n_part = plan.z;
   const int32_t* bt = a.block_table + (size_t)slot * a.max_pages;
   const int PS = a.page_size;
   const int n_tok = (int)min((long long)max(pos + 1, 0), (long long)a.max_pages * PS);
@@ -510,24 +521,32 @@ __global__ void __launch_bounds__(kTlThreads) tail_attn_kernel(SharedArgs a) {
   const int ranges = max(1, min(a.n_splits, units / (8 * kTlWarps)));
   if (split >= ranges) return;
   const int ub = u0 + (int)((long long)units * split / ranges), ue = u0 + (int)((long long)units * (split + 1) / ranges);
+  if (tid == 0) s_abort = 0;
+  if (lane == 0) {
+    for (int i = 0; i < STAGES; ++i) mbar_init(&full[warp][i], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
 
-  const uint32_t base = smem_u32(ring) + warp * STAGES * 2 * kHalf;
+  uint8_t* mine = ring + warp * STAGES * 2 * kHalf;
+  int page = 0;  // of the lane's unit among the 32 that come next: one read for them all, not one per unit in front of its copies
   auto fetch = [&](int i) {  // unit ub + warp + 4 i -> stage i % STAGES
-    const int u = ub + warp + i * kTlWarps;
-    if (u < ue) {
-      const int key = u * kTlKeys, page = bt[key / PS];
-      const size_t at = (((size_t)page * a.Hkv + kvh) * PS + key % PS) * D;
-      const uint32_t dst = base + (i % STAGES) * 2 * kHalf;
+    if ((i & 31) == 0) {
+      const int u = ub + warp + (i + lane) * kTlWarps;
+      page = u < ue ? bt[u * kTlKeys / PS] : 0;
+    }
+    const int u = ub + warp + i * kTlWarps, p = __shfl_sync(0xffffffffu, page, i & 31);
+    if (u < ue && lane == 0) {
+      uint64_t* bar = &full[warp][i % STAGES];
+      uint8_t* dst = mine + (i % STAGES) * 2 * kHalf;
+      mbar_expect_tx(bar, 2 * kHalf);
 #pragma unroll
-      for (int c = 0; c < kTlKeys * kChunks / 32; ++c) {
-        const int p = c * 32 + lane, r = p / kChunks, ch = p % kChunks;
-        const int n = key + r >= first && key + r < n_tok ? 16 : 0;  // (what is not the row's own becomes zeros)
-        const uint32_t d = dst + r * (D * 2) + ((ch ^ (r & 7)) << 4);
-        cp_async16(d, a.k_pages + at + (size_t)r * D + ch * 8, n);
-        cp_async16(d + kHalf, a.v_pages + at + (size_t)r * D + ch * 8, n);
+      for (int j = 0; j < D / 64; ++j) {
+        tma_load_4d(dst + j * 2048, &map_k, j * 64, u * kTlKeys % PS, kvh, p, bar);
+        tma_load_4d(dst + kHalf + j * 2048, &map_v, j * 64, u * kTlKeys % PS, kvh, p, bar);
       }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    __syncwarp();
   };
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) fetch(i);
@@ -552,18 +571,28 @@ __global__ void __launch_bounds__(kTlThreads) tail_attn_kernel(SharedArgs a) {
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   const int mr = lane & 7, mi = lane >> 3;  // row and matrix whose address this lane gives to ldmatrix
 
+  bool ok = true;
   for (int i = 0; ub + warp + i * kTlWarps < ue; ++i) {
     fetch(i + STAGES - 1);
-    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-    __syncwarp();
+    ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][i % STAGES], (i / STAGES) & 1, &s_abort));
+    if (!ok) break;
     const int key = (ub + warp + i * kTlWarps) * kTlKeys;
-    const uint32_t sk = base + (i % STAGES) * 2 * kHalf, sv = sk + kHalf;
+    uint8_t* stage = mine + (i % STAGES) * 2 * kHalf;
+    const uint32_t sk = smem_u32(stage), sv = sk + kHalf;
+    if (key < first || key + kTlKeys > n_tok) {  // what is not the row's own: its probabilities are 0, but 0 * NaN is not
+      for (int c = lane; c < kTlKeys * D / 8; c += 32) {
+        const int r = c % 128 / 8;  // (a sub-tile has 16 rows of eight pieces; a swizzled row stays inside its own 128 bytes)
+        if (key + r < first || key + r >= n_tok) *reinterpret_cast<uint4*>(stage + kHalf + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+    }
     float s[2][4] = {};
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {  // matrices: keys 0-7 and 8-15, columns 16 k and + 8
       uint32_t b[4];
       const int r = (mi >> 1) * 8 + mr, ch = 2 * k + (mi & 1);
-      ldsm4(sk + r * (D * 2) + ((ch ^ mr) << 4), b);
+      ldsm4(sk + (ch >> 3) * 2048 + r * 128 + (((ch & 7) ^ mr) << 4), b);
       mma16816(s[0], qa[k], b[0], b[1]);
       mma16816(s[1], qa[k], b[2], b[3]);
     }
@@ -600,7 +629,7 @@ __global__ void __launch_bounds__(kTlThreads) tail_attn_kernel(SharedArgs a) {
     for (int c = 0; c < D / 16; ++c) {  // matrices: keys 0-7 and 8-15 of columns 16 c, then of 16 c + 8
       uint32_t b[4];
       const int r = (mi & 1) * 8 + mr, ch = 2 * c + (mi >> 1);
-      ldsm4t(sv + r * (D * 2) + ((ch ^ mr) << 4), b);
+      ldsm4t(sv + (ch >> 3) * 2048 + r * 128 + (((ch & 7) ^ mr) << 4), b);
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         float(&d)[4] = o[2 * c + n];
@@ -611,8 +640,12 @@ __global__ void __launch_bounds__(kTlThreads) tail_attn_kernel(SharedArgs a) {
     }
     __syncwarp();  // (the next copy overwrites what was read here)
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if (!ok) {
+    s_abort = 1;
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);  // copies may still be in flight
+  }
   __syncthreads();  // every warp is done with the ring
+  if (s_abort && tid == 0 && a.status) atomicOr(a.status, 1);
 
   // ---- the four warps' results, joined with what the prefix's key ranges left ---------------------------------------------------
   float* acc = reinterpret_cast<float*>(ring);  // [warp][16][D]
@@ -667,7 +700,7 @@ __global__ void __launch_bounds__(kTlThreads) tail_attn_kernel(SharedArgs a) {
     if (ranges == 1) return make_float2(s_m[r][h], s_l[r][h]);
     return __ldcg(reinterpret_cast<const float2*>(a.own + (((size_t)t * a.Hq + h0 + h) * a.n_splits + r) * (D + 4) + D));
   };
-  const float* part0 = a.parts + ((size_t)pv.part[t] * a.Hq + h0) * (D + 4);
+  const float* part0 = a.parts + ((size_t)plan.y * a.Hq + h0) * (D + 4);
   const size_t part_step = (size_t)a.Hq * (D + 4);
   // factors exp2(m - M) / L of every range, 64 prefix ranges at a time in shared memory; the totals first
   const int h = tid / (kTlThreads / 16), sub = tid % (kTlThreads / 16);  // 8 threads per head
@@ -687,14 +720,15 @@ __global__ void __launch_bounds__(kTlThreads) tail_attn_kernel(SharedArgs a) {
     if (mn != -INFINITY) L = (M == -INFINITY ? 0.f : L * fast_exp2(M - mn)) + (mo == -INFINITY ? 0.f : lo * fast_exp2(mo - mn));
     M = mn;
   }
-  const float inv = L > 0.f ? 1.f / L : 0.f;
-  // outputs: 4 columns of a head per thread, D / 4 threads a head
+  const float inv = L > 0.f && !s_abort ? 1.f / L : 0.f;
+  // outputs: 4 columns of a head per thread, D / 4 threads a head; where there are few heads, several threads share the ranges
   constexpr int kPer = kTlThreads / (D / 4);           // heads in work at once
   constexpr int kSets = 16 / kPer;
+  const int hp = n_heads >= kPer ? kPer : n_heads > 2 ? 4 : n_heads, slices = kPer / hp;
   float4 sum[kSets];
 #pragma unroll
   for (int i = 0; i < kSets; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  const int c = tid % (D / 4), hs = tid / (D / 4);
+  const int c = tid % (D / 4), hs = tid / (D / 4) % hp, slice = tid / (D / 4) / hp;
   for (int r0 = 0; r0 < n_own + n_part; r0 += 64) {
     const int n = min(64, n_own + n_part - r0);
     __syncthreads();
@@ -707,10 +741,10 @@ __global__ void __launch_bounds__(kTlThreads) tail_attn_kernel(SharedArgs a) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kSets; ++i) {
-      const int hh = i * kPer + hs;
-      if (hh >= n_heads) continue;
+      const int hh = i * hp + hs;
+      if (hh >= n_heads || (i > 0 && hp < kPer)) continue;
 #pragma unroll 4
-      for (int r = 0; r < n; ++r) {
+      for (int r = slice; r < n; r += slices) {
         const int x = r0 + r;
         const float f = s_w[r][hh];
         float4 v;
@@ -721,22 +755,32 @@ __global__ void __launch_bounds__(kTlThreads) tail_attn_kernel(SharedArgs a) {
       }
     }
   }
+  if (slices > 1) {
+    float4* share = reinterpret_cast<float4*>(ring) + kTlWarps * 16 * D / 4;  // (behind the warps' results)
+    if (slice > 0) share[tid] = sum[0];
+    __syncthreads();
+    if (slice > 0) return;
+    for (int i = 1; i < slices; ++i) {
+      const float4 v = share[tid + i * hp * (D / 4)];
+      sum[0].x += v.x, sum[0].y += v.y, sum[0].z += v.z, sum[0].w += v.w;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < kSets; ++i) {
-    const int hh = i * kPer + hs;
-    if (hh >= n_heads) continue;
+    const int hh = i * hp + hs;
+    if (hh >= n_heads || (i > 0 && hp < kPer)) continue;
     __nv_bfloat162 b[2] = {__floats2bfloat162_rn(sum[i].x, sum[i].y), __floats2bfloat162_rn(sum[i].z, sum[i].w)};
     *reinterpret_cast<uint2*>(a.out + (size_t)t * a.ld_out + (size_t)(h0 + hh) * D + c * 4) = *reinterpret_cast<const uint2*>(b);
   }
 }
 
-// Pages [n_pages][Hkv][PS][D], a box of `pages` pages of one head, 64 columns: rows of 128 bytes, swizzled.
-int page_map(CUtensorMap* m, const void* ptr, int n_pages, int Hkv, int PS, int D, int pages) {
+// Pages [n_pages][Hkv][PS][D], a box of `keys` keys of `pages` pages of one head, 64 columns: rows of 128 bytes, swizzled.
+int page_map(CUtensorMap* m, const void* ptr, int n_pages, int Hkv, int PS, int D, int pages, int keys) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(MLORA_ECUDA, "paged_attention_shared: cuTensorMapEncodeTiled is not available from this driver");
   cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)PS, (cuuint64_t)Hkv, (cuuint64_t)n_pages};
   cuuint64_t strides[3] = {(cuuint64_t)D * 2, (cuuint64_t)PS * D * 2, (cuuint64_t)Hkv * PS * D * 2};
-  cuuint32_t box[4] = {64, (cuuint32_t)PS, 1, (cuuint32_t)pages};
+  cuuint32_t box[4] = {64, (cuuint32_t)keys, 1, (cuuint32_t)pages};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -761,26 +805,29 @@ constexpr int kTlStages = 3;
 template <int ND, int PS>
 int launch_shared(const SharedArgs& a, int n_pages_total, int max_items, cudaStream_t st) {
   constexpr int D = ND * 64;
-  CUtensorMap mk, mv, mkr, mvr;
-  int rc = page_map(&mk, a.k_pages, n_pages_total, a.Hkv, PS, D, 1);
-  if (!rc) rc = page_map(&mv, a.v_pages, n_pages_total, a.Hkv, PS, D, 1);
-  if (!rc) rc = page_map(&mkr, a.k_pages, n_pages_total, a.Hkv, PS, D, kTile / PS);
-  if (!rc) rc = page_map(&mvr, a.v_pages, n_pages_total, a.Hkv, PS, D, kTile / PS);
+  CUtensorMap mk, mv, mkr, mvr, mkt, mvt;  // a page, a block of them, 16 keys
+  int rc = page_map(&mk, a.k_pages, n_pages_total, a.Hkv, PS, D, 1, PS);
+  if (!rc) rc = page_map(&mv, a.v_pages, n_pages_total, a.Hkv, PS, D, 1, PS);
+  if (!rc) rc = page_map(&mkr, a.k_pages, n_pages_total, a.Hkv, PS, D, kTile / PS, PS);
+  if (!rc) rc = page_map(&mvr, a.v_pages, n_pages_total, a.Hkv, PS, D, kTile / PS, PS);
+  if (!rc) rc = page_map(&mkt, a.k_pages, n_pages_total, a.Hkv, PS, D, 1, kTlKeys);
+  if (!rc) rc = page_map(&mvt, a.v_pages, n_pages_total, a.Hkv, PS, D, 1, kTlKeys);
   if (rc) return rc;
-  constexpr int smem = 3 * ND * kSub + 1024, smem_tail = kTlWarps * kTlStages * 2 * kTlKeys * D * 2;
-  static_assert(smem_tail >= kTlWarps * 16 * D * 4, "the warps' results lie in the ring");
+  constexpr int smem = 3 * ND * kSub + 1024, smem_tail = kTlWarps * kTlStages * 2 * kTlKeys * D * 2 + 1024;
+  static_assert(smem_tail >= kTlWarps * 16 * D * 4 + kTlThreads * 16 + 1024, "the warps' results lie in the ring");
   static std::atomic<unsigned long long> done{0}, done_tail{0};
   rc = allow_smem(prefix_attn_kernel<ND, PS>, smem, done);
   if (!rc) rc = allow_smem(tail_attn_kernel<D, kTlStages>, smem_tail, done_tail);
   if (rc) return rc;
   if (max_items > 0) {
-    prefix_attn_kernel<ND, PS><<<(unsigned)max_items, kPxThreads, smem, st>>>(mk, mv, mkr, mvr, a);
+    const cudaError_t e = launch_pdl_if(pdl_enabled_tail(), prefix_attn_kernel<ND, PS>, dim3((unsigned)max_items), dim3(kPxThreads), smem, st, mk, mv, mkr, mvr, a);
+    if (e != cudaSuccess) return fail(MLORA_ECUDA, "prefix_attn_kernel: %s", cudaGetErrorString(e));
     count_launch();
     MLORA_CHECK_LAUNCH("prefix_attn_kernel");
   }
   const int head_tiles = (a.Hq / a.Hkv + 15) / 16;
   const cudaError_t e = launch_pdl_if(max_items > 0 && pdl_enabled_tail(), tail_attn_kernel<D, kTlStages>, dim3((unsigned)(a.Hkv * head_tiles), (unsigned)a.T, (unsigned)a.n_splits),
-                                      dim3(kTlThreads), smem_tail, st, a);
+                                      dim3(kTlThreads), smem_tail, st, mkt, mvt, a);
   if (e != cudaSuccess) return fail(MLORA_ECUDA, "tail_attn_kernel: %s", cudaGetErrorString(e));
   count_launch();
   MLORA_CHECK_LAUNCH("tail_attn_kernel");
@@ -796,9 +843,7 @@ SharedSizes sizes_of(int T, int Hq, int Hkv, int D) {
   SharedSizes s;
   const int rep = Hq / Hkv, ht = (rep + 15) / 16;
   s.target = 2 * sm_count();
-  // tiles: a group has at least kPlanMinRows rows and a full tile has more, so there are at most T / kPlanMinRows
-  const int tiles = T / kPlanMinRows;
-  s.max_items = tiles == 0 ? 0 : (int)((long long)tiles * Hkv > s.target ? (long long)tiles * Hkv : s.target);
+  s.max_items = max_items_of(T, Hkv, s.target);
   const long long ctas = (long long)T * Hkv * ht;
   s.n_splits = ctas >= s.target || ctas > kTickets ? 1 : (int)((s.target + ctas - 1) / (ctas > 0 ? ctas : 1));
   if (s.n_splits > 32) s.n_splits = 32;
@@ -818,8 +863,9 @@ bool shared_sizes_fit(int T, int Hq, int Hkv, int D) {
 
 using namespace mlora;
 
-extern "C" size_t mlora_prefix_plan_bytes(int32_t max_rows) {
-  return max_rows < 0 || max_rows > kPlanMaxRows ? 0 : 4u * (size_t)(kPlanHeader + 8 * (max_rows / kPlanMinRows + 1) + 4 * max_rows);
+extern "C" size_t mlora_prefix_plan_bytes(int32_t max_rows, int32_t Hkv) {
+  if (max_rows < 0 || max_rows > kPlanMaxRows || Hkv <= 0 || Hkv > 1024) return 0;
+  return 4u * (size_t)(kPlanHeader + 4 * max_rows + (max_rows + 3) / 4 * 4 + 8 * max_items_of(max_rows, Hkv, 2 * sm_count()));
 }
 
 extern "C" int mlora_prefix_plan(const int32_t* d_row_slot, int32_t T, const int32_t* d_prefix_id, const int32_t* d_prefix_len, int32_t n_slots,
@@ -829,7 +875,7 @@ extern "C" int mlora_prefix_plan(const int32_t* d_row_slot, int32_t T, const int
   MLORA_REQUIRE(d_row_slot && d_prefix_id && d_prefix_len && d_plan && aligned16(d_plan), "prefix_plan: null pointer or unaligned plan");
   if (T == 0) return MLORA_OK;
   const int rep = Hq / Hkv, target = 2 * sm_count();
-  const int threads = (T + 31) / 32 * 32;
+  const int threads = T <= 256 ? 256 : (T + 31) / 32 * 32;
   launch_pdl(prefix_plan_kernel, 1, threads, 0, (cudaStream_t)stream, d_row_slot, T, d_prefix_id, d_prefix_len, n_slots, tile_rows(rep), Hkv,
              target, (int)max_parts(T, rep, Hkv, target), d_plan, max_rows);
   count_launch();

@@ -997,7 +997,10 @@ class PrefixPlan:
         if not 0 < max_rows <= PREFIX_PLAN_MAX_ROWS:
             raise ValueError(f"mlora: a prefix plan holds 1 to {PREFIX_PLAN_MAX_ROWS} rows")
         self.max_rows, self.Hq, self.Hkv, self.T = int(max_rows), int(Hq), int(Hkv), 0
-        self.table = torch.zeros(_lib.lib().mlora_prefix_plan_bytes(self.max_rows) // 4, dtype=torch.int32, device=device)
+        n = _lib.lib().mlora_prefix_plan_bytes(self.max_rows, self.Hkv)
+        if not n:
+            raise ValueError(f"mlora: no prefix plan for {Hkv} key heads")
+        self.table = torch.zeros(n // 4, dtype=torch.int32, device=device)
 
 
 def prefix_plan(row_slot, prefix_id, prefix_len, plan: PrefixPlan):
