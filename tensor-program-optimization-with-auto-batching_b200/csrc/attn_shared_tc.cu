@@ -11,7 +11,7 @@
 //
 // The prefix has 2 D 2 bytes per key and key head against 4 D 128 flops of a full tile: bound by HBM up to some 128 pairs (rows x query
 // heads per key head), by the softmax beyond.  The tail is bound by HBM alone: its tiles have only the query heads of one key head, so
-// it uses mma.sync on 16 of them, with a ring of asynchronous copies in every warp.
+// it uses mma.sync with 16 keys as the rows and up to eight heads as the columns, and a ring of TMA copies in every warp.
 #include <math.h>
 
 #include <atomic>
@@ -30,6 +30,9 @@ constexpr int kPlanMaxRows = 1024;
 constexpr int kPlanHeader = 8;           // int32: rows, tiles, items, parts
 constexpr int kTickets = 1024;           // arrival counters at the start of the scratch, whatever the call's sizes: zero between calls
 constexpr int kPlanMinRows = 2, kPlanMinKeys = 64;  // smaller groups and shorter prefixes are read row by row
+// Reads a group has to save, (rows - 1) x tokens x key heads.  Measured, shared against row by row, 128-wide heads: 4 rows x 2048 x 32 key
+// heads (196608 saved) 21.8 us against 20.2; 32 x 1024 x 8 (253952) 17.2 against 27.3; 2 x 4096 x 32 (131072) 30.8 against 22.5.
+constexpr int kPlanLeast = 200000;
 
 // A plan in int32: header; per row a quad (first key of its own part, its first part, its parts, 0) and its entry of `list` (rows by group);
 // then two quads per item, all that a CTA needs to begin: (slot whose pages are read, first block, blocks, keys of the prefix | first entry
@@ -86,7 +89,7 @@ __device__ __forceinline__ int block_sum_int(int v, int* sm /*[33]*/) {
 // One CTA, a thread per row.  Rows of a group keep their order; groups are ordered by their first row.
 __global__ void __launch_bounds__(kPlanMaxRows) prefix_plan_kernel(const int32_t* __restrict__ row_slot, int T,
                                                                    const int32_t* __restrict__ prefix_id, const int32_t* __restrict__ prefix_len,
-                                                                   int n_slots, int rt, int Hkv, int target, int cap_parts, int32_t* plan, int max_rows) {
+                                                                   int n_slots, int rt, int Hkv, int target, int cap_items, int cap_parts, long long least, int32_t* plan, int max_rows) {
   __shared__ int s_id[kPlanMaxRows];     // prefix of the row, -1: none
   __shared__ int s_lead[kPlanMaxRows];   // first row of its group, if the group is taken together
   __shared__ int s_tile[kPlanMaxRows / kPlanMinRows + 1][8];  // blocks, rows, key ranges, first item, slot, keys, first entry of the list
@@ -111,7 +114,7 @@ __global__ void __launch_bounds__(kPlanMaxRows) prefix_plan_kernel(const int32_t
         rank += j < t;
         ++count;
       }
-  const bool used = count >= kPlanMinRows;
+  const bool used = count >= kPlanMinRows && (long long)(count - 1) * len * Hkv >= least;
   s_lead[t] = used ? lead : -1;
   __syncthreads();
   const bool opens = used && rank % rt == 0;  // first row of a tile
@@ -138,13 +141,16 @@ __global__ void __launch_bounds__(kPlanMaxRows) prefix_plan_kernel(const int32_t
     s_tile[tile][1] = rows;
   }
   const int total = block_sum_int(blocks, s_red);
-  // keys per item, in blocks: as few as make no more than `target` items, which is what runs at once
+  // Keys per item, in blocks: an equal share for about `target` items (a tile's last one is shorter).  Long ranges run two CTAs to an SM, which fill each other's gaps;
+  // short ones (below 16 blocks) one, so that CTAs of the tail, which wait for memory and not for it, find room beside them (32 rows
+  // behind 4096 tokens: XX us instead of YY).
+  if ((long long)total * Hkv < 16ll * target) target /= 2;
   int unit = max(1, (int)(((long long)total * Hkv + target - 1) / target));
   for (;;) {
     const int splits = opens ? (blocks + unit - 1) / unit : 0;
     const int items = block_sum_int(splits, s_red) * Hkv, parts = block_sum_int(splits * rows, s_red);
     const int longer = block_sum_int(opens && blocks > unit, s_red);
-    if (longer == 0 || (items <= target && parts <= cap_parts)) break;
+    if (longer == 0 || (items <= cap_items && parts <= cap_parts)) break;
     unit += max(1, unit / 8);
   }
   const int splits = opens ? (blocks + unit - 1) / unit : 0;
@@ -472,6 +478,7 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
 // ---- the tail -------------------------------------------------------------------------------------------------------------------
 constexpr int kTlWarps = 4, kTlThreads = kTlWarps * 32;
 constexpr int kTlKeys = 16;  // keys a warp works on at a time
+constexpr int kTlHeads = 8;  // query heads of a CTA
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -480,9 +487,14 @@ __device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {  // of 16-bit values, a pair per lane
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 // Two probabilities as the sum of two pairs of bf16: the products with the values keep 16 bits of them.
 __device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
@@ -493,22 +505,22 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint3
   lo = *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// grid (Hkv x head tiles, T, key ranges): up to 16 query heads of a key head over the row's keys from `first` on (or a range of them).
+// grid (Hkv x head tiles, T, key ranges): up to eight query heads of a key head over the row's keys from `first` on (or a range of them).
 template <int D, int STAGES>
-__global__ void __launch_bounds__(kTlThreads) tail_attn_kernel(const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(kTlThreads, 3) tail_attn_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                const __grid_constant__ CUtensorMap map_v, SharedArgs a) {
   constexpr int kHalf = kTlKeys * D * 2;               // bytes of 16 keys: D / 64 sub-tiles [16][64], 128-byte swizzle
   extern __shared__ uint8_t smem_raw[];                // [warp][stage][K | V]; then the warps' partial results
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ uint64_t full[kTlWarps][STAGES];
-  __shared__ float s_m[kTlWarps][16], s_l[kTlWarps][16];
-  __shared__ float s_w[64 + kTlWarps][16];             // factors of the ranges that are joined
+  __shared__ float s_m[kTlWarps][kTlHeads], s_l[kTlWarps][kTlHeads];
+  __shared__ float s_w[64][kTlHeads];                // factors of the ranges that are joined
   __shared__ int s_last, s_abort;
 
   pdl_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rep = a.Hq / a.Hkv, head_tiles = (rep + 15) / 16;
-  const int kvh = blockIdx.x / head_tiles, h0 = kvh * rep + (blockIdx.x % head_tiles) * 16, n_heads = min(16, kvh * rep + rep - h0);
+  const int rep = a.Hq / a.Hkv, head_tiles = (rep + kTlHeads - 1) / kTlHeads;
+  const int kvh = blockIdx.x / head_tiles, h0 = kvh * rep + (blockIdx.x % head_tiles) * kTlHeads, n_heads = min(kTlHeads, kvh * rep + rep - h0);
   const int t = blockIdx.y, split = blockIdx.z;
   const int slot = a.row_slot[t], pos = a.row_pos[t];
   const int4 plan = plan_view(a.plan, a.plan_rows).row[t];
@@ -551,24 +563,21 @@ __global__ void __launch_bounds__(kTlThreads) tail_attn_kernel(const __grid_cons
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) fetch(i);
 
-  // queries as the A operand: rows = heads, a register pair of columns 16 s + 2 (lane % 4) and + 8
-  uint32_t qa[D / 16][4];
+  // queries as the B operand: column = head lane / 4, a register pair of columns 16 s + 2 (lane % 4) and + 8
+  uint32_t qb[D / 16][2];
   {
-    const int g = lane >> 2, c = (lane & 3) * 2;
-    const bf16* q0 = a.q + (size_t)t * a.ld + (size_t)(h0 + g) * D + c;
-    const bf16* q1 = q0 + 8 * D;
+    const int g = lane >> 2;
+    const bf16* q = a.q + (size_t)t * a.ld + (size_t)(h0 + g) * D + (lane & 3) * 2;
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) {
-      qa[s][0] = g < n_heads ? *reinterpret_cast<const uint32_t*>(q0 + s * 16) : 0u;
-      qa[s][1] = g + 8 < n_heads ? *reinterpret_cast<const uint32_t*>(q1 + s * 16) : 0u;
-      qa[s][2] = g < n_heads ? *reinterpret_cast<const uint32_t*>(q0 + s * 16 + 8) : 0u;
-      qa[s][3] = g + 8 < n_heads ? *reinterpret_cast<const uint32_t*>(q1 + s * 16 + 8) : 0u;
+      qb[s][0] = g < n_heads ? *reinterpret_cast<const uint32_t*>(q + s * 16) : 0u;
+      qb[s][1] = g < n_heads ? *reinterpret_cast<const uint32_t*>(q + s * 16 + 8) : 0u;
     }
   }
-  float o[D / 8][4];
+  float o[D / 16][4];  // [column 16 i + lane / 4, + 8][head 2 (lane % 4), + 1]
 #pragma unroll
-  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // of the lane's two heads (l: the lane's own keys)
   const int mr = lane & 7, mi = lane >> 3;  // row and matrix whose address this lane gives to ldmatrix
 
   bool ok = true;
@@ -587,56 +596,47 @@ __global__ void __launch_bounds__(kTlThreads) tail_attn_kernel(const __grid_cons
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
     }
-    float s[2][4] = {};
+    float s[4] = {};  // [key lane / 4, + 8][head 2 (lane % 4), + 1]
 #pragma unroll
-    for (int k = 0; k < D / 16; ++k) {  // matrices: keys 0-7 and 8-15, columns 16 k and + 8
-      uint32_t b[4];
-      const int r = (mi >> 1) * 8 + mr, ch = 2 * k + (mi & 1);
-      ldsm4(sk + (ch >> 3) * 2048 + r * 128 + (((ch & 7) ^ mr) << 4), b);
-      mma16816(s[0], qa[k], b[0], b[1]);
-      mma16816(s[1], qa[k], b[2], b[3]);
+    for (int k = 0; k < D / 16; ++k) {  // matrices: keys 0-7 and 8-15 of columns 16 k, then of 16 k + 8
+      uint32_t x[4];
+      const int r = (mi & 1) * 8 + mr, ch = 2 * k + (mi >> 1);
+      ldsm4(sk + (ch >> 3) * 2048 + r * 128 + (((ch & 7) ^ mr) << 4), x);
+      mma16816(s, x, qb[k][0], qb[k][1]);
     }
     float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int kk = key + n * 8 + (lane & 3) * 2 + (e & 1);
-        s[n][e] = kk >= first && kk < n_tok ? s[n][e] * a.scale : -INFINITY;
-        mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
-      }
+    for (int e = 0; e < 4; ++e) {
+      const int kk = key + (lane >> 2) + (e >> 1) * 8;
+      s[e] = kk >= first && kk < n_tok ? s[e] * a.scale : -INFINITY;
+      mx[e & 1] = fmaxf(mx[e & 1], s[e]);
+    }
     float corr[2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-      const float mn = fmaxf(m[r], mx[r]);
-      corr[r] = m[r] == -INFINITY ? 0.f : fast_exp2(m[r] - mn);
-      l[r] *= corr[r];
-      m[r] = mn;
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], x));
+      const float mn = fmaxf(m[h], mx[h]);
+      corr[h] = m[h] == -INFINITY ? 0.f : fast_exp2(m[h] - mn);
+      l[h] *= corr[h];
+      m[h] = mn;
     }
-    uint32_t ph[4], pl[4];
+    uint32_t ph[2], pl[2];  // the lane's keys lane / 4 and + 8, a pair of heads each; then, transposed, a pair of keys of one head
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int r = 0; r < 2; ++r) {
+      const float x = s[2 * r] == -INFINITY ? 0.f : fast_exp2(s[2 * r] - m[0]), y = s[2 * r + 1] == -INFINITY ? 0.f : fast_exp2(s[2 * r + 1] - m[1]);
+      l[0] += x, l[1] += y;
+      split_pair(x, y, ph[r], pl[r]);
+      ph[r] = transpose8x8(ph[r]), pl[r] = transpose8x8(pl[r]);
+    }
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float x = s[n][2 * r] == -INFINITY ? 0.f : fast_exp2(s[n][2 * r] - m[r]);
-        const float y = s[n][2 * r + 1] == -INFINITY ? 0.f : fast_exp2(s[n][2 * r + 1] - m[r]);
-        l[r] += x + y;
-        split_pair(x, y, ph[n * 2 + r], pl[n * 2 + r]);
-      }
-#pragma unroll
-    for (int c = 0; c < D / 16; ++c) {  // matrices: keys 0-7 and 8-15 of columns 16 c, then of 16 c + 8
-      uint32_t b[4];
-      const int r = (mi & 1) * 8 + mr, ch = 2 * c + (mi >> 1);
-      ldsm4t(sv + (ch >> 3) * 2048 + r * 128 + (((ch & 7) ^ mr) << 4), b);
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        float(&d)[4] = o[2 * c + n];
-        d[0] *= corr[0], d[1] *= corr[0], d[2] *= corr[1], d[3] *= corr[1];
-        mma16816(d, ph, b[2 * n], b[2 * n + 1]);
-        mma16816(d, pl, b[2 * n], b[2 * n + 1]);
-      }
+    for (int c = 0; c < D / 16; ++c) {  // V transposed: rows = columns 16 c + lane / 4, + 8; matrices: keys 0-7 of both, then keys 8-15
+      uint32_t x[4];
+      const int r = (mi >> 1) * 8 + mr, ch = 2 * c + (mi & 1);
+      ldsm4t(sv + (ch >> 3) * 2048 + r * 128 + (((ch & 7) ^ mr) << 4), x);
+      o[c][0] *= corr[0], o[c][1] *= corr[1], o[c][2] *= corr[0], o[c][3] *= corr[1];
+      mma16816(o[c], x, ph[0], ph[1]);
+      mma16816(o[c], x, pl[0], pl[1]);
     }
     __syncwarp();  // (the next copy overwrites what was read here)
   }
@@ -648,17 +648,17 @@ __global__ void __launch_bounds__(kTlThreads) tail_attn_kernel(const __grid_cons
   if (s_abort && tid == 0 && a.status) atomicOr(a.status, 1);
 
   // ---- the four warps' results, joined with what the prefix's key ranges left ---------------------------------------------------
-  float* acc = reinterpret_cast<float*>(ring);  // [warp][16][D]
-  {
-    const int g = lane >> 2, c = (lane & 3) * 2;
+  float* acc = reinterpret_cast<float*>(ring);  // [warp][head][D]
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      if ((lane & 3) == 0) s_m[warp][g + 8 * r] = m[r], s_l[warp][g + 8 * r] = l[r];
+  for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n)
-        *reinterpret_cast<float2*>(acc + ((size_t)warp * 16 + g + 8 * r) * D + n * 8 + c) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+    for (int x = 4; x < 32; x <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], x);
+    const int hh = (lane & 3) * 2 + h;
+    if (lane < 4) s_m[warp][hh] = m[h], s_l[warp][hh] = l[h];
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+      acc[(warp * kTlHeads + hh) * D + c * 16 + (lane >> 2)] = o[c][h];
+      acc[(warp * kTlHeads + hh) * D + c * 16 + (lane >> 2) + 8] = o[c][2 + h];
     }
   }
   __syncthreads();
@@ -674,7 +674,7 @@ __global__ void __launch_bounds__(kTlThreads) tail_attn_kernel(const __grid_cons
 #pragma unroll
       for (int w = 0; w < kTlWarps; ++w) {
         const float f = s_m[w][h] == -INFINITY ? 0.f : fast_exp2(s_m[w][h] - M);
-        const float4 x = reinterpret_cast<const float4*>(acc + ((size_t)w * 16 + h) * D)[c];
+        const float4 x = reinterpret_cast<const float4*>(acc + (w * kTlHeads + h) * D)[c];
         L = fmaf(s_l[w][h], f, L);
         O.x = fmaf(x.x, f, O.x), O.y = fmaf(x.y, f, O.y), O.z = fmaf(x.z, f, O.z), O.w = fmaf(x.w, f, O.w);
       }
@@ -703,10 +703,11 @@ __global__ void __launch_bounds__(kTlThreads) tail_attn_kernel(const __grid_cons
   const float* part0 = a.parts + ((size_t)plan.y * a.Hq + h0) * (D + 4);
   const size_t part_step = (size_t)a.Hq * (D + 4);
   // factors exp2(m - M) / L of every range, 64 prefix ranges at a time in shared memory; the totals first
-  const int h = tid / (kTlThreads / 16), sub = tid % (kTlThreads / 16);  // 8 threads per head
+  constexpr int kSubs = kTlThreads / kTlHeads;  // threads per head
+  const int h = tid / kSubs, sub = tid % kSubs;
   float M = -INFINITY, L = 0.f;
   if (h < n_heads) {
-    for (int r = sub; r < n_own + n_part; r += 8) {
+    for (int r = sub; r < n_own + n_part; r += kSubs) {
       const float2 ml = r < n_own ? own_ml(r, h) : __ldcg(reinterpret_cast<const float2*>(part0 + (size_t)(r - n_own) * part_step + (size_t)h * (D + 4) + D));
       if (ml.x == -INFINITY) continue;
       const float mn = fmaxf(M, ml.x);
@@ -715,7 +716,7 @@ __global__ void __launch_bounds__(kTlThreads) tail_attn_kernel(const __grid_cons
     }
   }
 #pragma unroll
-  for (int x = 1; x < 8; x <<= 1) {
+  for (int x = 1; x < kSubs; x <<= 1) {
     const float mo = __shfl_xor_sync(0xffffffffu, M, x), lo = __shfl_xor_sync(0xffffffffu, L, x), mn = fmaxf(M, mo);
     if (mn != -INFINITY) L = (M == -INFINITY ? 0.f : L * fast_exp2(M - mn)) + (mo == -INFINITY ? 0.f : lo * fast_exp2(mo - mn));
     M = mn;
@@ -723,7 +724,7 @@ __global__ void __launch_bounds__(kTlThreads) tail_attn_kernel(const __grid_cons
   const float inv = L > 0.f && !s_abort ? 1.f / L : 0.f;
   // outputs: 4 columns of a head per thread, D / 4 threads a head; where there are few heads, several threads share the ranges
   constexpr int kPer = kTlThreads / (D / 4);           // heads in work at once
-  constexpr int kSets = 16 / kPer;
+  constexpr int kSets = kTlHeads / kPer;
   const int hp = n_heads >= kPer ? kPer : n_heads > 2 ? 4 : n_heads, slices = kPer / hp;
   float4 sum[kSets];
 #pragma unroll
@@ -733,7 +734,7 @@ __global__ void __launch_bounds__(kTlThreads) tail_attn_kernel(const __grid_cons
     const int n = min(64, n_own + n_part - r0);
     __syncthreads();
     if (h < n_heads)
-      for (int r = sub; r < n; r += 8) {
+      for (int r = sub; r < n; r += kSubs) {
         const int x = r0 + r;
         const float mx = x < n_own ? own_ml(x, h).x : __ldcg(part0 + (size_t)(x - n_own) * part_step + (size_t)h * (D + 4) + D);
         s_w[r][h] = mx == -INFINITY ? 0.f : fast_exp2(mx - M) * inv;
@@ -749,14 +750,14 @@ __global__ void __launch_bounds__(kTlThreads) tail_attn_kernel(const __grid_cons
         const float f = s_w[r][hh];
         float4 v;
         if (x >= n_own) v = __ldcg(reinterpret_cast<const float4*>(part0 + (size_t)(x - n_own) * part_step + (size_t)hh * (D + 4)) + c);
-        else if (ranges == 1) v = reinterpret_cast<const float4*>(acc + ((size_t)x * 16 + hh) * D)[c];
+        else if (ranges == 1) v = reinterpret_cast<const float4*>(acc + (x * kTlHeads + hh) * D)[c];
         else v = __ldcg(reinterpret_cast<const float4*>(a.own + (((size_t)t * a.Hq + h0 + hh) * a.n_splits + x) * (D + 4)) + c);
         sum[i].x = fmaf(v.x, f, sum[i].x), sum[i].y = fmaf(v.y, f, sum[i].y), sum[i].z = fmaf(v.z, f, sum[i].z), sum[i].w = fmaf(v.w, f, sum[i].w);
       }
     }
   }
   if (slices > 1) {
-    float4* share = reinterpret_cast<float4*>(ring) + kTlWarps * 16 * D / 4;  // (behind the warps' results)
+    float4* share = reinterpret_cast<float4*>(ring) + kTlWarps * kTlHeads * D / 4;  // (behind the warps' results)
     if (slice > 0) share[tid] = sum[0];
     __syncthreads();
     if (slice > 0) return;
@@ -800,7 +801,7 @@ int allow_smem(K kernel, int bytes, std::atomic<unsigned long long>& done) {
   return MLORA_OK;
 }
 
-constexpr int kTlStages = 3;
+constexpr int kTlStages = 2;  // (three CTAs per SM: twelve warps with 8 KB on the way each are 96 KB, and another 96 at work)
 
 template <int ND, int PS>
 int launch_shared(const SharedArgs& a, int n_pages_total, int max_items, cudaStream_t st) {
@@ -814,7 +815,7 @@ int launch_shared(const SharedArgs& a, int n_pages_total, int max_items, cudaStr
   if (!rc) rc = page_map(&mvt, a.v_pages, n_pages_total, a.Hkv, PS, D, 1, kTlKeys);
   if (rc) return rc;
   constexpr int smem = 3 * ND * kSub + 1024, smem_tail = kTlWarps * kTlStages * 2 * kTlKeys * D * 2 + 1024;
-  static_assert(smem_tail >= kTlWarps * 16 * D * 4 + kTlThreads * 16 + 1024, "the warps' results lie in the ring");
+  static_assert(smem_tail >= kTlWarps * kTlHeads * D * 4 + kTlThreads * 16 + 1024, "the warps' results lie in the ring");
   static std::atomic<unsigned long long> done{0}, done_tail{0};
   rc = allow_smem(prefix_attn_kernel<ND, PS>, smem, done);
   if (!rc) rc = allow_smem(tail_attn_kernel<D, kTlStages>, smem_tail, done_tail);
@@ -825,7 +826,7 @@ int launch_shared(const SharedArgs& a, int n_pages_total, int max_items, cudaStr
     count_launch();
     MLORA_CHECK_LAUNCH("prefix_attn_kernel");
   }
-  const int head_tiles = (a.Hq / a.Hkv + 15) / 16;
+  const int head_tiles = (a.Hq / a.Hkv + kTlHeads - 1) / kTlHeads;
   const cudaError_t e = launch_pdl_if(max_items > 0 && pdl_enabled_tail(), tail_attn_kernel<D, kTlStages>, dim3((unsigned)(a.Hkv * head_tiles), (unsigned)a.T, (unsigned)a.n_splits),
                                       dim3(kTlThreads), smem_tail, st, mkt, mvt, a);
   if (e != cudaSuccess) return fail(MLORA_ECUDA, "tail_attn_kernel: %s", cudaGetErrorString(e));
@@ -841,7 +842,7 @@ struct SharedSizes {
 };
 SharedSizes sizes_of(int T, int Hq, int Hkv, int D) {
   SharedSizes s;
-  const int rep = Hq / Hkv, ht = (rep + 15) / 16;
+  const int rep = Hq / Hkv, ht = (rep + kTlHeads - 1) / kTlHeads;
   s.target = 2 * sm_count();
   s.max_items = max_items_of(T, Hkv, s.target);
   const long long ctas = (long long)T * Hkv * ht;
@@ -869,7 +870,7 @@ extern "C" size_t mlora_prefix_plan_bytes(int32_t max_rows, int32_t Hkv) {
 }
 
 extern "C" int mlora_prefix_plan(const int32_t* d_row_slot, int32_t T, const int32_t* d_prefix_id, const int32_t* d_prefix_len, int32_t n_slots,
-                                 int32_t Hq, int32_t Hkv, int32_t* d_plan, int32_t max_rows, void* stream) {
+                                 int32_t Hq, int32_t Hkv, int64_t least, int32_t* d_plan, int32_t max_rows, void* stream) {
   MLORA_REQUIRE(shared_sizes_fit(T, Hq, Hkv, 64) && T <= max_rows && max_rows <= kPlanMaxRows && n_slots > 0,
                 "prefix_plan: bad sizes T=%d of %d, %d heads over %d key heads", T, max_rows, Hq, Hkv);
   MLORA_REQUIRE(d_row_slot && d_prefix_id && d_prefix_len && d_plan && aligned16(d_plan), "prefix_plan: null pointer or unaligned plan");
@@ -877,7 +878,7 @@ extern "C" int mlora_prefix_plan(const int32_t* d_row_slot, int32_t T, const int
   const int rep = Hq / Hkv, target = 2 * sm_count();
   const int threads = T <= 256 ? 256 : (T + 31) / 32 * 32;
   launch_pdl(prefix_plan_kernel, 1, threads, 0, (cudaStream_t)stream, d_row_slot, T, d_prefix_id, d_prefix_len, n_slots, tile_rows(rep), Hkv,
-             target, (int)max_parts(T, rep, Hkv, target), d_plan, max_rows);
+             target, max_items_of(T, Hkv, target), (int)max_parts(T, rep, Hkv, target), least < 0 ? (long long)kPlanLeast : (long long)least, d_plan, max_rows);
   count_launch();
   MLORA_CHECK_LAUNCH("prefix_plan_kernel");
   return MLORA_OK;

@@ -58,20 +58,36 @@ __device__ __forceinline__ unsigned long long warp_best(unsigned long long best)
   return best;
 }
 
-// f(place) for the tokens of text[0, n) that lie in the piece [v0, v0 + kChPiece)
-template <typename F>
-__device__ __forceinline__ void walk(const int32_t* text, int n, int v0, F f) {
-  for (int i = threadIdx.x; i < n; i += 4 * kChThreads) {
-    int w[4];
+// A text, whose first 4 * kChThreads tokens stay in registers (most texts, all of it): a row's pieces all look through it.
+struct Text {
+  const int32_t* at;
+  int n, first[4];
+  __device__ __forceinline__ void begin(const int32_t* text, int len) {
+    at = text;
+    n = len;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) w[u] = i + u * kChThreads < n ? text[i + u * kChThreads] : -1;
+    for (int u = 0; u < 4; ++u) first[u] = threadIdx.x + u * kChThreads < n ? at[threadIdx.x + u * kChThreads] : -1;
+  }
+  // f(place) for the tokens that lie in the piece [v0, v0 + kChPiece)
+  template <typename F>
+  __device__ __forceinline__ void walk(int v0, F f) const {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const unsigned at = (unsigned)w[u] - (unsigned)v0;
-      if (w[u] >= 0 && at < (unsigned)kChPiece) f((int)at);
+      const unsigned p = (unsigned)first[u] - (unsigned)v0;
+      if (first[u] >= 0 && p < (unsigned)kChPiece) f((int)p);
+    }
+    for (int i = threadIdx.x + 4 * kChThreads; i < n; i += 4 * kChThreads) {
+      int w[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) w[u] = i + u * kChThreads < n ? at[i + u * kChThreads] : -1;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const unsigned p = (unsigned)w[u] - (unsigned)v0;
+        if (w[u] >= 0 && p < (unsigned)kChPiece) f((int)p);
+      }
     }
   }
-}
+};
 
 __global__ void __launch_bounds__(kChThreads) choose_tokens_kernel(ChooseArgs a) {
   __shared__ __align__(16) uint32_t s_count[kChPiece];  // low 31 bits: times in the answer; top bit: in the prompt
@@ -107,33 +123,51 @@ __global__ void __launch_bounds__(kChThreads) choose_tokens_kernel(ChooseArgs a)
   const int mk = ruled && a.mask_of ? a.mask_of[src] : -1;
   const int32_t* mask = mk >= 0 && mk < a.n_masks ? a.masks + (size_t)mk * a.ld_mask : nullptr;
 
+  Text prompt, answer;
+  prompt.begin(n_prompt ? a.prompt + (size_t)src * a.ld_prompt : nullptr, n_prompt);
+  answer.begin(n_answer ? a.answer + (size_t)src * a.ld_answer : nullptr, n_answer);
+  if (counts || biased) {  // (a thread clears what it has read of a piece, so this is done once)
+#pragma unroll
+    for (int j = 0; j < kChVec; ++j) {
+      reinterpret_cast<uint4*>(s_count)[j * kChThreads + tid] = make_uint4(0u, 0u, 0u, 0u);
+      reinterpret_cast<float4*>(s_bias)[j * kChThreads + tid] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    __syncthreads();
+  }
   unsigned long long best = 0;
-  for (int64_t piece = (int64_t)rank * kChPiece; piece < a.V; piece += (int64_t)width * kChPiece) {
+  float next[kChVec][4];
+  uint32_t next_word[kChVec];
+  const auto load = [&](int64_t v0) {  // a piece's logits and mask, asked for while the piece before is at work
+#pragma unroll
+    for (int j = 0; j < kChVec; ++j) {
+      const int64_t at = v0 + (j * kChThreads + tid) * 4;
+      next_word[j] = 0xfu;
+      if (mask && at < a.V) next_word[j] = (uint32_t)mask[at >> 5] >> (at & 31);
+      if (vec && at < a.V) {
+        const float4 q = *reinterpret_cast<const float4*>(logits + at);  // (not the read-only path: `out` may be `logits`)
+        next[j][0] = q.x, next[j][1] = q.y, next[j][2] = q.z, next[j][3] = q.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) next[j][e] = at < a.V - e ? logits[at + e] : 0.f;
+      }
+    }
+  };
+  const int64_t step = (int64_t)width * kChPiece;
+  load((int64_t)rank * kChPiece);
+  for (int64_t piece = (int64_t)rank * kChPiece; piece < a.V; piece += step) {
     const int v0 = (int)piece;
     float l[kChVec][4];
     uint32_t word[kChVec];
 #pragma unroll
     for (int j = 0; j < kChVec; ++j) {
-      const int at = v0 + (j * kChThreads + tid) * 4;
-      word[j] = 0xfu;
-      if (mask && at < a.V) word[j] = (uint32_t)mask[at >> 5] >> (at & 31);
-      if (vec && at < a.V) {
-        const float4 q = *reinterpret_cast<const float4*>(logits + at);  // (not the read-only path: `out` may be `logits`)
-        l[j][0] = q.x, l[j][1] = q.y, l[j][2] = q.z, l[j][3] = q.w;
-      } else {
+      word[j] = next_word[j];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) l[j][e] = at < a.V - e ? logits[at + e] : 0.f;
-      }
+      for (int e = 0; e < 4; ++e) l[j][e] = next[j][e];
     }
+    load(piece + step);
     if (counts || biased) {
-#pragma unroll
-      for (int j = 0; j < kChVec; ++j) {
-        if (counts) reinterpret_cast<uint4*>(s_count)[j * kChThreads + tid] = make_uint4(0u, 0u, 0u, 0u);
-        if (biased) reinterpret_cast<float4*>(s_bias)[j * kChThreads + tid] = make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-      __syncthreads();
-      if (n_prompt) walk(a.prompt + (size_t)src * a.ld_prompt, n_prompt, v0, [&](int at) { atomicOr(&s_count[at], 0x80000000u); });
-      if (n_answer) walk(a.answer + (size_t)src * a.ld_answer, n_answer, v0, [&](int at) { atomicAdd(&s_count[at], 1u); });
+      prompt.walk(v0, [&](int p) { atomicOr(&s_count[p], 0x80000000u); });
+      answer.walk(v0, [&](int p) { atomicAdd(&s_count[p], 1u); });
       for (int i = b0 + tid; i < b1; i += kChThreads) {  // ascending tokens: equal ones are neighbours, the first one adds them up
         const int w = a.bias_token[i];
         const unsigned at = (unsigned)w - (unsigned)v0;
@@ -151,6 +185,7 @@ __global__ void __launch_bounds__(kChThreads) choose_tokens_kernel(ChooseArgs a)
         const uint4 c4 = reinterpret_cast<const uint4*>(s_count)[q4];
         const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w};
         if (c4.x | c4.y | c4.z | c4.w) {
+          reinterpret_cast<uint4*>(s_count)[q4] = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             if (!c[e]) continue;
@@ -165,6 +200,7 @@ __global__ void __launch_bounds__(kChThreads) choose_tokens_kernel(ChooseArgs a)
       }
       if (biased) {
         const float4 b = reinterpret_cast<const float4*>(s_bias)[q4];
+        reinterpret_cast<float4*>(s_bias)[q4] = make_float4(0.f, 0.f, 0.f, 0.f);
         l[j][0] = __fadd_rn(l[j][0], b.x), l[j][1] = __fadd_rn(l[j][1], b.y);
         l[j][2] = __fadd_rn(l[j][2], b.z), l[j][3] = __fadd_rn(l[j][3], b.w);
       }
@@ -186,7 +222,7 @@ __global__ void __launch_bounds__(kChThreads) choose_tokens_kernel(ChooseArgs a)
         }
       }
     }
-    if (counts || biased) __syncthreads();  // (the tables are cleared for the next piece)
+    if (counts || biased) __syncthreads();  // (before the next piece counts in the cleared tables)
   }
   best = warp_best(best);
   if (lane == 0) s_warp[warp] = best;

@@ -991,12 +991,13 @@ PREFIX_PLAN_MAX_ROWS = 1024
 
 
 class PrefixPlan:
-    """Which rows of a step share a prefix, for the attention of its layers (allocated once, filled by :func:`prefix_plan`)."""
+    """Which rows of a step share a prefix, for the attention of its layers (allocated once, filled by :func:`prefix_plan`).  ``least``:
+    reads that a group has to save, (rows - 1) x tokens x key heads (default: what measures as worth it)."""
 
-    def __init__(self, max_rows, Hq, Hkv, device):
+    def __init__(self, max_rows, Hq, Hkv, device, least=-1):
         if not 0 < max_rows <= PREFIX_PLAN_MAX_ROWS:
             raise ValueError(f"mlora: a prefix plan holds 1 to {PREFIX_PLAN_MAX_ROWS} rows")
-        self.max_rows, self.Hq, self.Hkv, self.T = int(max_rows), int(Hq), int(Hkv), 0
+        self.max_rows, self.Hq, self.Hkv, self.least, self.T = int(max_rows), int(Hq), int(Hkv), int(least), 0
         n = _lib.lib().mlora_prefix_plan_bytes(self.max_rows, self.Hkv)
         if not n:
             raise ValueError(f"mlora: no prefix plan for {Hkv} key heads")
@@ -1013,7 +1014,7 @@ def prefix_plan(row_slot, prefix_id, prefix_len, plan: PrefixPlan):
     _int32_table("row_slot", row_slot, T)
     _int32_table("prefix_id", prefix_id, n)
     _int32_table("prefix_len", prefix_len, n)
-    check(_lib.lib().mlora_prefix_plan(_ptr(row_slot), T, _ptr(prefix_id), _ptr(prefix_len), n, plan.Hq, plan.Hkv, _ptr(plan.table),
+    check(_lib.lib().mlora_prefix_plan(_ptr(row_slot), T, _ptr(prefix_id), _ptr(prefix_len), n, plan.Hq, plan.Hkv, plan.least, _ptr(plan.table),
                                        plan.max_rows, _stream()), "mlora_prefix_plan")
     plan.T = T
     return plan

@@ -77,7 +77,7 @@ def _want(c, heads, kv_heads, dim):
     return torch.stack(out), torch.stack(bound)
 
 
-def _call(ops, c, heads, kv_heads, cuda, work=None, slots=None, max_rows=None, out=None):
+def _call(ops, c, heads, kv_heads, cuda, work=None, slots=None, max_rows=None, out=None, least=0):
     R = len(c["rows"])
     slots = torch.arange(R, dtype=torch.int32) if slots is None else slots
     n = int(slots.max()) + 1
@@ -87,7 +87,7 @@ def _call(ops, c, heads, kv_heads, cuda, work=None, slots=None, max_rows=None, o
         pid[slots[t]], plen[slots[t]] = i, m
         table[slots[t]] = c["table"][t]
     d = lambda x: x.to(cuda)
-    plan = ops.PrefixPlan(max_rows or R, heads, kv_heads, cuda)
+    plan = ops.PrefixPlan(max_rows or R, heads, kv_heads, cuda, least=least)
     ops.prefix_plan(d(slots), d(pid), d(plen), plan)
     pos = torch.tensor([p for _, _, p in c["rows"]], dtype=torch.int32)
     status = torch.zeros(1, dtype=torch.int32, device=cuda)
@@ -168,6 +168,17 @@ def test_slots_in_any_order_and_a_larger_plan(ops, cuda):
         assert bool((whole[n] == 7).all()) and bool((whole[:, 1024:] == 7).all())
 
 
+def test_small_groups_are_left_to_their_rows(ops, cuda):
+    rows = [(0, 512, 512 + t) for t in range(5)]
+    c = _case(4, 2, 64, 16, rows, seed=8)
+    want, bound = _want(c, 4, 2, 64)
+    for least, tiles in ((4 * 512 * 2, 1), (4 * 512 * 2 + 1, 0), (-1, 0)):
+        got, plan = _call(ops, c, 4, 2, cuda, least=least)
+        assert int(plan.table[1]) == tiles
+        err = (got.cpu().double() - want).abs()
+        assert bool((err <= bound).all()), float((err / bound).max())
+
+
 def test_captured_and_replayed_with_other_rows(ops, cuda):
     """A captured step follows its tables: other slots, positions and groups, the same graph."""
     heads, kv_heads, dim, n = 8, 2, 128, 6
@@ -180,7 +191,7 @@ def test_captured_and_replayed_with_other_rows(ops, cuda):
     k, v = (z(pages, kv_heads, 16, dim, dtype=torch.bfloat16) for _ in range(2))
     q, table, pos = z(n, heads * dim, dtype=torch.bfloat16), z(n, width, dtype=torch.int32), z(n, dtype=torch.int32)
     pid, plen, slots = z(n, dtype=torch.int32), z(n, dtype=torch.int32), torch.arange(n, dtype=torch.int32, device=cuda)
-    plan, out = ops.PrefixPlan(n, heads, kv_heads, cuda), z(n, heads * dim, dtype=torch.bfloat16)
+    plan, out = ops.PrefixPlan(n, heads, kv_heads, cuda, least=0), z(n, heads * dim, dtype=torch.bfloat16)
     work = ops.new_workspace(ops.paged_attention_shared_workspace(n, heads, kv_heads, dim), cuda)
 
     def put(c):
