@@ -697,7 +697,7 @@ int mlora_paged_attention_shared(const void* d_q, int64_t ld, const void* d_k_pa
  *       l = l > 0 ? l / repetition[s] : l * repetition[s]
  *   c = how often the answer has v:  l = l - frequency[s] * c;  l = l - presence[s] where c > 0
  *   l = l + bias of v in set b = d_bias_set[s] (outside 0..n_sets-1: none): entries d_bias_start[b] .. d_bias_start[b + 1] of
- *       d_bias_token / d_bias_value [n_bias], ascending tokens (a token that is there twice gets the sum)
+ *       d_bias_token / d_bias_value [n_bias], in ascending order of tokens (one that is there twice gets the sum)
  *   l = -inf where bit v % 32 of d_masks[d_mask_of[s] * ld_mask + v / 32] is 0 (mask_of outside 0..n_masks-1: everything is allowed)
  * tok -1: no logit above -inf (a mask that allows nothing); NaN never wins, except that a mask turns it into -inf like any other.
  * d_logits_out (optional, row stride ld_out, may be d_logits): the logits after the rules.  Every table may be NULL with its

@@ -1,11 +1,12 @@
 // The next token of every row under the rules of its request: penalties for tokens that its text already has, biases, and a mask of
 // what its grammar allows (llama_exec_graph.py:134-137 picks the largest logit on the host; the rules have no reference counterpart).
 //
-// A cluster of up to eight CTAs shares a row.  A CTA takes pieces of 4096 tokens of the vocabulary: it asks for the piece's logits
-// first (eight a thread, in registers), then walks the row's text and counts in shared memory which of the piece's tokens occur how
-// often -- a table of counts in global memory would be another 4 bytes per token and row to read, the text is a few KB that the
-// row's CTAs find in L2 --, spreads the row's biases the same way, and only then touches the logits.  The best of a CTA is one
-// 64-bit key (value, then lowest index), so the order in which keys meet does not matter; the cluster's first CTA collects them
+// A cluster of up to eight CTAs shares a row.  A CTA takes pieces of 4096 tokens of the vocabulary: it asks for the piece's logits (eight
+// a thread, in registers; three CTAs on an SM have 48 KB on their way), then it looks through the row's text and counts in shared memory
+// which of the piece's tokens occur how often -- a table of counts in global memory would be another 4 bytes per token and row to read,
+// the text is a few KB that stays in registers --, marks the tokens that have a bias (which stay in registers too) and only then
+// touches the logits.  The best of a thread is kept as it goes, a later one only if it is larger, so the lowest index
+// wins; between threads a 64-bit key of value and index decides, in any order, and the cluster's first CTA collects the CTAs' keys
 // through distributed shared memory: one launch, no scratch.  Values are rounded step by step as the formula is written (no
 // contraction), so that the choice at a near tie is that of plain 32-bit arithmetic.
 #include "common.cuh"
@@ -89,9 +90,9 @@ struct Text {
   }
 };
 
-__global__ void __launch_bounds__(kChThreads) choose_tokens_kernel(ChooseArgs a) {
-  __shared__ __align__(16) uint32_t s_count[kChPiece];  // low 31 bits: times in the answer; top bit: in the prompt
-  __shared__ __align__(16) float s_bias[kChPiece];
+__global__ void __launch_bounds__(kChThreads, 3) choose_tokens_kernel(ChooseArgs a) {
+  __shared__ __align__(16) uint32_t s_count[kChPiece];  // low 30 bits: times in the answer; then: has a bias, is in the prompt
+  __shared__ float s_bias[kChPiece];                    // of the tokens that have one
   __shared__ unsigned long long s_warp[kChThreads / 32];
   __shared__ int s_best[2];
   pdl_launch_dependents();
@@ -130,88 +131,88 @@ __global__ void __launch_bounds__(kChThreads) choose_tokens_kernel(ChooseArgs a)
 #pragma unroll
     for (int j = 0; j < kChVec; ++j) {
       reinterpret_cast<uint4*>(s_count)[j * kChThreads + tid] = make_uint4(0u, 0u, 0u, 0u);
-      reinterpret_cast<float4*>(s_bias)[j * kChThreads + tid] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     __syncthreads();
   }
-  unsigned long long best = 0;
-  float next[kChVec][4];
-  uint32_t next_word[kChVec];
-  const auto load = [&](int64_t v0) {  // a piece's logits and mask, asked for while the piece before is at work
-#pragma unroll
-    for (int j = 0; j < kChVec; ++j) {
-      const int64_t at = v0 + (j * kChThreads + tid) * 4;
-      next_word[j] = 0xfu;
-      if (mask && at < a.V) next_word[j] = (uint32_t)mask[at >> 5] >> (at & 31);
-      if (vec && at < a.V) {
-        const float4 q = *reinterpret_cast<const float4*>(logits + at);  // (not the read-only path: `out` may be `logits`)
-        next[j][0] = q.x, next[j][1] = q.y, next[j][2] = q.z, next[j][3] = q.w;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) next[j][e] = at < a.V - e ? logits[at + e] : 0.f;
-      }
+  // the row's biases, one per thread, in ascending order of tokens: of equal ones the first has the sum
+  const auto bias_at = [&](int i, int& w, float& sum) {
+    w = i < b1 ? a.bias_token[i] : -1;
+    if (w < 0 || (i > b0 && a.bias_token[i - 1] == w)) {
+      w = -1;
+      return;
+    }
+    sum = a.bias_value[i];
+    for (int k = i + 1; k < b1 && a.bias_token[k] == w; ++k) sum += a.bias_value[k];
+  };
+  const auto set_bias = [&](int w, float value, int v0) {
+    const unsigned at = (unsigned)w - (unsigned)v0;
+    if (w >= 0 && at < (unsigned)kChPiece) {
+      atomicOr(&s_count[at], 0x40000000u);
+      s_bias[at] = value;
     }
   };
-  const int64_t step = (int64_t)width * kChPiece;
-  load((int64_t)rank * kChPiece);
-  for (int64_t piece = (int64_t)rank * kChPiece; piece < a.V; piece += step) {
+  int bias_w = -1;
+  float bias_v = 0.f;
+  if (biased) bias_at(b0 + tid, bias_w, bias_v);
+  float best_v = -INFINITY;  // (not a number, or not allowed: never above it)
+  int best_i = 0;
+  for (int64_t piece = (int64_t)rank * kChPiece; piece < a.V; piece += (int64_t)width * kChPiece) {
     const int v0 = (int)piece;
     float l[kChVec][4];
     uint32_t word[kChVec];
 #pragma unroll
     for (int j = 0; j < kChVec; ++j) {
-      word[j] = next_word[j];
+      const int at = v0 + (j * kChThreads + tid) * 4;
+      word[j] = 0xfu;
+      if (mask && at < a.V) word[j] = (uint32_t)mask[at >> 5] >> (at & 31);
+      if (vec && at < a.V) {
+        const float4 q = *reinterpret_cast<const float4*>(logits + at);  // (not the read-only path: `out` may be `logits`)
+        l[j][0] = q.x, l[j][1] = q.y, l[j][2] = q.z, l[j][3] = q.w;
+      } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) l[j][e] = next[j][e];
+        for (int e = 0; e < 4; ++e) l[j][e] = at < a.V - e ? logits[at + e] : -INFINITY;
+      }
     }
-    load(piece + step);
     if (counts || biased) {
       prompt.walk(v0, [&](int p) { atomicOr(&s_count[p], 0x80000000u); });
       answer.walk(v0, [&](int p) { atomicAdd(&s_count[p], 1u); });
-      for (int i = b0 + tid; i < b1; i += kChThreads) {  // ascending tokens: equal ones are neighbours, the first one adds them up
-        const int w = a.bias_token[i];
-        const unsigned at = (unsigned)w - (unsigned)v0;
-        if (w < 0 || at >= (unsigned)kChPiece || (i > b0 && a.bias_token[i - 1] == w)) continue;
-        float sum = a.bias_value[i];
-        for (int k = i + 1; k < b1 && a.bias_token[k] == w; ++k) sum += a.bias_value[k];
-        s_bias[at] = sum;
+      set_bias(bias_w, bias_v, v0);
+      for (int i = b0 + kChThreads + tid; i < b1; i += kChThreads) {
+        int w;
+        float value = 0.f;
+        bias_at(i, w, value);
+        set_bias(w, value, v0);
       }
       __syncthreads();
     }
 #pragma unroll
     for (int j = 0; j < kChVec; ++j) {
       const int q4 = j * kChThreads + tid, at = v0 + q4 * 4;
-      if (counts) {
+      if (counts || biased) {
         const uint4 c4 = reinterpret_cast<const uint4*>(s_count)[q4];
-        const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w};
         if (c4.x | c4.y | c4.z | c4.w) {
+          const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w};
           reinterpret_cast<uint4*>(s_count)[q4] = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             if (!c[e]) continue;
             float v = l[j][e];
-            v = v > 0.f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
-            const uint32_t times = c[e] & 0x7fffffffu;
-            v = __fsub_rn(v, __fmul_rn(freq, (float)times));
-            if (times) v = __fsub_rn(v, pres);
+            const uint32_t times = c[e] & 0x3fffffffu;
+            if (times || c[e] >> 31) v = v > 0.f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
+            if (times) v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, (float)times)), pres);
+            if (c[e] & 0x40000000u) v = __fadd_rn(v, s_bias[q4 * 4 + e]);
             l[j][e] = v;
           }
         }
       }
-      if (biased) {
-        const float4 b = reinterpret_cast<const float4*>(s_bias)[q4];
-        reinterpret_cast<float4*>(s_bias)[q4] = make_float4(0.f, 0.f, 0.f, 0.f);
-        l[j][0] = __fadd_rn(l[j][0], b.x), l[j][1] = __fadd_rn(l[j][1], b.y);
-        l[j][2] = __fadd_rn(l[j][2], b.z), l[j][3] = __fadd_rn(l[j][3], b.w);
+      if ((word[j] & 0xfu) != 0xfu) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (!(word[j] >> e & 1u)) l[j][e] = -INFINITY;
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (!(word[j] >> e & 1u)) l[j][e] = -INFINITY;
-        if (at < a.V - e) {
-          const unsigned long long k = choice_key(l[j][e], at + e);
-          best = k > best ? k : best;
-        }
-      }
+      for (int e = 0; e < 4; ++e)
+        if (l[j][e] > best_v) best_v = l[j][e], best_i = at + e;
       if (out && at < a.V) {
         if (vec) {
           *reinterpret_cast<float4*>(out + at) = make_float4(l[j][0], l[j][1], l[j][2], l[j][3]);
@@ -224,7 +225,7 @@ __global__ void __launch_bounds__(kChThreads) choose_tokens_kernel(ChooseArgs a)
     }
     if (counts || biased) __syncthreads();  // (before the next piece counts in the cleared tables)
   }
-  best = warp_best(best);
+  unsigned long long best = warp_best(choice_key(best_v, best_i));
   if (lane == 0) s_warp[warp] = best;
   __syncthreads();
   if (warp == 0) {
@@ -269,8 +270,10 @@ extern "C" int mlora_choose_tokens(const float* d_logits, int64_t ld, int32_t T,
                d_answer_len, ld_answer, d_bias_set, d_bias_start, d_bias_token, d_bias_value, n_sets, n_bias, d_mask_of, d_masks, n_masks,
                ld_mask, d_logits_out, ld_out, d_tok};
   const int pieces = (V + kChPiece - 1) / kChPiece;
+  // CTAs per row: some six per SM (256 rows x 128000 under all rules, in us: one 115, two 120, four 103, eight 108; 32 rows x 32000: one
+  // 21.7, four 8.8, eight 7.6)
   int width = 1;
-  while (width < kChCluster && width < pieces) width *= 2;
+  while (width < kChCluster && width < pieces && (long long)T * width < 6 * 148) width *= 2;
   MLORA_REQUIRE((long long)T * width <= 2147483647ll, "choose_tokens: too many rows");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(T * width));

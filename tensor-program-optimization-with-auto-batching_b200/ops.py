@@ -973,12 +973,18 @@ def delta_step(x, r: DeltaRule, eps, row_slot, row_pos, state, ring, out, status
 # ---------------------------------------------------------------- attention of a batch that shares prefixes
 def _one_device(*ts):
     """Checks that the tensors lie on one CUDA device; None, or a context that makes it the current one."""
-    _need_cuda(*ts)
-    devs = {t.get_device() for t in ts if t is not None}
-    if len(devs) > 1:
-        raise ValueError("mlora: tensors of one call lie on one device")
-    dev = devs.pop()
-    return None if dev == torch.cuda.current_device() else torch.cuda.device(dev)
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        d = t.get_device()
+        if d < 0:
+            raise ValueError("mlora operators need CUDA tensors (there is no CPU path)")
+        if dev is None:
+            dev = d
+        elif d != dev:
+            raise ValueError("mlora: tensors of one call lie on one device")
+    return None if dev is None or dev == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def _int32_table(what, t, *shape):
@@ -1142,6 +1148,18 @@ class LogitRules:
         """Requests that have rules (0: none has any)."""
         return next((t.shape[0] for t in (self.repetition, self.frequency, self.presence, self.bias_set, self.mask_of) if t is not None), 0)
 
+    def __setattr__(self, name, value):
+        object.__setattr__(self, name, value)
+        object.__setattr__(self, "_ready", None)  # (another table: checked again before the next call)
+
+    def _tables(self, V):
+        """(requests, device, arguments of the call), checked once for these tables."""
+        if self._ready is None or self._ready[0] != V:
+            at = _one_device(*(t for t in vars(self).values() if isinstance(t, torch.Tensor)))
+            del at
+            object.__setattr__(self, "_ready", (V, *self._check(V)))
+        return self._ready[1:]
+
     def _check(self, V):
         n = self.n
         for name in ("repetition", "frequency", "presence"):
@@ -1166,19 +1184,29 @@ class LogitRules:
             if self.masks is None or self.masks.dim() != 2 or self.masks.shape[1] < -(-V // 32):
                 raise ValueError(f"mlora: masks must be int32 [any, {-(-V // 32)}]")
             _int32_table("masks", self.masks, None, None)
-        return n
+        sets = 0 if self.bias_set is None else self.bias_start.numel() - 1
+        masks = 0 if self.mask_of is None else self.masks.shape[0]
+        bias = sets > 0 and self.bias_token.numel() > 0
+        pitch = lambda t: t.stride(0) if t is not None else 0
+        device = next((t.get_device() for t in vars(self).values() if isinstance(t, torch.Tensor)), None)
+        return n, device, (
+            n, _ptr(self.repetition), _ptr(self.frequency), _ptr(self.presence), _ptr(self.prompt), _ptr(self.prompt_len), pitch(self.prompt),
+            _ptr(self.answer), _ptr(self.answer_len), pitch(self.answer), _ptr(self.bias_set) if bias else None, _ptr(self.bias_start),
+            _ptr(self.bias_token), _ptr(self.bias_value), sets, self.bias_token.numel() if bias else 0, _ptr(self.mask_of) if masks else None,
+            _ptr(self.masks), masks, pitch(self.masks))
 
 
 def choose_tokens(logits, rules: LogitRules, row_src=None, out=None, logits_out=None):
     """The greedy tokens of the logits under ``rules`` (-1: none is allowed); ``row_src`` int32 [T]: the request of every row (default:
     its own number; outside the rules: none).  ``logits_out``: where the logits after the rules go (may be ``logits``)."""
-    r = rules
-    at = _one_device(logits, row_src, out, logits_out, *vars(r).values())
+    T, V = logits.shape
+    at = _one_device(logits, row_src, out, logits_out)
+    n, device, tables = rules._tables(V)
+    if device is not None and device != logits.get_device():
+        raise ValueError("mlora: tensors of one call lie on one device")
     if at is not None:
         with at:
             return choose_tokens(logits, rules, row_src, out, logits_out)
-    T, V = logits.shape
-    n = r._check(V)
     if out is None:
         out = torch.empty(T, dtype=torch.int32, device=logits.device)
     for t in (logits,) if logits_out is None else (logits, logits_out):
@@ -1189,15 +1217,6 @@ def choose_tokens(logits, rules: LogitRules, row_src=None, out=None, logits_out=
     elif n and T > n:
         raise ValueError(f"mlora: {T} rows, rules of {n} requests: row_src says which")
     _int32_table("out", out, T)
-    sets = 0 if r.bias_set is None else r.bias_start.numel() - 1
-    masks = 0 if r.mask_of is None else r.masks.shape[0]
-    bias = r.bias_set is not None and sets > 0 and r.bias_token.numel() > 0
-    check(_lib.lib().mlora_choose_tokens(
-        _ptr(logits), logits.stride(0), T, V, _ptr(row_src), n, _ptr(r.repetition), _ptr(r.frequency), _ptr(r.presence),
-        _ptr(r.prompt), _ptr(r.prompt_len), r.prompt.stride(0) if r.prompt is not None else 0,
-        _ptr(r.answer), _ptr(r.answer_len), r.answer.stride(0) if r.answer is not None else 0,
-        _ptr(r.bias_set) if bias else None, _ptr(r.bias_start), _ptr(r.bias_token), _ptr(r.bias_value), sets,
-        r.bias_token.numel() if bias else 0, _ptr(r.mask_of) if masks else None, _ptr(r.masks), masks,
-        r.masks.stride(0) if masks else 0, _ptr(logits_out), logits_out.stride(0) if logits_out is not None else 0, _ptr(out), _stream()),
-        "mlora_choose_tokens")
+    check(_lib.lib().mlora_choose_tokens(_ptr(logits), logits.stride(0), T, V, _ptr(row_src), *tables, _ptr(logits_out),
+                                         logits_out.stride(0) if logits_out is not None else 0, _ptr(out), _stream()), "mlora_choose_tokens")
     return out
