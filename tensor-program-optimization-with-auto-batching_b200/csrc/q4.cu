@@ -232,9 +232,13 @@ extern "C" int mlora_q4_linear(const void* d_x, int64_t ldx, const void* d_Wq, i
     if (lora) {
       s.a.u += (size_t)t0 * a.r_max * a.n_mod;
       s.a.slots += t0;
-      w.delta = delta;
-      const int rc = launch_q4_expand(s, delta, st);
-      if (rc) return rc;
+      if (s.a.T > kQ4InlineRows) {  // (fewer rows: where the sums are written)
+        w.delta = delta;
+        const int rc = launch_q4_expand(s, delta, st);
+        if (rc) return rc;
+      } else {
+        w.delta = nullptr;
+      }
     }
     const int rc = s.a.T <= kQ4SmallRows ? launch_q4_mm(s, w, st) : launch_q4_tc(s, w, st);
     if (rc) return rc;

@@ -88,6 +88,7 @@ int q4_ctas(long long tiles, int units);  // CTAs of a persistent launch over ti
 int launch_q4_expand(const Q4Args& p, float* delta, cudaStream_t st);
 int launch_q4_mm(const Q4Args& p, const Q4Work& w, cudaStream_t st);
 int launch_q4_tc(const Q4Args& p, const Q4Work& w, cudaStream_t st);
+constexpr int kQ4InlineRows = 8;  // rows whose adapters launch_q4_mm expands itself
 constexpr int kQ4SmallRows = 16;  // rows that launch_q4_mm is for
 
 __device__ __noinline__ static float q4_act(float v, int act) { return act_one(v, act); }  // (one copy of erf, not one per value)

@@ -265,7 +265,13 @@ __global__ void __launch_bounds__(kMmThreads, 1) q4_mm_kernel(const __grid_const
       } else {
         const int o = row0 + c;
         const bool there = o < a.out;
-        if (t.w.delta != nullptr) {
+        if constexpr (N8 == 1) {
+          if (a.u != nullptr && there) {  // (two values a thread: quicker here than a kernel of its own in front of this one)
+#pragma unroll
+            for (int k = 0; k < kMine; ++k)
+              if (tok0 + 4 * k < n_tok) v[k] += q4_adapter(a, t.p.packed_b, token0 + tok0 + 4 * k, o);
+          }
+        } else if (t.w.delta != nullptr) {
           float add[kMine];
 #pragma unroll
           for (int k = 0; k < kMine; ++k) add[k] = there && tok0 + 4 * k < n_tok ? __ldcg(t.w.delta + (size_t)(token0 + tok0 + 4 * k) * a.out + o) : 0.f;

@@ -251,6 +251,7 @@ class QuantWeight:
 
     def _pack(self, q, s, z, group):
         self.shape, self.group, self.zeros, self.dtype = tuple(q.shape), int(group), z is not None, torch.bfloat16
+        self.work_bytes = {}  # rows -> scratch of a projection
         n = _lib.lib().mlora_q4_bytes(*self.shape, group, int(self.zeros))
         if not n:
             raise ValueError(f"QuantWeight: no matrix of {self.shape}")
@@ -302,7 +303,9 @@ def _linear_q4(x, W: QuantWeight, stack, slots, u, flags, out, work):
         if stack.n_mod > 1 and not flags & SILU_MUL:
             mod = (C.c_int32 * (stack.n_mod + 1))(*stack.mod_offsets)
     flags = (flags & ~B_SPLIT) | (Q4_ZEROS if W.zeros else 0) | (B_PACKED if stack is not None and stack.b_packed else 0)
-    need = q4_linear_workspace(T, K, N)
+    need = W.work_bytes.get(T)
+    if need is None:
+        need = W.work_bytes[T] = q4_linear_workspace(T, K, N)
     if work is None and need:
         work = workspace(need, x.device, "linear")
     if work is not None and work.numel() < need:
