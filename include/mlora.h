@@ -650,10 +650,10 @@ int mlora_delta_step(const void* d_x, int64_t ld, int32_t C, int32_t taps, int32
  * mlora_q4_linear: mlora_linear with such weights: y = x W^T + scale[slot] * B_all[slot] u, MLORA_OUT_F32, MLORA_SILU_MUL (W's rows
  *   interleaved as there), MLORA_ACT_*, MLORA_B_PACKED; MLORA_Q4_ZEROS says that the weights have zero points.  The other flags of
  *   mlora_linear change nothing, but MLORA_B_SPLIT is refused.  The integers q - z are multiplied exactly, a group's sum and everything after it
- *   are fp32; only the result is rounded.  Up to 16 rows need no scratch; more run on another kernel (other order of sums) and take
- *   d_work of mlora_q4_linear_workspace bytes, zero-filled once before its first use; its status word and the caller's bytes are
- *   those of mlora_linear's scratch (bit 1: a bounded wait expired, the output is undefined and the buffer must be zero-filled
- *   again), and like that one it serves calls of any shape on one stream. */
+ *   are fp32; only the result is rounded.  The order of the sums depends on the number of rows, in and out.  d_work:
+ *   mlora_q4_linear_workspace bytes, zero-filled once before its first use: its own, not one that mlora_linear uses as well (the counters
+ *   lie elsewhere), for calls of any shape on one stream.  Its first int32 is a status word (bit 1: a bounded wait expired; the output
+ *   is undefined and the buffer must be zero-filled again), and the caller's bytes are those of mlora_linear's scratch. */
 #define MLORA_Q4_ZEROS 4096
 size_t mlora_q4_bytes(int32_t out, int32_t in, int32_t group, int32_t zeros);
 int mlora_q4_quantize(const void* d_W, int32_t out, int32_t in, int32_t group, void* d_q, void* d_scale, void* d_zero, void* stream);

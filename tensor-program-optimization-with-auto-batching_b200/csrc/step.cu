@@ -79,6 +79,11 @@ __global__ void decode_step_end_kernel(const int32_t* __restrict__ row_src, cons
   const int b = row_src[i];
   if (b < 0) return;
   const int tok = next_tok[i];
+  if (tok < 0) {  // (no token is allowed: the sequence ends with what it has)
+    live[b] = 0;
+    atomicSub(n_live_io, 1);
+    return;
+  }
   const int n = gen_count[b];
   if (n < ld_out) out_tokens[(size_t)b * ld_out + n] = tok;
   gen_count[b] = n + 1;

@@ -7,6 +7,7 @@ per sequence, ``capture_decode`` / :class:`DecodeSession` the same as a CUDA gra
 """
 from __future__ import annotations
 
+import dataclasses
 import struct
 
 import numpy as np
@@ -286,9 +287,13 @@ class DecodeSession:
     node's size); the host only learns the live count (4 bytes, every ``sync_every`` steps) to pick the bucket and
     to stop, and reads all generated tokens once at the end.
 
-    ``seq_ids`` must already be in bucketing order (``LlamaSeqInfo.order_seqs``): rows of one adapter adjacent."""
+    ``seq_ids`` must already be in bucketing order (``LlamaSeqInfo.order_seqs``): rows of one adapter adjacent.
 
-    def __init__(self, engine: EngineBase, seq_ids, adapter_slots, first_tokens, max_gen, eos_id=None, use_lora=True):
+    ``rules`` (:class:`ops.LogitRules` of the sequences, in their order): the tokens are chosen under them, with the session's own
+    tokens as the answers (the first ones included, which the caller chooses: ``ops.choose_tokens`` on the prompts' logits).  A
+    sequence whose rules allow no token ends."""
+
+    def __init__(self, engine: EngineBase, seq_ids, adapter_slots, first_tokens, max_gen, eos_id=None, use_lora=True, rules=None):
         self.eng, self.seq_ids, self.use_lora = engine, list(seq_ids), use_lora
         kv, dev, n = engine.kv, engine.m.device, len(seq_ids)
         self.n = n
@@ -310,6 +315,13 @@ class DecodeSession:
         for sid, g in zip(seq_ids, max_gen):
             kv.reserve(sid, kv.length(sid) + int(g) + 1)
         self.max_keys = max((kv.tokens_reserved(sid) for sid in seq_ids), default=1)
+        self.rules = rules
+        if rules is not None:
+            if rules.n not in (0, n):
+                raise ValueError(f"mlora: rules of {rules.n} requests for {n} sequences")
+            if getattr(engine.m, "tp_size", 1) > 1:
+                raise ValueError("mlora: rules look at whole rows of logits, a tensor-parallel rank has a slice")
+            self.rules = dataclasses.replace(rules, answer=self.out_tokens, answer_len=self.gen_count) if rules.n else None
         self._graphs = {}
         self.steps = 0
         self.d2h_bytes = 0
@@ -320,6 +332,8 @@ class DecodeSession:
                               self.row_src, e.row_slot, e.row_pos, e.slots, e.tokens, self.n_live)
         e.n_distinct, e.max_keys = self.n_distinct, self.max_keys
         e.forward(rows, True, self.use_lora)
+        if self.rules is not None:
+            ops.choose_tokens(e.logits[:rows], self.rules, row_src=self.row_src[:rows], out=e.next_tok[:rows])
         ops.decode_step_end(self.row_src, e.next_tok, rows, self.live, self.last_tok, self.gen_count, self.max_gen,
                             self.out_tokens, self.eos_id, self.n_live)
 

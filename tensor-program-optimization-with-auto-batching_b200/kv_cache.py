@@ -44,6 +44,8 @@ class PagedCache:
         self._slot_of = {}           # sid -> slot
         self._free_slots = list(range(self.max_batch - 1, -1, -1))
         self._n_pages_of = {}        # sid -> pages held
+        self._more_holders = {}      # page -> sequences that hold it beyond the first
+        self._shared_tokens = {}     # sid -> tokens in pages that it shares
         self._pending = None
 
     # -- sequences -----------------------------------------------------------------------------
@@ -71,8 +73,18 @@ class PagedCache:
     def remove_sequence(self, sid):
         slot = self._slot_of.pop(sid)
         n = self._n_pages_of.pop(sid)
-        self._free.extend(self._bt_host[slot, :n][::-1].tolist())
+        self._shared_tokens.pop(sid, None)
+        self._free.extend(p for p in self._bt_host[slot, :n][::-1].tolist() if not self._let_go(p))
         self._free_slots.append(slot)
+
+    def _let_go(self, page):
+        """Whether another sequence still holds the page."""
+        more = self._more_holders.get(page, 0)
+        if more == 1:
+            del self._more_holders[page]
+        elif more:
+            self._more_holders[page] = more - 1
+        return more > 0
 
     def slot(self, sid):
         return self._slot_of[sid]
@@ -111,6 +123,10 @@ class PagedCache:
     def _push_pages(self, changed):
         if not changed:
             return
+        if not self.block_table.is_cuda:
+            for slot, have, need in changed:
+                self.block_table[slot, have:need] = torch.from_numpy(self._bt_host[slot, have:need])
+            return
         lo, hi = min(c[0] for c in changed), max(c[0] for c in changed) + 1
         if len(changed) > 1 and (hi - lo) * self.max_pages <= self._ROWS_PER_COPY * len(changed):
             self._push(self.block_table[lo:hi], self._bt_host[lo:hi])
@@ -142,6 +158,9 @@ class PagedCache:
         seq_ids = [int(s) for s in seq_ids]
         append_lens = [int(a) for a in append_lens]
         both = list(zip(seq_ids, append_lens))  # (what one of them has more of has no rows)
+        for sid, n in both if self._shared_tokens else ():
+            if n < 0 and self.length(sid) + n < self._shared_tokens.get(sid, 0):
+                raise ValueError(f"sequence {sid} cannot take back tokens in pages that it shares")
         slots = np.array([self._slot_of[s] for s, _ in both], dtype=np.int32)
         lens = np.array([a for _, a in both], dtype=np.int64)
         first = self._len_host[slots]
@@ -193,6 +212,63 @@ class PagedKVCache(PagedCache):
         self.n_layers, self.Hkv, self.D = n_layers, n_kv_heads, head_dim
         self.pages = torch.zeros(n_layers, 2, self.n_pages, n_kv_heads, self.page_size, head_dim, dtype=torch.bfloat16,
                                  device=self.device)
+        # prefixes that several sequences share: by slot the prefix (-1: none) and its tokens, for :func:`ops.prefix_plan`
+        self.prefix_id = torch.full((self.max_batch,), -1, dtype=torch.int32, device=self.device)
+        self.prefix_len = torch.zeros(self.max_batch, dtype=torch.int32, device=self.device)
+        self._prefix_of = {}  # sid -> (prefix, tokens)
+        self._next_prefix = 0
+
+    # -- shared prefixes -------------------------------------------------------------------------
+    @property
+    def shares_prefixes(self) -> bool:
+        return bool(self._prefix_of)
+
+    def fork(self, sid, source, n_tokens=None):
+        """Adds sequence ``sid`` beginning with the first ``n_tokens`` tokens (default: all) of ``source``, whose whole pages it shares from
+        then on; returns how many tokens that are (a multiple of the page size): the rest of its prompt is for the caller to run.
+        Keys and values are those of the source's adapter.  A decode step reads a prefix that several of its rows share once.  Sequences
+        forked from one source form a group over the tokens that the first fork shared; one that shares fewer stays outside it."""
+        length = self.length(source)
+        n_tokens = length if n_tokens is None else int(n_tokens)
+        if not 0 <= n_tokens <= length:
+            raise ValueError(f"sequence {source} has {length} tokens, not {n_tokens}")
+        pages = n_tokens // self.page_size
+        tokens = pages * self.page_size
+        slot = self.add_sequence(sid)
+        if not pages:
+            return 0
+        self._bt_host[slot, :pages] = self._bt_host[self._slot_of[source], :pages]
+        for p in self._bt_host[slot, :pages].tolist():
+            self._more_holders[p] = self._more_holders.get(p, 0) + 1
+        self._n_pages_of[sid] = pages
+        self._len_host[slot] = tokens
+        for s in (sid, source):
+            self._shared_tokens[s] = max(self._shared_tokens.get(s, 0), tokens)
+        self._push_pages([(slot, 0, pages)])
+        self._push_value(self.seq_lens, slot, tokens)
+        if source not in self._prefix_of:
+            self._set_prefix(source, self._next_prefix, tokens)
+            self._next_prefix = (self._next_prefix + 1) % (1 << 31)
+        if tokens >= self._prefix_of[source][1]:
+            self._set_prefix(sid, *self._prefix_of[source])
+        return tokens
+
+    def remove_sequence(self, sid):
+        slot = self.slot(sid)
+        super().remove_sequence(sid)
+        if self._prefix_of.pop(sid, None) is not None:
+            self._push_value(self.prefix_id, slot, -1)
+
+    def _set_prefix(self, sid, prefix, tokens):
+        self._prefix_of[sid] = (prefix, tokens)
+        self._push_value(self.prefix_id, self._slot_of[sid], prefix)
+        self._push_value(self.prefix_len, self._slot_of[sid], tokens)
+
+    def _push_value(self, table, slot, value):
+        if table.is_cuda:
+            self._push(table[slot:slot + 1], np.array([value], dtype=np.int32))
+        else:
+            table[slot] = value
 
     # -- layer views -----------------------------------------------------------------------------
     def k_pages(self, layer):

@@ -62,8 +62,12 @@ class PackedLlama:
     Adapter ``i`` occupies slot ``i`` of every stack."""
 
     def __init__(self, cfg, weights, adapters=(), scales=(), device="cuda", n_layers=None, pack=True,
-                 tp_rank=0, tp_size=1, adapter_capacity=None, max_rank=None, adapter_targets=None):
-        """pack=True stores every projection matrix and adapter B stack in the pre-tiled layouts of
+                 tp_rank=0, tp_size=1, adapter_capacity=None, max_rank=None, adapter_targets=None, weight_bits=16, weight_group=128,
+                 weight_zeros=True):
+        """``weight_bits`` 4: the layers' projections are quantised at load, every ``weight_group`` inputs of an output with a scale (and a
+        zero point) of their own (:class:`ops.QuantWeight`); embeddings, norms, the head and the adapters stay as they are.
+
+        pack=True stores every projection matrix and adapter B stack in the pre-tiled layouts of
         mlora_pack_weight / mlora_pack_lora_b (one bulk copy per pipeline stage).
 
         tp_size > 1: Megatron-style tensor parallelism.  q/k/v and gate/up are column-parallel (this
@@ -96,6 +100,11 @@ class PackedLlama:
         self.eps, self.theta = float(c["rms_norm_eps"]), float(c["rope_theta"])
         if self.I % 8:
             raise ValueError("intermediate_size must be a multiple of 8")
+        if weight_bits not in (4, 16):
+            raise ValueError(f"weights have 16 or 4 bits, not {weight_bits}")
+        if weight_bits == 4 and (weight_group not in (32, 64, 128) or any(n % weight_group for n in (self.H, self.I, self.Hq * self.D))):
+            raise ValueError(f"groups of 32, 64 or 128 inputs must divide the projections' ({self.H}, {self.I}, {self.Hq * self.D}), got {weight_group}")
+        self.weight_bits = int(weight_bits)
         bf = lambda t: t.to(device=self.device, dtype=torch.bfloat16).contiguous()
         self.embed = bf(weights["model.embed_tokens.weight"])
         self.norm = bf(weights["model.norm.weight"])
@@ -122,7 +131,10 @@ class PackedLlama:
         for l in range(self.L):
             p = f"model.layers.{l}."
             w = lambda n: weights[p + n + ".weight"]
-            pk = lambda t: ops.PackedWeight(bf(t)) if pack else bf(t)
+            if weight_bits == 4:
+                pk = lambda t: ops.QuantWeight(bf(t), weight_group, weight_zeros)
+            else:
+                pk = lambda t: ops.PackedWeight(bf(t)) if pack else bf(t)
             lw = LayerWeights(
                 ln1=bf(w("input_layernorm")), ln2=bf(w("post_attention_layernorm")),
                 w_qkv=pk(torch.cat([w("self_attn.q_proj")[self._q_rows], w("self_attn.k_proj")[self._kv_rows],
@@ -254,10 +266,11 @@ class PackedLlama:
 
     def weight_bytes(self):
         """Bytes of base weights one decode step streams (all layers + final norm + lm_head)."""
-        n = self.norm.numel() + self.lm_head.numel()
+        n = 2 * (self.norm.numel() + self.lm_head.numel())
         for lw in self.layers:
-            n += lw.ln1.numel() + lw.ln2.numel() + lw.w_qkv.numel() + lw.w_o.numel() + lw.w_gu.numel() + lw.w_down.numel()
-        return 2 * n
+            n += 2 * (lw.ln1.numel() + lw.ln2.numel())
+            n += sum(w.data.numel() if self.weight_bits == 4 else 2 * w.numel() for w in (lw.w_qkv, lw.w_o, lw.w_gu, lw.w_down))
+        return n
 
     def lora_bytes_per_adapter(self):
         n = 0
@@ -303,6 +316,15 @@ class Engine(EngineBase):
         # engine and are never shared with (or outgrown by) other callers on the device.
         self.ws_linear = ops.new_workspace(need, dev)
         self.ws_attn = ops.new_workspace(lib.mlora_paged_attention_workspace(T, m.Hq, m.D, 16), dev)
+        # projections with 4-bit weights keep counters at other places than the others: a scratch buffer of their own
+        self.ws_q4 = None
+        if m.weight_bits == 4:
+            self.ws_q4 = ops.new_workspace(max(ops.q4_linear_workspace(T, k, n) for k, n in
+                                               ((m.H, qkv_out), (m.Hq * m.D, m.H), (m.H, 2 * m.I), (m.I, m.H))), dev)
+        # decode steps of sequences that share prefixes (their plan and scratch are made when the first such step runs)
+        self.shared_rows = min(T, ops.PREFIX_PLAN_MAX_ROWS) if m.D in (64, 128) and 128 * m.Hkv // m.Hq > 2 else 0
+        self.prefix_plan = self.ws_shared = None
+        self.prefix_least = -1  # reads that a group has to save (see ops.PrefixPlan)
         # the o-projection's shrink computed in the attention launch (decode passes): its own zero-initialised scratch.
         # Measured on the benchmark's step: 32 launches fewer but 0.035 ms slower (the tail sits on the attention
         # kernel's critical path, the separate shrink launch overlaps the projection's weight prefetch), so off unless asked for
@@ -319,13 +341,33 @@ class Engine(EngineBase):
         # projections' epilogues (mlora_linear_norm) -- one launch fewer per layer.  Measured on the benchmark's step: the
         # two folding projections run a kernel variant of their own (69 registers more per thread), and a step that
         # alternates between two variants loses more than the 32 launches save: 5.03 ms against 4.99, so off unless asked for
-        self.fold_norm = os.environ.get("MLORA_FOLD_NORM", "0") == "1"
+        self.fold_norm = os.environ.get("MLORA_FOLD_NORM", "0") == "1" and m.weight_bits == 16
         self.sumsq = torch.zeros(-(-m.H // 128) * 32, dtype=torch.float32, device=dev)
         # decode-size passes can run everything between two attention calls as one persistent launch
         # (mlora_decode_chain); measured slower than the separate launches on the benchmark's step, so off unless asked for
         self.use_chain = os.environ.get("MLORA_CHAIN", "0") == "1"
         # "2": only gate|up -> down (two projections with nothing between them) as one launch
         self.chain_mlp = os.environ.get("MLORA_CHAIN", "0") == "2"
+
+    def check_status(self):
+        super().check_status()
+        if self.ws_q4 is not None:
+            st = ops.status_word(self.ws_q4)
+            if st:
+                self.ws_q4.zero_()
+                raise RuntimeError(f"mlora: a projection kernel (status bits {st:#x}) gave up a bounded wait; the results of this pass are undefined")
+
+    def _shares_prefixes(self, T, fused_append):
+        return fused_append and 1 < T <= self.shared_rows and self.kv.shares_prefixes
+
+    def _plan_prefixes(self, T):
+        """Which rows of this step share a prefix: once for all layers."""
+        m, kv = self.m, self.kv
+        if self.prefix_plan is None:
+            self.prefix_plan = ops.PrefixPlan(self.shared_rows, m.Hq, m.Hkv, m.device, self.prefix_least)
+            self.ws_shared = ops.new_workspace(max(ops.paged_attention_shared_workspace(t, m.Hq, m.Hkv, m.D) for t in range(1, self.shared_rows + 1)),
+                                               m.device)
+        return ops.prefix_plan(self.row_slot[:T], kv.prefix_id, kv.prefix_len, self.prefix_plan)
 
     @staticmethod
     def _full_rank(stack):
@@ -389,10 +431,14 @@ class Engine(EngineBase):
             u = self.u.view(-1)[: T * r_tot].view(T, r_tot)
             ops.lora_shrink(x, stack, slots, out=u)
             return ops.linear(x, W, stack, slots, u=u, flags=ANY_SUMS | self._lora_flags(T, stack, flags), out=out,
-                              work=self.ws_linear)
+                              work=self._scratch())
         # a projection without adapters inside a pass that has some: same kernel variant as its neighbours
         return ops.linear(x, W, flags=flags | ANY_SUMS | (SHARE_LORA_KERNEL if slots is not None else 0), out=out,
-                          work=self.ws_linear)
+                          work=self._scratch())
+
+    def _scratch(self):
+        """Of the layers' projections."""
+        return self.ws_linear if self.ws_q4 is None else self.ws_q4
 
     # ------------------------------------------------------------------------------------------
     def _chain_plan(self, T, slots):
@@ -472,7 +518,8 @@ class Engine(EngineBase):
         each sequence); None = every row.  ``hidden`` (bf16 [T,H]) replaces the embedding lookup."""
         m, kv = self.m, self.kv
         tok, slots = self.tokens[:T], (self.slots[:T] if (use_lora and m.n_adapters) else None)
-        if fused_append and lm_rows is None:
+        plan = self._plan_prefixes(T) if self._shares_prefixes(T, fused_append) else None
+        if fused_append and lm_rows is None and plan is None:
             chains = self._chain_plan(T, slots)
             if chains is not None:
                 return self._forward_chained(T, chains, slots, hidden)
@@ -493,24 +540,27 @@ class Engine(EngineBase):
                 u = self.u.view(-1)[: T * r_tot].view(T, r_tot)
                 ops.residual_rmsnorm_shrink(delta, res, res_other, lw.ln1, m.eps, xn, st, slots, u)
                 res, res_other = res_other, res
-                ops.linear(xn, lw.w_qkv, st, slots, u=u, flags=ANY_SUMS | self._lora_flags(T, st, 0), out=qkv, work=self.ws_linear)
+                ops.linear(xn, lw.w_qkv, st, slots, u=u, flags=ANY_SUMS | self._lora_flags(T, st, 0), out=qkv, work=self._scratch())
             else:
                 self._reduce_norm(delta, res, lw.ln1, xn, reduce=l > 0)
                 self._proj(xn, lw.w_qkv, st, slots, qkv)
             kp, vp = kv.k_pages(l), kv.v_pages(l)
-            if not fused_append:
+            if not fused_append or plan is not None:
                 ops.kv_append_rope(qkv, kp, vp, kv.block_table, row_slot, row_pos, m.Hq, m.Hkv, m.D, kv.page_size,
                                    m.theta)
             st_o = lw.lora.get("o")
             lora_o = st_o is not None and slots is not None
             u_o = self.u.view(-1)[: T * st_o.r_max].view(T, st_o.r_max) if lora_o else None
-            if (lora_o and self.fuse_o_shrink and fused_append and T <= 1024
+            if (lora_o and self.fuse_o_shrink and fused_append and plan is None and T <= 1024
                     and ops.attention_shrink_fits(T, m.Hq, kv.block_table.shape[1], st_o)):
                 # attention and the o-projection's shrink in one launch; the projection then only expands
                 ops.paged_attention_shrink(qkv, kp, vp, kv.block_table, row_slot, row_pos, m.Hq, m.Hkv, m.D, kv.page_size,
                                            m.theta, fused_append, attn, st_o, slots, u_o, self.ws_oshrink)
             else:
-                if not fused_append and self.tc_prefill and self._n_pf_tiles > 0:
+                if plan is not None:
+                    ops.paged_attention_shared(qkv, kp, vp, kv.block_table, row_slot, row_pos, plan, m.Hq, out=attn, work=self.ws_shared,
+                                               status=self.pf_status)
+                elif not fused_append and self.tc_prefill and self._n_pf_tiles > 0:
                     ops.prefill_attention(qkv, kp, vp, kv.block_table, self.pf_tiles, self._n_pf_tiles, m.Hq, m.Hkv, m.D,
                                           kv.page_size, attn, self.pf_status)
                 else:
@@ -530,9 +580,9 @@ class Engine(EngineBase):
                 self._proj(act, lw.w_down, lw.lora.get("down"), slots, y)
             else:
                 if lora_o:
-                    ops.linear(attn, lw.w_o, st_o, slots, u=u_o, flags=fl_o | ANY_SUMS, out=y, work=self.ws_linear)
+                    ops.linear(attn, lw.w_o, st_o, slots, u=u_o, flags=fl_o | ANY_SUMS, out=y, work=self._scratch())
                 else:
-                    ops.linear(attn, lw.w_o, flags=fl_o | ANY_SUMS, out=y, work=self.ws_linear)
+                    ops.linear(attn, lw.w_o, flags=fl_o | ANY_SUMS, out=y, work=self._scratch())
                 # row-parallel partials (base + LoRA) -> full o_proj output, added to the residual, normalised
                 self._reduce_norm(y, res, lw.ln2, xn)
                 if not self._mlp_chained(T, lw, slots, xn, act, y):

@@ -307,7 +307,7 @@ def _linear_q4(x, W: QuantWeight, stack, slots, u, flags, out, work):
     if need is None:
         need = W.work_bytes[T] = q4_linear_workspace(T, K, N)
     if work is None and need:
-        work = workspace(need, x.device, "linear")
+        work = workspace(need, x.device, "linear_q4")
     if work is not None and work.numel() < need:
         raise ValueError(f"mlora.linear: scratch of {need} bytes needed, {work.numel()} given")
     lora = stack is not None

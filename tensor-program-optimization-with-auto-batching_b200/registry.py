@@ -19,13 +19,14 @@ from .tevudra import PackedTevudra
 @dataclass(frozen=True)
 class Design:
     name: str
-    pack: Callable     # (config, weights, adapters, scales, device, dtype) -> packed model with new_cache / new_engine
+    pack: Callable     # (config, weights, adapters, scales, device, dtype, **options) -> packed model with new_cache / new_engine
     dtypes: tuple
     adapters: bool     # takes LoRA adapters
+    options: tuple = ()  # keyword arguments of its class that a caller may give
 
 
-def _pack_llama(cfg, weights, adapters, scales, device, dtype):
-    return PackedLlama(cfg, weights, adapters, scales, device=device)
+def _pack_llama(cfg, weights, adapters, scales, device, dtype, **options):
+    return PackedLlama(cfg, weights, adapters, scales, device=device, **options)
 
 
 def _pack_tevudra(cfg, weights, adapters, scales, device, dtype):
@@ -37,7 +38,7 @@ def _pack_relidra(cfg, weights, adapters, scales, device, dtype):
 
 
 DESIGNS = {d.name: d for d in (
-    Design("LlamaForCausalLM", _pack_llama, (torch.bfloat16,), True),
+    Design("LlamaForCausalLM", _pack_llama, (torch.bfloat16,), True, ("weight_bits", "weight_group", "weight_zeros")),
     Design("Tevudra", _pack_tevudra, PackedTevudra.dtypes, False),
     Design("Relidra", _pack_relidra, PackedRelidra.dtypes, False),
 )}
@@ -54,19 +55,21 @@ def design_of(cfg: dict) -> Design:
     return DESIGNS[name]
 
 
-def build_model(cfg: dict, weights: dict, adapters=(), scales=(), device="cuda", dtype=torch.bfloat16):
-    """Packs ``weights`` on the device for the design ``cfg`` names."""
+def build_model(cfg: dict, weights: dict, adapters=(), scales=(), device="cuda", dtype=torch.bfloat16, **options):
+    """Packs ``weights`` on the device for the design ``cfg`` names (``options``: Llama's ``weight_bits``, ``weight_group``, ``weight_zeros``)."""
     d = design_of(cfg)
     if dtype not in d.dtypes:
         raise UnsupportedPrecision(f"{d.name} does not run in {dtype}")
     if len(adapters) and not d.adapters:
         raise ValueError(f"{d.name} takes no adapters")
-    return d.pack(cfg, weights, adapters, scales, device, dtype)
+    if any(o not in d.options for o in options):
+        raise ValueError(f"{d.name} takes {list(d.options)}, not {sorted(options)}")
+    return d.pack(cfg, weights, adapters, scales, device, dtype, **options)
 
 
-def load_model(model_dir: str, device="cuda", dtype=torch.bfloat16):
+def load_model(model_dir: str, device="cuda", dtype=torch.bfloat16, **options):
     """A packed model from a folder with ``config.json`` and ``model.safetensors``."""
     cfg = checkpoint.read_config(model_dir)
     if dtype not in design_of(cfg).dtypes:
         raise UnsupportedPrecision(f"{design_of(cfg).name} does not run in {dtype}")
-    return build_model(cfg, checkpoint.read_tensors(model_dir), device=device, dtype=dtype)
+    return build_model(cfg, checkpoint.read_tensors(model_dir), device=device, dtype=dtype, **options)
