@@ -73,7 +73,8 @@ __global__ void __launch_bounds__(kMmThreads, 1) q4_mm_kernel(const __grid_const
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);  // [stage][x | W | scales]
   float* sums = reinterpret_cast<float*>(ring + kStages * S::kBytes);                                            // [block][row of x][kMmPitch]
-  __shared__ uint64_t full[kStages], empty[kStages];
+  __shared__ uint64_t bars[2 * kStages];
+  uint64_t *const full = bars, *const empty = bars + kStages;
   __shared__ int s_abort;
 
   pdl_launch_dependents();
@@ -163,18 +164,25 @@ __global__ void __launch_bounds__(kMmThreads, 1) q4_mm_kernel(const __grid_const
     };
     clear();
     bool ok = true, waited = false;
+    // (the integer pipe is what this loop is bound by: running pointers, no remainders)
+    const uint8_t* stage = ring;
+    const uint8_t* const ring_end = ring + kStages * S::kBytes;
+    uint64_t* bar = full;
+    uint32_t par = 0;
+    const uint32_t x_lane = block * N8 * 1024 + (lane & 7) * 128;
+    const int w_lane = S::kX + block * kQ4TileBytes + quarter * 1024 + lane * 16, s_lane = S::kX + S::kW + (quarter * 32 + g) * kEntry;
+    const uint32_t x_piece[2] = {(uint32_t)(((lane >> 3) ^ (lane & 7)) << 4), (uint32_t)(((4 + (lane >> 3)) ^ (lane & 7)) << 4)};
+    const bool in_last = block < n_kb - (t.units - 1) * kMmBlocks;
     for (int i = 0; i < left;) {
       const int seg = min(left - i, t.units - u);  // stages of this tile
       const int u_first = u;
       for (int e = i + seg; i < e; ++i, ++u) {
-        const int slot = i % kStages;
-        ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], (i / kStages) & 1, abort));
+        ok = __all_sync(0xffffffffu, mbar_wait(bar, par, abort));
         if (!ok) break;
-        if (u * kMmBlocks + block < n_kb) {
-          const uint8_t* st = ring + slot * S::kBytes;
-          const uint32_t sx = smem_u32(st) + block * N8 * 1024 + (lane & 7) * 128;
-          const uint8_t* sw = st + S::kX + block * kQ4TileBytes + quarter * 1024 + lane * 16;
-          const uint8_t* ss = st + S::kX + S::kW + (quarter * 32 + g) * kEntry;
+        if (in_last || u + 1 < t.units) {
+          const uint32_t sx = smem_u32(stage) + x_lane;
+          const uint8_t* sw = stage + w_lane;
+          const uint8_t* ss = stage + s_lane;
           uint4 w4[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) w4[h] = *reinterpret_cast<const uint4*>(sw + h * 512);
@@ -182,7 +190,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) q4_mm_kernel(const __grid_const
 #pragma unroll
           for (int n = 0; n < N8; ++n)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) ldmatrix4(sx + n * 1024 + (((h * 4 + (lane >> 3)) ^ (lane & 7)) << 4), b[n][h]);
+            for (int h = 0; h < 2; ++h) ldmatrix4(sx + n * 1024 + x_piece[h], b[n][h]);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t w[4] = {w4[h].x, w4[h].y, w4[h].z, w4[h].w};
@@ -224,7 +232,10 @@ __global__ void __launch_bounds__(kMmThreads, 1) q4_mm_kernel(const __grid_const
           }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[slot]);
+        if (lane == 0) mbar_arrive(bar + kStages);
+        stage += S::kBytes;
+        ++bar;
+        if (stage == ring_end) stage = ring, bar = full, par ^= 1;
       }
       ok = mm_all(ok);  // (also: the sums before have been read)
       if (!ok) break;

@@ -24,7 +24,7 @@ namespace {
 constexpr int q4_weight_groups(int bn) { return bn == 32 ? 3 : 2; }
 constexpr int q4_out_warps(int bn) { return bn == 32 ? 4 : 8; }
 constexpr int q4_threads(int bn) { return 32 * (4 * q4_weight_groups(bn) + q4_out_warps(bn) + 3); }
-constexpr int q4_ring(int bn) { return bn == 32 ? 10 : bn == 64 ? 8 : 6; }  // packed units in shared memory
+constexpr int q4_ring(int bn) { return bn == 32 ? 9 : bn == 64 ? 8 : 6; }  // packed units in shared memory: as many for every weight warpgroup
 constexpr int q4_bufs(int bn) { return bn == 128 ? 4 : 6; }  // units of weights in TMEM, and of x in shared memory (from L2, 1 us away)
 // Units whose scales lie in shared memory.  A slot is filled again without asking: copies are at most q4_bufs units ahead of the MMAs,
 // which are at most as many accumulators (q4_sums, one or more a unit) ahead of the warps that read scales.
@@ -160,9 +160,11 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
       if (lane == 0) mbar_arrive(&full[told]);
       __syncwarp();
     };
+    static_assert(kWslots % kGroups == 0 && kBufs % kGroups == 0, "every warpgroup has slots and buffers of its own");
+    int slot = wg, buf = wg;
+    uint32_t w_par = 0, a_par = 1;
     for (int seq = wg; seq < n_units; seq += kGroups) {
-      const int slot = seq % kWslots, buf = seq % kBufs;
-      if (!__all_sync(0xffffffffu, mbar_wait(&w_full[slot], (seq / kWslots) & 1, abort))) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&w_full[slot], w_par, abort))) {
         s_abort = 1;
         told = -1;
         break;
@@ -190,7 +192,7 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
         }
         if (h == 0) {
           tell();
-          if (!__all_sync(0xffffffffu, mbar_wait(&empty[buf], ((seq / kBufs) & 1) ^ 1, abort))) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&empty[buf], a_par, abort))) {
             s_abort = 1;
             told = -1;
             break;
@@ -206,6 +208,8 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
         tmem_st_16x128b_x8(tmem_a + buf * 64 + (h >> 1) * 32 + ((uint32_t)(quarter * 32 + (h & 1) * 16) << 16), r);
       }
       if (told < 0) break;
+      if ((slot += kGroups) >= kWslots) slot = wg, w_par ^= 1;
+      if ((buf += kGroups) >= kBufs) buf = wg, a_par ^= 1;
     }
     tell();
   } else if (warp < kMma) {
@@ -218,16 +222,17 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
     pdl_wait();  // (scratch and outputs belong to earlier kernels until here)
     Cursor c(t, u_begin, u_end);
     long long unit = u_begin;
-    int seq = 0;  // units taken
+    int s_slot = 0;
     uint32_t d = 0, d_par = 0;
     const uint32_t d_full0 = smem_u32(d_full);
     bool ok = true;
     while (c.left > 0 && ok) {
       const int u0 = c.u, token0 = c.token_tile * BN + col0, n_units = min(c.left, t.units - u0);
       const long long seg_begin = unit, tile_begin = unit - u0, seg_end = unit + n_units;
-      for (int k = 0; k < n_units && ok; ++k, ++seq) {
+      for (int k = 0; k < n_units && ok; ++k) {
         const int n_g = min(kSums, t.p.n_groups - (u0 + k) * kSums);
-        const uint8_t* scales = ss + seq % kSlots * kScaleBytes + row * kEntry;
+        const uint8_t* scales = ss + s_slot * kScaleBytes + row * kEntry;
+        if (++s_slot == kSlots) s_slot = 0;
 #pragma unroll 1
         for (int g = 0; g < n_g; ++g, scales += kQ4Tile * kEntry) {
           // (a unit's scales arrive at the barrier of its rows of x, which the MMAs have waited for)
