@@ -28,8 +28,9 @@ __host__ __device__ inline long long q4_weight_bytes(int out, int in) {
 }
 
 __device__ __forceinline__ uint32_t q4_sub(uint32_t v, uint32_t z) {  // two bf16
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&z));
-  return *reinterpret_cast<const uint32_t*>(&r);
+  uint32_t r;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(z));
+  return r;
 }
 // The four registers of a word; z0, z1: twice 128 + z of the lane's two outputs.
 __device__ __forceinline__ void q4_expand(uint32_t w, uint32_t z0, uint32_t z1, uint32_t (&r)[4]) {

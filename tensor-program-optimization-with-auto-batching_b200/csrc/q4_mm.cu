@@ -18,7 +18,8 @@ namespace mlora {
 namespace {
 
 constexpr int kMmWarps = 16, kMmThreads = 32 * (kMmWarps + 1);  // and one warp for the copies
-constexpr int kMmBlocks = 4;                                    // of 64 inputs per stage
+constexpr int kMmBlocks = 8;                                    // of 64 inputs per stage
+constexpr int kMmSplit = 4;                                     // warps that share a range of outputs
 constexpr int kMmPitch = 132;                                   // floats between rows of x in the sums
 
 struct MmArgs {
@@ -58,10 +59,10 @@ __device__ __forceinline__ bool mm_all(bool ok) {
 // N8: rows of x in eights; ZERO: zero points; G: inputs per group
 template <int N8, bool ZERO, int G>
 struct MmStage {
-  static constexpr int kEntry = ZERO ? 4 : 2, kGroups = 256 / G;
+  static constexpr int kEntry = ZERO ? 4 : 2, kGroups = kMmBlocks * kQ4Block / G;
   static constexpr int kW = kMmBlocks * kQ4TileBytes, kX = kMmBlocks * N8 * 1024, kS = kGroups * kQ4Tile * kEntry;
   static constexpr int kBytes = (kW + kX + kS + 1023) / 1024 * 1024;  // (x is swizzled: 1024-byte places)
-  static constexpr int kSums = 4 * N8 * 8 * kMmPitch * 4;  // of the four blocks' warps
+  static constexpr int kSums = kMmSplit * N8 * 8 * kMmPitch * 4;
   static constexpr int kStages = (227 * 1024 - 1024 - 512 - kSums) / kBytes < 8 ? (227 * 1024 - 1024 - 512 - kSums) / kBytes : 8;
   static constexpr int kSmem = 1024 + kStages * kBytes + kSums;
 };
@@ -72,7 +73,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) q4_mm_kernel(const __grid_const
   constexpr int kStages = S::kStages, kEntry = S::kEntry;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);  // [stage][x | W | scales]
-  float* sums = reinterpret_cast<float*>(ring + kStages * S::kBytes);                                            // [block][row of x][kMmPitch]
+  float* sums = reinterpret_cast<float*>(ring + kStages * S::kBytes);                                            // [split][row of x][kMmPitch]
   __shared__ uint64_t bars[2 * kStages];
   uint64_t *const full = bars, *const empty = bars + kStages;
   __shared__ int s_abort;
@@ -169,28 +170,31 @@ __global__ void __launch_bounds__(kMmThreads, 1) q4_mm_kernel(const __grid_const
     const uint8_t* const ring_end = ring + kStages * S::kBytes;
     uint64_t* bar = full;
     uint32_t par = 0;
-    const uint32_t x_lane = block * N8 * 1024 + (lane & 7) * 128;
+    const uint32_t x_lane = block * N8 * 1024 + (lane & 7) * 128;  // (the warp's first block; the other lies kMmSplit blocks further)
     const int w_lane = S::kX + block * kQ4TileBytes + quarter * 1024 + lane * 16, s_lane = S::kX + S::kW + (quarter * 32 + g) * kEntry;
     const uint32_t x_piece[2] = {(uint32_t)(((lane >> 3) ^ (lane & 7)) << 4), (uint32_t)(((4 + (lane >> 3)) ^ (lane & 7)) << 4)};
-    const bool in_last = block < n_kb - (t.units - 1) * kMmBlocks;
+    const int last_blocks = n_kb - (t.units - 1) * kMmBlocks;
     for (int i = 0; i < left;) {
       const int seg = min(left - i, t.units - u);  // stages of this tile
       const int u_first = u;
       for (int e = i + seg; i < e; ++i, ++u) {
         ok = __all_sync(0xffffffffu, mbar_wait(bar, par, abort));
         if (!ok) break;
-        if (in_last || u + 1 < t.units) {
-          const uint32_t sx = smem_u32(stage) + x_lane;
-          const uint8_t* sw = stage + w_lane;
-          const uint8_t* ss = stage + s_lane;
+        const int blocks = u + 1 < t.units ? kMmBlocks : last_blocks;
+        const uint32_t sx = smem_u32(stage) + x_lane;
+        const uint8_t* sw = stage + w_lane;
+        const uint8_t* ss = stage + s_lane;
+#pragma unroll
+        for (int q = 0; q < kMmBlocks / kMmSplit; ++q) {
+          if (block + q * kMmSplit >= blocks) break;
           uint4 w4[2];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) w4[h] = *reinterpret_cast<const uint4*>(sw + h * 512);
+          for (int h = 0; h < 2; ++h) w4[h] = *reinterpret_cast<const uint4*>(sw + q * kMmSplit * kQ4TileBytes + h * 512);
           uint32_t b[N8][2][4];  // rows 8 n .. of x: inputs 32 h .. 32 h + 31 of the block
 #pragma unroll
           for (int n = 0; n < N8; ++n)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) ldmatrix4(sx + n * 1024 + x_piece[h], b[n][h]);
+            for (int h = 0; h < 2; ++h) ldmatrix4(sx + (q * kMmSplit * N8 + n) * 1024 + x_piece[h], b[n][h]);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t w[4] = {w4[h].x, w4[h].y, w4[h].z, w4[h].w};
@@ -200,8 +204,9 @@ __global__ void __launch_bounds__(kMmThreads, 1) q4_mm_kernel(const __grid_const
             for (int j = 0; j < 4; ++j) {
               constexpr int kWords = G == 32 ? 2 : 4;  // of a group in this block
               if (j % kWords == 0) {
+                const int at = block + q * kMmSplit;
                 // (inputs that end inside a block: its second group is not there, and x is 0)
-                const int group = G == 32 ? min(block * 2 + j / 2, t.p.n_groups - u * S::kGroups - 1) : G == 64 ? block : block / 2;
+                const int group = G == 32 ? min(at * 2 + j / 2, t.p.n_groups - u * S::kGroups - 1) : G == 64 ? at : at / 2;
                 const uint8_t* e = ss + (group * kQ4Tile + h * 16) * kEntry;
                 if constexpr (ZERO) {
                   const uint32_t e0 = *reinterpret_cast<const uint32_t*>(e), e1 = *reinterpret_cast<const uint32_t*>(e + 8 * 4);
@@ -367,12 +372,12 @@ int launch_mm_for(const MmArgs& t, int grid, cudaStream_t st) {
 }  // namespace
 
 int launch_q4_mm(const Q4Args& p, const Q4Work& w, cudaStream_t st) {
-  const int n8 = p.a.T <= 8 ? 1 : p.a.T <= 16 ? 2 : 4;
+  const int n8 = p.a.T <= 8 ? 1 : 2;
   MmArgs t{p, w, (p.a.out + kQ4Tile - 1) / kQ4Tile, (p.a.T + n8 * 8 - 1) / (n8 * 8), (p.n_kb + kMmBlocks - 1) / kMmBlocks};
   const long long all = (long long)t.row_tiles * t.token_tiles * t.units;
   if (all > 2147483647ll) return fail(MLORA_ESIZE, "q4_linear: too many tiles");
   const int grid = q4_ctas(t.row_tiles * (long long)t.token_tiles, t.units);
-  return n8 == 1 ? launch_mm_for<1>(t, grid, st) : n8 == 2 ? launch_mm_for<2>(t, grid, st) : launch_mm_for<4>(t, grid, st);
+  return n8 == 1 ? launch_mm_for<1>(t, grid, st) : launch_mm_for<2>(t, grid, st);
 }
 
 }  // namespace mlora
