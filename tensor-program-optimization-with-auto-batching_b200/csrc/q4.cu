@@ -117,19 +117,20 @@ int launch_q4_expand(const Q4Args& p, float* delta, cudaStream_t st) {
   return MLORA_OK;
 }
 
-static int q4_most_ctas() {
+static int q4_most_ctas(int per_sm) {
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
     cudaGetLastError();
     n = 148;
   }
+  n *= per_sm;
   return n < kQ4MaxCtas ? n : kQ4MaxCtas;
 }
 
-// One per SM at most.  Where nearly all of them can have equal shares of one tile each (a 4096-wide output: four CTAs a tile, 128 of
+// `per_sm` per SM at most.  Where nearly all of them can have equal shares of one tile each (a 4096-wide output: four CTAs a tile, 128 of
 // 148), they do: one sum to leave or to collect per CTA instead of two.
-int q4_ctas(long long tiles, int units) {
-  const int n = q4_most_ctas();
+int q4_ctas(long long tiles, int units, int per_sm) {
+  const int n = q4_most_ctas(per_sm);
   if (tiles <= n) {
     const int per = n / (int)tiles < units ? n / (int)tiles : units;
     if (tiles * per >= n * 85 / 100 || per == units) return (int)tiles * per;
@@ -139,7 +140,7 @@ int q4_ctas(long long tiles, int units) {
 
 // Counters and shares lie at places that no call's sizes move; behind them the adapters' share of a slice of rows.
 size_t q4_workspace(int T, int out) {
-  return kQ4Header + kQ4MaxCtas * 4 + (size_t)q4_most_ctas() * 128 * kQ4Tile * 4 + (size_t)(T < kQ4Slice ? T : kQ4Slice) * out * 4;
+  return kQ4Header + kQ4MaxCtas * 4 + (size_t)q4_most_ctas(2) * 128 * kQ4Tile * 4 + (size_t)(T < kQ4Slice ? T : kQ4Slice) * out * 4;
 }
 
 }  // namespace mlora

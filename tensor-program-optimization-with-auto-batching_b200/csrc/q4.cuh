@@ -85,7 +85,7 @@ struct Q4Work {
   const float* delta;  // [rows][out]: the adapters' share, or NULL
 };
 size_t q4_workspace(int T, int out);
-int q4_ctas(long long tiles, int units);  // CTAs of a persistent launch over tiles of so many units
+int q4_ctas(long long tiles, int units, int per_sm);  // CTAs of a persistent launch over tiles of so many units
 int launch_q4_expand(const Q4Args& p, float* delta, cudaStream_t st);
 int launch_q4_mm(const Q4Args& p, const Q4Work& w, cudaStream_t st);
 int launch_q4_tc(const Q4Args& p, const Q4Work& w, cudaStream_t st);

@@ -17,9 +17,9 @@
 namespace mlora {
 namespace {
 
-constexpr int kMmWarps = 16, kMmThreads = 32 * (kMmWarps + 1);  // and one warp for the copies
-constexpr int kMmBlocks = 8;                                    // of 64 inputs per stage
-constexpr int kMmSplit = 4;                                     // warps that share a range of outputs
+constexpr int kMmWarps = 8, kMmThreads = 32 * (kMmWarps + 1);  // and one warp for the copies
+constexpr int kMmBlocks = 4;                                    // of 64 inputs per stage
+constexpr int kMmSplit = 2;                                     // warps that share a range of outputs
 constexpr int kMmPitch = 132;                                   // floats between rows of x in the sums
 
 struct MmArgs {
@@ -41,14 +41,14 @@ __device__ __forceinline__ void mma_more(float (&d)[4], const uint32_t (&a)[4], 
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// One verdict of the 512 threads that multiply; see bar_all.
+// One verdict of the 256 threads that multiply; see bar_all.
 __device__ __forceinline__ bool mm_all(bool ok) {
   uint32_t r;
   __syncwarp();
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.and.aligned.pred q, 1, 512, p;\n\t"
+      "barrier.cta.red.and.aligned.pred q, 1, 256, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
       : "r"((uint32_t)ok)
@@ -63,12 +63,12 @@ struct MmStage {
   static constexpr int kW = kMmBlocks * kQ4TileBytes, kX = kMmBlocks * N8 * 1024, kS = kGroups * kQ4Tile * kEntry;
   static constexpr int kBytes = (kW + kX + kS + 1023) / 1024 * 1024;  // (x is swizzled: 1024-byte places)
   static constexpr int kSums = kMmSplit * N8 * 8 * kMmPitch * 4;
-  static constexpr int kStages = (227 * 1024 - 1024 - 512 - kSums) / kBytes < 8 ? (227 * 1024 - 1024 - 512 - kSums) / kBytes : 8;
+  static constexpr int kStages = (227 * 1024 / 2 - 1024 - 1536 - kSums) / kBytes;  // (two CTAs per SM)
   static constexpr int kSmem = 1024 + kStages * kBytes + kSums;
 };
 
 template <int N8, bool ZERO, int G>
-__global__ void __launch_bounds__(kMmThreads, 1) q4_mm_kernel(const __grid_constant__ CUtensorMap map_x, MmArgs t) {
+__global__ void __launch_bounds__(kMmThreads, 2) q4_mm_kernel(const __grid_constant__ CUtensorMap map_x, MmArgs t) {
   using S = MmStage<N8, ZERO, G>;
   constexpr int kStages = S::kStages, kEntry = S::kEntry;
   extern __shared__ uint8_t smem_raw[];
@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) q4_mm_kernel(const __grid_const
     }
   } else {
     // ---- products --------------------------------------------------------------------------------------------------------------------
-    const int quarter = warp >> 2, block = warp & 3, g = lane >> 2;
+    const int quarter = warp / kMmSplit, block = warp % kMmSplit, g = lane >> 2;
     float acc[2][N8][4];
     const auto clear = [&] {
 #pragma unroll
@@ -260,19 +260,24 @@ __global__ void __launch_bounds__(kMmThreads, 1) q4_mm_kernel(const __grid_const
       mm_all(true);
       const long long tile_begin = (long long)tile * t.units;
       const int row0 = tile % t.row_tiles * kQ4Tile, token0 = tile / t.row_tiles * (N8 * 8), n_tok = a.T - token0;
-      // a thread: one output of every fourth row of x
-      constexpr int kMine = N8 * 2;
+      // a thread: one output of every kApart-th row of x
+      constexpr int kApart = kMmWarps / 4, kMine = (N8 * 8 + kApart - 1) / kApart;
       const int c = tid & 127, tok0 = tid >> 7;
       float v[kMine];
 #pragma unroll
       for (int k = 0; k < kMine; ++k) {
-        const float* s = sums + (tok0 + 4 * k) * kMmPitch + c;
-        v[k] = (s[0] + s[N8 * 8 * kMmPitch]) + (s[2 * N8 * 8 * kMmPitch] + s[3 * N8 * 8 * kMmPitch]);
+        v[k] = 0.f;
+        if (tok0 + kApart * k < N8 * 8) {
+          const float* s = sums + (tok0 + kApart * k) * kMmPitch + c;
+#pragma unroll
+          for (int q = 0; q < kMmSplit; ++q) v[k] += s[q * N8 * 8 * kMmPitch];
+        }
       }
       if (u_first != 0) {
         float* mine = t.w.parts + (size_t)blockIdx.x * (kQ4Tile * kQ4Tile) + tok0 * kQ4Tile + c;
 #pragma unroll
-        for (int k = 0; k < kMine; ++k) __stcg(mine + 4 * k * kQ4Tile, v[k]);
+        for (int k = 0; k < kMine; ++k)
+          if (tok0 + kApart * k < N8 * 8) __stcg(mine + kApart * k * kQ4Tile, v[k]);
         mm_all(true);
         if (tid == 0) {
           __threadfence();
@@ -285,12 +290,12 @@ __global__ void __launch_bounds__(kMmThreads, 1) q4_mm_kernel(const __grid_const
           if (a.u != nullptr && there) {  // (two values a thread: quicker here than a kernel of its own in front of this one)
 #pragma unroll
             for (int k = 0; k < kMine; ++k)
-              if (tok0 + 4 * k < n_tok) v[k] += q4_adapter(a, t.p.packed_b, token0 + tok0 + 4 * k, o);
+              if (tok0 + kApart * k < n_tok) v[k] += q4_adapter(a, t.p.packed_b, token0 + tok0 + kApart * k, o);
           }
         } else if (t.w.delta != nullptr) {
           float add[kMine];
 #pragma unroll
-          for (int k = 0; k < kMine; ++k) add[k] = there && tok0 + 4 * k < n_tok ? __ldcg(t.w.delta + (size_t)(token0 + tok0 + 4 * k) * a.out + o) : 0.f;
+          for (int k = 0; k < kMine; ++k) add[k] = there && tok0 + kApart * k < n_tok ? __ldcg(t.w.delta + (size_t)(token0 + tok0 + kApart * k) * a.out + o) : 0.f;
 #pragma unroll
           for (int k = 0; k < kMine; ++k) v[k] += add[k];
         }
@@ -313,7 +318,8 @@ __global__ void __launch_bounds__(kMmThreads, 1) q4_mm_kernel(const __grid_const
           for (int part = blockIdx.x + 1; part <= last; ++part) {
             const float* from = t.w.parts + (size_t)part * (kQ4Tile * kQ4Tile) + tok0 * kQ4Tile + c;
 #pragma unroll
-            for (int k = 0; k < kMine; ++k) v[k] += __ldcg(from + 4 * k * kQ4Tile);
+            for (int k = 0; k < kMine; ++k)
+              if (tok0 + kApart * k < N8 * 8) v[k] += __ldcg(from + kApart * k * kQ4Tile);
           }
         }
         const bool silu = (a.flags & MLORA_SILU_MUL) != 0;
@@ -328,7 +334,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) q4_mm_kernel(const __grid_const
         if (there && (!silu || !(c & 8))) {
 #pragma unroll
           for (int k = 0; k < kMine; ++k)
-            if (tok0 + 4 * k < n_tok) store_out(a, token0 + tok0 + 4 * k, col, v[k]);
+            if (tok0 + kApart * k < n_tok) store_out(a, token0 + tok0 + kApart * k, col, v[k]);
         }
       }
       if (u == t.units) u = 0, ++tile;
@@ -376,7 +382,7 @@ int launch_q4_mm(const Q4Args& p, const Q4Work& w, cudaStream_t st) {
   MmArgs t{p, w, (p.a.out + kQ4Tile - 1) / kQ4Tile, (p.a.T + n8 * 8 - 1) / (n8 * 8), (p.n_kb + kMmBlocks - 1) / kMmBlocks};
   const long long all = (long long)t.row_tiles * t.token_tiles * t.units;
   if (all > 2147483647ll) return fail(MLORA_ESIZE, "q4_linear: too many tiles");
-  const int grid = q4_ctas(t.row_tiles * (long long)t.token_tiles, t.units);
+  const int grid = q4_ctas(t.row_tiles * (long long)t.token_tiles, t.units, 2);
   return n8 == 1 ? launch_mm_for<1>(t, grid, st) : launch_mm_for<2>(t, grid, st);
 }
 

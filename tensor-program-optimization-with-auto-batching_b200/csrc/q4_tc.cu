@@ -515,7 +515,7 @@ int launch_q4_tc(const Q4Args& p, const Q4Work& w, cudaStream_t st) {
   t.units = (p.n_kb + 1) / 2;
   const long long all = (long long)t.row_tiles * t.token_tiles * t.units;
   if (all > 2147483647ll) return fail(MLORA_ESIZE, "q4_linear: too many tiles");
-  const int grid = q4_ctas(t.row_tiles * (long long)t.token_tiles, t.units);
+  const int grid = q4_ctas(t.row_tiles * (long long)t.token_tiles, t.units, 1);
   return bn == 32 ? launch_tc_for<32>(t, grid, st) : bn == 64 ? launch_tc_for<64>(t, grid, st) : launch_tc_for<128>(t, grid, st);
 }
 
