@@ -91,6 +91,7 @@ __global__ void __launch_bounds__(kPlanMaxRows) prefix_plan_kernel(const int32_t
                                                                    const int32_t* __restrict__ prefix_id, const int32_t* __restrict__ prefix_len,
                                                                    int n_slots, int rt, int Hkv, int target, int cap_items, int cap_parts, long long least, int32_t* plan, int max_rows) {
   __shared__ int s_id[kPlanMaxRows];     // prefix of the row, -1: none
+  __shared__ int s_len[kPlanMaxRows];    // its tokens
   __shared__ int s_lead[kPlanMaxRows];   // first row of its group, if the group is taken together
   __shared__ int s_tile[kPlanMaxRows / kPlanMinRows + 1][8];  // blocks, rows, key ranges, first item, slot, keys, first entry of the list
   __shared__ int s_red[33];
@@ -105,12 +106,14 @@ __global__ void __launch_bounds__(kPlanMaxRows) prefix_plan_kernel(const int32_t
   }
   if (len < kPlanMinKeys) id = -1;
   s_id[t] = id;
+  s_len[t] = len;
   __syncthreads();
   int rank = 0, count = 0, lead = t;
   if (id >= 0)
     for (int j = 0; j < T; ++j)
       if (s_id[j] == id) {
         if (j < lead) lead = j;
+        len = min(len, s_len[j]);  // (of slots that say different things, what all of them share)
         rank += j < t;
         ++count;
       }
@@ -141,10 +144,7 @@ __global__ void __launch_bounds__(kPlanMaxRows) prefix_plan_kernel(const int32_t
     s_tile[tile][1] = rows;
   }
   const int total = block_sum_int(blocks, s_red);
-  // Keys per item, in blocks: an equal share for about `target` items (a tile's last one is shorter).  Long ranges run two CTAs to an SM, which fill each other's gaps;
-  // short ones (below 16 blocks) one, so that CTAs of the tail, which wait for memory and not for it, find room beside them (32 rows
-  // behind 4096 tokens: XX us instead of YY).
-  if ((long long)total * Hkv < 16ll * target) target /= 2;
+  // keys per item, in blocks: an equal share for about `target` items, two per SM (a tile's last one is shorter)
   int unit = max(1, (int)(((long long)total * Hkv + target - 1) / target));
   for (;;) {
     const int splits = opens ? (blocks + unit - 1) / unit : 0;
@@ -811,8 +811,11 @@ int launch_shared(const SharedArgs& a, int n_pages_total, int max_items, cudaStr
   if (!rc) rc = page_map(&mv, a.v_pages, n_pages_total, a.Hkv, PS, D, 1, PS);
   if (!rc) rc = page_map(&mkr, a.k_pages, n_pages_total, a.Hkv, PS, D, kTile / PS, PS);
   if (!rc) rc = page_map(&mvr, a.v_pages, n_pages_total, a.Hkv, PS, D, kTile / PS, PS);
-  if (!rc) rc = page_map(&mkt, a.k_pages, n_pages_total, a.Hkv, PS, D, 1, kTlKeys);
-  if (!rc) rc = page_map(&mvt, a.v_pages, n_pages_total, a.Hkv, PS, D, 1, kTlKeys);
+  mkt = mk, mvt = mv;  // (pages of 16: the same)
+  if (PS != kTlKeys) {
+    if (!rc) rc = page_map(&mkt, a.k_pages, n_pages_total, a.Hkv, PS, D, 1, kTlKeys);
+    if (!rc) rc = page_map(&mvt, a.v_pages, n_pages_total, a.Hkv, PS, D, 1, kTlKeys);
+  }
   if (rc) return rc;
   constexpr int smem = 3 * ND * kSub + 1024, smem_tail = kTlWarps * kTlStages * 2 * kTlKeys * D * 2 + 1024;
   static_assert(smem_tail >= kTlWarps * kTlHeads * D * 4 + kTlThreads * 16 + 1024, "the warps' results lie in the ring");

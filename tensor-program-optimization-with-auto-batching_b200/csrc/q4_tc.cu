@@ -19,10 +19,10 @@
 namespace mlora {
 namespace {
 
-// Warps: weight warpgroups, then those that sum and write (32 columns of BN 32 and 64 each, 64 of 128), then MMA issue, copies of x,
+// Warps: weight warpgroups, then those that sum and write (32 columns each), then MMA issue, copies of x,
 // copies of weights.
 constexpr int q4_weight_groups(int bn) { return bn == 32 ? 3 : 2; }
-constexpr int q4_out_warps(int bn) { return bn == 32 ? 4 : 8; }
+constexpr int q4_out_warps(int bn) { return bn / 8; }
 constexpr int q4_threads(int bn) { return 32 * (4 * q4_weight_groups(bn) + q4_out_warps(bn) + 3); }
 constexpr int q4_ring(int bn) { return bn == 32 ? 9 : bn == 64 ? 8 : 6; }  // packed units in shared memory: as many for every weight warpgroup
 constexpr int q4_bufs(int bn) { return bn == 128 ? 4 : 6; }  // units of weights in TMEM, and of x in shared memory (from L2, 1 us away)
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(q4_threads(BN), 1) q4_tc_kernel(const __grid_c
           tc_fence_after();
           const uint32_t from = tmem_d + d * BN + col0 + lanes;
           const float s = __uint_as_float((ZERO ? *reinterpret_cast<const uint32_t*>(scales) : (uint32_t)*reinterpret_cast<const uint16_t*>(scales)) << 16);
-          constexpr int kStep = kCols == 32 ? 32 : 16;  // (64 sums leave registers for 16 columns on their way)
+          constexpr int kStep = BN == 128 ? 16 : 32;  // (27 warps have registers for 16 columns on their way)
 #pragma unroll
           for (int c0 = 0; c0 < kCols; c0 += kStep) {
             float v[kStep];
