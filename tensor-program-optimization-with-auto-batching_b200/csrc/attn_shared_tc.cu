@@ -476,7 +476,6 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
 }
 
 // ---- the tail -------------------------------------------------------------------------------------------------------------------
-constexpr int kTlWarps = 4, kTlThreads = kTlWarps * 32;
 constexpr int kTlKeys = 16;  // keys a warp works on at a time
 constexpr int kTlHeads = 8;  // query heads of a CTA
 
@@ -506,9 +505,10 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint3
 }
 
 // grid (Hkv x head tiles, T, key ranges): up to eight query heads of a key head over the row's keys from `first` on (or a range of them).
-template <int D, int STAGES>
-__global__ void __launch_bounds__(kTlThreads, 3) tail_attn_kernel(const __grid_constant__ CUtensorMap map_k,
+template <int D, int STAGES, int W>
+__global__ void __launch_bounds__(W * 32, 12 / W) tail_attn_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                const __grid_constant__ CUtensorMap map_v, SharedArgs a) {
+  constexpr int kTlWarps = W, kTlThreads = W * 32;
   constexpr int kHalf = kTlKeys * D * 2;               // bytes of 16 keys: D / 64 sub-tiles [16][64], 128-byte swizzle
   extern __shared__ uint8_t smem_raw[];                // [warp][stage][K | V]; then the warps' partial results
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -801,7 +801,23 @@ int allow_smem(K kernel, int bytes, std::atomic<unsigned long long>& done) {
   return MLORA_OK;
 }
 
-constexpr int kTlStages = 2;  // (three CTAs per SM: twelve warps with 8 KB on the way each are 96 KB, and another 96 at work)
+constexpr int kTlStages = 2;  // (twelve warps per SM, in three or six CTAs: 96 KB on the way, and another 96 at work)
+
+template <int D, int W>
+int launch_tail(const CUtensorMap& mk, const CUtensorMap& mv, const SharedArgs& a, bool behind_prefix, cudaStream_t st) {
+  constexpr int smem = W * kTlStages * 2 * kTlKeys * D * 2 + 1024;
+  static_assert(smem >= W * kTlHeads * D * 4 + W * 32 * 16 + 1024, "the warps' results lie in the ring");
+  static std::atomic<unsigned long long> done{0};
+  const int rc = allow_smem(tail_attn_kernel<D, kTlStages, W>, smem, done);
+  if (rc) return rc;
+  const int head_tiles = (a.Hq / a.Hkv + kTlHeads - 1) / kTlHeads;
+  const cudaError_t e = launch_pdl_if(behind_prefix && pdl_enabled_tail(), tail_attn_kernel<D, kTlStages, W>,
+                                      dim3((unsigned)(a.Hkv * head_tiles), (unsigned)a.T, (unsigned)a.n_splits), dim3(W * 32), smem, st, mk, mv, a);
+  if (e != cudaSuccess) return fail(MLORA_ECUDA, "tail_attn_kernel: %s", cudaGetErrorString(e));
+  count_launch();
+  MLORA_CHECK_LAUNCH("tail_attn_kernel");
+  return MLORA_OK;
+}
 
 template <int ND, int PS>
 int launch_shared(const SharedArgs& a, int n_pages_total, int max_items, cudaStream_t st) {
@@ -817,11 +833,9 @@ int launch_shared(const SharedArgs& a, int n_pages_total, int max_items, cudaStr
     if (!rc) rc = page_map(&mvt, a.v_pages, n_pages_total, a.Hkv, PS, D, 1, kTlKeys);
   }
   if (rc) return rc;
-  constexpr int smem = 3 * ND * kSub + 1024, smem_tail = kTlWarps * kTlStages * 2 * kTlKeys * D * 2 + 1024;
-  static_assert(smem_tail >= kTlWarps * kTlHeads * D * 4 + kTlThreads * 16 + 1024, "the warps' results lie in the ring");
-  static std::atomic<unsigned long long> done{0}, done_tail{0};
+  constexpr int smem = 3 * ND * kSub + 1024;
+  static std::atomic<unsigned long long> done{0};
   rc = allow_smem(prefix_attn_kernel<ND, PS>, smem, done);
-  if (!rc) rc = allow_smem(tail_attn_kernel<D, kTlStages>, smem_tail, done_tail);
   if (rc) return rc;
   if (max_items > 0) {
     const cudaError_t e = launch_pdl_if(pdl_enabled_tail(), prefix_attn_kernel<ND, PS>, dim3((unsigned)max_items), dim3(kPxThreads), smem, st, mk, mv, mkr, mvr, a);
@@ -829,13 +843,9 @@ int launch_shared(const SharedArgs& a, int n_pages_total, int max_items, cudaStr
     count_launch();
     MLORA_CHECK_LAUNCH("prefix_attn_kernel");
   }
-  const int head_tiles = (a.Hq / a.Hkv + kTlHeads - 1) / kTlHeads;
-  const cudaError_t e = launch_pdl_if(max_items > 0 && pdl_enabled_tail(), tail_attn_kernel<D, kTlStages>, dim3((unsigned)(a.Hkv * head_tiles), (unsigned)a.T, (unsigned)a.n_splits),
-                                      dim3(kTlThreads), smem_tail, st, mkt, mvt, a);
-  if (e != cudaSuccess) return fail(MLORA_ECUDA, "tail_attn_kernel: %s", cudaGetErrorString(e));
-  count_launch();
-  MLORA_CHECK_LAUNCH("tail_attn_kernel");
-  return MLORA_OK;
+  // Many (row, key head) pairs: CTAs of two warps, whose ends hold up less of an SM (72 rows x 40 key heads: 159 us against 176 with
+  // four); few: four warps, which are through a row sooner (4 x 8: 12.1 us against 14.8, 128 x 8: 133 against 138).
+  return (long long)a.T * a.Hkv >= 2048 ? launch_tail<D, 2>(mkt, mvt, a, max_items > 0, st) : launch_tail<D, 4>(mkt, mvt, a, max_items > 0, st);
 }
 
 // How a call's scratch is laid out: tickets | own parts | prefix parts, in floats.

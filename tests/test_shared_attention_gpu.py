@@ -252,3 +252,27 @@ def test_refusals(ops, cuda):
         ops.prefix_plan(slots, pid, pid, ops.PrefixPlan(1, 4, 2, cuda))
     with pytest.raises(err, match="bad sizes"):
         ops.prefix_plan(slots, pid, pid, ops.PrefixPlan(2, 64, 1, cuda))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(40, 40, 64), (32, 16, 128), (64, 32, 128)])
+def test_many_rows_and_key_heads(ops, cuda, heads, kv_heads, dim):
+    """Enough pairs of rows and key heads for the smaller CTAs of the rows' own parts."""
+    n = 2100 // kv_heads + 3
+    rows = [(t % 3, (96, 160, 272)[t % 3], (96, 160, 272)[t % 3] + (t * 13) % 60) if t % 5 else (-1, 0, t % 40 - 1) for t in range(n)]
+    c = _case(heads, kv_heads, dim, 16, rows, seed=n)
+    got, plan = _call(ops, c, heads, kv_heads, cuda)
+    want, bound = _want(c, heads, kv_heads, dim)
+    err = (got.cpu().double() - want).abs()
+    assert bool((err <= bound).all()), float((err / bound.clamp(min=1e-30)).max())
+    assert int(plan.table[1]) >= 3
+
+
+def test_slots_that_disagree_share_the_shortest(ops, cuda):
+    """One prefix of which the slots give different lengths: the rows still see every token once."""
+    rows = [(0, 256, 300), (0, 160, 310), (0, 200, 290)]
+    c = _case(4, 2, 64, 16, [(0, 256, p) for _, _, p in rows], seed=11)
+    c["rows"] = rows
+    got, plan = _call(ops, c, 4, 2, cuda)
+    want, bound = _want(c, 4, 2, 64)
+    err = (got.cpu().double() - want).abs()
+    assert bool((err <= bound).all()) and int(plan.table[1]) == 1, float((err / bound).max())
