@@ -1,14 +1,17 @@
-// Projections with 4-bit weights for up to 64 rows (see q4.cuh for the layout): y = x W^T is bound by the weights' out in / 2 bytes, and on
-// the way there by the integer pipe, which takes 14 cycles for the eight weights of a word -- 224 per 8 KB and SM sub-core, against the
-// 350 in which HBM delivers them.  So nothing else may cost much: weights go from bulk copies in shared memory to registers and from
-// there, as the A operand, straight into mma.m16n8k16, whose fragments the packed order has; the legacy tensor path is a third busy at 32
-// rows.  (A tcgen05 form of this kernel needs the weights in TMEM, four kinds of barriers per block and a trip of every group's sums
-// through registers: 567 instructions per sub-core and 8 KB, 30 us at 32 rows x 4096 x 22016 against XX here.)
+// Projections with 4-bit weights for up to 16 rows (see q4.cuh for the layout): y = x W^T is bound by the weights' out in / 2 bytes, and on
+// the way there by the integer pipe: shifts and masks of the eight weights of a word are seven instructions of two cycles, 224 cycles per
+// 8 KB and SM sub-core against the 350 in which HBM delivers them.  So weights go from bulk copies in shared memory to registers and from
+// there, as the A operand, straight into mma.m16n8k16, whose fragments the packed order has (8.3 cycles each and sub-core: 134 per 8 KB
+// at up to eight rows); no TMEM, no hand-over between warps.  From 17 rows on the products of this path would cost more than the weights.
 //
-// A CTA's tile is 128 outputs x 8, 16 or 32 rows; stages of 256 inputs -- 16 KB of weights, their scales, the rows of x -- arrive by bulk and
-// TMA copies.  Sixteen warps: four ranges of 32 outputs x four blocks of 64 inputs.  Persistent, one CTA per SM, the stages of all tiles
-// dealt out in equal ranges; a tile that several CTAs share is finished by the one that begins it, from the sums that the others have
-// left in scratch -- the first thing each of them does.
+// A CTA's tile is 128 outputs x 8 or 16 rows; stages of 256 inputs -- 16 KB of weights, their scales, the rows of x -- arrive by bulk and
+// TMA copies.  Eight warps: four ranges of 32 outputs x two sets of blocks of 64 inputs.  Persistent, two CTAs per SM, the stages of all
+// tiles dealt out in equal ranges; a tile that several CTAs share is finished by the one that begins it, from the sums that the others
+// have left in scratch -- the first thing each of them does.
+//
+// Measured (weights from HBM, CUDA graph, groups of 128): 1 x 4096 x 22016 17.8 us, 8 rows 18.0, 16 rows 21.3; 1 x 4096 x 4096 7.4; 7 x 11008 x
+// 4096 in groups of 32 with zero points 14.2.  Without the products the copies alone take 13.4 us of the first, of which 5.7 are the
+// launch, the first copy and the last sums.  16 or 24 warps, or one CTA per SM, are no faster (18.8, 19.9, 19.0).
 #include "q4.cuh"
 #include "tc_ptx.cuh"
 

@@ -11,6 +11,12 @@
 // that begins it: the others leave their sums in scratch -- the first thing each of them does -- and it adds them up in the order of the
 // inputs.  Adapters are expanded by a kernel of their own in front of this one, into fp32 scratch that is added to the sums: a thread here
 // has one output and many rows, whose adapters' rows it would have to wait for one after the other.
+//
+// What bounds it: the warps that hand units on.  Their instructions come one after the other, some ten cycles each among the 17 to 27
+// warps of an SM: with one unit per barrier, counters instead of remainders and one barrier for weights and rows of x a unit takes 950
+// cycles at 32 rows, against 350 in which HBM delivers it and 128 in which it is multiplied.  Groups of 32 or 64 have an accumulator to
+// hand on for each of them.  Measured (CUDA graph): 32 x 4096 x 22016 25.6 us, 128 rows 36.3, 512 x 4096 x 11008 58.7 (787 TFLOP/s);
+// 32 x 4096 x 22016 in groups of 32 44.4.
 #include "q4.cuh"
 #include "tc_ptx.cuh"
 

@@ -290,8 +290,9 @@ class DecodeSession:
     ``seq_ids`` must already be in bucketing order (``LlamaSeqInfo.order_seqs``): rows of one adapter adjacent.
 
     ``rules`` (:class:`ops.LogitRules` of the sequences, in their order): the tokens are chosen under them, with the session's own
-    tokens as the answers (the first ones included, which the caller chooses: ``ops.choose_tokens`` on the prompts' logits).  A
-    sequence whose rules allow no token ends."""
+    tokens as the answers (the first ones included, which the caller chooses: ``ops.choose_tokens`` on the prompts' logits; a sequence
+    whose rules allow none has no place here).  A sequence whose rules allow no token ends; the cache then holds its last token too,
+    which that of any other sequence does not."""
 
     def __init__(self, engine: EngineBase, seq_ids, adapter_slots, first_tokens, max_gen, eos_id=None, use_lora=True, rules=None):
         self.eng, self.seq_ids, self.use_lora = engine, list(seq_ids), use_lora
@@ -321,6 +322,8 @@ class DecodeSession:
                 raise ValueError(f"mlora: rules of {rules.n} requests for {n} sequences")
             if getattr(engine.m, "tp_size", 1) > 1:
                 raise ValueError("mlora: rules look at whole rows of logits, a tensor-parallel rank has a slice")
+            if any(int(t) < 0 for t in first_tokens):
+                raise ValueError("mlora: a sequence without a first token (its rules allow none) cannot take part")
             self.rules = dataclasses.replace(rules, answer=self.out_tokens, answer_len=self.gen_count) if rules.n else None
         self._graphs = {}
         self.steps = 0
@@ -384,6 +387,10 @@ class DecodeSession:
         counts = self.gen_count.cpu().tolist()
         toks = self.out_tokens.cpu().tolist()
         self.d2h_bytes += 4 * (self.n + self.out_tokens.numel())
-        for sid, c in zip(self.seq_ids, counts):
-            self.eng.kv.note_device_decode([sid], c - 1)
+        if self.rules is not None:
+            self.eng.kv.note_device_lengths(self.seq_ids)
+            self.d2h_bytes += 4 * self.eng.kv.seq_lens.numel()
+        else:
+            for sid, c in zip(self.seq_ids, counts):
+                self.eng.kv.note_device_decode([sid], c - 1)
         return [t[:c] for t, c in zip(toks, counts)]

@@ -188,6 +188,13 @@ class PagedCache:
         for sid in seq_ids:
             self._len_host[self._slot_of[int(sid)]] += n_steps
 
+    def note_device_lengths(self, seq_ids):
+        """The same where the device decided how far each of these sequences went: their lengths are read back."""
+        lengths = self.seq_lens.cpu().numpy()
+        for sid in seq_ids:
+            slot = self._slot_of[int(sid)]
+            self._len_host[slot] = lengths[slot]
+
     def snapshot(self, seq_ids):
         """Whatever a step of these sequences changes and running it again would not put right (pages are simply written
         again): a function that puts it back."""

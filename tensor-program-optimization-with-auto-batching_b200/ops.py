@@ -43,9 +43,10 @@ def workspace(nbytes: int, device, tag="default"):
     on demand, never freed.  Zero-filled when created: the split-K arrival counters of ``mlora_linear``
     must start at zero (they reset themselves).  Long-lived users (``model.Engine``) own their scratch
     and pass it with ``work=`` instead."""
-    dev = torch.device(device)
-    idx = dev.index if dev.index is not None else torch.cuda.current_device()
-    key = (idx, torch.cuda.current_stream(idx).cuda_stream, tag)
+    idx = torch.device(device).index
+    if idx is None:
+        idx = torch.cuda.current_device()
+    key = (idx, torch._C._cuda_getCurrentRawStream(idx), tag)
     buf = _workspaces.get(key)
     if buf is None or buf.numel() < nbytes:
         if buf is not None:
@@ -381,6 +382,8 @@ def linear_norm(x, W, stack: LoraStack = None, slots=None, u=None, flags: int = 
     squares; consumer (``sumsq_in``, ``n_sumsq_in``, ``eps``, ``norm_dim``): output rows scaled by their input
     rows' 1/rms before the activation.  ``u`` must already hold the shrink outputs when ``stack`` is given."""
     _need_cuda(x, W)
+    if isinstance(W, QuantWeight):
+        raise ValueError("mlora.linear_norm: bf16 weights only; use linear and residual_rmsnorm with a QuantWeight")
     if isinstance(W, PackedWeight):
         flags |= W_PACKED
     if stack is not None and stack.b_packed:
@@ -461,6 +464,8 @@ def decode_chain(steps, slots, ranks, scales, n_adapters: int, work):
     T = steps[0].x.shape[0]
     for i, st in enumerate(steps):
         _need_cuda(st.x, st.y)
+        if not isinstance(st.W, PackedWeight):
+            raise ValueError(f"mlora.decode_chain: step {i} needs a PackedWeight, got {type(st.W).__name__}")
         ph = arr[i]
         ph.d_x, ph.ldx, ph.d_Wp = st.x.data_ptr(), st.x.stride(0), st.W.data_ptr()
         ph.d_y, ph.ldy = st.y.data_ptr(), st.y.stride(0)
@@ -992,7 +997,11 @@ def _one_device(*ts):
 
 def _int32_table(what, t, *shape):
     """A contiguous int32 tensor of this shape (None: any size)."""
-    if t.dtype != torch.int32 or not t.is_contiguous() or t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+    ok = t.dtype == torch.int32 and t.is_contiguous() and t.dim() == len(shape)
+    if ok:
+        for n, m in zip(shape, t.shape):
+            ok = ok and (n is None or n == m)
+    if not ok:
         raise ValueError(f"mlora: {what} must be contiguous int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
 
 
@@ -1011,6 +1020,7 @@ class PrefixPlan:
         if not n:
             raise ValueError(f"mlora: no prefix plan for {Hkv} key heads")
         self.table = torch.zeros(n // 4, dtype=torch.int32, device=device)
+        self.work_bytes = {}  # (rows, head size) -> scratch of their attention
 
 
 def prefix_plan(row_slot, prefix_id, prefix_len, plan: PrefixPlan):
@@ -1045,7 +1055,7 @@ def paged_attention_shared(q, k_pages, v_pages, block_table, row_slot, row_pos, 
         out = torch.empty(T, Hq * D, dtype=torch.bfloat16, device=q.device)
     if (plan.T, plan.Hq, plan.Hkv) != (T, Hq, Hkv):
         raise ValueError(f"mlora: the plan is for {plan.T} rows of {plan.Hq} heads over {plan.Hkv}, the call for {T} of {Hq} over {Hkv}")
-    if any(t.dtype != torch.bfloat16 for t in (q, k_pages, v_pages, out)) or v_pages.shape != k_pages.shape:
+    if not q.dtype == k_pages.dtype == v_pages.dtype == out.dtype == torch.bfloat16 or v_pages.shape != k_pages.shape:
         raise ValueError("mlora: shared attention takes bf16 queries, pages of one shape, and a bf16 result")
     if not (k_pages.is_contiguous() and v_pages.is_contiguous()) or q.stride(1) != 1 or out.stride(1) != 1 or q.shape[1] < Hq * D \
             or tuple(out.shape) != (T, Hq * D):
@@ -1053,8 +1063,10 @@ def paged_attention_shared(q, k_pages, v_pages, block_table, row_slot, row_pos, 
     _int32_table("block_table", block_table, None, None)
     _int32_table("row_slot", row_slot, T)
     _int32_table("row_pos", row_pos, T)
-    need = paged_attention_shared_workspace(T, Hq, Hkv, D)
     if work is None:
+        need = plan.work_bytes.get((T, D))
+        if need is None:
+            need = plan.work_bytes[T, D] = paged_attention_shared_workspace(T, Hq, Hkv, D)
         work = workspace(need, q.device, "attn_shared")
     check(_lib.lib().mlora_paged_attention_shared(
         _ptr(q), q.stride(0), _ptr(k_pages), _ptr(v_pages), n_pages, _ptr(block_table), block_table.shape[1], _ptr(row_slot), _ptr(row_pos),
@@ -1157,11 +1169,15 @@ class LogitRules:
 
     def _tables(self, V):
         """(requests, device, arguments of the call), checked once for these tables."""
-        if self._ready is None or self._ready[0] != V:
-            at = _one_device(*(t for t in vars(self).values() if isinstance(t, torch.Tensor)))
-            del at
-            object.__setattr__(self, "_ready", (V, *self._check(V)))
-        return self._ready[1:]
+        if self._ready is not None:
+            known, tensors, places, ready = self._ready
+            if known == V and places == [t.data_ptr() for t in tensors] + [t.numel() for t in tensors]:  # (no table was resized or replaced in place)
+                return ready
+        tensors = [t for t in vars(self).values() if isinstance(t, torch.Tensor)]
+        _one_device(*tensors)
+        ready = self._check(V)
+        object.__setattr__(self, "_ready", (V, tensors, [t.data_ptr() for t in tensors] + [t.numel() for t in tensors], ready))
+        return ready
 
     def _check(self, V):
         n = self.n

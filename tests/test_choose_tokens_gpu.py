@@ -176,3 +176,18 @@ def test_refusals(ops, cuda):
     for kw in (dict(biases=[{V: 1.0}, None]), dict(allowed=[[V], None]), dict(allowed=[[-1], None]), dict(prompts=[[1]]), dict(repetition=[1.0, 2.0, 3.0])):
         with pytest.raises(ValueError):
             ops.LogitRules.build(V, n, cuda, **kw)
+
+
+def test_a_table_that_grows_in_place(ops, cuda):
+    """Rules whose answers' buffer is resized in place between calls are read from where it lies then."""
+    V = 500
+    rules = ops.LogitRules(frequency=torch.full((2,), 100.0, device=cuda), answer=torch.full((2, 4), 7, dtype=torch.int32, device=cuda),
+                           answer_len=torch.tensor([1, 1], dtype=torch.int32, device=cuda))
+    logits = torch.zeros(2, V, device=cuda)
+    logits[:, 7], logits[:, 9], logits[:, 11] = 3.0, 2.0, 1.0
+    assert ops.choose_tokens(logits, rules).tolist() == [9, 9]
+    rules.answer.resize_(2, 100000)
+    rules.answer.zero_()
+    rules.answer[:, 0], rules.answer[:, 1], rules.answer[:, 2] = 7, 9, 5
+    rules.answer_len.fill_(3)
+    assert ops.choose_tokens(logits, rules).tolist() == [11, 11]

@@ -231,3 +231,15 @@ def test_empty_and_refusals(ops, cuda):
     with pytest.raises(err, match="sixteens"):
         q2, s2, z2, _ = _weights(40, 128, 64, True, seed=0)
         ops.linear(x, _packed(ops, q2, s2, z2, 64, cuda), flags=ops.SILU_MUL)
+
+
+def test_paths_without_integers_refuse_them(ops, cuda):
+    """The folded norm and the one-launch layer read bf16 weights: packed integers are refused before a launch."""
+    q, s, z, _ = _weights(64, 128, 64, True, seed=0)
+    W = _packed(ops, q, s, z, 64, cuda)
+    x = torch.zeros(4, 128, dtype=torch.bfloat16, device=cuda)
+    y = torch.zeros(4, 64, dtype=torch.bfloat16, device=cuda)
+    with pytest.raises(ValueError, match="bf16 weights"):
+        ops.linear_norm(x, W, res=torch.zeros(4, 64, device=cuda), norm_w=y[0], sumsq_out=torch.zeros(32, device=cuda))
+    with pytest.raises(ValueError, match="PackedWeight"):
+        ops.decode_chain([ops.ChainStep(x=x, W=W, y=y)], None, None, None, 0, ops.new_workspace(1 << 20, cuda))

@@ -171,3 +171,31 @@ def test_session_refusals(ops, cuda):
     with pytest.raises(ValueError):
         registry.build_model(CFG, w, device=cuda, nonsense=1)
     assert registry.build_model(CFG, w, device=cuda, weight_bits=4, weight_group=64).weight_bits == 4
+
+
+def test_the_cache_after_a_session_with_rules(ops, cuda):
+    """The host's lengths are the device's when a session ends, whichever way its sequences did, and a continuation gives the logits of the
+    whole text run at once."""
+    w, _, _ = _weights()
+    texts = [[5, 17, 3, 8], [9, 2, 40]]
+
+    def start():
+        eng = _engine(w, cuda)
+        for i, t in enumerate(texts):
+            eng.kv.add_sequence(i)
+        return eng, eng.extend(range(2), texts)[0]
+
+    eng, _ = start()
+    rules = ops.LogitRules.build(1000, 2, cuda, allowed=[None, []])
+    with pytest.raises(ValueError, match="first token"):
+        load("model").DecodeSession(eng, [0, 1], [-1, -1], [4, -1], [3, 3], rules=rules)
+    got = load("model").DecodeSession(eng, [0, 1], [-1, -1], [4, 7], [3, 3], rules=rules).run()
+    assert [len(g) for g in got] == [3, 1] and got[1] == [7]
+    lengths = eng.kv.seq_lens.cpu().tolist()
+    held = [eng.kv.length(i) for i in range(2)]
+    assert held == [lengths[eng.kv.slot(i)] for i in range(2)] == [4 + 2, 3 + 1]
+    more = [got[0][-1:] + [11], [11]]
+    a = eng.extend(range(2), more)[0].clone()
+    eng, _ = start()
+    b = eng.extend(range(2), [got[0][:-1] + more[0], got[1] + more[1]])[0]
+    torch.testing.assert_close(a, b, atol=2e-2, rtol=1e-2)
