@@ -91,6 +91,17 @@ __device__ __forceinline__ int block_sum_int(int v, int* sm /*[33]*/) {
   return s;
 }
 
+__device__ __forceinline__ int block_max_int(int v, int* sm /*[33]*/) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
+  __syncthreads();
+  int m = sm[0];
+  for (int w = 1; w < (int)(blockDim.x >> 5); ++w) m = max(m, sm[w]);
+  return m;
+}
+
 // One CTA, a thread per row.  Rows of a group keep their order; groups are ordered by their first row.
 __global__ void __launch_bounds__(kPlanMaxRows) prefix_plan_kernel(const int32_t* __restrict__ row_slot, int T,
                                                                    const int32_t* __restrict__ prefix_id, const int32_t* __restrict__ prefix_len,
@@ -149,15 +160,34 @@ __global__ void __launch_bounds__(kPlanMaxRows) prefix_plan_kernel(const int32_t
     s_tile[tile][1] = rows;
   }
   const int total = block_sum_int(blocks, s_red);
-  // keys per item, in blocks: an equal share for about `target` items, two per SM (a tile's last one is shorter)
-  int unit = max(1, (int)(((long long)total * Hkv + target - 1) / target));
-  for (;;) {
-    const int splits = opens ? (blocks + unit - 1) / unit : 0;
-    const int items = block_sum_int(splits, s_red) * Hkv, parts = block_sum_int(splits * rows, s_red);
-    const int longer = block_sum_int(opens && blocks > unit, s_red);
-    if (longer == 0 || (items <= cap_items && parts <= cap_parts)) break;
-    unit += max(1, unit / 8);
+  // Blocks per item: a candidate per thread, from a quarter of an equal share for `target` items -- two per SM -- upwards, and one item per
+  // tile and key head, which always has room.  The best one has the shortest way through: rounds of `target` items times the longest item,
+  // each with some two blocks' time before and behind.  (4 tiles x 256 blocks x 8 key heads: 320 items of 26, a round and a bit, 133 us;
+  // 288 of 29, one round, @@ us.)
+  __shared__ unsigned long long s_best;
+  const int longest = block_max_int(blocks, s_red);
+  if (t == 0) s_best = ~0ull;
+  const int base = max(1, (int)(((long long)total * Hkv + 4LL * target - 1) / (4LL * target)));
+  const auto candidate = [&](int i) { return i == 0 ? longest : base + (i - 1) * max(1, base / 16); };
+  __syncthreads();
+  {
+    const int unit = candidate(t);
+    long long items = 0, parts = 0;
+    int length = 0;
+    for (int i = 0; i < n_tiles && unit <= longest; ++i) {
+      const int n = s_tile[i][0], k = (n + unit - 1) / unit;
+      items += k;
+      parts += k * s_tile[i][1];
+      length = max(length, (n + k - 1) / k);
+    }
+    items *= Hkv;
+    if (n_tiles > 0 && unit <= longest && items <= cap_items && parts <= cap_parts) {
+      const unsigned long long cost = (unsigned long long)((items + target - 1) / target) * (length + 2);
+      atomicMin(&s_best, min(cost, (1ull << 29) - 1) << 34 | (unsigned long long)items << 10 | t);
+    }
   }
+  __syncthreads();
+  const int unit = max(1, candidate((int)(s_best & 1023)));
   const int splits = opens ? (blocks + unit - 1) / unit : 0;
   if (opens) s_tile[tile][2] = splits;
   __syncthreads();
