@@ -30,6 +30,9 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 128;               // (row, query head) pairs of a tile = keys of a block
 constexpr int kSub = kTile * 64 * 2;     // one [128 x 64] bf16 sub-tile: 16 KB
+// A pair's scores are taken against a reference that follows their running maximum only when that is more than 2^kGrow above it: exact all
+// the same -- the reference cancels, and fp32 sums and bf16 weights of up to 2^8 round no more than those of up to 1 --, and O stays in TMEM.
+constexpr float kGrow = 8.f;
 constexpr int kPxThreads = 160;          // warps 0..3: one thread per pair; warp 4: copies and MMA issue
 constexpr int kPlanMaxRows = 1024;
 constexpr int kPlanHeader = 8;           // int32: rows, tiles, items, parts
@@ -253,7 +256,7 @@ struct SharedArgs {
 
 // One item: a tile's pairs x a range of the prefix's blocks of 128 keys x one key head.  As in the prompt attention, S = Q K^T and
 // P V are tcgen05 products with S, P and O in TMEM, keys and values arrive page by page through the block table of the group's first
-// row, and one thread per pair runs the softmax against the exact running maximum.
+// row, and one thread per pair runs the softmax: a block's 128 scores in registers, and nothing to be taken out of TMEM but them.
 template <int ND, int PS>
 __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                      const __grid_constant__ CUtensorMap map_v,
@@ -266,8 +269,9 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
   uint8_t* sv = sk + ND * kSub;
   __shared__ uint64_t kbar, vbar;  // a block's keys / values have landed
   __shared__ uint64_t sbar;        // S = Q K^T has retired, and every P V before it
-  __shared__ uint64_t pbar;        // the four softmax warps have written P, and taken the P V before into O
+  __shared__ uint64_t pbar;        // the four softmax warps have written P, and O is at its reference
   __shared__ uint64_t obar;        // P V has retired
+  __shared__ uint64_t fbar;        // ... the last one
   __shared__ uint32_t tmem_slot;
   __shared__ int s_abort;
 
@@ -289,6 +293,7 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
     mbar_init(&sbar, 1);
     mbar_init(&pbar, 4);
     mbar_init(&obar, 1);
+    mbar_init(&fbar, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 4) {
@@ -387,8 +392,9 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < kTile / 16; ++k)
-          umma_bf16_ta(tmem_o, tmem_base + k * 8, make_smem_desc_mn(smem_u32(sv + k * 2048), kSub, 1024), idesc_pv, k > 0 ? 1u : 0u);
+          umma_bf16_ta(tmem_o, tmem_base + k * 8, make_smem_desc_mn(smem_u32(sv + k * 2048), kSub, 1024), idesc_pv, kb > 0 || k > 0 ? 1u : 0u);
         umma_commit(&obar);
+        if (kb + 1 == n_blocks) umma_commit(&fbar);
       }
       __syncwarp();
     }
@@ -399,9 +405,6 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
     const bool busy = warp * 32 < i1.y * rep;
     const int q_pos = row >= 0 ? a.row_pos[row] : -1;
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    float o[D];
-#pragma unroll
-    for (int i = 0; i < D; ++i) o[i] = 0.f;
     float m_run = -INFINITY, l_run = 0.f;
     bool ok = true;
     for (int kb = 0; kb < n_blocks && ok; ++kb) {
@@ -412,59 +415,55 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
       tc_fence_after();
       const uint32_t s_addr = tmem_base + lanes;
       const int hi = min(q_pos, n_keys - 1) - kstart;  // last key of the block that this pair sees
-      float corr = 0.f;
       if (busy) {
-        const bool need_mask = __any_sync(0xffffffffu, hi < kTile - 1);
-        float buf[2][16];  // 16 scores at work, the next 16 on their way
+        float v[kTile];
+#pragma unroll
+        for (int c = 0; c < kTile / 16; ++c) tmem_ld16_issue(s_addr + c * 16, v + c * 16);
+#pragma unroll
+        for (int c = 0; c < kTile / 16; ++c) tmem_wait_ld16(v + c * 16);
+        if (__any_sync(0xffffffffu, hi < kTile - 1)) {
+#pragma unroll
+          for (int i = 0; i < kTile; ++i)
+            if (i > hi) v[i] = -INFINITY;
+        }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        auto maximum = [&](auto masked) {
-          tmem_ld16_issue(s_addr, buf[0]);
 #pragma unroll
-          for (int c = 0; c < kTile / 16; ++c) {
-            tmem_wait_ld16(buf[c & 1]);
-            if (c + 1 < kTile / 16) tmem_ld16_issue(s_addr + (c + 1) * 16, buf[(c + 1) & 1]);
+        for (int i = 0; i < kTile; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale;
+        const bool grows = top > m_run + kGrow;  // (with nothing seen yet: as soon as there is a score)
+        if (__any_sync(0xffffffffu, grows)) {
+          const float corr = !grows ? 1.f : m_run == -INFINITY ? 0.f : fast_exp2(m_run - top);
+          if (grows) m_run = top;
+          l_run *= corr;
+          if (kb > 0)
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (!masked() || c * 16 + i <= hi) mx[i & 3] = fmaxf(mx[i & 3], buf[c & 1][i]);
-          }
-        };
-        if (need_mask)
-          maximum(std::true_type{});
-        else
-          maximum(std::false_type{});
-        const float m_new = fmaxf(m_run, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale);
-        corr = m_run == -INFINITY ? 0.f : fast_exp2(m_run - m_new);
-        const float neg_m = m_new == -INFINITY ? 0.f : -m_new;  // (-inf: nothing seen yet)
-        float sum = 0.f;
-        auto probabilities = [&](auto masked) {
-          tmem_ld16_issue(s_addr, buf[0]);
+            for (int c = 0; c < D / 16; ++c) {
+              float o[16];
+              tmem_ld16_issue(tmem_o + lanes + c * 16, o);
+              tmem_wait_ld16(o);
 #pragma unroll
-          for (int c = 0; c < kTile / 16; ++c) {
-            tmem_wait_ld16(buf[c & 1]);
-            if (c + 1 < kTile / 16) tmem_ld16_issue(s_addr + (c + 1) * 16, buf[(c + 1) & 1]);
-            uint32_t pk[8];
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              float p[2];
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                p[e] = fast_exp2(fmaf(buf[c & 1][i + e], a.scale, neg_m));
-                if (masked() && c * 16 + i + e > hi) p[e] = 0.f;
-                sum += p[e];
-              }
-              const __nv_bfloat162 b = __floats2bfloat162_rn(p[0], p[1]);
-              pk[i / 2] = *reinterpret_cast<const uint32_t*>(&b);
+              for (int i = 0; i < 16; ++i) o[i] *= corr;
+              tmem_st8_issue(tmem_o + lanes + c * 16, reinterpret_cast<const uint32_t*>(o));
+              tmem_st8_issue(tmem_o + lanes + c * 16 + 8, reinterpret_cast<const uint32_t*>(o + 8));
             }
-            tmem_st8_issue(s_addr + c * 8, pk);
+        }
+        const float neg_m = m_run == -INFINITY ? 0.f : -m_run;  // (-inf: nothing seen yet)
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < kTile / 16; ++c) {
+          uint32_t pk[8];
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const float p0 = fast_exp2(fmaf(v[c * 16 + i], a.scale, neg_m)), p1 = fast_exp2(fmaf(v[c * 16 + i + 1], a.scale, neg_m));
+            sum[i & 2] += p0;
+            sum[(i & 2) + 1] += p1;
+            const __nv_bfloat162 b = __floats2bfloat162_rn(p0, p1);
+            pk[i / 2] = *reinterpret_cast<const uint32_t*>(&b);
           }
-          tmem_wait_st();
-        };
-        if (need_mask)
-          probabilities(std::true_type{});
-        else
-          probabilities(std::false_type{});
-        l_run = fmaf(l_run, corr, sum);
-        m_run = m_new;
+          tmem_st8_issue(s_addr + c * 8, pk);
+        }
+        tmem_wait_st();
+        l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       }
       if (n_keys - kstart < kTile) {
         // the prefix ends inside this block: values of keys that are not its own are zeroed (0 * NaN is not 0)
@@ -481,27 +480,24 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&pbar);
-      ok = __all_sync(0xffffffffu, mbar_wait(&obar, par, &s_abort));
-      if (!ok) break;
-      tc_fence_after();
-      if (busy) {
-        float buf[2][16];
-        tmem_ld16_issue(tmem_o + lanes, buf[0]);
-#pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-          tmem_wait_ld16(buf[c & 1]);
-          if (c + 1 < D / 16) tmem_ld16_issue(tmem_o + lanes + (c + 1) * 16, buf[(c + 1) & 1]);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[c * 16 + i] = fmaf(o[c * 16 + i], corr, buf[c & 1][i]);
-        }
-      }
     }
+    if (ok && n_blocks > 0) ok = __all_sync(0xffffffffu, mbar_wait(&fbar, 0, &s_abort));
+    tc_fence_after();
     if (!ok) s_abort = 1;
-    if (row >= 0) {
-      float* dst = a.parts + ((size_t)(pv.row[row].y + split) * a.Hq + head) * (D + 4);
+    if (busy) {
+      float* dst = row < 0 ? nullptr : a.parts + ((size_t)(pv.row[row].y + split) * a.Hq + head) * (D + 4);
 #pragma unroll
-      for (int c = 0; c < D / 4; ++c) reinterpret_cast<float4*>(dst)[c] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
-      *reinterpret_cast<float2*>(dst + D) = ok ? make_float2(m_run, l_run) : make_float2(-INFINITY, 0.f);
+      for (int c = 0; c < D / 16; ++c) {
+        float o[16] = {};
+        if (ok && n_blocks > 0) {
+          tmem_ld16_issue(tmem_o + lanes + c * 16, o);
+          tmem_wait_ld16(o);
+        }
+        if (dst)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(dst)[c * 4 + i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+      }
+      if (dst) *reinterpret_cast<float2*>(dst + D) = ok ? make_float2(m_run, l_run) : make_float2(-INFINITY, 0.f);
     }
     if (!ok && tid == 0 && a.status) atomicOr(a.status, 1);
   }
