@@ -33,7 +33,7 @@ constexpr int kSub = kTile * 64 * 2;     // one [128 x 64] bf16 sub-tile: 16 KB
 // A pair's scores are taken against a reference that follows their running maximum only when that is more than 2^kGrow above it: exact all
 // the same -- the reference cancels, and fp32 sums and bf16 weights of up to 2^8 round no more than those of up to 1 --, and O stays in TMEM.
 constexpr float kGrow = 8.f;
-constexpr int kPxThreads = 160;          // warps 0..3: one thread per pair; warp 4: copies and MMA issue
+constexpr int kPxThreads = 192;          // warps 0..3: one thread per pair; 4: MMA issue; 5: copies
 constexpr int kPlanMaxRows = 1024;
 constexpr int kPlanHeader = 8;           // int32: rows, tiles, items, parts
 constexpr int kTickets = 1024;           // arrival counters at the start of the scratch, whatever the call's sizes: zero between calls
@@ -256,7 +256,7 @@ struct SharedArgs {
 
 // One item: a tile's pairs x a range of the prefix's blocks of 128 keys x one key head.  As in the prompt attention, S = Q K^T and
 // P V are tcgen05 products with S, P and O in TMEM, keys and values arrive page by page through the block table of the group's first
-// row, and one thread per pair runs the softmax: a block's 128 scores in registers, and nothing to be taken out of TMEM but them.
+// row, and one thread per pair runs the softmax: a block's 128 scores in registers, and nothing else to be taken out of TMEM.
 template <int ND, int PS>
 __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                      const __grid_constant__ CUtensorMap map_v,
@@ -325,10 +325,7 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
   tc_fence_after();
   const uint32_t tmem_base = tmem_slot, tmem_o = tmem_base + kTile;
 
-  if (warp == 4) {
-    // ---- copies and MMAs: lane 0 waits and issues, one lane per page copies -----------------------------------------------
-    constexpr uint32_t idesc = make_idesc(kTile, kTile);
-    constexpr uint32_t idesc_pv = make_idesc(kTile, D) | (1u << 16);  // B operand MN-major
+  if (warp >= 4) {
     auto wait = [&](uint64_t* bar, uint32_t par) {
       int w = 1;
       if (lane == 0) w = mbar_wait(bar, par, &s_abort) ? 1 : 0;
@@ -336,70 +333,76 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
       if (!w) s_abort = 1;
       return w != 0;
     };
-    auto page_of = [&](int kb) {  // read one block ahead
-      const int pg = (b0 + kb) * kPages + lane;
-      return lane < kPages && kb < n_blocks && pg < n_pages ? bt[pg] : -1;
-    };
-    auto copy = [&](int kb, int page, uint8_t* dst, const CUtensorMap* map, const CUtensorMap* map_run, uint64_t* bar) {
-      const int valid = min(kPages, n_pages - (b0 + kb) * kPages);
-      const int first = __shfl_sync(0xffffffffu, page, 0);
-      if (valid == kPages && __all_sync(0xffffffffu, lane >= kPages || page == first + lane)) {
-        // pages that follow each other in the pool: one copy per 64 columns
+    if (warp == 4) {
+      // ---- MMAs -----------------------------------------------------------------------------------------------------------
+      constexpr uint32_t idesc = make_idesc(kTile, kTile);
+      constexpr uint32_t idesc_pv = make_idesc(kTile, D) | (1u << 16);  // B operand MN-major
+      // (keys and values: atoms of 8 keys x 64 columns, those of the same keys beside each other)
+      const uint64_t qdesc = make_smem_desc(smem_u32(sq)), kdesc = make_smem_desc(smem_u32(sk)) + ((uint64_t)((ND - 1) * 1024 >> 4) << 32);
+      const uint64_t vdesc = make_smem_desc_mn(smem_u32(sv), 1024, ND * 1024);
+      for (int kb = 0; kb < n_blocks; ++kb) {
+        const uint32_t par = kb & 1;
+        if (!wait(&kbar, par)) break;
         if (lane == 0) {
-          mbar_expect_tx(bar, (uint32_t)(ND * kSub));
-          for (int j = 0; j < ND; ++j) tma_load_4d(dst + j * kSub, map_run, j * 64, 0, kvh, first, bar);
+          tc_fence_after();
+#pragma unroll
+          for (int j = 0; j < ND; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_bf16(tmem_base, qdesc + j * (kSub >> 4) + 2 * k, kdesc + j * (1024 >> 4) + 2 * k, idesc, (j > 0 || k > 0) ? 1u : 0u);
+          umma_commit(&sbar);
         }
         __syncwarp();
-        return;
-      }
-      if (lane == 0) mbar_expect_tx(bar, (uint32_t)(valid * ND * PS * 128));
-      __syncwarp();
-      if (lane < valid)
-        for (int j = 0; j < ND; ++j) tma_load_4d(dst + j * kSub + lane * (PS * 128), map, j * 64, 0, kvh, page, bar);
-      __syncwarp();
-    };
-    int page = page_of(0), page_next = page_of(1);
-    if (n_blocks > 0) {  // (a prefix longer than the block table is cut at its end)
-      copy(0, page, sk, &map_k, &map_kr, &kbar);
-      copy(0, page, sv, &map_v, &map_vr, &vbar);
-    }
-    for (int kb = 0; kb < n_blocks; ++kb) {
-      const uint32_t par = kb & 1;
-      if (!wait(&kbar, par)) break;
-      if (lane == 0) {
-        tc_fence_after();
+        if (!wait(&vbar, par) || !wait(&pbar, par)) break;
+        if (lane == 0) {
+          tc_fence_after();
 #pragma unroll
-        for (int j = 0; j < ND; ++j) {
-          const uint64_t adesc = make_smem_desc(smem_u32(sq + j * kSub));
-          const uint64_t bdesc = make_smem_desc(smem_u32(sk + j * kSub));
-#pragma unroll
-          for (int k = 0; k < 4; ++k) umma_bf16(tmem_base, adesc + 2 * k, bdesc + 2 * k, idesc, (j > 0 || k > 0) ? 1u : 0u);
+          for (int k = 0; k < kTile / 16; ++k)
+            umma_bf16_ta(tmem_o, tmem_base + k * 8, vdesc + k * (2 * ND * 1024 >> 4), idesc_pv, kb > 0 || k > 0 ? 1u : 0u);
+          umma_commit(&obar);
+          if (kb + 1 == n_blocks) umma_commit(&fbar);
         }
-        umma_commit(&sbar);
+        __syncwarp();
       }
-      if (kb > 0) {  // V's place is free once the P V before has retired
-        if (!wait(&obar, par ^ 1)) break;
+    } else {
+      // ---- copies: a block's values once the ones before are in O, the next one's keys once the scores are there.  Copies of single pages
+      // take their time to be issued, which is why the MMAs do not wait behind them --------------------------------------------
+      auto page_of = [&](int kb) {  // read one block ahead
+        const int pg = (b0 + kb) * kPages + lane;
+        return lane < kPages && kb < n_blocks && pg < n_pages ? bt[pg] : -1;
+      };
+      auto copy = [&](int kb, int page, uint8_t* dst, const CUtensorMap* map, const CUtensorMap* map_run, uint64_t* bar) {
+        const int valid = min(kPages, n_pages - (b0 + kb) * kPages);
+        int pg[kPages];
+#pragma unroll
+        for (int i = 0; i < kPages; ++i) pg[i] = __shfl_sync(0xffffffffu, page, i);
+        if (valid == kPages && __all_sync(0xffffffffu, lane >= kPages || page == pg[0] + lane)) {
+          // pages that follow each other in the pool: one copy
+          if (lane == 0) {
+            mbar_expect_tx(bar, (uint32_t)(ND * kSub));
+            tma_load_5d(dst, map_run, 0, 0, 0, kvh * (PS / 8), pg[0], bar);
+          }
+        } else if (lane == 0) {
+          mbar_expect_tx(bar, (uint32_t)(valid * ND * PS * 128));
+#pragma unroll
+          for (int i = 0; i < kPages; ++i)
+            if (i < valid) tma_load_5d(dst + i * (PS * D * 2), map, 0, 0, 0, kvh * (PS / 8), pg[i], bar);
+        }
+        __syncwarp();
+      };
+      int page = page_of(0), page_next = page_of(1);
+      if (n_blocks > 0) copy(0, page, sk, &map_k, &map_kr, &kbar);
+      for (int kb = 0; kb < n_blocks; ++kb) {
+        if (kb > 0 && !wait(&obar, (kb - 1) & 1)) break;
         copy(kb, page, sv, &map_v, &map_vr, &vbar);
-      }
-      if (kb + 1 < n_blocks) {
-        if (!wait(&sbar, par)) break;
+        if (kb + 1 == n_blocks || !wait(&sbar, kb & 1)) break;
         page = page_next;
         page_next = page_of(kb + 2);
         copy(kb + 1, page, sk, &map_k, &map_kr, &kbar);
       }
-      if (!wait(&vbar, par) || !wait(&pbar, par)) break;
-      if (lane == 0) {
-        tc_fence_after();
-#pragma unroll
-        for (int k = 0; k < kTile / 16; ++k)
-          umma_bf16_ta(tmem_o, tmem_base + k * 8, make_smem_desc_mn(smem_u32(sv + k * 2048), kSub, 1024), idesc_pv, kb > 0 || k > 0 ? 1u : 0u);
-        umma_commit(&obar);
-        if (kb + 1 == n_blocks) umma_commit(&fbar);
-      }
-      __syncwarp();
+      if (s_abort && lane == 0)  // copies may still be in flight: let them land before the shared memory goes to another CTA
+        for (int i = 0; i < 64; ++i) __nanosleep(1000);
     }
-    if (s_abort && lane == 0)  // copies may still be in flight: let them land before the shared memory goes to another CTA
-      for (int i = 0; i < 64; ++i) __nanosleep(1000);
   } else {
     // ---- softmax: one thread per pair; a warp without pairs only keeps step -------------------------------------------------
     const bool busy = warp * 32 < i1.y * rep;
@@ -473,7 +476,7 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
 #pragma unroll
           for (int half = 0; half < ND; ++half)
 #pragma unroll
-            for (int c = 0; c < 8; ++c) reinterpret_cast<uint4*>(sv + half * kSub + tid * 128)[c] = make_uint4(0u, 0u, 0u, 0u);
+            for (int c = 0; c < 8; ++c) reinterpret_cast<uint4*>(sv + (tid >> 3) * (ND * 1024) + half * 1024 + (tid & 7) * 128)[c] = make_uint4(0u, 0u, 0u, 0u);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
@@ -806,15 +809,29 @@ __global__ void __launch_bounds__(W * 32, 12 / W) tail_attn_kernel(const __grid_
   }
 }
 
-// Pages [n_pages][Hkv][PS][D], a box of `keys` keys of `pages` pages of one head, 64 columns: rows of 128 bytes, swizzled.
-int page_map(CUtensorMap* m, const void* ptr, int n_pages, int Hkv, int PS, int D, int pages, int keys) {
+// Pages [n_pages][Hkv][PS][D], a box of kTlKeys keys of one head, 64 columns: rows of 128 bytes, swizzled.
+int page_map(CUtensorMap* m, const void* ptr, int n_pages, int Hkv, int PS, int D) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(MLORA_ECUDA, "paged_attention_shared: cuTensorMapEncodeTiled is not available from this driver");
   cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)PS, (cuuint64_t)Hkv, (cuuint64_t)n_pages};
   cuuint64_t strides[3] = {(cuuint64_t)D * 2, (cuuint64_t)PS * D * 2, (cuuint64_t)Hkv * PS * D * 2};
-  cuuint32_t box[4] = {64, (cuuint32_t)keys, 1, (cuuint32_t)pages};
+  cuuint32_t box[4] = {64, (cuuint32_t)kTlKeys, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MLORA_ECUDA, "paged_attention_shared: cuTensorMapEncodeTiled failed with %d", (int)r);
+  return MLORA_OK;
+}
+
+// The same, `pages` whole pages of one head as atoms of 8 keys x 64 columns, those of the same keys beside each other: one copy has it all.
+int atom_map(CUtensorMap* m, const void* ptr, int n_pages, int Hkv, int PS, int D, int pages) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(MLORA_ECUDA, "paged_attention_shared: cuTensorMapEncodeTiled is not available from this driver");
+  cuuint64_t dims[5] = {64, 8, (cuuint64_t)D / 64, (cuuint64_t)Hkv * (PS / 8), (cuuint64_t)n_pages};
+  cuuint64_t strides[4] = {(cuuint64_t)D * 2, 128, (cuuint64_t)8 * D * 2, (cuuint64_t)Hkv * PS * D * 2};
+  cuuint32_t box[5] = {64, 8, (cuuint32_t)D / 64, (cuuint32_t)PS / 8, (cuuint32_t)pages};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(MLORA_ECUDA, "paged_attention_shared: cuTensorMapEncodeTiled failed with %d", (int)r);
   return MLORA_OK;
@@ -854,15 +871,12 @@ template <int ND, int PS>
 int launch_shared(const SharedArgs& a, int n_pages_total, int max_items, cudaStream_t st) {
   constexpr int D = ND * 64;
   CUtensorMap mk, mv, mkr, mvr, mkt, mvt;  // a page, a block of them, 16 keys
-  int rc = page_map(&mk, a.k_pages, n_pages_total, a.Hkv, PS, D, 1, PS);
-  if (!rc) rc = page_map(&mv, a.v_pages, n_pages_total, a.Hkv, PS, D, 1, PS);
-  if (!rc) rc = page_map(&mkr, a.k_pages, n_pages_total, a.Hkv, PS, D, kTile / PS, PS);
-  if (!rc) rc = page_map(&mvr, a.v_pages, n_pages_total, a.Hkv, PS, D, kTile / PS, PS);
-  mkt = mk, mvt = mv;  // (pages of 16: the same)
-  if (PS != kTlKeys) {
-    if (!rc) rc = page_map(&mkt, a.k_pages, n_pages_total, a.Hkv, PS, D, 1, kTlKeys);
-    if (!rc) rc = page_map(&mvt, a.v_pages, n_pages_total, a.Hkv, PS, D, 1, kTlKeys);
-  }
+  int rc = atom_map(&mk, a.k_pages, n_pages_total, a.Hkv, PS, D, 1);
+  if (!rc) rc = atom_map(&mv, a.v_pages, n_pages_total, a.Hkv, PS, D, 1);
+  if (!rc) rc = atom_map(&mkr, a.k_pages, n_pages_total, a.Hkv, PS, D, kTile / PS);
+  if (!rc) rc = atom_map(&mvr, a.v_pages, n_pages_total, a.Hkv, PS, D, kTile / PS);
+  if (!rc) rc = page_map(&mkt, a.k_pages, n_pages_total, a.Hkv, PS, D);
+  if (!rc) rc = page_map(&mvt, a.v_pages, n_pages_total, a.Hkv, PS, D);
   if (rc) return rc;
   constexpr int smem = 3 * ND * kSub + 1024;
   static std::atomic<unsigned long long> done{0};
