@@ -33,7 +33,7 @@ constexpr int kSub = kTile * 64 * 2;     // one [128 x 64] bf16 sub-tile: 16 KB
 // A pair's scores are taken against a reference that follows their running maximum only when that is more than 2^kGrow above it: exact all
 // the same -- the reference cancels, and fp32 sums and bf16 weights of up to 2^8 round no more than those of up to 1 --, and O stays in TMEM.
 constexpr float kGrow = 8.f;
-constexpr int kPxThreads = 192;          // warps 0..3: one thread per pair; 4: MMA issue; 5: copies
+constexpr int kPxThreads = 192;          // warps 0..3: one thread per pair; 4: MMA issue, copies of keys; 5: copies of values
 constexpr int kPlanMaxRows = 1024;
 constexpr int kPlanHeader = 8;           // int32: rows, tiles, items, parts
 constexpr int kTickets = 1024;           // arrival counters at the start of the scratch, whatever the call's sizes: zero between calls
@@ -333,13 +333,40 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
       if (!w) s_abort = 1;
       return w != 0;
     };
+    // Copies of a block's pages take some hundred cycles each to be issued: two warps share them, and the MMAs have time for half of them
+    // while the softmax runs.
+    auto page_of = [&](int kb) {  // read one block ahead
+      const int pg = (b0 + kb) * kPages + lane;
+      return lane < kPages && kb < n_blocks && pg < n_pages ? bt[pg] : -1;
+    };
+    auto copy = [&](int kb, int page, uint8_t* dst, const CUtensorMap* map, const CUtensorMap* map_run, uint64_t* bar) {
+      const int valid = min(kPages, n_pages - (b0 + kb) * kPages);
+      int pg[kPages];
+#pragma unroll
+      for (int i = 0; i < kPages; ++i) pg[i] = __shfl_sync(0xffffffffu, page, i);
+      if (valid == kPages && __all_sync(0xffffffffu, lane >= kPages || page == pg[0] + lane)) {
+        // pages that follow each other in the pool: one copy
+        if (lane == 0) {
+          mbar_expect_tx(bar, (uint32_t)(ND * kSub));
+          tma_load_5d(dst, map_run, 0, 0, 0, kvh * (PS / 8), pg[0], bar);
+        }
+      } else if (lane == 0) {
+        mbar_expect_tx(bar, (uint32_t)(valid * ND * PS * 128));
+#pragma unroll
+        for (int i = 0; i < kPages; ++i)
+          if (i < valid) tma_load_5d(dst + i * (PS * D * 2), map, 0, 0, 0, kvh * (PS / 8), pg[i], bar);
+      }
+      __syncwarp();
+    };
+    int page = page_of(0), page_next = page_of(1);
     if (warp == 4) {
-      // ---- MMAs -----------------------------------------------------------------------------------------------------------
+      // ---- MMAs, and copies of keys: the next block's once the scores are there -----------------------------------------------------------------------------------------------------------
       constexpr uint32_t idesc = make_idesc(kTile, kTile);
       constexpr uint32_t idesc_pv = make_idesc(kTile, D) | (1u << 16);  // B operand MN-major
       // (keys and values: atoms of 8 keys x 64 columns, those of the same keys beside each other)
       const uint64_t qdesc = make_smem_desc(smem_u32(sq)), kdesc = make_smem_desc(smem_u32(sk)) + ((uint64_t)((ND - 1) * 1024 >> 4) << 32);
       const uint64_t vdesc = make_smem_desc_mn(smem_u32(sv), 1024, ND * 1024);
+      if (n_blocks > 0) copy(0, page, sk, &map_k, &map_kr, &kbar);
       for (int kb = 0; kb < n_blocks; ++kb) {
         const uint32_t par = kb & 1;
         if (!wait(&kbar, par)) break;
@@ -353,6 +380,12 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
           umma_commit(&sbar);
         }
         __syncwarp();
+        if (kb + 1 < n_blocks) {
+          if (!wait(&sbar, par)) break;
+          page = page_next;
+          page_next = page_of(kb + 2);
+          copy(kb + 1, page, sk, &map_k, &map_kr, &kbar);
+        }
         if (!wait(&vbar, par) || !wait(&pbar, par)) break;
         if (lane == 0) {
           tc_fence_after();
@@ -365,44 +398,16 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
         __syncwarp();
       }
     } else {
-      // ---- copies: a block's values once the ones before are in O, the next one's keys once the scores are there.  Copies of single pages
-      // take their time to be issued, which is why the MMAs do not wait behind them --------------------------------------------
-      auto page_of = [&](int kb) {  // read one block ahead
-        const int pg = (b0 + kb) * kPages + lane;
-        return lane < kPages && kb < n_blocks && pg < n_pages ? bt[pg] : -1;
-      };
-      auto copy = [&](int kb, int page, uint8_t* dst, const CUtensorMap* map, const CUtensorMap* map_run, uint64_t* bar) {
-        const int valid = min(kPages, n_pages - (b0 + kb) * kPages);
-        int pg[kPages];
-#pragma unroll
-        for (int i = 0; i < kPages; ++i) pg[i] = __shfl_sync(0xffffffffu, page, i);
-        if (valid == kPages && __all_sync(0xffffffffu, lane >= kPages || page == pg[0] + lane)) {
-          // pages that follow each other in the pool: one copy
-          if (lane == 0) {
-            mbar_expect_tx(bar, (uint32_t)(ND * kSub));
-            tma_load_5d(dst, map_run, 0, 0, 0, kvh * (PS / 8), pg[0], bar);
-          }
-        } else if (lane == 0) {
-          mbar_expect_tx(bar, (uint32_t)(valid * ND * PS * 128));
-#pragma unroll
-          for (int i = 0; i < kPages; ++i)
-            if (i < valid) tma_load_5d(dst + i * (PS * D * 2), map, 0, 0, 0, kvh * (PS / 8), pg[i], bar);
-        }
-        __syncwarp();
-      };
-      int page = page_of(0), page_next = page_of(1);
-      if (n_blocks > 0) copy(0, page, sk, &map_k, &map_kr, &kbar);
+      // ---- copies of values: a block's once the ones before are in O -------------------------------------------------------
       for (int kb = 0; kb < n_blocks; ++kb) {
         if (kb > 0 && !wait(&obar, (kb - 1) & 1)) break;
         copy(kb, page, sv, &map_v, &map_vr, &vbar);
-        if (kb + 1 == n_blocks || !wait(&sbar, kb & 1)) break;
         page = page_next;
         page_next = page_of(kb + 2);
-        copy(kb + 1, page, sk, &map_k, &map_kr, &kbar);
       }
-      if (s_abort && lane == 0)  // copies may still be in flight: let them land before the shared memory goes to another CTA
-        for (int i = 0; i < 64; ++i) __nanosleep(1000);
     }
+    if (s_abort && lane == 0)  // copies may still be in flight: let them land before the shared memory goes to another CTA
+      for (int i = 0; i < 64; ++i) __nanosleep(1000);
   } else {
     // ---- softmax: one thread per pair; a warp without pairs only keeps step -------------------------------------------------
     const bool busy = warp * 32 < i1.y * rep;
