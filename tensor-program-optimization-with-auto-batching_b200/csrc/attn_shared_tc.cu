@@ -34,6 +34,7 @@ constexpr int kSub = kTile * 64 * 2;     // one [128 x 64] bf16 sub-tile: 16 KB
 // the same -- the reference cancels, and fp32 sums and bf16 weights of up to 2^8 round no more than those of up to 1 --, and O stays in TMEM.
 constexpr float kGrow = 8.f;
 constexpr int kPxThreads = 192;          // warps 0..3: one thread per pair; 4: MMA issue, copies of keys; 5: copies of values
+constexpr int kPxRegs = 128;             // two CTAs per SM leave room for the tail's
 constexpr int kPlanMaxRows = 1024;
 constexpr int kPlanHeader = 8;           // int32: rows, tiles, items, parts
 constexpr int kTickets = 1024;           // arrival counters at the start of the scratch, whatever the call's sizes: zero between calls
@@ -256,9 +257,9 @@ struct SharedArgs {
 
 // One item: a tile's pairs x a range of the prefix's blocks of 128 keys x one key head.  As in the prompt attention, S = Q K^T and
 // P V are tcgen05 products with S, P and O in TMEM, keys and values arrive page by page through the block table of the group's first
-// row, and one thread per pair runs the softmax: a block's 128 scores in registers, and nothing else to be taken out of TMEM.
+// row, and one thread per pair runs the softmax: 64 of a block's scores in registers at a time, and nothing else to be taken out of TMEM.
 template <int ND, int PS>
-__global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid_constant__ CUtensorMap map_k,
+__global__ void __maxnreg__(kPxRegs) prefix_attn_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                      const __grid_constant__ CUtensorMap map_v,
                                                                      const __grid_constant__ CUtensorMap map_kr,
                                                                      const __grid_constant__ CUtensorMap map_vr, SharedArgs a) {
@@ -360,7 +361,7 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
     };
     int page = page_of(0), page_next = page_of(1);
     if (warp == 4) {
-      // ---- MMAs, and copies of keys: the next block's once the scores are there -----------------------------------------------------------------------------------------------------------
+      // ---- MMAs, and copies of keys: the next block's once the scores are there -----------------------
       constexpr uint32_t idesc = make_idesc(kTile, kTile);
       constexpr uint32_t idesc_pv = make_idesc(kTile, D) | (1u << 16);  // B operand MN-major
       // (keys and values: atoms of 8 keys x 64 columns, those of the same keys beside each other)
@@ -424,19 +425,25 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
       const uint32_t s_addr = tmem_base + lanes;
       const int hi = min(q_pos, n_keys - 1) - kstart;  // last key of the block that this pair sees
       if (busy) {
-        float v[kTile];
-#pragma unroll
-        for (int c = 0; c < kTile / 16; ++c) tmem_ld16_issue(s_addr + c * 16, v + c * 16);
-#pragma unroll
-        for (int c = 0; c < kTile / 16; ++c) tmem_wait_ld16(v + c * 16);
-        if (__any_sync(0xffffffffu, hi < kTile - 1)) {
-#pragma unroll
-          for (int i = 0; i < kTile; ++i)
-            if (i > hi) v[i] = -INFINITY;
-        }
+        float v[64];
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        const auto scores = [&](int half) {
 #pragma unroll
-        for (int i = 0; i < kTile; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
+          for (int c = 0; c < 4; ++c) tmem_ld16_issue(s_addr + half * 64 + c * 16, v + c * 16);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_wait_ld16(v + c * 16);
+          if (__any_sync(0xffffffffu, hi < kTile - 1)) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i)
+              if (half * 64 + i > hi) v[i] = -INFINITY;
+          }
+        };
+#pragma unroll
+        for (int half = 1; half >= 0; --half) {
+          scores(half);
+#pragma unroll
+          for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
+        }
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale;
         const bool grows = top > m_run + kGrow;  // (with nothing seen yet: as soon as there is a score)
         if (__any_sync(0xffffffffu, grows)) {
@@ -458,17 +465,21 @@ __global__ void __launch_bounds__(kPxThreads, 2) prefix_attn_kernel(const __grid
         const float neg_m = m_run == -INFINITY ? 0.f : -m_run;  // (-inf: nothing seen yet)
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < kTile / 16; ++c) {
-          uint32_t pk[8];
+        for (int half = 0; half < 2; ++half) {
+          if (half) scores(half);  // (the first half is still there; its weights go over scores that have been read)
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            const float p0 = fast_exp2(fmaf(v[c * 16 + i], a.scale, neg_m)), p1 = fast_exp2(fmaf(v[c * 16 + i + 1], a.scale, neg_m));
-            sum[i & 2] += p0;
-            sum[(i & 2) + 1] += p1;
-            const __nv_bfloat162 b = __floats2bfloat162_rn(p0, p1);
-            pk[i / 2] = *reinterpret_cast<const uint32_t*>(&b);
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pk[8];
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const float p0 = fast_exp2(fmaf(v[c * 16 + i], a.scale, neg_m)), p1 = fast_exp2(fmaf(v[c * 16 + i + 1], a.scale, neg_m));
+              sum[i & 2] += p0;
+              sum[(i & 2) + 1] += p1;
+              const __nv_bfloat162 b = __floats2bfloat162_rn(p0, p1);
+              pk[i / 2] = *reinterpret_cast<const uint32_t*>(&b);
+            }
+            tmem_st8_issue(s_addr + half * 32 + c * 8, pk);
           }
-          tmem_st8_issue(s_addr + c * 8, pk);
         }
         tmem_wait_st();
         l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
