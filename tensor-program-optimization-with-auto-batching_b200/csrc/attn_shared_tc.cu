@@ -270,7 +270,7 @@ __global__ void __maxnreg__(kPxRegs) prefix_attn_kernel(const __grid_constant__ 
   uint8_t* sv = sk + ND * kSub;
   __shared__ uint64_t kbar, vbar;  // a block's keys / values have landed
   __shared__ uint64_t sbar;        // S = Q K^T has retired, and every P V before it
-  __shared__ uint64_t pbar;        // the four softmax warps have written P, and O is at its reference
+  __shared__ uint64_t pbar[2];     // the four softmax warps have written P of the block's first / last 64 keys; O is at its reference
   __shared__ uint64_t obar;        // P V has retired
   __shared__ uint64_t fbar;        // ... the last one
   __shared__ uint32_t tmem_slot;
@@ -292,7 +292,8 @@ __global__ void __maxnreg__(kPxRegs) prefix_attn_kernel(const __grid_constant__ 
     mbar_init(&kbar, 1);
     mbar_init(&vbar, 1);
     mbar_init(&sbar, 1);
-    mbar_init(&pbar, 4);
+    mbar_init(&pbar[0], 4);
+    mbar_init(&pbar[1], 4);
     mbar_init(&obar, 1);
     mbar_init(&fbar, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -387,15 +388,20 @@ __global__ void __maxnreg__(kPxRegs) prefix_attn_kernel(const __grid_constant__ 
           page_next = page_of(kb + 2);
           copy(kb + 1, page, sk, &map_k, &map_kr, &kbar);
         }
-        if (!wait(&vbar, par) || !wait(&pbar, par)) break;
-        if (lane == 0) {
-          tc_fence_after();
+        if (!wait(&vbar, par)) break;
+        bool ok = true;
+        for (int half = 0; half < 2 && ok; ++half) {  // (the products of the first half run while the softmax is at the second)
+          ok = wait(&pbar[half], par);
+          if (ok && lane == 0) {
+            tc_fence_after();
 #pragma unroll
-          for (int k = 0; k < kTile / 16; ++k)
-            umma_bf16_ta(tmem_o, tmem_base + k * 8, vdesc + k * (2 * ND * 1024 >> 4), idesc_pv, kb > 0 || k > 0 ? 1u : 0u);
-          umma_commit(&obar);
-          if (kb + 1 == n_blocks) umma_commit(&fbar);
+            for (int k = 0; k < 4; ++k)
+              umma_bf16_ta(tmem_o, tmem_base + half * 32 + k * 8, vdesc + (half * 4 + k) * (2 * ND * 1024 >> 4), idesc_pv, kb + half + k > 0 ? 1u : 0u);
+            if (half) umma_commit(&obar);
+            if (half && kb + 1 == n_blocks) umma_commit(&fbar);
+          }
         }
+        if (!ok) break;
         __syncwarp();
       }
     } else {
@@ -423,6 +429,18 @@ __global__ void __maxnreg__(kPxRegs) prefix_attn_kernel(const __grid_constant__ 
       if (!ok) break;
       tc_fence_after();
       const uint32_t s_addr = tmem_base + lanes;
+      if (n_keys - kstart < kTile) {
+        // the prefix ends inside this block: values of keys that are not its own are zeroed (0 * NaN is not 0)
+        ok = __all_sync(0xffffffffu, mbar_wait(&vbar, par, &s_abort));
+        if (!ok) break;
+        if (tid >= n_keys - kstart) {
+#pragma unroll
+          for (int half = 0; half < ND; ++half)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) reinterpret_cast<uint4*>(sv + (tid >> 3) * (ND * 1024) + half * 1024 + (tid & 7) * 128)[c] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
       const int hi = min(q_pos, n_keys - 1) - kstart;  // last key of the block that this pair sees
       if (busy) {
         float v[64];
@@ -480,25 +498,20 @@ __global__ void __maxnreg__(kPxRegs) prefix_attn_kernel(const __grid_constant__ 
             }
             tmem_st8_issue(s_addr + half * 32 + c * 8, pk);
           }
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pbar[half]);
         }
-        tmem_wait_st();
         l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       }
-      if (n_keys - kstart < kTile) {
-        // the prefix ends inside this block: values of keys that are not its own are zeroed (0 * NaN is not 0)
-        ok = __all_sync(0xffffffffu, mbar_wait(&vbar, par, &s_abort));
-        if (!ok) break;
-        if (tid >= n_keys - kstart) {
-#pragma unroll
-          for (int half = 0; half < ND; ++half)
-#pragma unroll
-            for (int c = 0; c < 8; ++c) reinterpret_cast<uint4*>(sv + (tid >> 3) * (ND * 1024) + half * 1024 + (tid & 7) * 128)[c] = make_uint4(0u, 0u, 0u, 0u);
+      if (!busy) {
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&pbar[0]);
+          mbar_arrive(&pbar[1]);
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&pbar);
     }
     if (ok && n_blocks > 0) ok = __all_sync(0xffffffffu, mbar_wait(&fbar, 0, &s_abort));
     tc_fence_after();
