@@ -1,7 +1,7 @@
 // Decode attention of a batch whose rows share long prefixes: the pages of a shared prefix are read once for all rows that have it
 // (the page-sharing counterpart of attention_with_fused_qkv, tvm/llama_auto_batcher/llama_for_causal_lm.py:55-64).
 //
-// softmax(q K^T) V over the keys of a row falls into ranges: with m, l and O the maximum, the sum of exp(s - m) and the sum of
+// softmax(q K^T) V over the keys of a row falls into ranges: with m, l and O the maximum (or what is near it), the sum of exp(s - m) and the sum of
 // exp(s - m) v of a range, two ranges make one with m = max(m1, m2), l = l1 e^(m1 - m) + l2 e^(m2 - m), O likewise.  So
 //
 //   prefix_plan_kernel     groups the rows of a step by the prefix their slot names (once a step, for all layers);
@@ -14,9 +14,10 @@
 // the softmax beyond.  The tail is bound by HBM alone: its tiles have only the query heads of one key head, so it uses mma.sync with 16
 // keys as the rows and up to eight heads as the columns, and a ring of TMA copies in every warp.  It is launched programmatically
 // dependent on the prefix and waits for it only before the join.
-// Measured (CUDA graph, three sets of inputs in turn): 32 rows x 32 heads behind 4096 tokens 60 us (3.9 TB/s of the keys and values read
-// once), 72 rows x 40 heads in four groups 159 us (5.6 TB/s), 128 rows x 32 heads over 8 key heads behind 32768 tokens 133 us (520
-// TFLOP/s), 4 rows behind 512 tokens 12 us.
+// Measured (CUDA graph, three sets of inputs in turn): 32 rows x 32 heads behind 4096 tokens 58.5 us (4.0 TB/s of the keys and values read
+// once), 72 rows x 40 heads in four groups 144 us (6.2 TB/s), 128 rows x 32 heads over 8 key heads behind 32768 tokens 124 us (560
+// TFLOP/s), 4 rows behind 512 tokens 12 us.  An eighth of the exponentials on the FMA units costs the third 3 us: it is instructions
+// that bound it, not exponentials alone.
 #include <math.h>
 
 #include <atomic>
@@ -34,14 +35,15 @@ constexpr int kSub = kTile * 64 * 2;     // one [128 x 64] bf16 sub-tile: 16 KB
 // the same -- the reference cancels, and fp32 sums and bf16 weights of up to 2^8 round no more than those of up to 1 --, and O stays in TMEM.
 constexpr float kGrow = 8.f;
 constexpr int kPxThreads = 192;          // warps 0..3: one thread per pair; 4: MMA issue, copies of keys; 5: copies of values
-constexpr int kPxRegs = 128;             // two CTAs per SM leave room for the tail's
+constexpr int kPxRegs = 128;             // two CTAs per SM leave room for the tail's (72 rows x 40 heads 146 us, with 168 160)
 constexpr int kPlanMaxRows = 1024;
 constexpr int kPlanHeader = 8;           // int32: rows, tiles, items, parts
 constexpr int kTickets = 1024;           // arrival counters at the start of the scratch, whatever the call's sizes: zero between calls
 constexpr int kPlanMinRows = 2, kPlanMinKeys = 64;  // smaller groups and shorter prefixes are read row by row
-// Reads a group has to save, (rows - 1) x tokens x key heads.  Measured, shared against row by row, 128-wide heads: 4 rows x 2048 x 32 key
-// heads (196608 saved) 21.8 us against 20.2; 32 x 1024 x 8 (253952) 17.2 against 27.3; 2 x 4096 x 32 (131072) 30.8 against 22.5.
-constexpr int kPlanLeast = 200000;
+// Reads a group has to save, (rows - 1) x tokens x key heads.  Measured, shared against row by row, 128-wide heads: 2 rows x 4096 x 8 key
+// heads (32768 saved) 22.9 us against 17.7; 8 x 1024 x 8 (57344) 13.9 against 15.9, 3 x 1024 x 32 (65536) 14.5 against 15.7; 2 x 4096 x 32
+// (131072) 22.8 against 22.3, 32 x 1024 x 8 (253952) 16.9 against 27.1.
+constexpr int kPlanLeast = 50000;
 
 // A plan in int32: header; per row a quad (first key of its own part, its first part, its parts, 0) and its entry of `list` (rows by group);
 // then two quads per item, all that a CTA needs to begin: (slot whose pages are read, first block, blocks, keys of the prefix | first entry
@@ -166,8 +168,8 @@ __global__ void __launch_bounds__(kPlanMaxRows) prefix_plan_kernel(const int32_t
   const int total = block_sum_int(blocks, s_red);
   // Blocks per item: a candidate per thread, from a quarter of an equal share for `target` items -- two per SM -- upwards, and one item per
   // tile and key head, which always has room.  The best one has the shortest way through: rounds of `target` items times the longest item,
-  // each with some two blocks' time before and behind.  (4 tiles x 256 blocks x 8 key heads: 320 items of 26, a round and a bit, 133 us;
-  // 288 of 29, one round, @@ us.)
+  // each with some two blocks' time before and behind.  (An equal
+  // share alone gives 4 tiles x 256 blocks x 8 key heads 320 items of 26 blocks, a round and a bit; 288 of 29 are one.)
   __shared__ unsigned long long s_best;
   const int longest = block_max_int(blocks, s_red);
   if (t == 0) s_best = ~0ull;
@@ -917,8 +919,8 @@ int launch_shared(const SharedArgs& a, int n_pages_total, int max_items, cudaStr
     count_launch();
     MLORA_CHECK_LAUNCH("prefix_attn_kernel");
   }
-  // Many (row, key head) pairs: CTAs of two warps, whose ends hold up less of an SM (72 rows x 40 key heads: 159 us against 176 with
-  // four); few: four warps, which are through a row sooner (4 x 8: 12.1 us against 14.8, 128 x 8: 133 against 138).
+  // Many (row, key head) pairs: CTAs of two warps, whose ends hold up less of an SM (72 rows x 40 key heads: 144 us against 151 with
+  // four); few: four warps, which are through a row sooner (4 x 8: 12.1 us against 14.8, 128 x 8: 124 against 128).
   return (long long)a.T * a.Hkv >= 2048 ? launch_tail<D, 2>(mkt, mvt, a, max_items > 0, st) : launch_tail<D, 4>(mkt, mvt, a, max_items > 0, st);
 }
 

@@ -20,6 +20,9 @@ ANY_SUMS = 2048
 Q4_ZEROS = 4096
 
 
+_data_ptr, _numel = torch.Tensor.data_ptr, torch.Tensor.numel
+
+
 def _ptr(t):  # (plain numbers: the prototypes convert them)
     return None if t is None else t.data_ptr()
 
@@ -1170,13 +1173,14 @@ class LogitRules:
     def _tables(self, V):
         """(requests, device, arguments of the call), checked once for these tables."""
         if self._ready is not None:
-            known, tensors, places, ready = self._ready
-            if known == V and places == [t.data_ptr() for t in tensors] + [t.numel() for t in tensors]:  # (no table was resized or replaced in place)
+            known, tensors, places, wide, sizes, ready = self._ready
+            if known == V and places == list(map(_data_ptr, tensors)) and sizes == list(map(_numel, wide)):  # (no table was resized or replaced in place)
                 return ready
         tensors = [t for t in vars(self).values() if isinstance(t, torch.Tensor)]
         _one_device(*tensors)
+        wide = [t for t in (self.prompt, self.answer, self.bias_start, self.bias_token, self.masks) if t is not None] + tensors[:1]
         ready = self._check(V)
-        object.__setattr__(self, "_ready", (V, tensors, [t.data_ptr() for t in tensors] + [t.numel() for t in tensors], ready))
+        object.__setattr__(self, "_ready", (V, tensors, list(map(_data_ptr, tensors)), wide, list(map(_numel, wide)), ready))
         return ready
 
     def _check(self, V):
