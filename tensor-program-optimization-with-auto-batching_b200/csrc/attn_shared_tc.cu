@@ -11,13 +11,13 @@
 //
 // The prefix has 2 D 2 bytes per key and key head against 4 D 128 flops of a full tile: bound by HBM up to some 128 pairs (rows x query
 // heads per key head) -- for few pairs by the chain scores, softmax, products of a block, which 32 of a tile's rows do not shorten --, by
-// the softmax beyond.  The tail is bound by HBM alone: its tiles have only the query heads of one key head, so it uses mma.sync with 16
+// what comes through L2 beyond.  The tail is bound by HBM alone: its tiles have only the query heads of one key head, so it uses mma.sync with 16
 // keys as the rows and up to eight heads as the columns, and a ring of TMA copies in every warp.  It is launched programmatically
 // dependent on the prefix and waits for it only before the join.
 // Measured (CUDA graph, three sets of inputs in turn): 32 rows x 32 heads behind 4096 tokens 58.5 us (4.0 TB/s of the keys and values read
 // once), 72 rows x 40 heads in four groups 144 us (6.2 TB/s), 128 rows x 32 heads over 8 key heads behind 32768 tokens 124 us (560
-// TFLOP/s), 4 rows behind 512 tokens 12 us.  An eighth of the exponentials on the FMA units costs the third 3 us: it is instructions
-// that bound it, not exponentials alone.
+// TFLOP/s; every tile reads the prefix through L2: 537 MB, 6.3 TB/s), 4 rows behind 512 tokens 12 us.  Exponentials partly on the FMA
+// units (126 us) and steps of 64 keys with two places for everything (146) are no faster in the third.
 #include <math.h>
 
 #include <atomic>
