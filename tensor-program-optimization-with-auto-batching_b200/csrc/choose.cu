@@ -11,6 +11,8 @@
 // contraction), so that the choice at a near tie is that of plain 32-bit arithmetic.
 // Measured (CUDA graph): one row of 32000 4.8 us, 32 rows 7.6, 256 rows of 128000 with the logits kept 103 us (59 without rules, a copy
 // 42): what the rules cost there is looking through the texts once per piece, and its barriers.
+#include <atomic>
+
 #include "common.cuh"
 #include "tc_ptx.cuh"
 
@@ -20,6 +22,7 @@ namespace {
 constexpr int kChThreads = 512;
 constexpr int kChVec = 2;                                 // float4 of logits a thread keeps
 constexpr int kChPiece = kChThreads * kChVec * 4;         // tokens of a piece
+constexpr int kChSmem = 2 * kChPiece * 8;  // counts and biases of two pieces
 constexpr int kChCluster = 8;
 
 struct ChooseArgs {
@@ -93,8 +96,10 @@ struct Text {
 };
 
 __global__ void __launch_bounds__(kChThreads, 3) choose_tokens_kernel(ChooseArgs a) {
-  __shared__ __align__(16) uint32_t s_count[kChPiece];  // low 30 bits: times in the answer; then: has a bias, is in the prompt
-  __shared__ float s_bias[kChPiece];                    // of the tokens that have one
+  // of every second piece: its counts are made while other threads are still at the piece before
+  extern __shared__ __align__(16) uint32_t s_tables[];
+  uint32_t* s_counts = s_tables;                                           // low 30 bits: times in the answer; then: has a bias, is in the prompt
+  float* s_biases = reinterpret_cast<float*>(s_tables + 2 * kChPiece);     // of the tokens that have one
   __shared__ unsigned long long s_warp[kChThreads / 32];
   __shared__ int s_best[2];
   pdl_launch_dependents();
@@ -131,8 +136,9 @@ __global__ void __launch_bounds__(kChThreads, 3) choose_tokens_kernel(ChooseArgs
   answer.begin(n_answer ? a.answer + (size_t)src * a.ld_answer : nullptr, n_answer);
   if (counts || biased) {  // (a thread clears what it has read of a piece, so this is done once)
 #pragma unroll
-    for (int j = 0; j < kChVec; ++j) {
-      reinterpret_cast<uint4*>(s_count)[j * kChThreads + tid] = make_uint4(0u, 0u, 0u, 0u);
+    for (int j = 0; j < 2 * kChVec; ++j) {
+      if (j >= kChVec && (int64_t)(rank + width) * kChPiece >= a.V) break;  // (one piece only)
+      reinterpret_cast<uint4*>(s_counts)[j * kChThreads + tid] = make_uint4(0u, 0u, 0u, 0u);
     }
     __syncthreads();
   }
@@ -146,6 +152,8 @@ __global__ void __launch_bounds__(kChThreads, 3) choose_tokens_kernel(ChooseArgs
     sum = a.bias_value[i];
     for (int k = i + 1; k < b1 && a.bias_token[k] == w; ++k) sum += a.bias_value[k];
   };
+  uint32_t* s_count = s_counts;
+  float* s_bias = s_biases;
   const auto set_bias = [&](int w, float value, int v0) {
     const unsigned at = (unsigned)w - (unsigned)v0;
     if (w >= 0 && at < (unsigned)kChPiece) {
@@ -225,7 +233,9 @@ __global__ void __launch_bounds__(kChThreads, 3) choose_tokens_kernel(ChooseArgs
         }
       }
     }
-    if (counts || biased) __syncthreads();  // (before the next piece counts in the cleared tables)
+    // (the other tables: nobody counts in these again before everybody has met behind the counts of the next piece)
+    s_count = s_count == s_counts ? s_counts + kChPiece : s_counts;
+    s_bias = s_bias == s_biases ? s_biases + kChPiece : s_biases;
   }
   unsigned long long best = warp_best(choice_key(best_v, best_i));
   if (lane == 0) s_warp[warp] = best;
@@ -280,7 +290,16 @@ extern "C" int mlora_choose_tokens(const float* d_logits, int64_t ld, int32_t T,
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(T * width));
   cfg.blockDim = dim3(kChThreads);
+  cfg.dynamicSmemBytes = kChSmem;
   cfg.stream = (cudaStream_t)stream;
+  static std::atomic<unsigned long long> allowed{0};  // by device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!((allowed.load(std::memory_order_acquire) >> (dev & 63)) & 1ull)) {
+    const cudaError_t e = cudaFuncSetAttribute(choose_tokens_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kChSmem);
+    if (e != cudaSuccess) return fail(MLORA_ECUDA, "choose_tokens: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    allowed.fetch_or(1ull << (dev & 63), std::memory_order_release);
+  }
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)width;
