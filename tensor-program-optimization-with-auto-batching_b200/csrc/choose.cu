@@ -9,8 +9,9 @@
 // wins; between threads a 64-bit key of value and index decides, in any order, and the cluster's first CTA collects the CTAs' keys
 // through distributed shared memory: one launch, no scratch.  Values are rounded step by step as the formula is written (no
 // contraction), so that the choice at a near tie is that of plain 32-bit arithmetic.
-// Measured (CUDA graph): one row of 32000 4.8 us, 32 rows 7.6, 256 rows of 128000 with the logits kept 103 us (59 without rules, a copy
-// 42): what the rules cost there is looking through the texts once per piece, and its barriers.
+// Measured (CUDA graph): one row of 32000 4.6 us, 32 rows 7.5, 256 rows of 128000 with the logits kept 92 us (a copy 42): what the rules
+// cost there is looking through the texts once per piece, and its barrier.  Two tables in turn save the other barrier of a piece (104 us
+// without); the next piece's logits on their way cost a CTA per SM and lose (99).
 #include <atomic>
 
 #include "common.cuh"
@@ -282,8 +283,8 @@ extern "C" int mlora_choose_tokens(const float* d_logits, int64_t ld, int32_t T,
                d_answer_len, ld_answer, d_bias_set, d_bias_start, d_bias_token, d_bias_value, n_sets, n_bias, d_mask_of, d_masks, n_masks,
                ld_mask, d_logits_out, ld_out, d_tok};
   const int pieces = (V + kChPiece - 1) / kChPiece;
-  // CTAs per row: some six per SM (256 rows x 128000 under all rules, in us: one 115, two 120, four 103, eight 108; 32 rows x 32000: one
-  // 21.7, four 8.8, eight 7.6)
+  // CTAs per row: some six per SM (256 rows x 128000 under all rules, in us: one 99, two 104, four 92, eight 101; 32 rows x 32000: one
+  // 19.1, eight 7.5)
   int width = 1;
   while (width < kChCluster && width < pieces && (long long)T * width < 6 * 148) width *= 2;
   MLORA_REQUIRE((long long)T * width <= 2147483647ll, "choose_tokens: too many rows");
