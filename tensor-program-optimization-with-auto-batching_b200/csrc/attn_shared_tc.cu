@@ -1,7 +1,7 @@
 // Decode attention of a batch whose rows share long prefixes: the pages of a shared prefix are read once for all rows that have it
 // (the page-sharing counterpart of attention_with_fused_qkv, tvm/llama_auto_batcher/llama_for_causal_lm.py:55-64).
 //
-// softmax(q K^T) V over the keys of a row falls into ranges: with m, l and O the maximum (or what is near it), the sum of exp(s - m) and the sum of
+// softmax(q K^T) V over the keys of a row falls into ranges: with m, l and O the maximum the sum of exp(s - m) and the sum of
 // exp(s - m) v of a range, two ranges make one with m = max(m1, m2), l = l1 e^(m1 - m) + l2 e^(m2 - m), O likewise.  So
 //
 //   prefix_plan_kernel     groups the rows of a step by the prefix their slot names (once a step, for all layers);
@@ -15,9 +15,9 @@
 // keys as the rows and up to eight heads as the columns, and a ring of TMA copies in every warp.  It is launched programmatically
 // dependent on the prefix and waits for it only before the join.
 // Measured (CUDA graph, three sets of inputs in turn): 32 rows x 32 heads behind 4096 tokens 58.5 us (4.0 TB/s of the keys and values read
-// once), 72 rows x 40 heads in four groups 144 us (6.2 TB/s), 128 rows x 32 heads over 8 key heads behind 32768 tokens 124 us (560
-// TFLOP/s; every tile reads the prefix through L2: 537 MB, 6.3 TB/s), 4 rows behind 512 tokens 12 us.  Exponentials partly on the FMA
-// units (126 us) and steps of 64 keys with two places for everything (146) are no faster in the third.
+// once), 72 rows x 40 heads in four groups 146 us (6.1 TB/s), 128 rows x 32 heads over 8 key heads behind 32768 tokens 131 us (525
+// TFLOP/s; every tile reads the prefix through L2: 537 MB), 4 rows behind 512 tokens 12 us.  Exponentials partly on the FMA
+// units (2 % more) and steps of 64 keys with two places for everything (18 % more) are no faster in the third.
 #include <math.h>
 
 #include <atomic>
@@ -31,9 +31,6 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 128;               // (row, query head) pairs of a tile = keys of a block
 constexpr int kSub = kTile * 64 * 2;     // one [128 x 64] bf16 sub-tile: 16 KB
-// A pair's scores are taken against a reference that follows their running maximum only when that is more than 2^kGrow above it: exact all
-// the same -- the reference cancels, and fp32 sums and bf16 weights of up to 2^8 round no more than those of up to 1 --, and O stays in TMEM.
-constexpr float kGrow = 8.f;
 constexpr int kPxThreads = 192;          // warps 0..3: one thread per pair; 4: MMA issue, copies of keys; 5: copies of values
 constexpr int kPxRegs = 128;             // two CTAs per SM leave room for the tail's (72 rows x 40 heads 146 us, with 168 160)
 constexpr int kPlanMaxRows = 1024;
@@ -465,8 +462,10 @@ __global__ void __maxnreg__(kPxRegs) prefix_attn_kernel(const __grid_constant__ 
           for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
         }
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale;
-        const bool grows = top > m_run + kGrow;  // (with nothing seen yet: as soon as there is a score)
+        const bool grows = top > m_run;
         if (__any_sync(0xffffffffu, grows)) {
+          // (following the maximum only every 2^8 saves 6 % at 128 x 32768, but the largest weight is then no longer 1, which bf16 has
+          // exactly: error 0.0023 instead of 0.0019, of which 0.0017 are the result's own rounding)
           const float corr = !grows ? 1.f : m_run == -INFINITY ? 0.f : fast_exp2(m_run - top);
           if (grows) m_run = top;
           l_run *= corr;
@@ -919,8 +918,8 @@ int launch_shared(const SharedArgs& a, int n_pages_total, int max_items, cudaStr
     count_launch();
     MLORA_CHECK_LAUNCH("prefix_attn_kernel");
   }
-  // Many (row, key head) pairs: CTAs of two warps, whose ends hold up less of an SM (72 rows x 40 key heads: 144 us against 151 with
-  // four); few: four warps, which are through a row sooner (4 x 8: 12.1 us against 14.8, 128 x 8: 124 against 128).
+  // Many (row, key head) pairs: CTAs of two warps, whose ends hold up less of an SM (72 rows x 40 key heads: 146 us, with four
+  // 5 % more); few: four warps, which are through a row sooner (4 x 8: 12.1 us against 14.8 with two, 128 x 8: 131, with two 3 % more).
   return (long long)a.T * a.Hkv >= 2048 ? launch_tail<D, 2>(mkt, mvt, a, max_items > 0, st) : launch_tail<D, 4>(mkt, mvt, a, max_items > 0, st);
 }
 
