@@ -787,9 +787,10 @@ __global__ void __launch_bounds__(W * 32, 12 / W) tail_attn_kernel(const __grid_
   }
   const float inv = L > 0.f && !s_abort ? 1.f / L : 0.f;
   // outputs: 4 columns of a head per thread, D / 4 threads a head; where there are few heads, several threads share the ranges
-  constexpr int kPer = kTlThreads / (D / 4);           // heads in work at once
+  constexpr int kPer = kTlThreads / (D / 4);           // heads in work at once: 2, 4 or 8
   constexpr int kSets = kTlHeads / kPer;
-  const int hp = n_heads >= kPer ? kPer : n_heads > 2 ? 4 : n_heads, slices = kPer / hp;
+  // (a part of them, a power of two, only where it has all heads: those are done in one set)
+  const int hp = n_heads > kPer / 2 ? kPer : n_heads > 2 ? 4 : n_heads, slices = kPer / hp;
   float4 sum[kSets];
 #pragma unroll
   for (int i = 0; i < kSets; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
