@@ -1,7 +1,7 @@
 // Decode attention of a batch whose rows share long prefixes: the pages of a shared prefix are read once for all rows that have it
 // (the page-sharing counterpart of attention_with_fused_qkv, tvm/llama_auto_batcher/llama_for_causal_lm.py:55-64).
 //
-// softmax(q K^T) V over the keys of a row falls into ranges: with m, l and O the maximum the sum of exp(s - m) and the sum of
+// softmax(q K^T) V over the keys of a row falls into ranges: with m, l and O the maximum (or what is near it), the sum of exp(s - m) and the sum of
 // exp(s - m) v of a range, two ranges make one with m = max(m1, m2), l = l1 e^(m1 - m) + l2 e^(m2 - m), O likewise.  So
 //
 //   prefix_plan_kernel     groups the rows of a step by the prefix their slot names (once a step, for all layers);
@@ -14,8 +14,8 @@
 // what comes through L2 beyond.  The tail is bound by HBM alone: its tiles have only the query heads of one key head, so it uses mma.sync with 16
 // keys as the rows and up to eight heads as the columns, and a ring of TMA copies in every warp.  It is launched programmatically
 // dependent on the prefix and waits for it only before the join.
-// Measured (CUDA graph, three sets of inputs in turn): 32 rows x 32 heads behind 4096 tokens 58.5 us (4.0 TB/s of the keys and values read
-// once), 72 rows x 40 heads in four groups 146 us (6.1 TB/s), 128 rows x 32 heads over 8 key heads behind 32768 tokens 131 us (525
+// Measured (CUDA graph, three sets of inputs in turn): 32 rows x 32 heads behind 4096 tokens 60.3 us (3.9 TB/s of the keys and values read
+// once), 72 rows x 40 heads in four groups 151 us (5.9 TB/s), 128 rows x 32 heads over 8 key heads behind 32768 tokens 143 us (480
 // TFLOP/s; every tile reads the prefix through L2: 537 MB), 4 rows behind 512 tokens 12 us.  Exponentials partly on the FMA
 // units (2 % more) and steps of 64 keys with two places for everything (18 % more) are no faster in the third.
 #include <math.h>
@@ -31,6 +31,10 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 128;               // (row, query head) pairs of a tile = keys of a block
 constexpr int kSub = kTile * 64 * 2;     // one [128 x 64] bf16 sub-tile: 16 KB
+// A pair's scores are taken against a reference that follows their running maximum only when that is more than 2^kGrow above it: the
+// reference cancels, fp32 sums and weights of 16 bits round those of up to 2^8 no more than those of up to 1, and O stays in TMEM (128 x
+// 32768 143 us, following every maximum 150).
+constexpr float kGrow = 8.f;
 constexpr int kPxThreads = 192;          // warps 0..3: one thread per pair; 4: MMA issue, copies of keys; 5: copies of values
 constexpr int kPxRegs = 128;             // two CTAs per SM leave room for the tail's (72 rows x 40 heads 146 us, with 168 160)
 constexpr int kPlanMaxRows = 1024;
@@ -232,6 +236,17 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 
+// Two weights as the sum of two pairs of bf16: what a truncation leaves is rounded, so that the products with the values see them to 2^-15
+// and the sum l, which is taken before, fits them.  Decode attention without shared prefixes has fp32 weights; with bf16
+// ones a row's error was 0.0019 of the result in place of 0.0017, which is the result's own rounding (128 x 32768: 132 us).  Truncating is
+// a byte permutation; rounding the first part as well costs 6 % there.
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+  hi = __byte_perm(a, b, 0x7632);
+  const __nv_bfloat162 r = __floats2bfloat162_rn(x - __uint_as_float(a & 0xffff0000u), y - __uint_as_float(b & 0xffff0000u));
+  lo = *reinterpret_cast<const uint32_t*>(&r);
+}
+
 struct SharedArgs {
   const bf16* q;
   int64_t ld;
@@ -394,8 +409,9 @@ __global__ void __maxnreg__(kPxRegs) prefix_attn_kernel(const __grid_constant__ 
           if (ok && lane == 0) {
             tc_fence_after();
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma_bf16_ta(tmem_o, tmem_base + half * 32 + k * 8, vdesc + (half * 4 + k) * (2 * ND * 1024 >> 4), idesc_pv, kb + half + k > 0 ? 1u : 0u);
+            for (int k = 0; k < 8; ++k)  // (both parts of 16 keys' weights, then the next 16)
+              umma_bf16_ta(tmem_o, tmem_base + half * 64 + (k & 1) * 32 + (k >> 1) * 8, vdesc + (half * 4 + (k >> 1)) * (2 * ND * 1024 >> 4), idesc_pv,
+                           kb + half + k > 0 ? 1u : 0u);
             if (half) umma_commit(&obar);
             if (half && kb + 1 == n_blocks) umma_commit(&fbar);
           }
@@ -462,10 +478,8 @@ __global__ void __maxnreg__(kPxRegs) prefix_attn_kernel(const __grid_constant__ 
           for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
         }
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale;
-        const bool grows = top > m_run;
+        const bool grows = top > m_run + kGrow;  // (with nothing seen yet: as soon as there is a score)
         if (__any_sync(0xffffffffu, grows)) {
-          // (following the maximum only every 2^8 saves 6 % at 128 x 32768, but the largest weight is then no longer 1, which bf16 has
-          // exactly: error 0.0023 instead of 0.0019, of which 0.0017 are the result's own rounding)
           const float corr = !grows ? 1.f : m_run == -INFINITY ? 0.f : fast_exp2(m_run - top);
           if (grows) m_run = top;
           l_run *= corr;
@@ -488,16 +502,16 @@ __global__ void __maxnreg__(kPxRegs) prefix_attn_kernel(const __grid_constant__ 
           if (half) scores(half);  // (the first half is still there; its weights go over scores that have been read)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            uint32_t pk[8];
+            uint32_t hi[8], lo[8];
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
               const float p0 = fast_exp2(fmaf(v[c * 16 + i], a.scale, neg_m)), p1 = fast_exp2(fmaf(v[c * 16 + i + 1], a.scale, neg_m));
               sum[i & 2] += p0;
               sum[(i & 2) + 1] += p1;
-              const __nv_bfloat162 b = __floats2bfloat162_rn(p0, p1);
-              pk[i / 2] = *reinterpret_cast<const uint32_t*>(&b);
+              split_pair(p0, p1, hi[i / 2], lo[i / 2]);
             }
-            tmem_st8_issue(s_addr + half * 32 + c * 8, pk);
+            tmem_st8_issue(s_addr + half * 64 + c * 8, hi);
+            tmem_st8_issue(s_addr + half * 64 + 32 + c * 8, lo);
           }
           tmem_wait_st();
           tc_fence_before();
@@ -558,14 +572,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {  // of 16-bit val
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
-}
-// Two probabilities as the sum of two pairs of bf16: the products with the values keep 16 bits of them.
-__device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-  const float2 f = __bfloat1622float2(h);
-  const __nv_bfloat162 r = __floats2bfloat162_rn(x - f.x, y - f.y);
-  hi = *reinterpret_cast<const uint32_t*>(&h);
-  lo = *reinterpret_cast<const uint32_t*>(&r);
 }
 
 // grid (Hkv x head tiles, T, key ranges): up to eight query heads of a key head over the row's keys from `first` on (or a range of them).
