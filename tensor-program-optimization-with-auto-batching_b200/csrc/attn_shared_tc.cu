@@ -15,7 +15,7 @@
 // keys as the rows and up to eight heads as the columns, and a ring of TMA copies in every warp.  It is launched programmatically
 // dependent on the prefix and waits for it only before the join.
 // Measured (CUDA graph, three sets of inputs in turn): 32 rows x 32 heads behind 4096 tokens 60.3 us (3.9 TB/s of the keys and values read
-// once), 72 rows x 40 heads in four groups 151 us (5.9 TB/s), 128 rows x 32 heads over 8 key heads behind 32768 tokens 143 us (480
+// once), 72 rows x 40 heads in four groups 152 us (5.9 TB/s), 128 rows x 32 heads over 8 key heads behind 32768 tokens 143 us (480
 // TFLOP/s; every tile reads the prefix through L2: 537 MB), 4 rows behind 512 tokens 12 us.  Exponentials partly on the FMA
 // units (2 % more) and steps of 64 keys with two places for everything (18 % more) are no faster in the third.
 #include <math.h>
@@ -253,7 +253,7 @@ struct SharedArgs {
   const bf16* k_pages;
   const bf16* v_pages;
   const int32_t* block_table;
-  int max_pages;
+  int max_pages, n_pages;
   const int32_t* row_slot;
   const int32_t* row_pos;
   int T, Hq, Hkv, page_size;
@@ -268,6 +268,42 @@ struct SharedArgs {
   float scale;      // of the scores, times log2(e)
   int32_t* status;
 };
+
+// The matrix products multiply every value of a block with every pair's weight: a value that is infinite or none makes the sums NaN for pairs
+// that do not see its key (weight 0) or whose weight has no second part.  A sum that has met one stays infinite or NaN, so that is looked at
+// once, at the end, and the few pairs whose sums are not finite are weighed again by this function, a warp for a pair, key by key in fp32:
+// keys that the pair does not see or scores -inf are left out, whatever their values are.
+// dst[c] = sum of exp2(scale q k - m) v[c] over the keys of [lo, hi) in the units of 16 from k0 on, every `step` keys.
+template <int D>
+__device__ __noinline__ void weigh_again(const bf16* q, const bf16* k_pages, const bf16* v_pages, int n_pages, const int32_t* bt, int Hkv, int kvh, int PS,
+                                         int k0, int step, int lo, int hi, float scale, float m, float* dst) {
+  constexpr int kCols = D / 32;
+  const int lane = threadIdx.x & 31;
+  float qf[kCols], o[kCols];
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) qf[c] = __bfloat162float(q[lane * kCols + c]), o[c] = 0.f;
+  for (int u = k0; u < hi; u += step) {
+    const int page = bt[u / PS];
+    const bool there = page >= 0 && page < n_pages;  // (else the copies have read zeros)
+    const size_t at = (((size_t)(there ? page : 0) * Hkv + kvh) * PS + u % PS) * D + lane * kCols;
+#pragma unroll 4
+    for (int i = 0; i < 16; ++i) {
+      if (u + i < lo || u + i >= hi) continue;
+      float d = 0.f;
+      if (there)
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) d = fmaf(qf[c], __bfloat162float(k_pages[at + i * D + c]), d);
+      d = warp_sum(d);
+      if (d == -INFINITY) continue;
+      const float w = fast_exp2(fmaf(d, scale, -m));
+      if (there)
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) o[c] = fmaf(w, __bfloat162float(v_pages[at + i * D + c]), o[c]);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) dst[lane * kCols + c] = o[c];
+}
 
 // One item: a tile's pairs x a range of the prefix's blocks of 128 keys x one key head.  As in the prompt attention, S = Q K^T and
 // P V are tcgen05 products with S, P and O in TMEM, keys and values arrive page by page through the block table of the group's first
@@ -533,6 +569,8 @@ __global__ void __maxnreg__(kPxRegs) prefix_attn_kernel(const __grid_constant__ 
     if (!ok) s_abort = 1;
     if (busy) {
       float* dst = row < 0 ? nullptr : a.parts + ((size_t)(pv.row[row].y + split) * a.Hq + head) * (D + 4);
+      const bool seen = ok && n_blocks > 0 && m_run > -INFINITY;  // (the sums of a pair that has seen nothing are 0, whatever the values are)
+      float odd = 0.f;
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) {
         float o[16] = {};
@@ -540,11 +578,24 @@ __global__ void __maxnreg__(kPxRegs) prefix_attn_kernel(const __grid_constant__ 
           tmem_ld16_issue(tmem_o + lanes + c * 16, o);
           tmem_wait_ld16(o);
         }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (!seen) o[i] = 0.f;
+          odd = fmaf(o[i], 0.f, odd);
+        }
         if (dst)
 #pragma unroll
           for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(dst)[c * 4 + i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
       }
       if (dst) *reinterpret_cast<float2*>(dst + D) = ok ? make_float2(m_run, l_run) : make_float2(-INFINITY, 0.f);
+      for (uint32_t left = __ballot_sync(0xffffffffu, dst && odd != 0.f); left; left &= left - 1) {  // (NaN, where a sum is not finite)
+        const int from = __ffs(left) - 1, r = __shfl_sync(0xffffffffu, row, from), h = __shfl_sync(0xffffffffu, head, from);
+        const int end = min(__shfl_sync(0xffffffffu, q_pos, from) + 1, min(n_keys, (b0 + n_blocks) * kTile));
+        const float m = __shfl_sync(0xffffffffu, m_run, from);
+        __syncwarp();
+        weigh_again<D>(a.q + (size_t)r * a.ld + (size_t)h * D, a.k_pages, a.v_pages, a.n_pages, bt, a.Hkv, kvh, PS, b0 * kTile, 16, 0, end, a.scale, m,
+                       a.parts + ((size_t)(pv.row[r].y + split) * a.Hq + h) * (D + 4));
+      }
     }
     if (!ok && tid == 0 && a.status) atomicOr(a.status, 1);
   }
@@ -725,10 +776,21 @@ __global__ void __launch_bounds__(W * 32, 12 / W) tail_attn_kernel(const __grid_
     for (int x = 4; x < 32; x <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], x);
     const int hh = (lane & 3) * 2 + h;
     if (lane < 4) s_m[warp][hh] = m[h], s_l[warp][hh] = l[h];
+    float odd = 0.f;
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) {
       acc[(warp * kTlHeads + hh) * D + c * 16 + (lane >> 2)] = o[c][h];
       acc[(warp * kTlHeads + hh) * D + c * 16 + (lane >> 2) + 8] = o[c][2 + h];
+      odd = fmaf(o[c][h], 0.f, fmaf(o[c][2 + h], 0.f, odd));
+    }
+    const uint32_t lanes = __ballot_sync(0xffffffffu, odd != 0.f);  // (NaN, where a sum is not finite)
+    for (int x = 0; lanes && ok && x < 4 && 2 * x + h < n_heads; ++x) {
+      if (!(lanes & (0x11111111u << x))) continue;
+      const int hx = 2 * x + h;
+      const float mx = __shfl_sync(0xffffffffu, m[h], x);
+      __syncwarp();
+      weigh_again<D>(a.q + (size_t)t * a.ld + (size_t)(h0 + hx) * D, a.k_pages, a.v_pages, a.n_pages, bt, a.Hkv, kvh, PS, (ub + warp) * kTlKeys,
+                     kTlWarps * kTlKeys, first, mx > -INFINITY ? min(ue * kTlKeys, n_tok) : 0, a.scale, mx, acc + (warp * kTlHeads + hx) * D);
     }
   }
   __syncthreads();
@@ -1004,8 +1066,8 @@ extern "C" int mlora_paged_attention_shared(const void* d_q, int64_t ld, const v
   if (!d_work || work_bytes < 4 * (size_t)(s.tickets + s.own + s.parts))
     return fail(MLORA_ESIZE, "paged_attention_shared: scratch of %zu bytes needed, %zu given", 4 * (size_t)(s.tickets + s.own + s.parts), work_bytes);
   float* w = (float*)d_work;
-  SharedArgs a{(const bf16*)d_q, ld, (const bf16*)d_k_pages, (const bf16*)d_v_pages, d_block_table, max_pages, d_row_slot, d_row_pos, T, Hq, Hkv,
-               page_size, const_cast<int32_t*>(d_plan), plan_rows, w + s.tickets + s.own, w + s.tickets, (int32_t*)w, s.n_splits, (bf16*)d_out, ld_out,
+  SharedArgs a{(const bf16*)d_q, ld, (const bf16*)d_k_pages, (const bf16*)d_v_pages, d_block_table, max_pages, n_pages_total, d_row_slot, d_row_pos, T, Hq,
+               Hkv, page_size, const_cast<int32_t*>(d_plan), plan_rows, w + s.tickets + s.own, w + s.tickets, (int32_t*)w, s.n_splits, (bf16*)d_out, ld_out,
                scale * kLog2e, d_status};
   cudaStream_t st = (cudaStream_t)stream;
   if (D == 64) return page_size == 16 ? launch_shared<1, 16>(a, n_pages_total, s.max_items, st) : launch_shared<1, 32>(a, n_pages_total, s.max_items, st);
