@@ -45,7 +45,7 @@ class PagedCache:
         self._free_slots = list(range(self.max_batch - 1, -1, -1))
         self._n_pages_of = {}        # sid -> pages held
         self._more_holders = {}      # page -> sequences that hold it beyond the first
-        self._shared_tokens = {}     # sid -> tokens in pages that it shares
+        self._shared_tokens = {}     # sid -> tokens in pages that it has shared at some time
         self._pending = None
 
     # -- sequences -----------------------------------------------------------------------------
@@ -85,6 +85,11 @@ class PagedCache:
         elif more:
             self._more_holders[page] = more - 1
         return more > 0
+
+    def _shares_page(self, sid, pos):
+        """Whether another sequence holds the page of this position too (shared pages come first: then so are all before it)."""
+        i = max(pos, 0) // self.page_size
+        return i < self._n_pages_of[sid] and int(self._bt_host[self._slot_of[sid], i]) in self._more_holders
 
     def slot(self, sid):
         return self._slot_of[sid]
@@ -159,7 +164,7 @@ class PagedCache:
         append_lens = [int(a) for a in append_lens]
         both = list(zip(seq_ids, append_lens))  # (what one of them has more of has no rows)
         for sid, n in both if self._shared_tokens else ():
-            if n < 0 and self.length(sid) + n < self._shared_tokens.get(sid, 0):
+            if n < 0 and self.length(sid) + n < self._shared_tokens.get(sid, 0) and self._shares_page(sid, self.length(sid) + n):
                 raise ValueError(f"sequence {sid} cannot take back tokens in pages that it shares")
         slots = np.array([self._slot_of[s] for s, _ in both], dtype=np.int32)
         lens = np.array([a for _, a in both], dtype=np.int64)

@@ -1,0 +1,58 @@
+"""What is left of sharing when sequences leave: who may take tokens back, and whether a decode step has rows that share a prefix."""
+import pytest
+
+from conftest import load
+
+
+@pytest.fixture
+def kv():
+    return load("kv_cache").PagedKVCache(1, 2, 64, 6, 1600, 64, 16, "cpu", max_seq_len=320)
+
+
+def _grow(kv, sid, n):
+    kv.begin_rows([sid], [n])
+    kv._len_host[kv.slot(sid)] += n
+    kv._pending = None
+
+
+def test_the_only_holder_takes_tokens_back(kv):
+    kv.add_sequence(0)
+    _grow(kv, 0, 100)
+    kv.fork(1, 0)         # 96 tokens
+    kv.fork(2, 0, 40)     # 32
+    _grow(kv, 1, 10)
+    with pytest.raises(ValueError, match="take back"):
+        kv.begin_rows([0], [-5])
+    kv.begin_rows([0], [-4])
+    kv._pending = None
+    kv.remove_sequence(1)
+    _grow(kv, 0, -5)      # (page 5 is the source's alone again)
+    _grow(kv, 0, -60)
+    assert kv.length(0) == 35
+    for sid in (0, 2):    # the first two pages are still shared
+        with pytest.raises(ValueError, match="take back"):
+            kv.begin_rows([sid], [31 - kv.length(sid)])
+    kv.begin_rows([0], [-3])
+    kv._pending = None
+    kv.remove_sequence(0)
+    _grow(kv, 2, -32)     # (a fork whose source has gone)
+    assert kv.length(2) == 0
+    kv.remove_sequence(2)
+    assert not kv._more_holders and len(kv._free) == kv.n_pages
+
+
+def test_pages_that_changed_hands(kv):
+    """A sequence that never shared is not asked about the pages that its slot or its numbers had before."""
+    kv.add_sequence(0)
+    _grow(kv, 0, 64)
+    kv.fork(1, 0)
+    kv.remove_sequence(1)
+    kv.remove_sequence(0)
+    kv.add_sequence(1)
+    _grow(kv, 1, 64)
+    kv.add_sequence(5)
+    kv.fork(6, 1, 16)
+    _grow(kv, 1, -48)
+    with pytest.raises(ValueError, match="take back"):
+        kv.begin_rows([1], [-1])
+    kv.begin_rows([5], [0])
