@@ -228,12 +228,14 @@ class PagedKVCache(PagedCache):
         self.prefix_id = torch.full((self.max_batch,), -1, dtype=torch.int32, device=self.device)
         self.prefix_len = torch.zeros(self.max_batch, dtype=torch.int32, device=self.device)
         self._prefix_of = {}  # sid -> (prefix, tokens)
+        self._with_prefix = {}  # prefix -> how many sequences begin with it
         self._next_prefix = 0
 
     # -- shared prefixes -------------------------------------------------------------------------
     @property
     def shares_prefixes(self) -> bool:
-        return bool(self._prefix_of)
+        """Whether any two sequences begin with one prefix."""
+        return any(n > 1 for n in self._with_prefix.values())
 
     def fork(self, sid, source, n_tokens=None):
         """Adds sequence ``sid`` beginning with the first ``n_tokens`` tokens (default: all) of ``source``, whose whole pages it shares from
@@ -258,7 +260,8 @@ class PagedKVCache(PagedCache):
             self._shared_tokens[s] = max(self._shared_tokens.get(s, 0), tokens)
         self._push_pages([(slot, 0, pages)])
         self._push_value(self.seq_lens, slot, tokens)
-        if source not in self._prefix_of:
+        known = self._prefix_of.get(source)
+        if known is None or (self._with_prefix[known[0]] == 1 and tokens < known[1]):  # (whoever began like it has gone)
             self._set_prefix(source, self._next_prefix, tokens)
             self._next_prefix = (self._next_prefix + 1) % (1 << 31)
         if tokens >= self._prefix_of[source][1]:
@@ -268,11 +271,21 @@ class PagedKVCache(PagedCache):
     def remove_sequence(self, sid):
         slot = self.slot(sid)
         super().remove_sequence(sid)
-        if self._prefix_of.pop(sid, None) is not None:
+        if self._leave_prefix(sid):
             self._push_value(self.prefix_id, slot, -1)
 
+    def _leave_prefix(self, sid):
+        prefix = self._prefix_of.pop(sid, None)
+        if prefix is not None:
+            self._with_prefix[prefix[0]] -= 1
+            if not self._with_prefix[prefix[0]]:
+                del self._with_prefix[prefix[0]]
+        return prefix is not None
+
     def _set_prefix(self, sid, prefix, tokens):
+        self._leave_prefix(sid)
         self._prefix_of[sid] = (prefix, tokens)
+        self._with_prefix[prefix] = self._with_prefix.get(prefix, 0) + 1
         self._push_value(self.prefix_id, self._slot_of[sid], prefix)
         self._push_value(self.prefix_len, self._slot_of[sid], tokens)
 

@@ -56,3 +56,27 @@ def test_pages_that_changed_hands(kv):
     with pytest.raises(ValueError, match="take back"):
         kv.begin_rows([1], [-1])
     kv.begin_rows([5], [0])
+
+
+def test_a_prefix_that_one_sequence_is_left_with(kv):
+    """A cache shares prefixes while two sequences begin with one; the one that is left can begin a group of fewer tokens."""
+    for sid in (0, 9):
+        kv.add_sequence(sid)
+        _grow(kv, sid, 200)
+    kv.fork(1, 0)
+    assert kv.shares_prefixes
+    kv.remove_sequence(1)
+    assert not kv.shares_prefixes
+    kv.fork(2, 0, 100)
+    assert kv.shares_prefixes
+    one, two = (kv.slot(s) for s in (0, 2))
+    assert int(kv.prefix_id[one]) == int(kv.prefix_id[two]) >= 0 and int(kv.prefix_len[one]) == int(kv.prefix_len[two]) == 96
+    kv.fork(3, 9, 32)
+    assert int(kv.prefix_id[kv.slot(3)]) == int(kv.prefix_id[kv.slot(9)]) != int(kv.prefix_id[one])
+    kv.fork(4, 0, 64)  # (while others are in the group, one that shares fewer stays outside)
+    assert int(kv.prefix_id[kv.slot(4)]) == -1 and int(kv.prefix_len[one]) == 96
+    kv.remove_sequence(0)
+    assert kv.shares_prefixes  # (3 and 9)
+    kv.remove_sequence(9)
+    assert not kv.shares_prefixes
+    assert int(kv.prefix_id[two]) >= 0  # (a graph captured earlier finds no second row with it)
