@@ -51,6 +51,7 @@ class EngineBase:
         self.iota = torch.arange(T, **i32)
         self.n_distinct = 0  # distinct adapters among the rows staged for the next pass (set with self.slots)
         self.max_keys = kv.max_pages * kv.page_size  # bound of the context of the rows staged for the next pass
+        self.step_seqs = None  # sequences of a captured step, which the cache does not know of
         self.ws_linear = None
 
     def forward(self, T, fused_append, use_lora=True, lm_rows=None, n_lm=None, hidden=None):
@@ -211,7 +212,9 @@ class EngineBase:
 
         def step():
             ops.kv_begin_decode(self.row_slot[:B], kv.seq_lens, self.row_pos[:B])
+            self.step_seqs = seq_ids
             self.forward(B, True, use_lora)
+            self.step_seqs = None
             if feed_back:  # the greedy tokens become the next step's input without leaving the device
                 self.tokens[:B].copy_(self.next_tok[:B])
 
@@ -334,7 +337,9 @@ class DecodeSession:
         ops.decode_step_begin(self.live, self.seq_slot, self.adapter_slot, self.last_tok, rows, e.kv.seq_lens,
                               self.row_src, e.row_slot, e.row_pos, e.slots, e.tokens, self.n_live)
         e.n_distinct, e.max_keys = self.n_distinct, self.max_keys
+        e.step_seqs = self.seq_ids
         e.forward(rows, True, self.use_lora)
+        e.step_seqs = None
         if self.rules is not None:
             ops.choose_tokens(e.logits[:rows], self.rules, row_src=self.row_src[:rows], out=e.next_tok[:rows])
         ops.decode_step_end(self.row_src, e.next_tok, rows, self.live, self.last_tok, self.gen_count, self.max_gen,

@@ -237,6 +237,13 @@ class PagedKVCache(PagedCache):
         """Whether any two sequences begin with one prefix."""
         return any(n > 1 for n in self._with_prefix.values())
 
+    def shared_by(self, seq_ids) -> bool:
+        """Whether two of these do."""
+        if not self.shares_prefixes:
+            return False
+        known = [self._prefix_of[s][0] for s in seq_ids if s in self._prefix_of]
+        return len(set(known)) < len(known)
+
     def fork(self, sid, source, n_tokens=None):
         """Adds sequence ``sid`` beginning with the first ``n_tokens`` tokens (default: all) of ``source``, whose whole pages it shares from
         then on; returns how many tokens that are (a multiple of the page size): the rest of its prompt is for the caller to run.

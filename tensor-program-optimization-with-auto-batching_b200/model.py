@@ -358,7 +358,11 @@ class Engine(EngineBase):
                 raise RuntimeError(f"mlora: a projection kernel (status bits {st:#x}) gave up a bounded wait; the results of this pass are undefined")
 
     def _shares_prefixes(self, T, fused_append):
-        return fused_append and 1 < T <= self.shared_rows and self.kv.shares_prefixes
+        """Whether two rows of this decode step may begin with one prefix: of its sequences, where they are known, else of the cache's."""
+        if not (fused_append and 1 < T <= self.shared_rows and self.kv.shares_prefixes):
+            return False
+        seqs = self.kv._pending[0] if self.kv._pending is not None else self.step_seqs
+        return seqs is None or self.kv.shared_by(seqs)
 
     def _plan_prefixes(self, T):
         """Which rows of this step share a prefix: once for all layers."""

@@ -80,3 +80,25 @@ def test_a_prefix_that_one_sequence_is_left_with(kv):
     kv.remove_sequence(9)
     assert not kv.shares_prefixes
     assert int(kv.prefix_id[two]) >= 0  # (a graph captured earlier finds no second row with it)
+
+
+def test_steps_whose_rows_share_nothing(kv):
+    """The engine takes the route for shared prefixes only where two sequences of the step begin with one."""
+    engine = load("model").Engine
+    eng = engine.__new__(engine)
+    eng.kv, eng.shared_rows, eng.step_seqs = kv, 256, None
+    for sid in (0, 7, 8):
+        kv.add_sequence(sid)
+        _grow(kv, sid, 100)
+    kv.fork(1, 0)
+    kv.fork(2, 0)
+    kv.fork(9, 8)
+    assert kv.shared_by([0, 7, 1]) and kv.shared_by([1, 2]) and not kv.shared_by([0, 7]) and not kv.shared_by([0, 8, 7]) and not kv.shared_by([])
+    for seqs, shares in (([7, 8, 0], False), ([2, 9], False), ([1, 2, 7], True), ([9, 1, 8], True)):
+        kv.begin_rows(seqs, [1] * len(seqs))  # (an eager step)
+        assert eng._shares_prefixes(len(seqs), True) == shares and not eng._shares_prefixes(len(seqs), False)
+        kv._pending = None
+        eng.step_seqs = seqs  # (a captured one)
+        assert eng._shares_prefixes(len(seqs), True) == shares
+        eng.step_seqs = None
+        assert eng._shares_prefixes(len(seqs), True)  # (a caller's own: any sequences of the cache)
