@@ -110,7 +110,7 @@ __device__ __forceinline__ int block_max_int(int v, int* sm /*[33]*/) {
 }
 
 // One CTA, a thread per row.  Rows of a group keep their order; groups are ordered by their first row.
-__global__ void __launch_bounds__(kPlanMaxRows) prefix_plan_kernel(const int32_t* __restrict__ row_slot, int T,
+__global__ void __launch_bounds__(kPlanMaxRows) prefix_plan_kernel(const int32_t* __restrict__ row_slot, const int32_t* __restrict__ row_pos, int T,
                                                                    const int32_t* __restrict__ prefix_id, const int32_t* __restrict__ prefix_len,
                                                                    int n_slots, int rt, int Hkv, int target, int cap_items, int cap_parts, long long least, int32_t* plan, int max_rows) {
   __shared__ int s_id[kPlanMaxRows];     // prefix of the row, -1: none
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kPlanMaxRows) prefix_plan_kernel(const int32_t
   int id = -1, len = 0, slot = 0;
   if (t < T) {
     slot = row_slot[t];
-    if (slot >= 0 && slot < n_slots) id = prefix_id[slot], len = prefix_len[slot];
+    if (slot >= 0 && slot < n_slots && (row_pos == nullptr || row_pos[t] >= 0)) id = prefix_id[slot], len = prefix_len[slot];
   }
   if (len < kPlanMinKeys) id = -1;
   s_id[t] = id;
@@ -1028,14 +1028,20 @@ extern "C" size_t mlora_prefix_plan_bytes(int32_t max_rows, int32_t Hkv) {
 
 extern "C" int mlora_prefix_plan(const int32_t* d_row_slot, int32_t T, const int32_t* d_prefix_id, const int32_t* d_prefix_len, int32_t n_slots,
                                  int32_t Hq, int32_t Hkv, int64_t least, int32_t* d_plan, int32_t max_rows, void* stream) {
+  return mlora_prefix_plan_rows(d_row_slot, nullptr, T, d_prefix_id, d_prefix_len, n_slots, Hq, Hkv, least, d_plan, max_rows, stream);
+}
+
+extern "C" int mlora_prefix_plan_rows(const int32_t* d_row_slot, const int32_t* d_row_pos, int32_t T, const int32_t* d_prefix_id,
+                                      const int32_t* d_prefix_len, int32_t n_slots, int32_t Hq, int32_t Hkv, int64_t least, int32_t* d_plan,
+                                      int32_t max_rows, void* stream) {
   MLORA_REQUIRE(shared_sizes_fit(T, Hq, Hkv, 64) && T <= max_rows && max_rows <= kPlanMaxRows && n_slots > 0,
                 "prefix_plan: bad sizes T=%d of %d, %d heads over %d key heads", T, max_rows, Hq, Hkv);
   MLORA_REQUIRE(d_row_slot && d_prefix_id && d_prefix_len && d_plan && aligned16(d_plan), "prefix_plan: null pointer or unaligned plan");
   if (T == 0) return MLORA_OK;
   const int rep = Hq / Hkv, target = 2 * sm_count();
   const int threads = T <= 256 ? 256 : (T + 31) / 32 * 32;
-  launch_pdl(prefix_plan_kernel, 1, threads, 0, (cudaStream_t)stream, d_row_slot, T, d_prefix_id, d_prefix_len, n_slots, tile_rows(rep), Hkv,
-             target, max_items_of(T, Hkv, target), (int)max_parts(T, rep, Hkv, target), least < 0 ? (long long)kPlanLeast : (long long)least, d_plan, max_rows);
+  launch_pdl(prefix_plan_kernel, 1, threads, 0, (cudaStream_t)stream, d_row_slot, d_row_pos, T, d_prefix_id, d_prefix_len, n_slots, tile_rows(rep),
+             Hkv, target, max_items_of(T, Hkv, target), (int)max_parts(T, rep, Hkv, target), least < 0 ? (long long)kPlanLeast : (long long)least, d_plan, max_rows);
   count_launch();
   MLORA_CHECK_LAUNCH("prefix_plan_kernel");
   return MLORA_OK;

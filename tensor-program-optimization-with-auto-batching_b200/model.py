@@ -371,7 +371,7 @@ class Engine(EngineBase):
             self.prefix_plan = ops.PrefixPlan(self.shared_rows, m.Hq, m.Hkv, m.device, self.prefix_least)
             self.ws_shared = ops.new_workspace(max(ops.paged_attention_shared_workspace(t, m.Hq, m.Hkv, m.D) for t in range(1, self.shared_rows + 1)),
                                                m.device)
-        return ops.prefix_plan(self.row_slot[:T], kv.prefix_id, kv.prefix_len, self.prefix_plan)
+        return ops.prefix_plan(self.row_slot[:T], kv.prefix_id, kv.prefix_len, self.prefix_plan, self.row_pos[:T])
 
     @staticmethod
     def _full_rank(stack):

@@ -1026,18 +1026,20 @@ class PrefixPlan:
         self.work_bytes = {}  # (rows, head size) -> scratch of their attention
 
 
-def prefix_plan(row_slot, prefix_id, prefix_len, plan: PrefixPlan):
-    """Groups the rows by the prefix their slots begin with; see ``mlora_prefix_plan``."""
-    at = _one_device(row_slot, prefix_id, prefix_len, plan.table)
+def prefix_plan(row_slot, prefix_id, prefix_len, plan: PrefixPlan, row_pos=None):
+    """Groups the rows by the prefix their slots begin with; see ``mlora_prefix_plan``.  ``row_pos``: rows of padding (< 0) stay outside."""
+    at = _one_device(row_slot, prefix_id, prefix_len, plan.table, row_pos)
     if at is not None:
         with at:
-            return prefix_plan(row_slot, prefix_id, prefix_len, plan)
+            return prefix_plan(row_slot, prefix_id, prefix_len, plan, row_pos)
     T, n = row_slot.numel(), prefix_id.numel()
     _int32_table("row_slot", row_slot, T)
     _int32_table("prefix_id", prefix_id, n)
     _int32_table("prefix_len", prefix_len, n)
-    check(_lib.lib().mlora_prefix_plan(_ptr(row_slot), T, _ptr(prefix_id), _ptr(prefix_len), n, plan.Hq, plan.Hkv, plan.least, _ptr(plan.table),
-                                       plan.max_rows, _stream()), "mlora_prefix_plan")
+    if row_pos is not None:
+        _int32_table("row_pos", row_pos, T)
+    check(_lib.lib().mlora_prefix_plan_rows(_ptr(row_slot), _ptr(row_pos), T, _ptr(prefix_id), _ptr(prefix_len), n, plan.Hq, plan.Hkv, plan.least,
+                                            _ptr(plan.table), plan.max_rows, _stream()), "mlora_prefix_plan")
     plan.T = T
     return plan
 
