@@ -66,10 +66,17 @@ class EngineBase:
     def _check_prompt_status(self):
         pass
 
+    def _projection_scratch(self):
+        """Scratch buffers of the projections, each with a status word."""
+        return [self.ws_linear]
+
     def status_word(self) -> int:
-        """Status word of the projection kernels' scratch (synchronises): non-zero after a bounded wait expired
-        somewhere since the buffer was last cleared; the outputs since then are undefined."""
-        return ops.status_word(self.ws_linear)
+        """Status words of the projection kernels' scratch (synchronises): non-zero after a bounded wait expired
+        somewhere since the buffers were last cleared; the outputs since then are undefined."""
+        st = 0
+        for work in self._projection_scratch():
+            st |= ops.status_word(work)
+        return st
 
     def _own_status_word(self):
         """The word of the projection scratch's header that is the caller's, for the engine's other kernels with bounded waits:
@@ -81,9 +88,13 @@ class EngineBase:
         after such a failure) so that the engine stays usable."""
         words = self.ws_linear[:ops.WORK_CALLER_OFFSET + 4].view(torch.int32).tolist()
         st, own = words[0], words[-1]
+        scratch = self._projection_scratch()
+        for work in scratch[1:]:
+            st |= ops.status_word(work)
         if not st and not own:
             return
-        self.ws_linear.zero_()
+        for work in scratch:
+            work.zero_()
         who = ([f"a projection kernel (status bits {st:#x})"] if st else []) + (["an attention kernel"] if own else [])
         raise RuntimeError(f"mlora: {' and '.join(who)} gave up a bounded wait; the results of this pass are undefined")
 

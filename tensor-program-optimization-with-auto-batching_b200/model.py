@@ -349,13 +349,8 @@ class Engine(EngineBase):
         # "2": only gate|up -> down (two projections with nothing between them) as one launch
         self.chain_mlp = os.environ.get("MLORA_CHAIN", "0") == "2"
 
-    def check_status(self):
-        super().check_status()
-        if self.ws_q4 is not None:
-            st = ops.status_word(self.ws_q4)
-            if st:
-                self.ws_q4.zero_()
-                raise RuntimeError(f"mlora: a projection kernel (status bits {st:#x}) gave up a bounded wait; the results of this pass are undefined")
+    def _projection_scratch(self):
+        return [self.ws_linear] + ([] if self.ws_q4 is None else [self.ws_q4])
 
     def _shares_prefixes(self, T, fused_append):
         """Whether two rows of this decode step may begin with one prefix: of its sequences, where they are known, else of the cache's."""
