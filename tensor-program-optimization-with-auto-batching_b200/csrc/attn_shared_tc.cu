@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(kPlanMaxRows) prefix_plan_kernel(const int32_t
   int blocks = 0, rows = 0;
   if (opens) {
     rows = min(rt, count - rank);
-    blocks = (len + kTile - 1) / kTile;
+    blocks = (len - 1) / kTile + 1;  // (any 32-bit length)
     s_tile[tile][0] = blocks;
     s_tile[tile][1] = rows;
   }

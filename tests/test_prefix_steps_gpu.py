@@ -89,3 +89,18 @@ def test_a_session_whose_bucket_is_part_padding(ops, cuda):
     assert [len(x) for x in got] == [9, 3, 9, 9, 2] and 4 in session._graphs
     assert _tiles(eng.prefix_plan) == ({(0, 3, eng.kv.slot(1))}, [0, 1, 2])
     eng.check_status()
+
+
+@pytest.mark.parametrize("length", [2 ** 31 - 1, 2 ** 31 - 127, 4096])
+def test_a_prefix_longer_than_the_block_table_is_cut(ops, cuda, length):
+    """Rows that end inside what their slots call a prefix: all of their tokens are the prefix's, whatever its length is said to be."""
+    from test_shared_attention_gpu import _call, _case, _want
+
+    c = _case(8, 2, 64, 16, [(0, 320, 319), (0, 320, 319), (0, 320, 200)], seed=6)
+    c["table"] = c["table"][:, :20].contiguous()
+    want, bound = _want(c, 8, 2, 64)
+    c["rows"] = [(0, length, p) for _, _, p in c["rows"]]
+    got, plan = _call(ops, c, 8, 2, cuda)
+    assert _tiles(plan)[1] == [0, 1, 2]
+    err = (got.cpu().double() - want).abs()
+    assert bool((err <= bound).all()), float((err / bound).max())
