@@ -14,8 +14,8 @@
 // what comes through L2 beyond.  The tail is bound by HBM alone: its tiles have only the query heads of one key head, so it uses mma.sync with 16
 // keys as the rows and up to eight heads as the columns, and a ring of TMA copies in every warp.  It is launched programmatically
 // dependent on the prefix and waits for it only before the join.
-// Measured (CUDA graph, three sets of inputs in turn): 32 rows x 32 heads behind 4096 tokens 60.3 us (3.9 TB/s of the keys and values read
-// once), 72 rows x 40 heads in four groups 152 us (5.9 TB/s), 128 rows x 32 heads over 8 key heads behind 32768 tokens 143 us (480
+// Measured (CUDA graph, three sets of inputs in turn): 32 rows x 32 heads behind 4096 tokens 60.2 us (3.9 TB/s of the keys and values read
+// once), 72 rows x 40 heads in four groups 153 us (5.9 TB/s), 128 rows x 32 heads over 8 key heads behind 32768 tokens 137 us (502
 // TFLOP/s; every tile reads the prefix through L2: 537 MB), 4 rows behind 512 tokens 12 us.  Exponentials partly on the FMA
 // units (2 % more) and steps of 64 keys with two places for everything (18 % more) are no faster in the third.
 #include <math.h>
@@ -45,6 +45,10 @@ constexpr int kPlanMinRows = 2, kPlanMinKeys = 64;  // smaller groups and shorte
 // heads (32768 saved) 22.9 us against 17.7; 8 x 1024 x 8 (57344) 13.9 against 15.9, 3 x 1024 x 32 (65536) 14.5 against 15.7; 2 x 4096 x 32
 // (131072) 22.8 against 22.3, 32 x 1024 x 8 (253952) 16.9 against 27.1.
 constexpr int kPlanLeast = 50000;
+// Key ranges that a row's CTA joins in the time of a block, with kJoin of them on their way: some 0.15 us against 2.5 (2 rows behind 32768
+// tokens of one key head, 256 blocks: in 256 ranges 178 us with one range after the other and 72 with kJoin, in some 50 ranges 35; ranges
+// chosen with 6 here in place of 18 cost 5 to 12 % on average over 2 to 32 rows behind 2048 to 32768 tokens of 1 to 40 key heads).
+constexpr int kBlockParts = 18;
 
 // A plan in int32: header; per row a quad (first key of its own part, its first part, its parts, 0) and its entry of `list` (rows by group);
 // then two quads per item, all that a CTA needs to begin: (slot whose pages are read, first block, blocks, keys of the prefix | first entry
@@ -169,7 +173,7 @@ __global__ void __launch_bounds__(kPlanMaxRows) prefix_plan_kernel(const int32_t
   const int total = block_sum_int(blocks, s_red);
   // Blocks per item: a candidate per thread, from a quarter of an equal share for `target` items -- two per SM -- upwards, and one item per
   // tile and key head, which always has room.  The best one has the shortest way through: rounds of `target` items times the longest item,
-  // each with some two blocks' time before and behind.  (An equal
+  // each with some two blocks' time before and behind, and then the join of a row's ranges.  (An equal
   // share alone gives 4 tiles x 256 blocks x 8 key heads 320 items of 26 blocks, a round and a bit; 288 of 29 are one.)
   __shared__ unsigned long long s_best;
   const int longest = block_max_int(blocks, s_red);
@@ -180,16 +184,17 @@ __global__ void __launch_bounds__(kPlanMaxRows) prefix_plan_kernel(const int32_t
   {
     const int unit = candidate(t);
     long long items = 0, parts = 0;
-    int length = 0;
+    int length = 0, most = 0;
     for (int i = 0; i < n_tiles && unit <= longest; ++i) {
       const int n = s_tile[i][0], k = (n + unit - 1) / unit;
       items += k;
       parts += k * s_tile[i][1];
       length = max(length, (n + k - 1) / k);
+      most = max(most, k);
     }
     items *= Hkv;
     if (n_tiles > 0 && unit <= longest && items <= cap_items && parts <= cap_parts) {
-      const unsigned long long cost = (unsigned long long)((items + target - 1) / target) * (length + 2);
+      const unsigned long long cost = (unsigned long long)((items + target - 1) / target) * (length + 2) * kBlockParts + most;
       atomicMin(&s_best, min(cost, (1ull << 29) - 1) << 34 | (unsigned long long)items << 10 | t);
     }
   }
@@ -607,6 +612,7 @@ __global__ void __maxnreg__(kPxRegs) prefix_attn_kernel(const __grid_constant__ 
 // ---- the tail -------------------------------------------------------------------------------------------------------------------
 constexpr int kTlKeys = 16;  // keys a warp works on at a time
 constexpr int kTlHeads = 8;  // query heads of a CTA
+constexpr int kJoin = 8;     // ranges whose results a thread has on their way when it joins them
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -839,12 +845,21 @@ __global__ void __launch_bounds__(W * 32, 12 / W) tail_attn_kernel(const __grid_
   const int h = tid / kSubs, sub = tid % kSubs;
   float M = -INFINITY, L = 0.f;
   if (h < n_heads) {
-    for (int r = sub; r < n_own + n_part; r += kSubs) {
-      const float2 ml = r < n_own ? own_ml(r, h) : __ldcg(reinterpret_cast<const float2*>(part0 + (size_t)(r - n_own) * part_step + (size_t)h * (D + 4) + D));
-      if (ml.x == -INFINITY) continue;
+    const auto take = [&](const float2& ml) {
+      if (ml.x == -INFINITY) return;
       const float mn = fmaxf(M, ml.x);
       L = L * fast_exp2(M - mn) + ml.y * fast_exp2(ml.x - mn);
       M = mn;
+    };
+    for (int r = sub; r < n_own; r += kSubs) take(own_ml(r, h));
+    const float* from = part0 + (size_t)h * (D + 4) + D;
+    for (int r = sub; r < n_part; r += kSubs * kJoin) {
+      float2 ml[kJoin];
+#pragma unroll
+      for (int j = 0; j < kJoin; ++j)
+        ml[j] = r + j * kSubs < n_part ? __ldcg(reinterpret_cast<const float2*>(from + (size_t)(r + j * kSubs) * part_step)) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int j = 0; j < kJoin; ++j) take(ml[j]);
     }
   }
 #pragma unroll
@@ -877,15 +892,23 @@ __global__ void __launch_bounds__(W * 32, 12 / W) tail_attn_kernel(const __grid_
     for (int i = 0; i < kSets; ++i) {
       const int hh = i * hp + hs;
       if (hh >= n_heads || (i > 0 && hp < kPer)) continue;
-#pragma unroll 4
-      for (int r = slice; r < n; r += slices) {
-        const int x = r0 + r;
-        const float f = s_w[r][hh];
-        float4 v;
-        if (x >= n_own) v = __ldcg(reinterpret_cast<const float4*>(part0 + (size_t)(x - n_own) * part_step + (size_t)hh * (D + 4)) + c);
-        else if (ranges == 1) v = reinterpret_cast<const float4*>(acc + (x * kTlHeads + hh) * D)[c];
-        else v = __ldcg(reinterpret_cast<const float4*>(a.own + (((size_t)t * a.Hq + h0 + hh) * a.n_splits + x) * (D + 4)) + c);
+      const auto add = [&](const float4& v, float f) {
         sum[i].x = fmaf(v.x, f, sum[i].x), sum[i].y = fmaf(v.y, f, sum[i].y), sum[i].z = fmaf(v.z, f, sum[i].z), sum[i].w = fmaf(v.w, f, sum[i].w);
+      };
+      int r = slice;
+      for (; r < n && r0 + r < n_own; r += slices) {
+        const int x = r0 + r;
+        add(ranges == 1 ? reinterpret_cast<const float4*>(acc + (x * kTlHeads + hh) * D)[c]
+                        : __ldcg(reinterpret_cast<const float4*>(a.own + (((size_t)t * a.Hq + h0 + hh) * a.n_splits + x) * (D + 4)) + c), s_w[r][hh]);
+      }
+      const float* from = part0 + (size_t)(r0 + r - n_own) * part_step + (size_t)hh * (D + 4) + 4 * c;
+      for (; r < n; r += slices * kJoin, from += slices * kJoin * part_step) {
+        float4 v[kJoin];
+#pragma unroll
+        for (int j = 0; j < kJoin; ++j)
+          v[j] = r + j * slices < n ? __ldcg(reinterpret_cast<const float4*>(from + j * slices * part_step)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < kJoin; ++j) add(v[j], r + j * slices < n ? s_w[r + j * slices][hh] : 0.f);
       }
     }
   }
