@@ -41,10 +41,20 @@ constexpr int kPlanMaxRows = 1024;
 constexpr int kPlanHeader = 8;           // int32: rows, tiles, items, parts
 constexpr int kTickets = 1024;           // arrival counters at the start of the scratch, whatever the call's sizes: zero between calls
 constexpr int kPlanMinRows = 2, kPlanMinKeys = 64;  // smaller groups and shorter prefixes are read row by row
-// Reads a group has to save, (rows - 1) x tokens x key heads.  Measured, shared against row by row, 128-wide heads: 2 rows x 4096 x 8 key
-// heads (32768 saved) 22.9 us against 17.7; 8 x 1024 x 8 (57344) 13.9 against 15.9, 3 x 1024 x 32 (65536) 14.5 against 15.7; 2 x 4096 x 32
-// (131072) 22.8 against 22.3, 32 x 1024 x 8 (253952) 16.9 against 27.1.
-constexpr int kPlanLeast = 50000;
+// Groups that are taken together where the caller does not say what they have to save: the second kernel has a chain of blocks and a join to go
+// through, so it takes rows enough to read a prefix again for, and a prefix that is long, or saves many reads ((rows - 1) x tokens x key
+// heads).  Measured, shared and row by row, us, one group of rows x tokens, heads of 128 (8 key heads
+// of 4 query heads | 32 of one | one of 8) and of 64 (8 of 4):
+//    2 x 8192    21.5  21.0 |  44.1  37.1 |  21.1  22.4 |  17.6  16.3
+//    2 x 32768   44.9  42.3 |   122   116 |  34.0  37.5 |  36.0  32.0
+//    4 x 1024    13.2  15.1 |  17.3  16.7 |  12.5  14.5 |  11.5  13.3
+//    4 x 8192    21.9  24.6 |  44.0  51.5 |  21.3  22.8 |  17.9  19.3
+//    8 x 512     12.8  13.0 |  16.7  15.9 |  12.8  12.3 |  10.7  11.1
+//    8 x 1024    13.3  16.1 |  18.2  28.2 |  12.9  14.5 |  11.3  14.0
+//   32 x 512     15.8  15.8 |  28.6  40.5 |  14.3  12.6 |  12.5  12.9
+//   32 x 8192    31.0   127 |  56.8   347 |  23.5  28.0 |  22.1  62.6
+// Over 784 such cases (2 to 32 rows, 256 to 32768 tokens, 1 to 40 key heads) no group that is taken together loses more than 9 %.
+constexpr int kPlanEnoughRows = 4, kPlanLongKeys = 1024, kPlanManyReads = 200000;
 // Key ranges that a row's CTA joins in the time of a block, with kJoin of them on their way: some 0.15 us against 2.5 (2 rows behind 32768
 // tokens of one key head, 256 blocks: in 256 ranges 178 us with one range after the other and 72 with kJoin, in some 50 ranges 35; ranges
 // chosen with 6 here in place of 18 cost 5 to 12 % on average over 2 to 32 rows behind 2048 to 32768 tokens of 1 to 40 key heads).
@@ -144,7 +154,9 @@ __global__ void __launch_bounds__(kPlanMaxRows) prefix_plan_kernel(const int32_t
         rank += j < t;
         ++count;
       }
-  const bool used = count >= kPlanMinRows && (long long)(count - 1) * len * Hkv >= least;
+  const long long saved = (long long)(count - 1) * len * Hkv;
+  const bool used = count >= kPlanMinRows &&
+                    (least >= 0 ? saved >= least : count >= kPlanEnoughRows && (len >= kPlanLongKeys || saved >= kPlanManyReads));
   s_lead[t] = used ? lead : -1;
   __syncthreads();
   const bool opens = used && rank % rt == 0;  // first row of a tile
@@ -1064,7 +1076,7 @@ extern "C" int mlora_prefix_plan_rows(const int32_t* d_row_slot, const int32_t* 
   const int rep = Hq / Hkv, target = 2 * sm_count();
   const int threads = T <= 256 ? 256 : (T + 31) / 32 * 32;
   launch_pdl(prefix_plan_kernel, 1, threads, 0, (cudaStream_t)stream, d_row_slot, d_row_pos, T, d_prefix_id, d_prefix_len, n_slots, tile_rows(rep),
-             Hkv, target, max_items_of(T, Hkv, target), (int)max_parts(T, rep, Hkv, target), least < 0 ? (long long)kPlanLeast : (long long)least, d_plan, max_rows);
+             Hkv, target, max_items_of(T, Hkv, target), (int)max_parts(T, rep, Hkv, target), (long long)least, d_plan, max_rows);
   count_launch();
   MLORA_CHECK_LAUNCH("prefix_plan_kernel");
   return MLORA_OK;

@@ -37,3 +37,14 @@ def test_many_ranges_of_the_prefix_and_of_the_rows_own_tokens(ops, cuda, dim, kv
     want, bound = _want(c, kv_heads * rep, kv_heads, dim)
     err = (got.cpu().double() - want).abs()
     assert bool((err <= bound).all()), float((err / bound).nan_to_num(9).max())
+
+
+@pytest.mark.parametrize("rows,tokens,kv_heads,together", [(2, 8192, 8, False), (2, 65536, 32, False), (3, 32768, 8, False), (4, 1024, 1, True), (4, 1023, 8, False),
+                                                           (8, 512, 8, False), (32, 512, 32, True), (32, 208, 32, True),  # (31 x 208 x 32 = 206336)
+                                                           (32, 192, 32, False), (128, 64, 32, True)])
+def test_which_groups_are_taken_together(ops, cuda, rows, tokens, kv_heads, together):
+    """Where the caller does not say what a group has to save: rows enough, and a long prefix or many reads."""
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda)
+    plan = ops.PrefixPlan(rows + 1, kv_heads, kv_heads, cuda)
+    ops.prefix_plan(i32(list(range(rows + 1))), i32([-1] + [3] * rows), i32([0] + [tokens] * rows), plan)
+    assert bool(int(plan.table[1])) == together
