@@ -1022,8 +1022,9 @@ int launch_shared(const SharedArgs& a, int n_pages_total, int max_items, cudaStr
     count_launch();
     MLORA_CHECK_LAUNCH("prefix_attn_kernel");
   }
-  // Many (row, key head) pairs: CTAs of two warps, whose ends hold up less of an SM (72 rows x 40 key heads: 146 us, with four
-  // 5 % more); few: four warps, which are through a row sooner (4 x 8: 12.1 us against 14.8 with two, 128 x 8: 131, with two 3 % more).
+  // Many (row, key head) pairs: CTAs of two warps, whose ends hold up less of an SM.  Against four warps, behind 1024 shared tokens: from 2048
+  // pairs on 10 to 29 % less time with 48 tokens of the rows' own, 0 to 9 % with 400, and rows that share nothing take up to 9 % more (heads
+  // of 128) or 19 % (64); at 1024 pairs 0 to 16 % less with 48 tokens, but 9 to 30 % more with 2000, and up to 18 or 44 % more without a prefix.
   return (long long)a.T * a.Hkv >= 2048 ? launch_tail<D, 2>(mkt, mvt, a, max_items > 0, st) : launch_tail<D, 4>(mkt, mvt, a, max_items > 0, st);
 }
 
