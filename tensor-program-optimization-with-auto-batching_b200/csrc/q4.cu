@@ -20,8 +20,11 @@ __global__ void q4_quantize_kernel(const bf16* __restrict__ W, int out, int in, 
   // with zero points the 16 values span [lo, hi], else -7 .. 7 spans the larger side
   const bf16 sb = __float2bfloat16_rn(zero ? (hi - lo) / 15.f : fmaxf(hi, -lo) / 7.f);
   const float s = __bfloat162float(sb), inv = s > 0.f ? 1.f / s : 0.f;
-  const int z = zero ? min(max(__float2int_rn(-lo * inv), 0), 15) : 8;
-  for (int i = lane; i < G; i += 32) q[at + i] = (uint8_t)min(max(__float2int_rn(__bfloat162float(W[at + i]) * inv) + z, 0), 15);
+  const int z = zero ? min(max(__float2int_rn(isinf(inv) ? -lo / s : -lo * inv), 0), 15) : 8;
+  for (int i = lane; i < G; i += 32) {
+    const float v = __bfloat162float(W[at + i]);
+    q[at + i] = (uint8_t)min(max(__float2int_rn(isinf(inv) ? v / s : v * inv) + z, 0), 15);  // (scales below 2^-128 have no reciprocal)
+  }
   if (lane == 0) {
     scale[w] = sb;
     if (zero) zero[w] = (uint8_t)z;
