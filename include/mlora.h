@@ -673,7 +673,8 @@ int mlora_q4_linear(const void* d_x, int64_t ldx, const void* d_Wq, int32_t grou
  * mlora_prefix_plan: groups the rows of a step (d_row_slot [T]) by prefix, once for all layers.  Prefixes of fewer than 64 tokens
  *   and groups of one row are left to the rows, and so is a group that saves fewer than `least` reads, counted as (rows - 1) x tokens x
  *   key heads (< 0: what measures as worth the second kernel's work).  d_plan: mlora_prefix_plan_bytes(max_rows, Hkv) bytes, 16-byte aligned; max_rows <= 1024.
- * mlora_prefix_plan_rows: the same, without the rows of padding (d_row_pos [T] < 0), which otherwise count as rows of their slot.
+ * mlora_prefix_together: whether a plan takes a group of so many rows behind so many shared tokens together (1) or leaves it to the rows (0).
+ * mlora_prefix_plan_rows: the same as mlora_prefix_plan, without the rows of padding (d_row_pos [T] < 0), which otherwise count as rows of their slot.
  * mlora_paged_attention_shared: out[t, h*D..] = softmax(scale q_t k^T) v over tokens 0..pos_t of the row's sequence (rows with
  *   pos < 0: zeros), q as mlora_kv_append_rope leaves it (row stride ld) and the tokens' keys and values in the pages.  d_plan: of the
  *   same rows, T, Hq and Hkv.  D 64 or 128, pages of 16 or 32, up to 42 query heads per key head.  Results do not depend on which
@@ -686,6 +687,7 @@ int mlora_prefix_plan(const int32_t* d_row_slot, int32_t T, const int32_t* d_pre
                       int32_t Hq, int32_t Hkv, int64_t least, int32_t* d_plan, int32_t max_rows, void* stream);
 int mlora_prefix_plan_rows(const int32_t* d_row_slot, const int32_t* d_row_pos, int32_t T, const int32_t* d_prefix_id, const int32_t* d_prefix_len,
                            int32_t n_slots, int32_t Hq, int32_t Hkv, int64_t least, int32_t* d_plan, int32_t max_rows, void* stream);
+int mlora_prefix_together(int32_t rows, int32_t tokens, int32_t Hkv, int64_t least);
 size_t mlora_paged_attention_shared_workspace(int32_t T, int32_t Hq, int32_t Hkv, int32_t D);
 int mlora_paged_attention_shared(const void* d_q, int64_t ld, const void* d_k_pages, const void* d_v_pages, int32_t n_pages_total,
                                  const int32_t* d_block_table, int32_t max_pages, const int32_t* d_row_slot,

@@ -128,6 +128,7 @@ PROTOTYPES = {
     "mlora_prefix_plan_bytes": (_sz, [_i32, _i32]),
     "mlora_prefix_plan": (C.c_int, [_vp, _i32, _vp, _vp, _i32, _i32, _i32, _i64, _vp, _i32, _vp]),
     "mlora_prefix_plan_rows": (C.c_int, [_vp, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _i64, _vp, _i32, _vp]),
+    "mlora_prefix_together": (C.c_int, [_i32, _i32, _i32, _i64]),
     "mlora_paged_attention_shared_workspace": (_sz, [_i32, _i32, _i32, _i32]),
     "mlora_paged_attention_shared": (C.c_int, [_vp, _i64, _vp, _vp, _i32, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _f32, _vp,
                                                _i32, _vp, _i64, _vp, _sz, _vp, _vp]),

@@ -55,6 +55,11 @@ constexpr int kPlanMinRows = 2, kPlanMinKeys = 64;  // smaller groups and shorte
 //   32 x 8192    31.0   127 |  56.8   347 |  23.5  28.0 |  22.1  62.6
 // Over 784 such cases (2 to 32 rows, 256 to 32768 tokens, 1 to 40 key heads) no group that is taken together loses more than 9 %.
 constexpr int kPlanEnoughRows = 4, kPlanLongKeys = 1024, kPlanManyReads = 200000;
+__host__ __device__ inline bool taken_together(int rows, int keys, int Hkv, long long least) {
+  const long long saved = (long long)(rows - 1) * keys * Hkv;
+  return rows >= kPlanMinRows && keys >= kPlanMinKeys &&
+         (least >= 0 ? saved >= least : rows >= kPlanEnoughRows && (keys >= kPlanLongKeys || saved >= kPlanManyReads));
+}
 // Key ranges that a row's CTA joins in the time of a block, with kJoin of them on their way: some 0.15 us against 2.5 (2 rows behind 32768
 // tokens of one key head, 256 blocks: in 256 ranges 178 us with one range after the other and 72 with kJoin, in some 50 ranges 35; ranges
 // chosen with 6 here in place of 18 cost 5 to 12 % on average over 2 to 32 rows behind 2048 to 32768 tokens of 1 to 40 key heads).
@@ -154,9 +159,7 @@ __global__ void __launch_bounds__(kPlanMaxRows) prefix_plan_kernel(const int32_t
         rank += j < t;
         ++count;
       }
-  const long long saved = (long long)(count - 1) * len * Hkv;
-  const bool used = count >= kPlanMinRows &&
-                    (least >= 0 ? saved >= least : count >= kPlanEnoughRows && (len >= kPlanLongKeys || saved >= kPlanManyReads));
+  const bool used = id >= 0 && taken_together(count, len, Hkv, least);
   s_lead[t] = used ? lead : -1;
   __syncthreads();
   const bool opens = used && rank % rt == 0;  // first row of a tile
@@ -1082,6 +1085,8 @@ extern "C" int mlora_prefix_plan_rows(const int32_t* d_row_slot, const int32_t* 
   MLORA_CHECK_LAUNCH("prefix_plan_kernel");
   return MLORA_OK;
 }
+
+extern "C" int mlora_prefix_together(int32_t rows, int32_t tokens, int32_t Hkv, int64_t least) { return taken_together(rows, tokens, Hkv, least); }
 
 extern "C" size_t mlora_paged_attention_shared_workspace(int32_t T, int32_t Hq, int32_t Hkv, int32_t D) {
   if (!shared_sizes_fit(T, Hq, Hkv, D)) return 0;

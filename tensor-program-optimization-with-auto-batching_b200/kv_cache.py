@@ -14,6 +14,8 @@ will append must be reserved ahead with :meth:`reserve`.
 """
 from __future__ import annotations
 
+from collections import Counter
+
 import numpy as np
 import torch
 
@@ -237,12 +239,12 @@ class PagedKVCache(PagedCache):
         """Whether any two sequences begin with one prefix."""
         return any(n > 1 for n in self._with_prefix.values())
 
-    def shared_by(self, seq_ids) -> bool:
-        """Whether two of these do."""
+    def shared_by(self, seq_ids, least=0) -> bool:
+        """Whether the plan of a step of these takes any of them together (``least``: see :class:`ops.PrefixPlan`)."""
         if not self.shares_prefixes:
             return False
-        known = [self._prefix_of[s][0] for s in seq_ids if s in self._prefix_of]
-        return len(set(known)) < len(known)
+        groups = Counter(self._prefix_of[s] for s in seq_ids if s in self._prefix_of)
+        return any(n > 1 and ops.prefix_together(n, tokens, self.Hkv, least) for (_, tokens), n in groups.items())
 
     def fork(self, sid, source, n_tokens=None):
         """Adds sequence ``sid`` beginning with the first ``n_tokens`` tokens (default: all) of ``source``, whose whole pages it shares from

@@ -353,11 +353,11 @@ class Engine(EngineBase):
         return [self.ws_linear] + ([] if self.ws_q4 is None else [self.ws_q4])
 
     def _shares_prefixes(self, T, fused_append):
-        """Whether two rows of this decode step may begin with one prefix: of its sequences, where they are known, else of the cache's."""
+        """Whether rows of this decode step may be taken together: of its sequences, where they are known, else of any in the cache."""
         if not (fused_append and 1 < T <= self.shared_rows and self.kv.shares_prefixes):
             return False
         seqs = self.kv._pending[0] if self.kv._pending is not None else self.step_seqs
-        return seqs is None or self.kv.shared_by(seqs)
+        return seqs is None or self.kv.shared_by(seqs, self.prefix_least)
 
     def _plan_prefixes(self, T):
         """Which rows of this step share a prefix: once for all layers."""

@@ -1044,6 +1044,11 @@ def prefix_plan(row_slot, prefix_id, prefix_len, plan: PrefixPlan, row_pos=None)
     return plan
 
 
+def prefix_together(rows, tokens, Hkv, least=-1) -> bool:
+    """Whether a plan takes a group of so many rows behind so many shared tokens together."""
+    return bool(_lib.lib().mlora_prefix_together(rows, tokens, Hkv, least))
+
+
 def paged_attention_shared_workspace(T, Hq, Hkv, D) -> int:
     return int(_lib.lib().mlora_paged_attention_shared_workspace(T, Hq, Hkv, D))
 

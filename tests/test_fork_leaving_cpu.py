@@ -86,7 +86,7 @@ def test_steps_whose_rows_share_nothing(kv):
     """The engine takes the route for shared prefixes only where two sequences of the step begin with one."""
     engine = load("model").Engine
     eng = engine.__new__(engine)
-    eng.kv, eng.shared_rows, eng.step_seqs = kv, 256, None
+    eng.kv, eng.shared_rows, eng.step_seqs, eng.prefix_least = kv, 256, None, 0
     for sid in (0, 7, 8):
         kv.add_sequence(sid)
         _grow(kv, sid, 100)
@@ -102,3 +102,25 @@ def test_steps_whose_rows_share_nothing(kv):
         assert eng._shares_prefixes(len(seqs), True) == shares
         eng.step_seqs = None
         assert eng._shares_prefixes(len(seqs), True)  # (a caller's own: any sequences of the cache)
+
+
+def test_steps_whose_groups_are_not_worth_a_plan():
+    """Groups that the plan would leave to their rows: the engine does not make one."""
+    kv = load("kv_cache").PagedKVCache(1, 8, 64, 8, 20000, 64, 16, "cpu", max_seq_len=4000)
+    engine = load("model").Engine
+    eng = engine.__new__(engine)
+    eng.kv, eng.shared_rows, eng.prefix_least = kv, 256, -1
+    for sid, n in ((0, 2000), (10, 900)):
+        kv.add_sequence(sid)
+        _grow(kv, sid, n)
+    for sid in (1, 2, 3):
+        kv.fork(sid, 0)
+    kv.fork(11, 10)
+    for least, shares in ((-1, [True, False, False, False]), (0, [True, True, True, False]), (40000, [True, False, False, False])):
+        eng.prefix_least = least
+        for seqs, want in zip(([0, 1, 2, 3], [3, 1, 2], [10, 11], [0, 10]), shares):
+            eng.step_seqs = seqs
+            assert eng._shares_prefixes(len(seqs), True) == want, (least, seqs)
+    together = load("ops").prefix_together
+    assert together(4, 1024, 1) and not together(3, 32768, 40) and not together(4, 1023, 8) and together(32, 208, 32) and not together(32, 192, 32)
+    assert together(2, 64, 1, 64) and not together(2, 64, 1, 65) and not together(2, 63, 1, 0) and not together(1, 4096, 8, 0)
