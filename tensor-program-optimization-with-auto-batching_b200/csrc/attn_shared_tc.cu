@@ -14,10 +14,11 @@
 // what comes through L2 beyond.  The tail is bound by HBM alone: its tiles have only the query heads of one key head, so it uses mma.sync with 16
 // keys as the rows and up to eight heads as the columns, and a ring of TMA copies in every warp.  It is launched programmatically
 // dependent on the prefix and waits for it only before the join.
-// Measured (CUDA graph, three sets of inputs in turn): 32 rows x 32 heads behind 4096 tokens 60.2 us (3.9 TB/s of the keys and values read
-// once), 72 rows x 40 heads in four groups 153 us (5.9 TB/s), 128 rows x 32 heads over 8 key heads behind 32768 tokens 137 us (502
-// TFLOP/s; every tile reads the prefix through L2: 537 MB), 4 rows behind 512 tokens 12 us.  Exponentials partly on the FMA
-// units (2 % more) and steps of 64 keys with two places for everything (18 % more) are no faster in the third.
+// Measured (CUDA graph, three or four sets of inputs in turn): 32 rows x 32 heads behind 4096 tokens 60.5 us (3.9 TB/s of the keys and values
+// read once), 72 rows x 40 heads in four groups 153 us (5.8 TB/s), 128 rows x 32 heads over 8 key heads behind 32768 tokens 138 us (498
+// TFLOP/s; every tile reads the prefix through L2: 537 MB), 4 rows behind 512 tokens 12.2 us.  Call after call the second and third come to the
+// power limit and take 158 and 147 us.  Exponentials partly on the FMA units (2 % more) and steps of 64 keys with two places for everything
+// (18 % more) were no faster in the third.
 #include <math.h>
 
 #include <atomic>
@@ -32,11 +33,11 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 128;               // (row, query head) pairs of a tile = keys of a block
 constexpr int kSub = kTile * 64 * 2;     // one [128 x 64] bf16 sub-tile: 16 KB
 // A pair's scores are taken against a reference that follows their running maximum only when that is more than 2^kGrow above it: the
-// reference cancels, fp32 sums and weights of 16 bits round those of up to 2^8 no more than those of up to 1, and O stays in TMEM (128 x
-// 32768 143 us, following every maximum 150).
+// reference cancels, fp32 sums and weights of 16 bits round those of up to 2^8 no more than those of up to 1, and O stays in TMEM (following
+// every maximum takes 128 x 32768 5 % more).
 constexpr float kGrow = 8.f;
 constexpr int kPxThreads = 192;          // warps 0..3: one thread per pair; 4: MMA issue, copies of keys; 5: copies of values
-constexpr int kPxRegs = 128;             // two CTAs per SM leave room for the tail's (72 rows x 40 heads 146 us, with 168 160)
+constexpr int kPxRegs = 128;             // two CTAs per SM leave room for the tail's (72 rows x 40 heads: 10 % more time with 168)
 constexpr int kPlanMaxRows = 1024;
 constexpr int kPlanHeader = 8;           // int32: rows, tiles, items, parts
 constexpr int kTickets = 1024;           // arrival counters at the start of the scratch, whatever the call's sizes: zero between calls
@@ -258,8 +259,9 @@ __device__ __forceinline__ float fast_exp2(float x) {
 
 // Two weights as the sum of two pairs of bf16: what a truncation leaves is rounded, so that the products with the values see them to 2^-15
 // and the sum l, which is taken before, fits them.  Decode attention without shared prefixes has fp32 weights; with bf16
-// ones a row's error was 0.0019 of the result in place of 0.0017, which is the result's own rounding (128 x 32768: 132 us).  Truncating is
-// a byte permutation; rounding the first part as well costs 6 % there.
+// ones a row's error was 0.0019 of the result in place of 0.0017, which is the result's own rounding; twice the products and as many stores
+// to TMEM cost 3 % at 32 x 4096, 5 % at four groups of 40 heads and, with the reference that lags behind, 4 to 10 % at 128 x 32768.  Truncating
+// is a byte permutation; rounding the first part as well costs 6 % more there.
 __device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
   const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
   hi = __byte_perm(a, b, 0x7632);
@@ -279,8 +281,8 @@ struct SharedArgs {
   int T, Hq, Hkv, page_size;
   int32_t* plan;
   int plan_rows;
-  float* parts;     // [part][Hq][D + 2]: O, m, l of a row's key range (base-2 logarithms)
-  float* own;       // [T][Hq][n_splits][D + 2]
+  float* parts;     // [part][Hq][D + 4]: O, m, l of a row's key range (base-2 logarithms)
+  float* own;       // [T][Hq][n_splits][D + 4]
   int32_t* tickets; // [T][Hkv][head tiles], zero between calls
   int n_splits;
   bf16* out;
@@ -292,7 +294,8 @@ struct SharedArgs {
 // The matrix products multiply every value of a block with every pair's weight: a value that is infinite or none makes the sums NaN for pairs
 // that do not see its key (weight 0) or whose weight has no second part.  A sum that has met one stays infinite or NaN, so that is looked at
 // once, at the end, and the few pairs whose sums are not finite are weighed again by this function, a warp for a pair, key by key in fp32:
-// keys that the pair does not see or scores -inf are left out, whatever their values are.
+// keys that the pair does not see or scores -inf are left out, whatever their values are.  (Looking at the sums costs 1 %; one infinite value in
+// 32768 tokens that 512 pairs share costs some 55 ms, in 4096 tokens of 32 pairs 8.)
 // dst[c] = sum of exp2(scale q k - m) v[c] over the keys of [lo, hi) in the units of 16 from k0 on, every `step` keys.
 template <int D>
 __device__ __noinline__ void weigh_again(const bf16* q, const bf16* k_pages, const bf16* v_pages, int n_pages, const int32_t* bt, int Hkv, int kvh, int PS,
@@ -684,7 +687,7 @@ __global__ void __launch_bounds__(W * 32, 12 / W) tail_attn_kernel(const __grid_
 
   uint8_t* mine = ring + warp * STAGES * 2 * kHalf;
   int page = 0;  // of the lane's unit among the 32 that come next: one read for them all, not one per unit in front of its copies
-  auto fetch = [&](int i) {  // unit ub + warp + 4 i -> stage i % STAGES
+  auto fetch = [&](int i) {  // unit ub + warp + W i -> stage i % STAGES
     if ((i & 31) == 0) {
       const int u = ub + warp + (i + lane) * kTlWarps;
       page = u < ue ? bt[u * kTlKeys / PS] : 0;
@@ -789,7 +792,7 @@ __global__ void __launch_bounds__(W * 32, 12 / W) tail_attn_kernel(const __grid_
   __syncthreads();  // every warp is done with the ring
   if (s_abort && tid == 0 && a.status) atomicOr(a.status, 1);
 
-  // ---- the four warps' results, joined with what the prefix's key ranges left ---------------------------------------------------
+  // ---- the warps' results, joined with what the prefix's key ranges left ---------------------------------------------------
   float* acc = reinterpret_cast<float*>(ring);  // [warp][head][D]
 #pragma unroll
   for (int h = 0; h < 2; ++h) {

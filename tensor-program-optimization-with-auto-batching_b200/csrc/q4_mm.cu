@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(kMmThreads, 2) q4_mm_kernel(const __grid_const
       }
       ok = mm_all(ok);  // (also: the sums before have been read)
       if (!ok) break;
-      // ---- the segment is done: the four blocks' sums, then output, or a share of a tile that another CTA finishes -----------------
+      // ---- the segment is done: the two warps' sums, then output, or a share of a tile that another CTA finishes -----------------
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll

@@ -4,7 +4,7 @@
 // bf16 integers q - z and write them to TMEM (tcgen05.st.16x128b has the lanes where the packed order has them): weights go DRAM -> shared
 // memory -> registers -> TMEM and are never written to shared memory as bf16, whose 32 KB per 8 KB of weights would be more than its
 // bandwidth.  The MMA takes them from there as its A operand -- 16 cycles per m128n32k16, against 40 from shared memory -- and the rows of
-// x (TMA, 128-byte swizzle) as B.  A group's sums have an accumulator of their own, which four or eight warps scale in fp32 registers
+// x (TMA, 128-byte swizzle) as B.  A group's sums have an accumulator of their own, which 4, 8 or 16 warps scale in fp32 registers
 // while the next ones are filled: nothing but the output is rounded.
 //
 // Persistent, one CTA per SM; the units of all tiles are dealt out in equal ranges.  A tile that several CTAs share is finished by the one
@@ -12,7 +12,7 @@
 // inputs.  Adapters are expanded by a kernel of their own in front of this one, into fp32 scratch that is added to the sums: a thread here
 // has one output and many rows, whose adapters' rows it would have to wait for one after the other.
 //
-// What bounds it: the warps that hand units on.  Their instructions come one after the other, some ten cycles each among the 17 to 27
+// What bounds it: the warps that hand units on.  Their instructions come one after the other, some ten cycles each among the 19 or 27
 // warps of an SM: with one unit per barrier, counters instead of remainders and one barrier for weights and rows of x a unit takes 950
 // cycles at 32 rows, against 350 in which HBM delivers it and 128 in which it is multiplied.  Groups of 32 or 64 have an accumulator to
 // hand on for each of them.  Measured (CUDA graph): 32 x 4096 x 22016 25.6 us, 128 rows 36.3, 512 x 4096 x 11008 58.7 (787 TFLOP/s);
