@@ -673,7 +673,8 @@ int mlora_q4_linear(const void* d_x, int64_t ldx, const void* d_Wq, int32_t grou
  * mlora_prefix_plan: groups the rows of a step (d_row_slot [T]) by prefix, once for all layers.  Prefixes of fewer than 64 tokens
  *   and groups of one row are left to the rows, and so is a group that saves fewer than `least` reads, counted as (rows - 1) x tokens x
  *   key heads (< 0: what measures as worth the second kernel's work).  d_plan: mlora_prefix_plan_bytes(max_rows, Hkv) bytes, 16-byte aligned; max_rows <= 1024.
- * mlora_prefix_together: whether a plan takes a group of so many rows behind so many shared tokens together (1) or leaves it to the rows (0).
+ * mlora_prefix_together: whether a plan takes a group of so many rows behind so many shared tokens together (1) or leaves it to the rows (0);
+ *   negative: an error.
  * mlora_prefix_plan_rows: the same as mlora_prefix_plan, without the rows of padding (d_row_pos [T] < 0), which otherwise count as rows of their slot.
  * mlora_paged_attention_shared: out[t, h*D..] = softmax(scale q_t k^T) v over tokens 0..pos_t of the row's sequence (rows with
  *   pos < 0: zeros), q as mlora_kv_append_rope leaves it (row stride ld) and the tokens' keys and values in the pages.  d_plan: of the

@@ -1089,7 +1089,10 @@ extern "C" int mlora_prefix_plan_rows(const int32_t* d_row_slot, const int32_t* 
   return MLORA_OK;
 }
 
-extern "C" int mlora_prefix_together(int32_t rows, int32_t tokens, int32_t Hkv, int64_t least) { return taken_together(rows, tokens, Hkv, least); }
+extern "C" int mlora_prefix_together(int32_t rows, int32_t tokens, int32_t Hkv, int64_t least) {
+  MLORA_REQUIRE(rows >= 0 && tokens >= 0 && Hkv > 0, "prefix_together: bad sizes %d rows, %d tokens, %d key heads", rows, tokens, Hkv);
+  return taken_together(rows, tokens, Hkv, least) ? 1 : 0;
+}
 
 extern "C" size_t mlora_paged_attention_shared_workspace(int32_t T, int32_t Hq, int32_t Hkv, int32_t D) {
   if (!shared_sizes_fit(T, Hq, Hkv, D)) return 0;

@@ -1046,7 +1046,10 @@ def prefix_plan(row_slot, prefix_id, prefix_len, plan: PrefixPlan, row_pos=None)
 
 def prefix_together(rows, tokens, Hkv, least=-1) -> bool:
     """Whether a plan takes a group of so many rows behind so many shared tokens together."""
-    return bool(_lib.lib().mlora_prefix_together(rows, tokens, Hkv, least))
+    yes = _lib.lib().mlora_prefix_together(rows, tokens, Hkv, least)
+    if yes < 0:
+        check(yes, "mlora_prefix_together")
+    return bool(yes)
 
 
 def paged_attention_shared_workspace(T, Hq, Hkv, D) -> int:

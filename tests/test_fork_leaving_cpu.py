@@ -124,3 +124,9 @@ def test_steps_whose_groups_are_not_worth_a_plan():
     together = load("ops").prefix_together
     assert together(4, 1024, 1) and not together(3, 32768, 40) and not together(4, 1023, 8) and together(32, 208, 32) and not together(32, 192, 32)
     assert together(2, 64, 1, 64) and not together(2, 64, 1, 65) and not together(2, 63, 1, 0) and not together(1, 4096, 8, 0)
+
+
+@pytest.mark.parametrize("rows,tokens,kv_heads", [(-1, 64, 8), (4, -1, 8), (4, 1024, 0)])
+def test_groups_of_no_size_are_refused(rows, tokens, kv_heads):
+    with pytest.raises(load("_lib").MloraError, match="bad sizes"):
+        load("ops").prefix_together(rows, tokens, kv_heads)
